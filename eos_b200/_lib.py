@@ -36,6 +36,10 @@ class TokenPoolDesc(C.Structure):
                 ("hidden_projection", C.c_void_p), ("projection", C.c_void_p)]
 
 
+class KvStrides(C.Structure):
+    _fields_ = [("key_token", C.c_int64), ("key_head", C.c_int64), ("value_token", C.c_int64), ("value_head", C.c_int64)]
+
+
 class EncoderTimes(C.Structure):
     _fields_ = [("steps", C.c_int32), ("gemm_launches", C.c_int32), ("attention_launches", C.c_int32),
                 ("layernorm_launches", C.c_int32), ("other_launches", C.c_int32), ("gemm_ms", C.c_float),
@@ -163,6 +167,16 @@ SYMBOLS = {
                                             C.c_int, _P, C.POINTER(Stats), _ERR]),
     "eos_b200_turbo_sparse_attention": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                                   C.c_int, _P, C.POINTER(Stats), _ERR]),
+    "eos_b200_kv_cache_create": (C.c_int, [_P, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(_P), _ERR]),
+    "eos_b200_kv_cache_destroy": (None, [_P]),
+    "eos_b200_kv_cache_page_bytes": (C.c_int64, [_P]),
+    "eos_b200_kv_cache_append_device": (C.c_int, [_P, _P, _P, C.c_int, C.c_int64, C.POINTER(KvStrides), C.c_int, _P, C.c_int, _P,
+                                                  _P, _P, C.POINTER(Stats), _ERR]),
+    "eos_b200_kv_cache_read_device": (C.c_int, [_P, _P, _P, C.c_int, C.c_int64, C.POINTER(KvStrides), C.c_int, _P, C.c_int, _P,
+                                                _P, _P, C.POINTER(Stats), _ERR]),
+    "eos_b200_kv_cache_attend_device": (C.c_int, [_P, _P, C.c_int, C.c_int, C.c_int64, C.c_int64, C.c_int, _P, C.c_int, _P,
+                                                  C.c_float, C.c_int, _P, _P, _P, C.POINTER(Stats), _ERR]),
+    "eos_b200_kv_cache_sync": (C.c_int, [_P, _P, _ERR]),
     "eos_b200_synth_gaussian_device": (C.c_int, [_P, C.c_uint64, C.c_int64, C.c_int64, C.c_int, C.c_int, _P, _P,
                                                  _ERR]),
 }

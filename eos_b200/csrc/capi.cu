@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -18,6 +19,7 @@
 #include "attention_tc.cuh"
 #include "encoder_kernels.cuh"
 #include "gemm_tc.cuh"
+#include "kv_cache.cuh"
 #include "sparse_attention.cuh"
 #include "token_pool.cuh"
 #include "turboquant.cuh"
@@ -112,6 +114,8 @@ int read_status(EosB200Runtime* rt, cudaStream_t s, char** err) {
     if (st == kStatusBadTokenId) what = "input_ids value out of range [0, vocab)";
     else if (st == kStatusBadTypeId) what = "token_type_ids value out of range";
     else if (st == kStatusBadPosition) what = "sequence longer than max_positions";
+    else if (st == kStatusBadPage) what = "page id outside the cache, or a position behind the sequence's page table";
+    else if (st == kStatusBadSequence) what = "length, start or row offset of a sequence out of range";
     else if (st == kStatusPipelineTimeout) what = "a bounded wait inside a kernel ran out (pipeline timeout)";
     return fail(err, std::string("device status ") + std::to_string(st) + ": " + what, EOS_B200_DEVICE_STATUS);
 }
@@ -3693,6 +3697,190 @@ int eos_b200_token_pool_encode(EosB200TokenPool* tp, const int32_t* h_tokens, co
             return fail(err, "token_pool_encode: span [" + std::to_string(starts[i]) + "," + std::to_string(ends[i]) +
                                  ") has no active tokens");
     return EOS_B200_OK;
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------------------
+// paged key-value cache
+// ------------------------------------------------------------------------------------------------
+struct EosB200KvCache {
+    EosB200Runtime* rt = nullptr;
+    KvPool pool{};
+};
+
+namespace {
+
+int type_bytes(int type) { return type == EOS_B200_TYPE_F32 ? 4 : 2; }
+
+bool aligned16(const void* p, int64_t stride_a, int64_t stride_b, int type) {
+    const int64_t es = type_bytes(type);
+    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride_a * es % 16 == 0 && stride_b * es % 16 == 0;
+}
+
+// What append and read check alike; fills the kernels' views.
+std::string kv_rows_check(const EosB200KvCache* c, const void* key, const void* value, int type, int64_t tokens,
+                          const EosB200KvStrides* st, int batch, const int32_t* table, int max_pages, const int32_t* starts,
+                          const int32_t* cu, KvSeqs* seqs, KvRows* k, KvRows* v) {
+    if (type < EOS_B200_TYPE_F32 || type > EOS_B200_TYPE_BF16) return "unknown element type";
+    if (tokens < 0 || batch < 0) return "negative token or sequence count";
+    if (tokens > 0x7fffffffLL) return "more than 2^31 - 1 tokens in one call";
+    if (cu == nullptr && tokens != batch) return "without row offsets there is one token per sequence (tokens == batch)";
+    if (tokens == 0 || batch == 0) return "";
+    if (key == nullptr || value == nullptr || table == nullptr || starts == nullptr) return "null argument";
+    if (max_pages <= 0) return "max_pages must be positive";
+    const int64_t dim = c->pool.dim, row = dim * c->pool.heads;
+    EosB200KvStrides s = {row, dim, row, dim};
+    if (st != nullptr) s = *st;
+    if (s.key_token < 0 || s.key_head < 0 || s.value_token < 0 || s.value_head < 0) return "negative stride";
+    if (reinterpret_cast<uintptr_t>(key) % type_bytes(type) != 0 || reinterpret_cast<uintptr_t>(value) % type_bytes(type) != 0)
+        return "key or value is not aligned to its element type";
+    // blocks of eight warps, one (record, head) each
+    if ((tokens / kKvRecord + 2 * (int64_t)batch + 1) * c->pool.heads / 8 >= 0x7fffffffLL) return "too many tokens x heads in one call";
+    *seqs = {table, max_pages, batch, starts, cu, nullptr};
+    *k = {const_cast<void*>(key), s.key_token, s.key_head, aligned16(key, s.key_token, s.key_head, type) ? 1 : 0};
+    *v = {const_cast<void*>(value), s.value_token, s.value_head, aligned16(value, s.value_token, s.value_head, type) ? 1 : 0};
+    return "";
+}
+
+}  // namespace
+
+extern "C" {
+
+int eos_b200_kv_cache_create(EosB200Runtime* rt, int64_t pages, int page_size, int kv_heads, int head_dim, int format,
+                             EosB200KvCache** out, char** err) {
+    if (rt == nullptr || out == nullptr) return fail(err, "kv_cache_create: null argument");
+    *out = nullptr;
+    if (format < EOS_B200_KV_F16 || format > EOS_B200_KV_MX4) return fail(err, "kv_cache_create: unknown format");
+    if (head_dim != 32 && head_dim != 64 && head_dim != 96 && head_dim != 128 && head_dim != 192 && head_dim != 256)
+        return fail(err, "kv_cache_create: head_dim must be 32, 64, 96, 128, 192 or 256");
+    if (page_size < kKvRecord || page_size > 65536 || page_size % kKvRecord != 0)
+        return fail(err, "kv_cache_create: page_size must be a multiple of 16, at most 65536");
+    if (kv_heads <= 0 || kv_heads > 4096) return fail(err, "kv_cache_create: kv_heads must be in [1, 4096]");
+    if (pages <= 0 || pages > 0x7fffffffLL) return fail(err, "kv_cache_create: pages must be in [1, 2^31)");
+    KvPool p{};
+    p.pages = pages;
+    p.heads = kv_heads;
+    p.dim = head_dim;
+    p.blocks = head_dim / 32;
+    p.format = format;
+    p.records_per_page = page_size / kKvRecord;
+    p.record_bytes = kv_record_bytes(format, p.blocks);
+    const int64_t page_bytes = (int64_t)p.records_per_page * p.record_bytes * kv_heads;
+    if (pages > (int64_t)(rt->prop.totalGlobalMem / (size_t)page_bytes))
+        return fail(err, "kv_cache_create: " + std::to_string(pages) + " pages of " + std::to_string(page_bytes) +
+                             " bytes exceed the device's memory");
+    CUDA_TRY(cudaSetDevice(rt->device));
+    CUDA_TRY(kv_attend_init(format, p.blocks));
+    CUDA_TRY(dev_alloc(&p.base, (size_t)(pages * page_bytes)));
+    cudaError_t e = cudaMemsetAsync(p.base, 0, (size_t)(pages * page_bytes), rt->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(rt->stream);
+    EosB200KvCache* c = e == cudaSuccess ? new (std::nothrow) EosB200KvCache() : nullptr;
+    if (c == nullptr) {
+        cudaGetLastError();
+        cudaFree(p.base);
+        return fail(err, std::string("kv_cache_create: ") + (e != cudaSuccess ? cudaGetErrorString(e) : "out of host memory"));
+    }
+    c->rt = rt;
+    c->pool = p;
+    *out = c;
+    return EOS_B200_OK;
+}
+
+void eos_b200_kv_cache_destroy(EosB200KvCache* c) {
+    if (c == nullptr) return;
+    cudaSetDevice(c->rt->device);
+    dev_free(c->pool.base);
+    delete c;
+}
+
+int64_t eos_b200_kv_cache_page_bytes(const EosB200KvCache* c) {
+    return c == nullptr ? 0 : (int64_t)c->pool.records_per_page * c->pool.record_bytes * c->pool.heads;
+}
+
+int eos_b200_kv_cache_append_device(EosB200KvCache* c, const void* d_key, const void* d_value, int type, int64_t tokens,
+                                    const EosB200KvStrides* strides, int batch, const int32_t* d_page_table, int max_pages,
+                                    const int32_t* d_starts, const int32_t* d_cu_tokens, void* stream, EosB200Stats* stats,
+                                    char** err) {
+    if (c == nullptr) return fail(err, "kv_cache_append: null cache");
+    KvSeqs seqs{};
+    KvRows k{}, v{};
+    const std::string why = kv_rows_check(c, d_key, d_value, type, tokens, strides, batch, d_page_table, max_pages, d_starts,
+                                          d_cu_tokens, &seqs, &k, &v);
+    if (!why.empty()) return fail(err, "kv_cache_append: " + why);
+    if (stats != nullptr) std::memset(stats, 0, sizeof(*stats));
+    if (tokens == 0 || batch == 0) return EOS_B200_OK;
+    CUDA_TRY(cudaSetDevice(c->rt->device));
+    launch_kv_append(c->pool, seqs, k, v, type, tokens, c->rt->d_status, pick_stream(c->rt, stream));
+    CUDA_TRY(cudaGetLastError());
+    if (stats != nullptr) stats->kernel_launches = 1;
+    return EOS_B200_OK;
+}
+
+int eos_b200_kv_cache_read_device(EosB200KvCache* c, void* d_key, void* d_value, int type, int64_t tokens,
+                                  const EosB200KvStrides* strides, int batch, const int32_t* d_page_table, int max_pages,
+                                  const int32_t* d_starts, const int32_t* d_cu_tokens, void* stream, EosB200Stats* stats,
+                                  char** err) {
+    if (c == nullptr) return fail(err, "kv_cache_read: null cache");
+    KvSeqs seqs{};
+    KvRows k{}, v{};
+    const std::string why = kv_rows_check(c, d_key, d_value, type, tokens, strides, batch, d_page_table, max_pages, d_starts,
+                                          d_cu_tokens, &seqs, &k, &v);
+    if (!why.empty()) return fail(err, "kv_cache_read: " + why);
+    if (stats != nullptr) std::memset(stats, 0, sizeof(*stats));
+    if (tokens == 0 || batch == 0) return EOS_B200_OK;
+    CUDA_TRY(cudaSetDevice(c->rt->device));
+    launch_kv_read(c->pool, seqs, k, v, type, tokens, c->rt->d_status, pick_stream(c->rt, stream));
+    CUDA_TRY(cudaGetLastError());
+    if (stats != nullptr) stats->kernel_launches = 1;
+    return EOS_B200_OK;
+}
+
+int eos_b200_kv_cache_attend_device(EosB200KvCache* c, const void* d_query, int type, int q_heads, int64_t query_seq_stride,
+                                    int64_t query_head_stride, int batch, const int32_t* d_page_table, int max_pages,
+                                    const int32_t* d_lengths, float scale, int window, void* d_out, float* d_lse, void* stream,
+                                    EosB200Stats* stats, char** err) {
+    if (c == nullptr) return fail(err, "kv_cache_attend: null cache");
+    if (type < EOS_B200_TYPE_F32 || type > EOS_B200_TYPE_BF16) return fail(err, "kv_cache_attend: unknown element type");
+    if (batch < 0 || batch > 65535) return fail(err, "kv_cache_attend: batch must be in [0, 65535]");
+    if (q_heads <= 0 || q_heads % c->pool.heads != 0)
+        return fail(err, "kv_cache_attend: q_heads " + std::to_string(q_heads) + " is not a multiple of the cache's " +
+                             std::to_string(c->pool.heads) + " key heads");
+    if (q_heads > 65536) return fail(err, "kv_cache_attend: more than 65536 query heads");
+    if (!std::isfinite(scale)) return fail(err, "kv_cache_attend: scale must be finite");
+    if (window < 0) return fail(err, "kv_cache_attend: negative window");
+    if (query_seq_stride < 0 || query_head_stride < 0) return fail(err, "kv_cache_attend: negative stride");
+    if (stats != nullptr) std::memset(stats, 0, sizeof(*stats));
+    if (batch == 0) return EOS_B200_OK;
+    if (d_query == nullptr || d_page_table == nullptr || d_lengths == nullptr || d_out == nullptr)
+        return fail(err, "kv_cache_attend: null argument");
+    if (max_pages <= 0) return fail(err, "kv_cache_attend: max_pages must be positive");
+    if (reinterpret_cast<uintptr_t>(d_query) % type_bytes(type) != 0 || reinterpret_cast<uintptr_t>(d_out) % type_bytes(type) != 0)
+        return fail(err, "kv_cache_attend: query or out is not aligned to its element type");
+    KvSeqs seqs = {d_page_table, max_pages, batch, nullptr, nullptr, d_lengths};
+    KvAttend a{};
+    a.query = d_query;
+    a.head_stride = query_head_stride > 0 ? query_head_stride : c->pool.dim;
+    a.seq_stride = query_seq_stride > 0 ? query_seq_stride : (int64_t)q_heads * c->pool.dim;
+    a.vec = aligned16(d_query, a.seq_stride, a.head_stride, type) ? 1 : 0;
+    a.type = type;
+    a.q_heads = q_heads;
+    a.group = q_heads / c->pool.heads;
+    a.out = d_out;
+    a.lse = d_lse;
+    a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+    a.window = window;
+    CUDA_TRY(cudaSetDevice(c->rt->device));
+    const int launches = launch_kv_attend(c->pool, seqs, a, c->rt->d_status, pick_stream(c->rt, stream));
+    CUDA_TRY(cudaGetLastError());
+    if (stats != nullptr) stats->kernel_launches = launches;
+    return EOS_B200_OK;
+}
+
+int eos_b200_kv_cache_sync(EosB200KvCache* c, void* stream, char** err) {
+    if (c == nullptr) return fail(err, "kv_cache_sync: null cache");
+    CUDA_TRY(cudaSetDevice(c->rt->device));
+    return read_status(c->rt, pick_stream(c->rt, stream), err);
 }
 
 }  // extern "C"

@@ -14,7 +14,9 @@ enum : int {
     kStatusBadTokenId = 1,      // input id outside [0, vocab)
     kStatusBadTypeId = 2,       // token type id outside [0, type_vocab)
     kStatusBadPosition = 3,     // position >= max positions
-    kStatusPipelineTimeout = 4  // a bounded mbarrier wait inside a kernel ran out
+    kStatusPipelineTimeout = 4, // a bounded mbarrier wait inside a kernel ran out
+    kStatusBadPage = 5,         // page id outside the cache, or a position behind the sequence's page table
+    kStatusBadSequence = 6      // lengths, starts or row offsets of a sequence out of range
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }

@@ -1,0 +1,502 @@
+// One new token a sequence attends over its cached keys and values: the kernel template (one instance per format, head
+// size and row tiles; kv_attend_*.cu compile them).
+//
+//     out = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),   x_j = scale log2(e) q . k_j,   one pass with a running maximum m
+//
+// A warp takes one record (16 tokens of one key head) at a time with mma.sync m16n8k16: the query heads that share the
+// key head are the rows.  At most 8 heads use a tile's 16 rows: rows 0-7 hold the upper half of every fp32 factor
+// (query or weight) and rows 8-15 what the rounding to 16 bits left over, so the products carry 22 bits (f16 operands)
+// at no extra instruction -- each thread finds both halves of its sums in its own registers.  The factor is split, not
+// the cached value, which is exact in its operand type.
+//
+// The maxima are integers, and lag: m is set 7 below the largest score and moves only when a score passes m + 15, so most
+// records do no rescaling and no shuffles, and weights use f16's range from both ends: they stay below 2^15, and what
+// f16 cannot hold (2^-25) is 2^-31 of the row's largest weight.  A weight and its value's scale are multiplied before the
+// split: w = 2^(x + e - M) with e the largest scale exponent of the token's blocks and M a second lagging maximum, so that
+// the bound holds whatever the scales; the blocks' own exponents (relative to e) are applied to the codes as f16 factors,
+// shifted up as far as the codes allow: what falls below f16 there is 2^-33 of the token's largest value.
+#pragma once
+#include "kv_dev.cuh"
+
+namespace eosb {
+
+constexpr float kKvMaxInit = -1e30f;   // below every score; finite, so that 2^(x - m) of a masked score is 0 and not NaN
+constexpr float kKvHead = 7.f, kKvLag = 15.f;   // m = ceil(largest score) - 7; weights up to 2^15
+constexpr int kKvQueryExp = 13;                  // query rows are scaled to a largest magnitude in [2^13, 2^14)
+// exponent that the blocks' relative scales are shifted up by: the largest code, 448 or 6, times 2^this is below 65504
+__host__ __device__ constexpr int kv_rel_shift(int format) { return format == kKvMx8 ? 6 : 13; }
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+template <bool kBf>
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                            uint32_t b1) {
+    if constexpr (kBf)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// a pair of fp32 values as the sum of two 16-bit pairs
+template <bool kBf>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
+    if constexpr (kBf) {
+        hi = bf16x2_of(a, b);
+        const float2 f = bf16x2_floats(hi);
+        lo = bf16x2_of(a - f.x, b - f.y);
+    } else {
+        hi = f16x2_of(a, b);
+        const float2 f = f16x2_floats(hi);
+        lo = f16x2_of(a - f.x, b - f.y);
+    }
+}
+
+// The bytes of one lane at `plane0`, BYTES of them (see kv_lane_offset)
+template <int BYTES>
+__device__ __forceinline__ void load_lane(const uint8_t* plane0, int lane, uint32_t (&w)[BYTES / 4]) {
+#pragma unroll
+    for (int p = 0; p + 16 <= BYTES; p += 16) {
+        const uint4 v = *reinterpret_cast<const uint4*>(plane0 + p * 32 + lane * 16);
+        w[p / 4] = v.x, w[p / 4 + 1] = v.y, w[p / 4 + 2] = v.z, w[p / 4 + 3] = v.w;
+    }
+    constexpr int r = BYTES & 15, p = BYTES - r;
+    if constexpr (r >= 8) {
+        const uint2 v = *reinterpret_cast<const uint2*>(plane0 + p * 32 + lane * 8);
+        w[p / 4] = v.x, w[p / 4 + 1] = v.y;
+    }
+    if constexpr ((r & 7) != 0)
+        w[BYTES / 4 - 1] = *reinterpret_cast<const uint32_t*>(plane0 + p * 32 + (r >= 8 ? 256 : 0) + lane * 4);
+}
+
+// Scale bytes of two neighbouring tokens, packed four to a word
+template <int NB>
+__device__ __forceinline__ void load_scales(const uint8_t* p, uint32_t (&a)[(NB + 3) / 4], uint32_t (&b)[(NB + 3) / 4]) {
+    if constexpr (NB == 1) {
+        const uint32_t w = *reinterpret_cast<const uint16_t*>(p);
+        a[0] = w & 0xffu, b[0] = w >> 8;
+    } else if constexpr (NB == 2) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+        a[0] = w & 0xffffu, b[0] = w >> 16;
+    } else if constexpr (NB <= 4) {
+        const uint2 w = *reinterpret_cast<const uint2*>(p);
+        a[0] = w.x, b[0] = w.y;
+    } else {
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        a[0] = w.x, a[1] = w.y, b[0] = w.z, b[1] = w.w;
+    }
+}
+// exponent field of byte i as a float 2^(byte - 127); 255 becomes infinity, which times the zero codes of such a block is NaN
+__device__ __forceinline__ float scale_at(uint32_t word, int i) {
+    return __uint_as_float(i == 3 ? (word >> 1) & 0x7f800000u
+                                  : (i == 2 ? (word << 7) & 0x7f800000u
+                                            : (i == 1 ? (word << 15) & 0x7f800000u : (word << 23) & 0x7f800000u)));
+}
+
+template <int FMT, int NB, int RT>
+struct KvWarp {
+    static constexpr bool kMx = FMT >= kKvMx8, kBf = FMT == kKvBf16;
+    static constexpr int KP = kv_key_piece(FMT), VP = kv_value_piece(FMT), D = 32 * NB;
+
+    uint32_t q[RT][NB][8];      // per block: 4 upper words, 4 lower words (8 elements of the lane's row)
+    float qs[RT];               // factor of the raw sums: scale log2(e) 2^(query exponent)
+    float m[RT], big[RT], l[RT];   // lagging maxima of x and of x + e (mx formats), this lane's part of the sum of weights
+    float o[RT][4 * NB][4];
+
+    __device__ __forceinline__ void reset() {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            m[r] = big[r] = kKvMaxInit;
+            l[r] = 0.f;
+#pragma unroll
+            for (int n = 0; n < 4 * NB; ++n) o[r][n][0] = o[r][n][1] = o[r][n][2] = o[r][n][3] = 0.f;
+        }
+    }
+
+    // Query rows [row0, row0 + 8 RT) of a unit, those from `rows` on are zero.  f16 operands: each row is divided by a
+    // power of two first, so that no magnitude leaves f16's range.
+    __device__ __forceinline__ void load_query(const KvAttend& a, int64_t at, int row0, int rows, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const int row = row0 + 8 * r + g;
+            const int64_t p = at + (int64_t)row * a.head_stride + 8 * t;
+            float x[NB][8];
+            uint32_t top = 0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if (row < rows) load_row<8>(a.query, p + 32 * b, a.type, a.vec, x[b]);
+                else
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[b][i] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[b][i]) & 0x7fffffffu);
+            }
+            float inv = 1.f;
+            qs[r] = a.scale_log2;
+            if constexpr (!kBf) {
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const uint32_t e = min(max(top >> 23, kKvQueryExp + 1u), 254u);
+                inv = __uint_as_float((254u + kKvQueryExp - e) << 23);
+                qs[r] *= __uint_as_float((e - kKvQueryExp) << 23);
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) split_pair<kBf>(x[b][2 * i] * inv, x[b][2 * i + 1] * inv, q[r][b][i], q[r][b][4 + i]);
+        }
+    }
+
+    // One record; its tokens [lo, hi) of 0..15 count.
+    __device__ __forceinline__ void record(const uint8_t* rec, int lo, int hi, int lane) {
+        const int t = lane & 3;
+        float x[RT][4];   // scores of row g: tokens 2t, 2t+1, 2t+8, 2t+9
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            uint32_t k[NB * KP / 4];
+            load_lane<NB * KP>(rec + j * 32 * NB * KP, lane, k);
+            float s0[RT], s1[RT];
+            if constexpr (!kMx) {
+                float c[RT][4];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) c[r][0] = c[r][1] = c[r][2] = c[r][3] = 0.f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s)
+#pragma unroll
+                        for (int r = 0; r < RT; ++r)
+                            mma_16x8x16<kBf>(c[r], q[r][b][2 * s], q[r][b][4 + 2 * s], q[r][b][2 * s + 1],
+                                             q[r][b][4 + 2 * s + 1], k[4 * b + 2 * s], k[4 * b + 2 * s + 1]);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) s0[r] = c[r][0] + c[r][2], s1[r] = c[r][1] + c[r][3];
+            } else {
+                uint32_t sa[(NB + 3) / 4], sb[(NB + 3) / 4];
+                load_scales<NB>(rec + kv_key_scale_offset(FMT, NB) + (8 * j + 2 * t) * kv_scale_stride(NB), sa, sb);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) s0[r] = s1[r] = 0.f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    uint32_t f[4];
+                    if constexpr (FMT == kKvMx8) {
+                        f16_of_e4m3x4(k[2 * b], f[0], f[1]);
+                        f16_of_e4m3x4(k[2 * b + 1], f[2], f[3]);
+                    } else {
+                        f16_of_e2m1x8(k[b], f[0], f[1], f[2], f[3]);
+                    }
+                    const float ca = scale_at(sa[b / 4], b & 3), cb = scale_at(sb[b / 4], b & 3);
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        float c[4] = {0.f, 0.f, 0.f, 0.f};
+                        mma_16x8x16<false>(c, q[r][b][0], q[r][b][4], q[r][b][1], q[r][b][5], f[0], f[1]);
+                        mma_16x8x16<false>(c, q[r][b][2], q[r][b][6], q[r][b][3], q[r][b][7], f[2], f[3]);
+                        s0[r] = fmaf(c[0] + c[2], ca, s0[r]);
+                        s1[r] = fmaf(c[1] + c[3], cb, s1[r]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) x[r][2 * j] = s0[r] * qs[r], x[r][2 * j + 1] = s1[r] * qs[r];
+        }
+        const bool edge = lo > 0 || hi < kKvRecord;
+        uint32_t live = 15u;
+        if (edge) {
+            live = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int tok = 2 * t + (i & 1) + 8 * (i >> 1);
+                if (tok >= lo && tok < hi) live |= 1u << i;
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+                    if (!(live >> i & 1)) x[r][i] = -INFINITY;
+            }
+        }
+        // value scales: largest exponent of each token, and every block's exponent relative to it as f16 pairs
+        float te[4];
+        uint32_t rel[2][NB];
+        if constexpr (kMx) {
+            uint32_t sc[4][(NB + 3) / 4];
+            const uint8_t* p = rec + kv_value_scale_offset(FMT, NB) + 2 * t * kv_scale_stride(NB);
+            load_scales<NB>(p, sc[0], sc[1]);
+            load_scales<NB>(p + 8 * kv_scale_stride(NB), sc[2], sc[3]);
+            int top[4];
+            uint32_t bad = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t v = 0;
+#pragma unroll
+                for (int w = 0; w < (NB + 3) / 4; ++w) {
+                    const uint32_t nan = __vcmpeq4(sc[i][w], 0xffffffffu);
+                    bad |= nan;
+                    v = __vmaxu4(v, sc[i][w] & ~nan);
+                }
+                if constexpr (NB > 2) v = __vmaxu4(v, v >> 16);
+                if constexpr (NB > 1) v = __vmaxu4(v, v >> 8);
+                top[i] = max((int)(v & 0xffu), 1);
+                te[i] = (float)(top[i] - 127 - kv_rel_shift(FMT));
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    // 2^(s - top + shift) as f16; 0 where the exponent leaves the float's
+                    const int sa = (int)(sc[2 * i][b / 4] >> (8 * (b & 3)) & 0xffu), sb = (int)(sc[2 * i + 1][b / 4] >> (8 * (b & 3)) & 0xffu);
+                    const float fa = __uint_as_float((uint32_t)max(sa - top[2 * i] + 127 + kv_rel_shift(FMT), 0) << 23);
+                    const float fb = __uint_as_float((uint32_t)max(sb - top[2 * i + 1] + 127 + kv_rel_shift(FMT), 0) << 23);
+                    rel[i][b] = f16x2_of(fa, fb);
+                }
+            if (bad != 0) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if ((sc[i][b / 4] >> (8 * (b & 3)) & 0xffu) == 255u) rel[i >> 1][b] |= (i & 1) ? 0x7fff0000u : 0x7fffu;
+            }
+            if (edge) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!(live >> i & 1)) rel[i >> 1][b] &= (i & 1) ? 0x0000ffffu : 0xffff0000u;
+            }
+        }
+        // softmax
+        uint32_t whi[RT][2], wlo[RT][2];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            float top = fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]));
+            if (__any_sync(0xffffffffu, top > m[r] + kKvLag)) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float to = top > m[r] + kKvLag ? ceilf(top) - kKvHead : m[r];
+                const float f = ex2(m[r] - to);
+                m[r] = to;
+                l[r] *= f;
+                if constexpr (!kMx) {
+#pragma unroll
+                    for (int n = 0; n < 4 * NB; ++n) o[r][n][0] *= f, o[r][n][1] *= f, o[r][n][2] *= f, o[r][n][3] *= f;
+                }
+            }
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = ex2(x[r][i] - m[r]);
+            l[r] += (w[0] + w[1]) + (w[2] + w[3]);
+            if constexpr (kMx) {
+                float high = fmaxf(fmaxf(x[r][0] + te[0], x[r][1] + te[1]), fmaxf(x[r][2] + te[2], x[r][3] + te[3]));
+                if (__any_sync(0xffffffffu, high > big[r] + kKvLag)) {
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
+                    const float to = high > big[r] + kKvLag ? ceilf(high) - kKvHead : big[r];
+                    const float f = ex2(big[r] - to);
+                    big[r] = to;
+#pragma unroll
+                    for (int n = 0; n < 4 * NB; ++n) o[r][n][0] *= f, o[r][n][1] *= f, o[r][n][2] *= f, o[r][n][3] *= f;
+                }
+                const float d = m[r] - big[r] + 127.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = fminf(fmaxf(te[i] + d, 0.f), 254.f);   // an integer
+                    w[i] *= __uint_as_float((uint32_t)(int)e << 23);
+                }
+            }
+            split_pair<kBf>(w[0], w[1], whi[r][0], wlo[r][0]);
+            split_pair<kBf>(w[2], w[3], whi[r][1], wlo[r][1]);
+        }
+        // values
+        uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
+        if (!kMx && edge) {   // what lies in the places that do not count may be anything
+            keep0 = (live & 1 ? 0xffffu : 0u) | (live & 2 ? 0xffff0000u : 0u);
+            keep1 = (live & 4 ? 0xffffu : 0u) | (live & 8 ? 0xffff0000u : 0u);
+        }
+        uint32_t v[NB * VP / 4];
+        load_lane<NB * VP>(rec + kv_value_offset(FMT, NB), lane, v);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            uint32_t f[8];
+            if constexpr (!kMx) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    f[2 * e] = v[8 * b + 2 * e], f[2 * e + 1] = v[8 * b + 2 * e + 1];
+                    if (edge) f[2 * e] &= keep0, f[2 * e + 1] &= keep1;
+                }
+            } else {
+                if constexpr (FMT == kKvMx8) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f16_of_e4m3x4(v[4 * b + e], f[2 * e], f[2 * e + 1]);
+                } else {
+                    f16_of_e2m1x8(v[2 * b], f[0], f[1], f[2], f[3]);
+                    f16_of_e2m1x8(v[2 * b + 1], f[4], f[5], f[6], f[7]);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&f[e]), *reinterpret_cast<const __half2*>(&rel[e & 1][b]));
+                    f[e] = *reinterpret_cast<const uint32_t*>(&y);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+                    mma_16x8x16<kBf>(o[r][4 * b + e], whi[r][0], wlo[r][0], whi[r][1], wlo[r][1], f[2 * e], f[2 * e + 1]);
+        }
+    }
+
+    // Partial result of this warp's rows: numerators (times 2^big), denominators (times 2^m).
+    __device__ __forceinline__ void store_partial(float* o_rows, float* stats, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            float s = l[r];
+            s += __shfl_xor_sync(0xffffffffu, s, 1);
+            s += __shfl_xor_sync(0xffffffffu, s, 2);
+            const int row = 8 * r + g;
+            if (t == 0) {
+                stats[3 * row] = m[r];
+                stats[3 * row + 1] = kMx ? big[r] : m[r];
+                stats[3 * row + 2] = s;
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                float4 lo4, hi4;   // elements 32 b + 8 t .. + 3 and .. + 7
+                lo4.x = o[r][4 * b][0] + o[r][4 * b][2], lo4.y = o[r][4 * b + 1][0] + o[r][4 * b + 1][2];
+                lo4.z = o[r][4 * b + 2][0] + o[r][4 * b + 2][2], lo4.w = o[r][4 * b + 3][0] + o[r][4 * b + 3][2];
+                hi4.x = o[r][4 * b][1] + o[r][4 * b][3], hi4.y = o[r][4 * b + 1][1] + o[r][4 * b + 1][3];
+                hi4.z = o[r][4 * b + 2][1] + o[r][4 * b + 2][3], hi4.w = o[r][4 * b + 3][1] + o[r][4 * b + 3][3];
+                float* dst = o_rows + (int64_t)row * D + 32 * b + 8 * t;
+                *reinterpret_cast<float4*>(dst) = lo4;
+                *reinterpret_cast<float4*>(dst + 4) = hi4;
+            }
+        }
+    }
+};
+
+// numerator 2^big * o over denominator 2^m * l; nothing attended to: 0 and -infinity
+__device__ __forceinline__ float kv_quotient(float o, float l, float big, float m) {
+    return l == 0.f ? 0.f : ldexpf(o / l, (int)fminf(fmaxf(big - m, -1000.f), 1000.f));
+}
+__device__ __forceinline__ float kv_lse(float l, float m) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f; }
+
+// positions of sequence b that are attended to: [lo, hi)
+__device__ __forceinline__ void kv_span(const KvPool& pool, const KvSeqs& s, int window, int b, int& lo, int& hi, int* status) {
+    const int n = __ldg(s.lengths + b);
+    const int64_t room = (int64_t)s.max_pages * pool.records_per_page * kKvRecord;
+    hi = (int)min((int64_t)max(n, 0), room);
+    lo = window > 0 ? max(hi - window, 0) : 0;
+    if (n < 0 || n > room) atomicExch(status, kStatusBadSequence);
+}
+
+template <int FMT, int NB, int RT>
+__global__ void __launch_bounds__(256) kv_attend_kernel(KvPool pool, KvSeqs seqs, KvAttend a, int chunks, int* status) {
+    constexpr int D = 32 * NB, kRows = 8 * RT, kWarps = 8;
+    extern __shared__ float4 smem4[];
+    float* so = reinterpret_cast<float*>(smem4);
+    float* ss = so + kWarps * kRows * D;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int chunk = blockIdx.x % chunks, h = blockIdx.x / chunks, b = blockIdx.y;
+    int lo, hi;
+    kv_span(pool, seqs, a.window, b, lo, hi, status);
+    KvWarp<FMT, NB, RT> w;
+    w.reset();
+    w.load_query(a, (int64_t)b * a.seq_stride + (int64_t)h * a.group * a.head_stride, chunk * kRows, a.group, lane);
+    for (int rec = lo / kKvRecord + warp; rec * kKvRecord < hi; rec += kWarps) {
+        const uint8_t* p = kv_record(pool, seqs, b, rec, h);
+        if (p == nullptr) {
+            if (lane == 0) atomicExch(status, kStatusBadPage);
+            continue;
+        }
+        w.record(p, max(lo - rec * kKvRecord, 0), min(hi - rec * kKvRecord, kKvRecord), lane);
+    }
+    w.store_partial(so + warp * kRows * D, ss + warp * kRows * 3, lane);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kRows * D; i += blockDim.x) {
+        const int row = i / D, d = i - row * D, head = chunk * kRows + row;
+        if (head >= a.group) break;
+        float m = kKvMaxInit, big = kKvMaxInit;
+        for (int k = 0; k < kWarps; ++k) {
+            m = fmaxf(m, ss[(k * kRows + row) * 3]);
+            big = fmaxf(big, ss[(k * kRows + row) * 3 + 1]);
+        }
+        float l = 0.f, o = 0.f;
+        for (int k = 0; k < kWarps; ++k) {
+            const float* s = ss + (k * kRows + row) * 3;
+            l += s[2] * ex2(s[0] - m);
+            o += so[(k * kRows + row) * D + d] * ex2(s[1] - big);
+        }
+        const int64_t out_row = (int64_t)b * a.q_heads + (int64_t)h * a.group + head;
+        const float y = kv_quotient(o, l, big, m);
+        if (a.type == kTypeF32) static_cast<float*>(a.out)[out_row * D + d] = y;
+        else if (a.type == kTypeF16) static_cast<__half*>(a.out)[out_row * D + d] = __float2half_rn(y);
+        else static_cast<__nv_bfloat16*>(a.out)[out_row * D + d] = __float2bfloat16_rn(y);
+        if (d == 0 && a.lse != nullptr) a.lse[out_row] = kv_lse(l, m);
+    }
+}
+
+template <int FMT, int NB, int RT>
+struct KvAttendInstance {
+    static constexpr int kSmem = 8 * 8 * RT * (32 * NB + 3) * 4;
+    static cudaError_t init() {
+        return cudaFuncSetAttribute(kv_attend_kernel<FMT, NB, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    }
+    static int launch(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, int* status, cudaStream_t stream) {
+        const int chunks = (a.group + 8 * RT - 1) / (8 * RT);
+        kv_attend_kernel<FMT, NB, RT><<<dim3(chunks * pool.heads, seqs.batch), 256, kSmem, stream>>>(pool, seqs, a, chunks, status);
+        return 1;
+    }
+};
+
+// Two row tiles (16 heads) where a key head serves more than 8 query heads and the accumulators of two tiles fit the
+// registers (head sizes up to 128).
+template <int FMT, int NB>
+int kv_attend_rows(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, int* status, cudaStream_t stream) {
+    if constexpr (NB <= 4)
+        if (a.group > 8) return KvAttendInstance<FMT, NB, 2>::launch(pool, seqs, a, status, stream);
+    return KvAttendInstance<FMT, NB, 1>::launch(pool, seqs, a, status, stream);
+}
+template <int FMT, int NB>
+cudaError_t kv_attend_rows_init() {
+    cudaError_t e = KvAttendInstance<FMT, NB, 1>::init();
+    if constexpr (NB <= 4)
+        if (e == cudaSuccess) e = KvAttendInstance<FMT, NB, 2>::init();
+    return e;
+}
+
+template <int FMT>
+int kv_attend_format(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, int* status, cudaStream_t stream) {
+    switch (pool.blocks) {
+        case 1: return kv_attend_rows<FMT, 1>(pool, seqs, a, status, stream);
+        case 2: return kv_attend_rows<FMT, 2>(pool, seqs, a, status, stream);
+        case 3: return kv_attend_rows<FMT, 3>(pool, seqs, a, status, stream);
+        case 4: return kv_attend_rows<FMT, 4>(pool, seqs, a, status, stream);
+        case 6: return kv_attend_rows<FMT, 6>(pool, seqs, a, status, stream);
+        default: return kv_attend_rows<FMT, 8>(pool, seqs, a, status, stream);
+    }
+}
+template <int FMT>
+cudaError_t kv_attend_format_init(int blocks) {
+    switch (blocks) {
+        case 1: return kv_attend_rows_init<FMT, 1>();
+        case 2: return kv_attend_rows_init<FMT, 2>();
+        case 3: return kv_attend_rows_init<FMT, 3>();
+        case 4: return kv_attend_rows_init<FMT, 4>();
+        case 6: return kv_attend_rows_init<FMT, 6>();
+        default: return kv_attend_rows_init<FMT, 8>();
+    }
+}
+
+int kv_attend_f16(const KvPool&, const KvSeqs&, const KvAttend&, int*, cudaStream_t);
+int kv_attend_bf16(const KvPool&, const KvSeqs&, const KvAttend&, int*, cudaStream_t);
+int kv_attend_mx8(const KvPool&, const KvSeqs&, const KvAttend&, int*, cudaStream_t);
+int kv_attend_mx4(const KvPool&, const KvSeqs&, const KvAttend&, int*, cudaStream_t);
+cudaError_t kv_attend_f16_init(int blocks);
+cudaError_t kv_attend_bf16_init(int blocks);
+cudaError_t kv_attend_mx8_init(int blocks);
+cudaError_t kv_attend_mx4_init(int blocks);
+
+}  // namespace eosb

@@ -1,0 +1,11 @@
+// Attention over a paged cache: the kernels of the mx4 format (kv_attend.cuh).
+#include "kv_attend.cuh"
+
+namespace eosb {
+
+int kv_attend_mx4(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, int* status, cudaStream_t stream) {
+    return kv_attend_format<kKvMx4>(pool, seqs, a, status, stream);
+}
+cudaError_t kv_attend_mx4_init(int blocks) { return kv_attend_format_init<kKvMx4>(blocks); }
+
+}  // namespace eosb

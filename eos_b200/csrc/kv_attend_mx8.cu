@@ -1,0 +1,11 @@
+// Attention over a paged cache: the kernels of the mx8 format (kv_attend.cuh).
+#include "kv_attend.cuh"
+
+namespace eosb {
+
+int kv_attend_mx8(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, int* status, cudaStream_t stream) {
+    return kv_attend_format<kKvMx8>(pool, seqs, a, status, stream);
+}
+cudaError_t kv_attend_mx8_init(int blocks) { return kv_attend_format_init<kKvMx8>(blocks); }
+
+}  // namespace eosb

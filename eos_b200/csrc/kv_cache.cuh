@@ -1,0 +1,95 @@
+// Paged key-value cache: host-side interface of its kernels (kv_cache.cu, kv_attend_*.cu) and the page layout.
+//
+// A page holds page_size tokens of every head; the unit of the layout is the RECORD: the keys and values of 16
+// consecutive tokens of one head, contiguous, 16-byte aligned,
+//     key codes | value codes | key scales | value scales           (scales only in the block-scaled formats)
+// page p, head h, record r of the page sit at ((p * heads + h) * (page_size / 16) + r) * record_bytes.
+//
+// Inside a record the codes are stored in the order in which the 32 lanes of a warp feed them to mma.sync m16n8k16, so
+// that the attention kernel reads them with conflict-free 16-byte loads and no shuffle.  With lane = 4 g + t
+// (g = 0..7, t = 0..3) and blocks b of 32 elements:
+//     keys    two tiles j of 8 tokens; lane (g, t) holds token 8 j + g, elements 32 b + 8 t .. + 7 of every block b
+//             (an mma sums over elements, so any order of them serves as long as the query uses the same one)
+//     values  lane (g, t) holds tokens {2t, 2t+1, 2t+8, 2t+9}, elements 32 b + 4 g + {0..3}, element-major: the two
+//             tokens of one 32-bit operand register are neighbours
+// A lane's bytes are cut into 16-byte pieces (then 8, then 4); piece i of all lanes is one contiguous plane.
+// Scales are one byte per token and block, [16][blocks rounded up to 1, 2, 4 or 8].
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace eosb {
+
+constexpr int kKvF16 = 0, kKvBf16 = 1, kKvMx8 = 2, kKvMx4 = 3;        // EOS_B200_KV_*
+constexpr int kTypeF32 = 0, kTypeF16 = 1, kTypeBf16 = 2;              // EOS_B200_TYPE_*
+constexpr int kKvRecord = 16;                                         // tokens of a record
+
+// bytes of one lane and one 32-element block: keys (one token tile) and values (all 16 tokens)
+__host__ __device__ constexpr int kv_key_piece(int format) { return format <= kKvBf16 ? 16 : format == kKvMx8 ? 8 : 4; }
+__host__ __device__ constexpr int kv_value_piece(int format) { return 2 * kv_key_piece(format); }
+__host__ __device__ constexpr int kv_scale_stride(int blocks) { return blocks <= 2 ? blocks : blocks <= 4 ? 4 : 8; }
+__host__ __device__ constexpr int kv_scale_bytes(int format, int blocks) {
+    return format <= kKvBf16 ? 0 : kKvRecord * kv_scale_stride(blocks);
+}
+__host__ __device__ constexpr int kv_value_offset(int format, int blocks) { return 64 * blocks * kv_key_piece(format); }
+__host__ __device__ constexpr int kv_key_scale_offset(int format, int blocks) {
+    return kv_value_offset(format, blocks) + 32 * blocks * kv_value_piece(format);
+}
+__host__ __device__ constexpr int kv_value_scale_offset(int format, int blocks) {
+    return kv_key_scale_offset(format, blocks) + kv_scale_bytes(format, blocks);
+}
+__host__ __device__ constexpr int kv_record_bytes(int format, int blocks) {
+    return kv_value_scale_offset(format, blocks) + kv_scale_bytes(format, blocks);
+}
+// offset of byte p of a lane's `bytes` bytes (planes of 16, then 8, then 4 bytes per lane)
+__host__ __device__ constexpr int kv_lane_offset(int bytes, int lane, int p) {
+    const int plane = p >> 4, in = p & 15, rest = bytes - (plane << 4);
+    if (rest >= 16) return plane * 512 + lane * 16 + in;
+    if (rest >= 8 && in < 8) return plane * 512 + lane * 8 + in;
+    return plane * 512 + (rest >= 8 ? 256 + lane * 4 + in - 8 : lane * 4 + in);
+}
+
+struct KvPool {
+    uint8_t* base;
+    int64_t pages;
+    int heads, dim, blocks, format;
+    int records_per_page, record_bytes;
+};
+
+// The sequences of a call: row b of table lists the pages of sequence b in order.
+struct KvSeqs {
+    const int32_t* table;   // [batch, max_pages]
+    int max_pages, batch;
+    const int32_t* starts;  // [batch] position of the first token of the call (append / read)
+    const int32_t* cu;      // [batch + 1] first row of each sequence's tokens; null: one token each
+    const int32_t* lengths; // [batch] cached tokens (attend)
+};
+
+struct KvRows {             // keys or values of a call, [tokens, heads, dim] with strides in elements
+    void* p;
+    int64_t token_stride, head_stride;
+    int vec;                // 16-byte accesses are aligned
+};
+
+void launch_kv_append(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type,
+                      int64_t tokens, int* status, cudaStream_t stream);
+void launch_kv_read(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
+                    int* status, cudaStream_t stream);
+
+struct KvAttend {
+    const void* query;      // [batch, q_heads, dim], strides in elements
+    int64_t seq_stride, head_stride;
+    int vec;                // 16-byte loads of the query are aligned
+    int type;               // of query and out
+    int q_heads, group;
+    void* out;              // [batch, q_heads, dim]
+    float* lse;             // [batch, q_heads] or null
+    float scale_log2;       // score scale times log2(e)
+    int window;             // 0: all positions
+};
+
+// cudaSuccess once the kernels of this format and dim are ready on the current device
+cudaError_t kv_attend_init(int format, int blocks);
+int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, int* status, cudaStream_t stream);
+
+}  // namespace eosb

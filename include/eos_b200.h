@@ -549,6 +549,73 @@ EOS_B200_API int eos_b200_token_pool_encode(EosB200TokenPool* tp, const int32_t*
                                             float* h_children, int max_children, int* n_children, EosB200Stats* stats,
                                             char** err);
 
+/* ---- paged key-value cache ------------------------------------------------------------------------
+ * No counterpart in Eos (its attention over compressed keys and values, eos_b200_turbo_sparse_attention above, takes
+ * the whole of them from the host in every call): keys and values of growing sequences stay on the device, in pages of
+ * page_size tokens that the caller hands out through page tables, and are quantised as they are written.
+ * Formats: F16 and BF16 hold the rounded values.  MX8 (e4m3 codes) and MX4 (e2m1 codes) add one scale byte for every 32
+ * consecutive elements of a head's vector: scale 2^e with the smallest e >= -126 for which max|x| <= 448 * 2^e (MX8) or
+ * 6 * 2^e (MX4), codes x / 2^e rounded to nearest even.  A block that holds an infinity or a NaN reads back as NaN.
+ * Rounding to F16 or BF16 overflows to infinity.
+ * head_dim: 32, 64, 96, 128, 192 or 256; page_size: a multiple of 16, at most 65536. */
+#define EOS_B200_TYPE_F32 0
+#define EOS_B200_TYPE_F16 1
+#define EOS_B200_TYPE_BF16 2
+#define EOS_B200_KV_F16 0
+#define EOS_B200_KV_BF16 1
+#define EOS_B200_KV_MX8 2
+#define EOS_B200_KV_MX4 3
+typedef struct EosB200KvCache EosB200KvCache;
+/* Allocates `pages` pages (zeroed) of page_size tokens x kv_heads heads, keys and values. */
+EOS_B200_API int eos_b200_kv_cache_create(EosB200Runtime* rt, int64_t pages, int page_size, int kv_heads, int head_dim, int format,
+                                          EosB200KvCache** out, char** err);
+EOS_B200_API void eos_b200_kv_cache_destroy(EosB200KvCache* cache);
+/* Device bytes of one page: codes and scales of keys and values of all heads. */
+EOS_B200_API int64_t eos_b200_kv_cache_page_bytes(const EosB200KvCache* cache);
+/* Distances between the tokens and heads of a call's tensors, in elements; a head's vector is contiguous. */
+typedef struct {
+    int64_t key_token, key_head, value_token, value_head;
+} EosB200KvStrides;
+/* Writes new tokens.  d_key, d_value: [tokens, kv_heads, head_dim] of `type` (strides NULL: contiguous).  Sequence b owns
+ * rows d_cu_tokens[b] .. d_cu_tokens[b + 1] - 1 and writes them to positions d_starts[b], d_starts[b] + 1, ...;
+ * position p is token p % page_size of page d_page_table[b * max_pages + p / page_size].  d_cu_tokens is [batch + 1],
+ * ascending, its last entry at most `tokens`; NULL: one token per sequence (tokens == batch).  Rows behind the last
+ * sequence are not read.  Nothing else of a page changes.  The positions written by one call must be distinct (no page
+ * twice among the pages written); tokens of other positions may be read by other calls meanwhile.
+ * Enqueued on `stream` (NULL: the runtime's stream) without synchronising, allocation-free, and may be captured into a
+ * graph; all arrays are device memory and are read when the kernel runs.  Sequences whose entries are out of range
+ * (negative, behind the page table, a page id outside the cache) are skipped as far as they are, and
+ * eos_b200_kv_cache_sync reports it. */
+EOS_B200_API int eos_b200_kv_cache_append_device(EosB200KvCache* cache, const void* d_key, const void* d_value, int type,
+                                                 int64_t tokens, const EosB200KvStrides* strides, int batch,
+                                                 const int32_t* d_page_table, int max_pages, const int32_t* d_starts,
+                                                 const int32_t* d_cu_tokens, void* stream, EosB200Stats* stats, char** err);
+/* Reads cached tokens back as the values that their codes stand for, rounded to `type`: the inverse of the call above
+ * with the same arguments.  Rows that belong to no sequence, and rows of sequences that are out of range, are left as
+ * they were. */
+EOS_B200_API int eos_b200_kv_cache_read_device(EosB200KvCache* cache, void* d_key, void* d_value, int type, int64_t tokens,
+                                               const EosB200KvStrides* strides, int batch, const int32_t* d_page_table,
+                                               int max_pages, const int32_t* d_starts, const int32_t* d_cu_tokens, void* stream,
+                                               EosB200Stats* stats, char** err);
+/* Attention of one new token per sequence: query [batch, q_heads, head_dim] of `type`, query head i reads key head
+ * i / (q_heads / kv_heads).  Sequence b attends to positions [max(0, n - window), n), n = d_lengths[b] (window 0: all
+ * of them):  out = sum_j softmax_j(scale q . k_j) v_j in fp32, rounded to `type` into d_out [batch, q_heads, head_dim]
+ * (contiguous); d_lse (nullable) [batch, q_heads] fp32 receives ln sum_j exp(scale q . k_j).  A sequence with n = 0 gives zeros
+ * and -infinity.  query_seq_stride / query_head_stride in elements, 0: contiguous.  The new token's own key and value
+ * are appended before the call when it attends to itself.
+ * Positions on a page that is out of range are left out and eos_b200_kv_cache_sync reports it; a length that is negative
+ * or longer than the page table is cut, and reported too.  Rows that meet an infinity or a NaN are not finite; other rows are not touched by it.
+ * Enqueued, allocation-free and capturable as above; calls of one cache share its workspace and must be ordered (one
+ * stream, or events between streams). */
+EOS_B200_API int eos_b200_kv_cache_attend_device(EosB200KvCache* cache, const void* d_query, int type, int q_heads,
+                                                 int64_t query_seq_stride, int64_t query_head_stride, int batch,
+                                                 const int32_t* d_page_table, int max_pages, const int32_t* d_lengths, float scale,
+                                                 int window, void* d_out, float* d_lse, void* stream, EosB200Stats* stats,
+                                                 char** err);
+/* Waits for `stream` (NULL: the runtime's stream) and returns EOS_B200_DEVICE_STATUS if a kernel of the calls above met
+ * a page, position or length out of range, or gave up on a bounded wait. */
+EOS_B200_API int eos_b200_kv_cache_sync(EosB200KvCache* cache, void* stream, char** err);
+
 /* Seeded synthetic data on the device (bench / tests): n rows of dim N(0,1) values, optionally
  * L2-normalised, row r generated from (seed, row_offset + r) only. */
 EOS_B200_API int eos_b200_synth_gaussian_device(EosB200Runtime* rt, uint64_t seed, int64_t row_offset, int64_t n, int dim,

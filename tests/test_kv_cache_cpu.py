@@ -1,0 +1,101 @@
+"""Paged key-value cache, what needs no device: the record layout is a bijection within its bounds, the work units of an
+append cover every record once, and bad arguments are refused before a device is touched."""
+import ctypes as C
+import os
+import random
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+LAYOUT_CHECK = r"""
+#include <cstdio>
+#include <vector>
+#include "kv_cache.cuh"
+using namespace eosb;
+int main() {
+    const int dims[] = {32, 64, 96, 128, 192, 256};
+    for (int format = 0; format < 4; ++format)
+        for (int dim : dims) {
+            const int nb = dim / 32, kp = kv_key_piece(format), vp = kv_value_piece(format), total = kv_record_bytes(format, nb);
+            if (total % 16 || kv_value_offset(format, nb) % 16 || kv_key_scale_offset(format, nb) % 16 ||
+                kv_value_scale_offset(format, nb) % 16) return 1;
+            std::vector<int> seen(total, 0);
+            auto piece = [&](int base, int bytes, int lane, int p, int size) {   // one access of `size` bytes
+                const int at = base + kv_lane_offset(bytes, lane, p);
+                if (at % (size < 16 ? size : 16) != 0) return false;
+                for (int i = 0; i < size; ++i) {
+                    if (base + kv_lane_offset(bytes, lane, p + i) != at + i || at + i >= total) return false;
+                    seen[at + i]++;
+                }
+                return true;
+            };
+            for (int lane = 0; lane < 32; ++lane)
+                for (int b = 0; b < nb; ++b) {
+                    for (int j = 0; j < 2; ++j)
+                        if (!piece(j * 32 * nb * kp, nb * kp, lane, b * kp, kp)) return 2;
+                    const int step = vp < 16 ? vp : 16;
+                    for (int p = 0; p < vp; p += step)
+                        if (!piece(kv_value_offset(format, nb), nb * vp, lane, b * vp + p, step)) return 3;
+                }
+            for (int i = 0; i < kv_key_scale_offset(format, nb); ++i)
+                if (seen[i] != 1) return 4;
+            if (format >= kKvMx8) {   // scales of 16 tokens behind the codes
+                if (kv_scale_stride(nb) < nb || kv_scale_bytes(format, nb) != 16 * kv_scale_stride(nb)) return 5;
+                if (kv_value_scale_offset(format, nb) + 16 * kv_scale_stride(nb) != total) return 6;
+            } else if (kv_key_scale_offset(format, nb) != total) return 7;
+        }
+    std::puts("ok");
+}
+"""
+
+
+def test_record_layout_is_a_bijection(tmp_path):
+    src = tmp_path / "layout.cpp"
+    src.write_text(LAYOUT_CHECK)
+    exe = tmp_path / "layout"
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    subprocess.check_call(["g++", "-std=c++17", "-I", os.path.join(ROOT, "eos_b200", "csrc"), "-I", os.path.join(cuda, "include"),
+                           str(src), "-o", str(exe)])
+    assert subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout == "ok\n"
+
+
+def test_work_units_cover_every_record_once():
+    """The unit arithmetic of an append / read: sequence b starts at unit cu[b] // 16 + 2 b, unit i of a sequence is its
+    i-th touched record, and tokens // 16 + 2 batch units are enough."""
+    rng = random.Random(5)
+    for _ in range(300):
+        batch = rng.randrange(1, 40)
+        counts = [rng.choice([0, 1, 2, 15, 16, 17, 31, rng.randrange(0, 200)]) for _ in range(batch)]
+        starts = [rng.randrange(0, 100) for _ in range(batch)]
+        cu = [0]
+        for n in counts:
+            cu.append(cu[-1] + n)
+        spare = rng.randrange(0, 20)                      # rows behind the last sequence
+        units = (cu[-1] + spare) // 16 + 2 * batch
+        done = {}
+        for u in range(units):
+            b = max(i for i in range(batch) if i == 0 or cu[i] // 16 + 2 * i <= u)
+            rec = starts[b] // 16 + u - (cu[b] // 16 + 2 * b)
+            if counts[b] and rec >= starts[b] // 16 and rec * 16 < starts[b] + counts[b]:
+                done[b, rec] = done.get((b, rec), 0) + 1
+        want = {(b, r) for b in range(batch) if counts[b]
+                for r in range(starts[b] // 16, (starts[b] + counts[b] - 1) // 16 + 1)}
+        assert set(done) == want and set(done.values()) <= {1}
+
+
+def test_refusals_without_a_device():
+    import eos_b200
+    from eos_b200 import _lib
+    with pytest.raises(ValueError, match="format"):
+        eos_b200.KvCache(None, 1, 16, 1, 64, "fp3")
+    for name, args in (("eos_b200_kv_cache_create", (None, 1, 16, 1, 64, 0, C.byref(C.c_void_p()))),
+                       ("eos_b200_kv_cache_append_device", (None, None, None, 0, 0, None, 0, None, 0, None, None, None, None)),
+                       ("eos_b200_kv_cache_read_device", (None, None, None, 0, 0, None, 0, None, 0, None, None, None, None)),
+                       ("eos_b200_kv_cache_attend_device", (None, None, 0, 1, 0, 0, 0, None, 0, None, 1.0, 0, None, None, None, None)),
+                       ("eos_b200_kv_cache_sync", (None, None))):
+        with pytest.raises(eos_b200.EosB200Error, match="null"):
+            _lib.call(name, *args)
+    assert _lib.lib().eos_b200_kv_cache_page_bytes(None) == 0
+    _lib.lib().eos_b200_kv_cache_destroy(None)
