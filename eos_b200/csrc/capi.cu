@@ -3707,6 +3707,7 @@ int eos_b200_token_pool_encode(EosB200TokenPool* tp, const int32_t* h_tokens, co
 struct EosB200KvCache {
     EosB200Runtime* rt = nullptr;
     KvPool pool{};
+    KvWork work{};
 };
 
 namespace {
@@ -3772,17 +3773,22 @@ int eos_b200_kv_cache_create(EosB200Runtime* rt, int64_t pages, int page_size, i
                              " bytes exceed the device's memory");
     CUDA_TRY(cudaSetDevice(rt->device));
     CUDA_TRY(kv_attend_init(format, p.blocks));
-    CUDA_TRY(dev_alloc(&p.base, (size_t)(pages * page_bytes)));
-    cudaError_t e = cudaMemsetAsync(p.base, 0, (size_t)(pages * page_bytes), rt->stream);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(rt->stream);
-    EosB200KvCache* c = e == cudaSuccess ? new (std::nothrow) EosB200KvCache() : nullptr;
-    if (c == nullptr) {
-        cudaGetLastError();
-        cudaFree(p.base);
-        return fail(err, std::string("kv_cache_create: ") + (e != cudaSuccess ? cudaGetErrorString(e) : "out of host memory"));
-    }
+    EosB200KvCache* c = new (std::nothrow) EosB200KvCache();
+    if (c == nullptr) return fail(err, "kv_cache_create: out of host memory");
     c->rt = rt;
+    c->work.ctas = rt->sm_count;
+    cudaError_t e = dev_alloc(&p.base, (size_t)(pages * page_bytes));
     c->pool = p;
+    if (e == cudaSuccess) e = dev_alloc(&c->work.partial, kv_work_floats(rt->sm_count, head_dim));
+    if (e == cudaSuccess) e = dev_alloc(&c->work.unit, (size_t)2 * rt->sm_count);
+    if (e == cudaSuccess) e = dev_alloc(&c->work.more, (size_t)rt->sm_count);
+    if (e == cudaSuccess) e = cudaMemsetAsync(p.base, 0, (size_t)(pages * page_bytes), rt->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(rt->stream);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        eos_b200_kv_cache_destroy(c);
+        return fail(err, std::string("kv_cache_create: ") + cudaGetErrorString(e));
+    }
     *out = c;
     return EOS_B200_OK;
 }
@@ -3791,6 +3797,9 @@ void eos_b200_kv_cache_destroy(EosB200KvCache* c) {
     if (c == nullptr) return;
     cudaSetDevice(c->rt->device);
     dev_free(c->pool.base);
+    dev_free(c->work.partial);
+    dev_free(c->work.unit);
+    dev_free(c->work.more);
     delete c;
 }
 
@@ -3867,11 +3876,12 @@ int eos_b200_kv_cache_attend_device(EosB200KvCache* c, const void* d_query, int 
     a.q_heads = q_heads;
     a.group = q_heads / c->pool.heads;
     a.out = d_out;
+    a.out_vec = reinterpret_cast<uintptr_t>(d_out) % 16 == 0 ? 1 : 0;
     a.lse = d_lse;
     a.scale_log2 = (float)((double)scale * 1.4426950408889634);
     a.window = window;
     CUDA_TRY(cudaSetDevice(c->rt->device));
-    const int launches = launch_kv_attend(c->pool, seqs, a, c->rt->d_status, pick_stream(c->rt, stream));
+    const int launches = launch_kv_attend(c->pool, seqs, a, c->work, c->rt->d_status, pick_stream(c->rt, stream));
     CUDA_TRY(cudaGetLastError());
     if (stats != nullptr) stats->kernel_launches = launches;
     return EOS_B200_OK;

@@ -348,14 +348,25 @@ struct KvWarp {
         }
     }
 
+    // numerators of row g of tile r, block b: the 8 elements 32 b + 8 t .. + 7
+    __device__ __forceinline__ void numerators(int r, int b, float (&y)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            y[e] = o[r][4 * b + e][0] + o[r][4 * b + e][2];
+            y[4 + e] = o[r][4 * b + e][1] + o[r][4 * b + e][3];
+        }
+    }
+    __device__ __forceinline__ float denominator(int r) const {
+        float s = l[r];
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        return s + __shfl_xor_sync(0xffffffffu, s, 2);
+    }
     // Partial result of this warp's rows: numerators (times 2^big), denominators (times 2^m).
-    __device__ __forceinline__ void store_partial(float* o_rows, float* stats, int lane) {
+    __device__ __forceinline__ void store_partial(float* o_rows, float* stats, int lane) const {
         const int g = lane >> 2, t = lane & 3;
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            float s = l[r];
-            s += __shfl_xor_sync(0xffffffffu, s, 1);
-            s += __shfl_xor_sync(0xffffffffu, s, 2);
+            const float s = denominator(r);
             const int row = 8 * r + g;
             if (t == 0) {
                 stats[3 * row] = m[r];
@@ -364,100 +375,332 @@ struct KvWarp {
             }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                float4 lo4, hi4;   // elements 32 b + 8 t .. + 3 and .. + 7
-                lo4.x = o[r][4 * b][0] + o[r][4 * b][2], lo4.y = o[r][4 * b + 1][0] + o[r][4 * b + 1][2];
-                lo4.z = o[r][4 * b + 2][0] + o[r][4 * b + 2][2], lo4.w = o[r][4 * b + 3][0] + o[r][4 * b + 3][2];
-                hi4.x = o[r][4 * b][1] + o[r][4 * b][3], hi4.y = o[r][4 * b + 1][1] + o[r][4 * b + 1][3];
-                hi4.z = o[r][4 * b + 2][1] + o[r][4 * b + 2][3], hi4.w = o[r][4 * b + 3][1] + o[r][4 * b + 3][3];
-                float* dst = o_rows + (int64_t)row * D + 32 * b + 8 * t;
-                *reinterpret_cast<float4*>(dst) = lo4;
-                *reinterpret_cast<float4*>(dst + 4) = hi4;
+                float y[8];
+                numerators(r, b, y);
+                float* dst = o_rows + row * D + 32 * b + 8 * t;
+                *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<float4*>(dst + 4) = make_float4(y[4], y[5], y[6], y[7]);
             }
         }
     }
 };
 
-// numerator 2^big * o over denominator 2^m * l; nothing attended to: 0 and -infinity
-__device__ __forceinline__ float kv_quotient(float o, float l, float big, float m) {
-    return l == 0.f ? 0.f : ldexpf(o / l, (int)fminf(fmaxf(big - m, -1000.f), 1000.f));
-}
-__device__ __forceinline__ float kv_lse(float l, float m) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f; }
+// The quotient of a numerator 2^big o and a denominator 2^m l.  The power of two is applied in two halves: the scales of
+// the values span fp32's exponents, and their product with 1 / l alone could leave them.  Nothing attended to gives 0.
+struct KvQuotient {
+    float inv, p, q, lse;
+    __device__ __forceinline__ KvQuotient(float l, float big, float m) {
+        const int k = (int)fminf(fmaxf(big - m, -252.f), 252.f), half = k / 2;   // an integer
+        inv = l == 0.f ? 0.f : 1.f / l;
+        p = __uint_as_float((uint32_t)(half + 127) << 23);
+        q = __uint_as_float((uint32_t)(k - half + 127) << 23);
+        lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
+    }
+    __device__ __forceinline__ float operator()(float o) const { return o * inv * p * q; }
+};
+
+// ------------------------------------------------------------------------------------------------
+// Split of the work.  Units are (sequence, key head, chunk of query heads); the records of all units, one unit after
+// the other, are cut into equal ranges, one for each CTA and within it for each warp, wherever the cuts fall: lengths may
+// differ as they like.  A warp writes what it holds of units that lie in its range altogether; at most its first and its
+// last unit are partial.  Partial results are joined in shared memory by the CTA, and what is still partial then (at most
+// two units a CTA) through the workspace by the join kernel.  All joins run in a fixed order: same bits every time.
+// ------------------------------------------------------------------------------------------------
+constexpr int kKvThreads = 256, kKvWarps = 8;
+constexpr int kKvMinRecords = 8;    // records of a CTA, at least
+
+struct KvSplit {
+    int chunks;                     // chunks of query heads per key head
+    int row_warps;                  // warps that share a record, each with its own rows (1, 2, 4, 8)
+    float* partial;                 // [ctas][2][rows][dim + 3]: numerators of all rows, then (m, big, l) of each
+    int64_t* unit;                  // [ctas][2] unit of each partial, -1: none
+    int* more;                      // [ctas] CTAs behind this one that hold parts of its last unit
+};
 
 // positions of sequence b that are attended to: [lo, hi)
-__device__ __forceinline__ void kv_span(const KvPool& pool, const KvSeqs& s, int window, int b, int& lo, int& hi, int* status) {
+__device__ __forceinline__ bool kv_span(const KvPool& pool, const KvSeqs& s, int window, int b, int& lo, int& hi) {
     const int n = __ldg(s.lengths + b);
     const int64_t room = (int64_t)s.max_pages * pool.records_per_page * kKvRecord;
     hi = (int)min((int64_t)max(n, 0), room);
     lo = window > 0 ? max(hi - window, 0) : 0;
-    if (n < 0 || n > room) atomicExch(status, kStatusBadSequence);
+    return n >= 0 && n <= room;
 }
+__device__ __forceinline__ int kv_records(int lo, int hi) { return hi > lo ? (hi + kKvRecord - 1) / kKvRecord - lo / kKvRecord : 0; }
+
 
 template <int FMT, int NB, int RT>
-__global__ void __launch_bounds__(256) kv_attend_kernel(KvPool pool, KvSeqs seqs, KvAttend a, int chunks, int* status) {
-    constexpr int D = 32 * NB, kRows = 8 * RT, kWarps = 8;
+__global__ void __launch_bounds__(kKvThreads) kv_attend_kernel(KvPool pool, KvSeqs seqs, KvAttend a, KvSplit split, int* status) {
+    constexpr int D = 32 * NB, kRows = 8 * RT;
     extern __shared__ float4 smem4[];
-    float* so = reinterpret_cast<float*>(smem4);
-    float* ss = so + kWarps * kRows * D;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int chunk = blockIdx.x % chunks, h = blockIdx.x / chunks, b = blockIdx.y;
-    int lo, hi;
-    kv_span(pool, seqs, a.window, b, lo, hi, status);
-    KvWarp<FMT, NB, RT> w;
-    w.reset();
-    w.load_query(a, (int64_t)b * a.seq_stride + (int64_t)h * a.group * a.head_stride, chunk * kRows, a.group, lane);
-    for (int rec = lo / kKvRecord + warp; rec * kKvRecord < hi; rec += kWarps) {
-        const uint8_t* p = kv_record(pool, seqs, b, rec, h);
-        if (p == nullptr) {
-            if (lane == 0) atomicExch(status, kStatusBadPage);
-            continue;
-        }
-        w.record(p, max(lo - rec * kKvRecord, 0), min(hi - rec * kKvRecord, kKvRecord), lane);
+    float* so = reinterpret_cast<float*>(smem4);              // [2 * warps][kRows][D]
+    float* ss = so + 2 * kKvWarps * kRows * D;                // [2 * warps][kRows][3]
+    __shared__ int64_t s_before[kKvThreads];                  // records of the sequences before thread i's
+    __shared__ int64_t s_warp[kKvWarps];
+    __shared__ int64_t s_unit[2 * kKvWarps];
+    __shared__ int s_ends[2 * kKvWarps];                      // bit 0: the unit begins there, bit 1: it ends there
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t per_seq = (int64_t)pool.heads * split.chunks;   // units of a sequence
+    const int chunk_rows = kRows * split.row_warps;
+
+    // ---- records of all sequences, scanned by the CTA
+    const int per = (seqs.batch + kKvThreads - 1) / kKvThreads;
+    int64_t mine = 0;
+    for (int b = tid * per; b < min((tid + 1) * per, seqs.batch); ++b) {
+        int lo, hi;
+        if (!kv_span(pool, seqs, a.window, b, lo, hi) && blockIdx.x == 0) atomicExch(status, kStatusBadSequence);
+        mine += kv_records(lo, hi);
     }
-    w.store_partial(so + warp * kRows * D, ss + warp * kRows * 3, lane);
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) s_warp[warp] = upto;
+    if (tid < 2 * kKvWarps) s_unit[tid] = -1;
     __syncthreads();
-    for (int i = threadIdx.x; i < kRows * D; i += blockDim.x) {
-        const int row = i / D, d = i - row * D, head = chunk * kRows + row;
-        if (head >= a.group) break;
-        float m = kKvMaxInit, big = kKvMaxInit;
-        for (int k = 0; k < kWarps; ++k) {
-            m = fmaxf(m, ss[(k * kRows + row) * 3]);
-            big = fmaxf(big, ss[(k * kRows + row) * 3 + 1]);
-        }
-        float l = 0.f, o = 0.f;
-        for (int k = 0; k < kWarps; ++k) {
-            const float* s = ss + (k * kRows + row) * 3;
-            l += s[2] * ex2(s[0] - m);
-            o += so[(k * kRows + row) * D + d] * ex2(s[1] - big);
-        }
-        const int64_t out_row = (int64_t)b * a.q_heads + (int64_t)h * a.group + head;
-        const float y = kv_quotient(o, l, big, m);
-        if (a.type == kTypeF32) static_cast<float*>(a.out)[out_row * D + d] = y;
-        else if (a.type == kTypeF16) static_cast<__half*>(a.out)[out_row * D + d] = __float2half_rn(y);
-        else static_cast<__nv_bfloat16*>(a.out)[out_row * D + d] = __float2bfloat16_rn(y);
-        if (d == 0 && a.lse != nullptr) a.lse[out_row] = kv_lse(l, m);
+    int64_t base = 0, total = 0;
+#pragma unroll
+    for (int i = 0; i < kKvWarps; ++i) {
+        if (i < warp) base += s_warp[i];
+        total += s_warp[i];
     }
+    s_before[tid] = base + upto - mine;
+    __syncthreads();
+    total *= per_seq;
+    const int64_t part = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kKvMinRecords);
+    const int64_t c0 = min((int64_t)blockIdx.x * part, total), c1 = min(c0 + part, total);
+    const int teams = kKvWarps / split.row_warps, team = warp / split.row_warps, rw = warp % split.row_warps;
+    const int64_t tpart = (c1 - c0 + teams - 1) / teams;
+    const int64_t t0 = min(c0 + team * tpart, c1), t1 = min(t0 + tpart, c1);
+
+    int64_t left = t1 - t0;
+    if (left > 0) {
+        // the sequence that record t0 belongs to
+        const int64_t q = t0 / per_seq;
+        int i = 31 - __clz(__ballot_sync(0xffffffffu, s_before[lane * (kKvThreads / 32)] <= q)), step = kKvThreads / 32;
+        i = i * step + 31 - __clz(__ballot_sync(0xffffffffu, lane < step && s_before[min(i * step + lane, kKvThreads - 1)] <= q));
+        int b = i * per, lo = 0, hi = 0, n = 0;
+        int64_t first = s_before[i];
+        for (;; ++b) {
+            kv_span(pool, seqs, a.window, b, lo, hi);
+            n = kv_records(lo, hi);
+            if (first + n > q) break;
+            first += n;
+        }
+        int64_t at = t0 - first * per_seq;
+        int hu = (int)(at / n), r = (int)(at - (int64_t)hu * n);
+        KvWarp<FMT, NB, RT> w;
+        while (true) {
+            const int seg = (int)min((int64_t)(n - r), left);
+            const bool begins = r == 0, ends = r + seg == n;
+            const int h = hu / split.chunks, row0 = (hu - h * split.chunks) * chunk_rows + rw * kRows;
+            w.reset();
+            w.load_query(a, (int64_t)b * a.seq_stride + (int64_t)h * a.group * a.head_stride, row0, a.group, lane);
+            const int rec0 = lo / kKvRecord + r;
+            for (int j = 0; j < seg; ++j) {
+                const int rec = rec0 + j;
+                const uint8_t* p = kv_record(pool, seqs, b, rec, h);
+                if (p == nullptr) {
+                    if (lane == 0) atomicExch(status, kStatusBadPage);
+                    continue;
+                }
+                w.record(p, max(lo - rec * kKvRecord, 0), min(hi - rec * kKvRecord, kKvRecord), lane);
+            }
+            if (begins && ends) {
+                const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+                for (int k = 0; k < RT; ++k) {
+                    const float l = w.denominator(k);
+                    const int row = row0 + 8 * k + g;
+                    if (row >= a.group) continue;
+                    const int64_t out_row = (int64_t)b * a.q_heads + (int64_t)h * a.group + row;
+                    const float big = FMT >= kKvMx8 ? w.big[k] : w.m[k];
+                    const KvQuotient f(l, big, w.m[k]);
+                    if (t == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
+#pragma unroll
+                    for (int blk = 0; blk < NB; ++blk) {
+                        float y[8];
+                        w.numerators(k, blk, y);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = f(y[e]);
+                        store_row<8>(a.out, out_row * D + 32 * blk + 8 * t, a.type, a.out_vec, y);
+                    }
+                }
+            } else {
+                const int slot = 2 * warp + (begins ? 1 : 0);
+                w.store_partial(so + slot * kRows * D, ss + slot * kRows * 3, lane);
+                if (lane == 0) {
+                    s_unit[slot] = (int64_t)b * per_seq + hu;
+                    s_ends[slot] = (begins ? 1 : 0) | (ends ? 2 : 0);
+                }
+            }
+            left -= seg;
+            if (left <= 0) break;
+            r = 0;
+            if (++hu == per_seq) {
+                hu = 0;
+                do {
+                    kv_span(pool, seqs, a.window, ++b, lo, hi);
+                    n = kv_records(lo, hi);
+                } while (n == 0);
+            }
+        }
+    }
+    __syncthreads();
+
+    // ---- join of the CTA's partial results: runs of equal units, in order
+    if (tid < 2) split.unit[2 * (int64_t)blockIdx.x + tid] = -1;
+    __syncthreads();
+    const int slots = 2 * teams;
+    auto slot_of = [&](int e, int k) { return 2 * ((e >> 1) * split.row_warps + k) + (e & 1); };   // entry e, row warp k
+    for (int e = 0; e < slots; ++e) {
+        const int64_t u = s_unit[slot_of(e, 0)];
+        if (u < 0) continue;
+        int e1 = e + 1, ends = s_ends[slot_of(e, 0)];
+        for (; e1 < slots; ++e1) {
+            const int64_t v = s_unit[slot_of(e1, 0)];
+            if (v >= 0 && v != u) break;
+            if (v == u) ends |= s_ends[slot_of(e1, 0)];
+        }
+        const int64_t b = u / per_seq;
+        const int hu = (int)(u - b * per_seq), h = hu / split.chunks, row0 = (hu - h * split.chunks) * chunk_rows;
+        const int which = ends & 1;
+        float* po = split.partial + (2 * (int64_t)blockIdx.x + which) * chunk_rows * (D + 3);
+        float* ps = po + chunk_rows * D;
+        for (int i = tid; i < chunk_rows * (D / 4); i += kKvThreads) {
+            const int row = i / (D / 4), d = 4 * (i - row * (D / 4)), k = row / kRows, in = row - k * kRows;
+            float m = kKvMaxInit, big = kKvMaxInit;
+            for (int f = e; f < e1; ++f) {
+                const int sl = slot_of(f, k);
+                if (s_unit[sl] < 0) continue;
+                m = fmaxf(m, ss[(sl * kRows + in) * 3]);
+                big = fmaxf(big, ss[(sl * kRows + in) * 3 + 1]);
+            }
+            float l = 0.f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int f = e; f < e1; ++f) {
+                const int sl = slot_of(f, k);
+                if (s_unit[sl] < 0) continue;
+                const float* s = ss + (sl * kRows + in) * 3;
+                l += s[2] * ex2(s[0] - m);
+                const float c = ex2(s[1] - big);
+                const float4 y = *reinterpret_cast<const float4*>(so + (sl * kRows + in) * D + d);
+                o.x = fmaf(y.x, c, o.x), o.y = fmaf(y.y, c, o.y), o.z = fmaf(y.z, c, o.z), o.w = fmaf(y.w, c, o.w);
+            }
+            if (ends == 3) {
+                if (row0 + row < a.group) {
+                    const int64_t out_row = b * a.q_heads + (int64_t)h * a.group + row0 + row;
+                    const KvQuotient f(l, big, m);
+                    const float y[4] = {f(o.x), f(o.y), f(o.z), f(o.w)};
+                    store_row<4>(a.out, out_row * D + d, a.type, a.out_vec, y);
+                    if (d == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
+                }
+            } else {
+                *reinterpret_cast<float4*>(po + row * D + d) = o;
+                if (d == 0) ps[3 * row] = m, ps[3 * row + 1] = big, ps[3 * row + 2] = l;
+            }
+        }
+        if (ends != 3 && tid == 0) {
+            split.unit[2 * (int64_t)blockIdx.x + which] = u;
+            if (which == 1) {
+                // CTA of the unit's last record
+                int lo, hi;
+                kv_span(pool, seqs, a.window, (int)b, lo, hi);
+                const int n = kv_records(lo, hi);
+                int64_t first = s_before[b / per];
+                for (int64_t i = b / per * per; i < b; ++i) {
+                    int l2, h2;
+                    kv_span(pool, seqs, a.window, (int)i, l2, h2);
+                    first += kv_records(l2, h2);
+                }
+                split.more[blockIdx.x] = (int)((first * per_seq + (int64_t)(hu + 1) * n - 1) / part) - (int)blockIdx.x;
+            }
+        }
+        e = e1 - 1;
+    }
+
+    // ---- sequences with nothing to attend to
+    for (int64_t b = blockIdx.x; b < seqs.batch; b += gridDim.x) {
+        int lo, hi;
+        kv_span(pool, seqs, a.window, (int)b, lo, hi);
+        if (hi > lo) continue;
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int i = tid; i < a.q_heads * (D / 4); i += kKvThreads)
+            store_row<4>(a.out, b * a.q_heads * D + 4 * i, a.type, a.out_vec, zero);
+        if (a.lse != nullptr)
+            for (int i = tid; i < a.q_heads; i += kKvThreads) a.lse[b * a.q_heads + i] = -INFINITY;
+    }
+}
+
+// Units that several CTAs hold parts of: block (c, y) joins rows of the unit that begins in CTA c and goes on behind it.
+template <int NB>
+__global__ void __launch_bounds__(kKvThreads) kv_join_kernel(KvPool pool, KvAttend a, KvSplit split, int chunk_rows) {
+    constexpr int D = 32 * NB, kD4 = D / 4;
+    const int c = blockIdx.x;
+    const int64_t u = split.unit[2 * (int64_t)c + 1];
+    if (u < 0) return;
+    const int more = split.more[c];
+    const int64_t per_seq = (int64_t)pool.heads * split.chunks, b = u / per_seq;
+    const int hu = (int)(u - b * per_seq), h = hu / split.chunks, row0 = (hu - h * split.chunks) * chunk_rows;
+    const int i = blockIdx.y * kKvThreads + threadIdx.x, row = i / kD4, d = 4 * (i - row * kD4);
+    if (row >= chunk_rows || row0 + row >= a.group) return;
+    const int64_t stride = (int64_t)chunk_rows * (D + 3);
+    auto part = [&](int k) { return split.partial + (2 * (int64_t)(c + k) + (k == 0 ? 1 : 0)) * stride; };
+    float m = kKvMaxInit, big = kKvMaxInit;
+#pragma unroll 4
+    for (int k = 0; k <= more; ++k) {
+        const float* s = part(k) + chunk_rows * D + 3 * row;
+        m = fmaxf(m, s[0]);
+        big = fmaxf(big, s[1]);
+    }
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k <= more; ++k) {
+        const float* s = part(k) + chunk_rows * D + 3 * row;
+        const float4 y = *reinterpret_cast<const float4*>(part(k) + row * D + d);
+        l += s[2] * ex2(s[0] - m);
+        const float f = ex2(s[1] - big);
+        o.x = fmaf(y.x, f, o.x), o.y = fmaf(y.y, f, o.y), o.z = fmaf(y.z, f, o.z), o.w = fmaf(y.w, f, o.w);
+    }
+    const int64_t out_row = b * a.q_heads + (int64_t)h * a.group + row0 + row;
+    const KvQuotient f(l, big, m);
+    const float y[4] = {f(o.x), f(o.y), f(o.z), f(o.w)};
+    store_row<4>(a.out, out_row * D + d, a.type, a.out_vec, y);
+    if (d == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
 }
 
 template <int FMT, int NB, int RT>
 struct KvAttendInstance {
-    static constexpr int kSmem = 8 * 8 * RT * (32 * NB + 3) * 4;
+    static constexpr int kSmem = 2 * kKvWarps * 8 * RT * (32 * NB + 3) * 4;
     static cudaError_t init() {
         return cudaFuncSetAttribute(kv_attend_kernel<FMT, NB, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     }
-    static int launch(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, int* status, cudaStream_t stream) {
-        const int chunks = (a.group + 8 * RT - 1) / (8 * RT);
-        kv_attend_kernel<FMT, NB, RT><<<dim3(chunks * pool.heads, seqs.batch), 256, kSmem, stream>>>(pool, seqs, a, chunks, status);
-        return 1;
+    static int launch(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
+                      cudaStream_t stream) {
+        KvSplit split{};
+        split.row_warps = 1;
+        while (split.row_warps < kKvWarps && split.row_warps * 8 * RT < a.group) split.row_warps *= 2;
+        const int chunk_rows = split.row_warps * 8 * RT;
+        split.chunks = (a.group + chunk_rows - 1) / chunk_rows;
+        split.unit = work.unit;
+        split.more = work.more;
+        split.partial = work.partial;
+        kv_attend_kernel<FMT, NB, RT><<<work.ctas, kKvThreads, kSmem, stream>>>(pool, seqs, a, split, status);
+        kv_join_kernel<NB><<<dim3(work.ctas, (chunk_rows * 8 * NB + kKvThreads - 1) / kKvThreads), kKvThreads, 0, stream>>>(
+            pool, a, split, chunk_rows);
+        return 2;
     }
 };
 
-// Two row tiles (16 heads) where a key head serves more than 8 query heads and the accumulators of two tiles fit the
-// registers (head sizes up to 128).
+// Two row tiles (16 heads) a warp where a key head serves more than 8 query heads and the accumulators of two tiles fit
+// the registers (head sizes up to 128).
 template <int FMT, int NB>
-int kv_attend_rows(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, int* status, cudaStream_t stream) {
+int kv_attend_rows(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status, cudaStream_t stream) {
     if constexpr (NB <= 4)
-        if (a.group > 8) return KvAttendInstance<FMT, NB, 2>::launch(pool, seqs, a, status, stream);
-    return KvAttendInstance<FMT, NB, 1>::launch(pool, seqs, a, status, stream);
+        if (a.group > 8) return KvAttendInstance<FMT, NB, 2>::launch(pool, seqs, a, work, status, stream);
+    return KvAttendInstance<FMT, NB, 1>::launch(pool, seqs, a, work, status, stream);
 }
 template <int FMT, int NB>
 cudaError_t kv_attend_rows_init() {
@@ -468,14 +711,14 @@ cudaError_t kv_attend_rows_init() {
 }
 
 template <int FMT>
-int kv_attend_format(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, int* status, cudaStream_t stream) {
+int kv_attend_format(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status, cudaStream_t stream) {
     switch (pool.blocks) {
-        case 1: return kv_attend_rows<FMT, 1>(pool, seqs, a, status, stream);
-        case 2: return kv_attend_rows<FMT, 2>(pool, seqs, a, status, stream);
-        case 3: return kv_attend_rows<FMT, 3>(pool, seqs, a, status, stream);
-        case 4: return kv_attend_rows<FMT, 4>(pool, seqs, a, status, stream);
-        case 6: return kv_attend_rows<FMT, 6>(pool, seqs, a, status, stream);
-        default: return kv_attend_rows<FMT, 8>(pool, seqs, a, status, stream);
+        case 1: return kv_attend_rows<FMT, 1>(pool, seqs, a, work, status, stream);
+        case 2: return kv_attend_rows<FMT, 2>(pool, seqs, a, work, status, stream);
+        case 3: return kv_attend_rows<FMT, 3>(pool, seqs, a, work, status, stream);
+        case 4: return kv_attend_rows<FMT, 4>(pool, seqs, a, work, status, stream);
+        case 6: return kv_attend_rows<FMT, 6>(pool, seqs, a, work, status, stream);
+        default: return kv_attend_rows<FMT, 8>(pool, seqs, a, work, status, stream);
     }
 }
 template <int FMT>
@@ -490,10 +733,10 @@ cudaError_t kv_attend_format_init(int blocks) {
     }
 }
 
-int kv_attend_f16(const KvPool&, const KvSeqs&, const KvAttend&, int*, cudaStream_t);
-int kv_attend_bf16(const KvPool&, const KvSeqs&, const KvAttend&, int*, cudaStream_t);
-int kv_attend_mx8(const KvPool&, const KvSeqs&, const KvAttend&, int*, cudaStream_t);
-int kv_attend_mx4(const KvPool&, const KvSeqs&, const KvAttend&, int*, cudaStream_t);
+int kv_attend_f16(const KvPool&, const KvSeqs&, const KvAttend&, const KvWork&, int*, cudaStream_t);
+int kv_attend_bf16(const KvPool&, const KvSeqs&, const KvAttend&, const KvWork&, int*, cudaStream_t);
+int kv_attend_mx8(const KvPool&, const KvSeqs&, const KvAttend&, const KvWork&, int*, cudaStream_t);
+int kv_attend_mx4(const KvPool&, const KvSeqs&, const KvAttend&, const KvWork&, int*, cudaStream_t);
 cudaError_t kv_attend_f16_init(int blocks);
 cudaError_t kv_attend_bf16_init(int blocks);
 cudaError_t kv_attend_mx8_init(int blocks);

@@ -3,8 +3,9 @@
 
 namespace eosb {
 
-int kv_attend_bf16(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, int* status, cudaStream_t stream) {
-    return kv_attend_format<kKvBf16>(pool, seqs, a, status, stream);
+int kv_attend_bf16(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
+                 cudaStream_t stream) {
+    return kv_attend_format<kKvBf16>(pool, seqs, a, work, status, stream);
 }
 cudaError_t kv_attend_bf16_init(int blocks) { return kv_attend_format_init<kKvBf16>(blocks); }
 

@@ -3,8 +3,9 @@
 
 namespace eosb {
 
-int kv_attend_mx8(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, int* status, cudaStream_t stream) {
-    return kv_attend_format<kKvMx8>(pool, seqs, a, status, stream);
+int kv_attend_mx8(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
+                 cudaStream_t stream) {
+    return kv_attend_format<kKvMx8>(pool, seqs, a, work, status, stream);
 }
 cudaError_t kv_attend_mx8_init(int blocks) { return kv_attend_format_init<kKvMx8>(blocks); }
 

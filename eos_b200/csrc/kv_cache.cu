@@ -365,12 +365,13 @@ void launch_kv_read(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, c
     }
 }
 
-int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, int* status, cudaStream_t stream) {
+int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
+                     cudaStream_t stream) {
     switch (pool.format) {
-        case kKvF16: return kv_attend_f16(pool, seqs, a, status, stream);
-        case kKvBf16: return kv_attend_bf16(pool, seqs, a, status, stream);
-        case kKvMx8: return kv_attend_mx8(pool, seqs, a, status, stream);
-        default: return kv_attend_mx4(pool, seqs, a, status, stream);
+        case kKvF16: return kv_attend_f16(pool, seqs, a, work, status, stream);
+        case kKvBf16: return kv_attend_bf16(pool, seqs, a, work, status, stream);
+        case kKvMx8: return kv_attend_mx8(pool, seqs, a, work, status, stream);
+        default: return kv_attend_mx4(pool, seqs, a, work, status, stream);
     }
 }
 

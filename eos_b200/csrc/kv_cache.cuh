@@ -83,13 +83,25 @@ struct KvAttend {
     int type;               // of query and out
     int q_heads, group;
     void* out;              // [batch, q_heads, dim]
+    int out_vec;            // 16-byte stores of out are aligned
     float* lse;             // [batch, q_heads] or null
     float scale_log2;       // score scale times log2(e)
     int window;             // 0: all positions
 };
 
+// Workspace of a cache's attention calls, of a fixed size: captured graphs keep its addresses.
+struct KvWork {
+    int ctas;               // one per SM
+    float* partial;         // kv_work_floats(ctas, dim)
+    int64_t* unit;          // [ctas][2]
+    int* more;              // [ctas]
+};
+constexpr int kKvMaxRows = 128;   // query heads of one unit, at most
+inline size_t kv_work_floats(int ctas, int dim) { return (size_t)ctas * 2 * kKvMaxRows * (dim + 3); }
+
 // cudaSuccess once the kernels of this format and dim are ready on the current device
 cudaError_t kv_attend_init(int format, int blocks);
-int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, int* status, cudaStream_t stream);
+int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
+                     cudaStream_t stream);
 
 }  // namespace eosb
