@@ -406,8 +406,26 @@ struct KvQuotient {
 // last unit are partial.  Partial results are joined in shared memory by the CTA, and what is still partial then (at most
 // two units a CTA) through the workspace by the join kernel.  All joins run in a fixed order: same bits every time.
 // ------------------------------------------------------------------------------------------------
-constexpr int kKvThreads = 256, kKvWarps = 8;
+constexpr int kKvJoinThreads = 256;
 constexpr int kKvMinRecords = 8;    // records of a CTA, at least
+
+// Shape of a CTA.  Each warp (or team of warps that share records) has a ring of records in shared memory, filled by
+// bulk copies: one copy a record, since a record is contiguous.  Beside the rings every warp has room for the partial
+// result of its first unit; that of its last one goes into its ring, which is empty by then.
+template <int FMT, int NB, int RT>
+struct KvShape {
+    static constexpr int kWarps = FMT <= kKvBf16 && NB > 4 ? 4 : 8;
+    static constexpr int kThreads = 32 * kWarps;
+    static constexpr int kRows = 8 * RT;
+    static constexpr int kPartial = kRows * (32 * NB + 3) * 4 + (kRows * 3 * 4 % 16 ? 16 - kRows * 3 * 4 % 16 : 0);
+    static constexpr int kRecord = kv_record_bytes(FMT, NB);
+    static constexpr int kSmemMax = 232448 - 5120;               // of a CTA, less the static part
+    static constexpr int kRoom = (kSmemMax / kWarps - kPartial) / kRecord;
+    static constexpr int kStages = kRoom > 8 ? 8 : kRoom;        // of one warp's ring
+    static constexpr int kRing = kStages * kRecord;
+    static constexpr int kSmem = kWarps * (kRing + kPartial);
+    static_assert(kStages >= 2 && kRing >= kPartial && kPartial % 16 == 0 && kRing % 16 == 0, "ring");
+};
 
 struct KvSplit {
     int chunks;                     // chunks of query heads per key head
@@ -428,22 +446,70 @@ __device__ __forceinline__ bool kv_span(const KvPool& pool, const KvSeqs& s, int
 __device__ __forceinline__ int kv_records(int lo, int hi) { return hi > lo ? (hi + kKvRecord - 1) / kKvRecord - lo / kKvRecord : 0; }
 
 
+// A walk over the records of a range, in order: the unit (b, hu) and the record r of its n.
+struct KvWalk {
+    int b, hu, r, n, lo, hi;
+
+    // to the record `at` of all records; i0 / first: a sequence at or before its own, and the records before that
+    __device__ __forceinline__ void seek(const KvPool& pool, const KvSeqs& s, int window, int64_t per_seq, int64_t at, int i0,
+                                         int64_t first) {
+        const int64_t q = at / per_seq;
+        for (b = i0;; ++b) {
+            kv_span(pool, s, window, b, lo, hi);
+            n = kv_records(lo, hi);
+            if (first + n > q) break;
+            first += n;
+        }
+        at -= first * per_seq;
+        hu = (int)(at / n);
+        r = (int)(at - (int64_t)hu * n);
+    }
+    // to the first record of the next unit (there is one)
+    __device__ __forceinline__ void next_unit(const KvPool& pool, const KvSeqs& s, int window, int per_seq) {
+        r = 0;
+        if (++hu < per_seq) return;
+        hu = 0;
+        do {
+            kv_span(pool, s, window, ++b, lo, hi);
+            n = kv_records(lo, hi);
+        } while (n == 0);
+    }
+};
+
+// One bulk copy of a record into shared memory, its bytes counted on the mbarrier.
+__device__ __forceinline__ void kv_copy_record(uint32_t dst, const uint8_t* src, uint32_t bytes, uint32_t bar) {
+    mbar_arrive_expect_tx(bar, bytes);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
 template <int FMT, int NB, int RT>
-__global__ void __launch_bounds__(kKvThreads) kv_attend_kernel(KvPool pool, KvSeqs seqs, KvAttend a, KvSplit split, int* status) {
-    constexpr int D = 32 * NB, kRows = 8 * RT;
-    extern __shared__ float4 smem4[];
-    float* so = reinterpret_cast<float*>(smem4);              // [2 * warps][kRows][D]
-    float* ss = so + 2 * kKvWarps * kRows * D;                // [2 * warps][kRows][3]
-    __shared__ int64_t s_before[kKvThreads];                  // records of the sequences before thread i's
-    __shared__ int64_t s_warp[kKvWarps];
-    __shared__ int64_t s_unit[2 * kKvWarps];
-    __shared__ int s_ends[2 * kKvWarps];                      // bit 0: the unit begins there, bit 1: it ends there
+__global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
+    kv_attend_kernel(KvPool pool, KvSeqs seqs, KvAttend a, KvSplit split, int* status) {
+    using Shape = KvShape<FMT, NB, RT>;
+    constexpr int D = 32 * NB, kRows = Shape::kRows, kWarps = Shape::kWarps, kThreads = Shape::kThreads;
+    constexpr int kMaxStages = 16;
+    extern __shared__ __align__(128) uint8_t smem[];          // rings, then the warps' partial results
+    __shared__ int64_t s_before[kThreads];                    // records of the sequences before thread i's
+    __shared__ int64_t s_warp[kWarps];
+    __shared__ int64_t s_unit[2 * kWarps];
+    __shared__ int s_ends[2 * kWarps];                        // bit 0: the unit begins there, bit 1: it ends there
+    __shared__ __align__(8) uint64_t s_full[kWarps][kMaxStages], s_empty[kWarps][kMaxStages];
+    __shared__ uint8_t s_ok[kWarps][kMaxStages];              // whether the record could be fetched
+    __shared__ int s_abort, s_drain[kWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t per_seq = (int64_t)pool.heads * split.chunks;   // units of a sequence
+    const int per_seq = pool.heads * split.chunks;            // units of a sequence
     const int chunk_rows = kRows * split.row_warps;
+    const int teams = kWarps / split.row_warps, team = warp / split.row_warps, rw = warp % split.row_warps;
+    const int stages = min(kMaxStages, Shape::kStages * split.row_warps);   // of the team's ring
+    // partial results: slot 0 (a unit that began before the warp's range), slot 1 (one that goes on behind it)
+    auto slot_rows = [&](int w, int which) {
+        return reinterpret_cast<float*>(which ? smem + w * Shape::kRing : smem + kWarps * Shape::kRing + w * Shape::kPartial);
+    };
 
     // ---- records of all sequences, scanned by the CTA
-    const int per = (seqs.batch + kKvThreads - 1) / kKvThreads;
+    const int per = (seqs.batch + kThreads - 1) / kThreads;
     int64_t mine = 0;
     for (int b = tid * per; b < min((tid + 1) * per, seqs.batch); ++b) {
         int lo, hi;
@@ -457,11 +523,17 @@ __global__ void __launch_bounds__(kKvThreads) kv_attend_kernel(KvPool pool, KvSe
         if (lane >= o) upto += v;
     }
     if (lane == 31) s_warp[warp] = upto;
-    if (tid < 2 * kKvWarps) s_unit[tid] = -1;
+    if (tid < 2 * kWarps) s_unit[tid] = -1;
+    if (tid == 0) s_abort = 0;
+    if (rw == 0 && lane < stages) {
+        mbar_init(smem_u32(&s_full[team][lane]), 1);
+        mbar_init(smem_u32(&s_empty[team][lane]), split.row_warps);
+    }
+    mbar_fence_init();
     __syncthreads();
     int64_t base = 0, total = 0;
 #pragma unroll
-    for (int i = 0; i < kKvWarps; ++i) {
+    for (int i = 0; i < kWarps; ++i) {
         if (i < warp) base += s_warp[i];
         total += s_warp[i];
     }
@@ -470,42 +542,90 @@ __global__ void __launch_bounds__(kKvThreads) kv_attend_kernel(KvPool pool, KvSe
     total *= per_seq;
     const int64_t part = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kKvMinRecords);
     const int64_t c0 = min((int64_t)blockIdx.x * part, total), c1 = min(c0 + part, total);
-    const int teams = kKvWarps / split.row_warps, team = warp / split.row_warps, rw = warp % split.row_warps;
     const int64_t tpart = (c1 - c0 + teams - 1) / teams;
     const int64_t t0 = min(c0 + team * tpart, c1), t1 = min(t0 + tpart, c1);
 
-    int64_t left = t1 - t0;
-    if (left > 0) {
-        // the sequence that record t0 belongs to
-        const int64_t q = t0 / per_seq;
-        int i = 31 - __clz(__ballot_sync(0xffffffffu, s_before[lane * (kKvThreads / 32)] <= q)), step = kKvThreads / 32;
-        i = i * step + 31 - __clz(__ballot_sync(0xffffffffu, lane < step && s_before[min(i * step + lane, kKvThreads - 1)] <= q));
-        int b = i * per, lo = 0, hi = 0, n = 0;
-        int64_t first = s_before[i];
-        for (;; ++b) {
-            kv_span(pool, seqs, a.window, b, lo, hi);
-            n = kv_records(lo, hi);
-            if (first + n > q) break;
-            first += n;
+    if (t1 > t0) {
+        KvWalk at;
+        {
+            const int64_t q = t0 / per_seq;
+            constexpr int kStep = kThreads / 32;
+            int i = 31 - __clz(__ballot_sync(0xffffffffu, s_before[lane * kStep] <= q));
+            i = i * kStep + 31 - __clz(__ballot_sync(0xffffffffu, lane < kStep && s_before[min(i * kStep + lane, kThreads - 1)] <= q));
+            at.seek(pool, seqs, a.window, per_seq, t0, i * per, s_before[i]);
         }
-        int64_t at = t0 - first * per_seq;
-        int hu = (int)(at / n), r = (int)(at - (int64_t)hu * n);
+        // ---- the copies: the walk of the records to fetch runs `stages` ahead of the one below
+        KvWalk ahead = at;
+        int64_t to_fetch = t1 - t0;
+        const int rpp = pool.records_per_page;
+        int slot = 0, in = 0, page = -1, next_page = -1;   // page slot of the record to fetch, record in the page, page ids
+        auto page_at = [&](int s) { return s < seqs.max_pages ? __ldg(seqs.table + (int64_t)ahead.b * seqs.max_pages + s) : -1; };
+        auto enter_unit = [&]() {
+            const int rec = ahead.lo / kKvRecord + ahead.r;
+            slot = rec / rpp;
+            in = rec - slot * rpp;
+            page = page_at(slot);
+            next_page = page_at(slot + 1);
+        };
+        auto fetch = [&](int stage) {   // the next record, if there is one, into `stage`
+            if (to_fetch == 0) return;
+            const bool ok = page >= 0 && page < pool.pages;
+            if (lane == 0) {
+                const uint32_t bar = smem_u32(&s_full[team][stage]);
+                s_ok[team][stage] = ok;
+                if (ok) {
+                    const int64_t rec = ((int64_t)page * pool.heads + ahead.hu / split.chunks) * rpp + in;
+                    kv_copy_record(smem_u32(smem + team * split.row_warps * Shape::kRing + stage * Shape::kRecord),
+                                   pool.base + rec * Shape::kRecord, Shape::kRecord, bar);
+                } else {
+                    atomicExch(status, kStatusBadPage);
+                    mbar_arrive(bar);
+                }
+            }
+            if (--to_fetch == 0) return;
+            if (++ahead.r == ahead.n) {
+                ahead.next_unit(pool, seqs, a.window, per_seq);
+                enter_unit();
+            } else if (++in == rpp) {
+                in = 0;
+                ++slot;
+                page = next_page;
+                next_page = page_at(slot + 1);
+            }
+        };
+        if (rw == 0) {
+            enter_unit();
+            for (int i = 0; i < stages; ++i) fetch(i);
+        }
+        int stage = 0;
+        uint32_t phase = 0;
+        bool alive = true;          // no wait has run out
+        int dead_stage = -1;         // the last stage that a wait was good for, and its phase
+        uint32_t dead_phase = 0;
+        int64_t left = t1 - t0;
+        const uint8_t* ring = smem + team * split.row_warps * Shape::kRing;
         KvWarp<FMT, NB, RT> w;
         while (true) {
-            const int seg = (int)min((int64_t)(n - r), left);
-            const bool begins = r == 0, ends = r + seg == n;
-            const int h = hu / split.chunks, row0 = (hu - h * split.chunks) * chunk_rows + rw * kRows;
+            const int b = at.b, seg = (int)min((int64_t)(at.n - at.r), left);
+            const bool begins = at.r == 0, ends = at.r + seg == at.n;
+            const int h = at.hu / split.chunks, row0 = (at.hu - h * split.chunks) * chunk_rows + rw * kRows;
             w.reset();
             w.load_query(a, (int64_t)b * a.seq_stride + (int64_t)h * a.group * a.head_stride, row0, a.group, lane);
-            const int rec0 = lo / kKvRecord + r;
-            for (int j = 0; j < seg; ++j) {
-                const int rec = rec0 + j;
-                const uint8_t* p = kv_record(pool, seqs, b, rec, h);
-                if (p == nullptr) {
-                    if (lane == 0) atomicExch(status, kStatusBadPage);
-                    continue;
+            int first = (at.lo / kKvRecord + at.r) * kKvRecord;   // position of the record's first token
+            for (int j = 0; j < seg; ++j, first += kKvRecord) {
+                alive = alive && mbar_wait(smem_u32(&s_full[team][stage]), phase, &s_abort);
+                if (alive && s_ok[team][stage])
+                    w.record(ring + stage * Shape::kRecord, max(at.lo - first, 0), min(at.hi - first, kKvRecord), lane);
+                __syncwarp();
+                if (split.row_warps > 1) {
+                    if (lane == 0) mbar_arrive(smem_u32(&s_empty[team][stage]));
+                    if (rw == 0 && to_fetch > 0) alive = alive && mbar_wait(smem_u32(&s_empty[team][stage]), phase, &s_abort);
                 }
-                w.record(p, max(lo - rec * kKvRecord, 0), min(hi - rec * kKvRecord, kKvRecord), lane);
+                if (alive) {
+                    if (rw == 0) fetch(stage);
+                    dead_stage = stage, dead_phase = phase;
+                }
+                if (++stage == stages) stage = 0, phase ^= 1;
             }
             if (begins && ends) {
                 const int g = lane >> 2, t = lane & 3;
@@ -528,22 +648,25 @@ __global__ void __launch_bounds__(kKvThreads) kv_attend_kernel(KvPool pool, KvSe
                     }
                 }
             } else {
-                const int slot = 2 * warp + (begins ? 1 : 0);
-                w.store_partial(so + slot * kRows * D, ss + slot * kRows * 3, lane);
+                const int which = begins ? 1 : 0;
+                if (begins && split.row_warps > 1) named_bar_sync(1 + team, 32 * split.row_warps);   // the ring is free
+                float* rows = slot_rows(warp, which);
+                w.store_partial(rows, rows + kRows * D, lane);
                 if (lane == 0) {
-                    s_unit[slot] = (int64_t)b * per_seq + hu;
-                    s_ends[slot] = (begins ? 1 : 0) | (ends ? 2 : 0);
+                    s_unit[2 * warp + which] = (int64_t)b * per_seq + at.hu;
+                    s_ends[2 * warp + which] = (begins ? 1 : 0) | (ends ? 2 : 0);
                 }
             }
             left -= seg;
-            if (left <= 0) break;
-            r = 0;
-            if (++hu == per_seq) {
-                hu = 0;
-                do {
-                    kv_span(pool, seqs, a.window, ++b, lo, hi);
-                    n = kv_records(lo, hi);
-                } while (n == 0);
+            if (left == 0) break;
+            at.next_unit(pool, seqs, a.window, per_seq);
+        }
+        if (!alive && lane == 0) {
+            atomicExch(status, kStatusPipelineTimeout);
+            // the copies still under way (of the stages behind the last good one) must land before the CTA leaves
+            for (int i = 0; rw == 0 && i < stages; ++i) {
+                s_drain[warp] = 0;
+                mbar_wait_limit(smem_u32(&s_full[team][i]), i > dead_stage ? dead_phase : dead_phase ^ 1u, &s_drain[warp], 100000000LL);
             }
         }
     }
@@ -568,24 +691,26 @@ __global__ void __launch_bounds__(kKvThreads) kv_attend_kernel(KvPool pool, KvSe
         const int which = ends & 1;
         float* po = split.partial + (2 * (int64_t)blockIdx.x + which) * chunk_rows * (D + 3);
         float* ps = po + chunk_rows * D;
-        for (int i = tid; i < chunk_rows * (D / 4); i += kKvThreads) {
+        for (int i = tid; i < chunk_rows * (D / 4); i += kThreads) {
             const int row = i / (D / 4), d = 4 * (i - row * (D / 4)), k = row / kRows, in = row - k * kRows;
             float m = kKvMaxInit, big = kKvMaxInit;
             for (int f = e; f < e1; ++f) {
                 const int sl = slot_of(f, k);
                 if (s_unit[sl] < 0) continue;
-                m = fmaxf(m, ss[(sl * kRows + in) * 3]);
-                big = fmaxf(big, ss[(sl * kRows + in) * 3 + 1]);
+                const float* st = slot_rows(sl >> 1, sl & 1) + kRows * D + 3 * in;
+                m = fmaxf(m, st[0]);
+                big = fmaxf(big, st[1]);
             }
             float l = 0.f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int f = e; f < e1; ++f) {
                 const int sl = slot_of(f, k);
                 if (s_unit[sl] < 0) continue;
-                const float* s = ss + (sl * kRows + in) * 3;
-                l += s[2] * ex2(s[0] - m);
-                const float c = ex2(s[1] - big);
-                const float4 y = *reinterpret_cast<const float4*>(so + (sl * kRows + in) * D + d);
+                const float* rows = slot_rows(sl >> 1, sl & 1);
+                const float* st = rows + kRows * D + 3 * in;
+                l += st[2] * ex2(st[0] - m);
+                const float c = ex2(st[1] - big);
+                const float4 y = *reinterpret_cast<const float4*>(rows + in * D + d);
                 o.x = fmaf(y.x, c, o.x), o.y = fmaf(y.y, c, o.y), o.z = fmaf(y.z, c, o.z), o.w = fmaf(y.w, c, o.w);
             }
             if (ends == 3) {
@@ -626,16 +751,16 @@ __global__ void __launch_bounds__(kKvThreads) kv_attend_kernel(KvPool pool, KvSe
         kv_span(pool, seqs, a.window, (int)b, lo, hi);
         if (hi > lo) continue;
         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int i = tid; i < a.q_heads * (D / 4); i += kKvThreads)
+        for (int i = tid; i < a.q_heads * (D / 4); i += kThreads)
             store_row<4>(a.out, b * a.q_heads * D + 4 * i, a.type, a.out_vec, zero);
         if (a.lse != nullptr)
-            for (int i = tid; i < a.q_heads; i += kKvThreads) a.lse[b * a.q_heads + i] = -INFINITY;
+            for (int i = tid; i < a.q_heads; i += kThreads) a.lse[b * a.q_heads + i] = -INFINITY;
     }
 }
 
 // Units that several CTAs hold parts of: block (c, y) joins rows of the unit that begins in CTA c and goes on behind it.
 template <int NB>
-__global__ void __launch_bounds__(kKvThreads) kv_join_kernel(KvPool pool, KvAttend a, KvSplit split, int chunk_rows) {
+__global__ void __launch_bounds__(kKvJoinThreads) kv_join_kernel(KvPool pool, KvAttend a, KvSplit split, int chunk_rows) {
     constexpr int D = 32 * NB, kD4 = D / 4;
     const int c = blockIdx.x;
     const int64_t u = split.unit[2 * (int64_t)c + 1];
@@ -643,7 +768,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_join_kernel(KvPool pool, KvAtte
     const int more = split.more[c];
     const int64_t per_seq = (int64_t)pool.heads * split.chunks, b = u / per_seq;
     const int hu = (int)(u - b * per_seq), h = hu / split.chunks, row0 = (hu - h * split.chunks) * chunk_rows;
-    const int i = blockIdx.y * kKvThreads + threadIdx.x, row = i / kD4, d = 4 * (i - row * kD4);
+    const int i = blockIdx.y * kKvJoinThreads + threadIdx.x, row = i / kD4, d = 4 * (i - row * kD4);
     if (row >= chunk_rows || row0 + row >= a.group) return;
     const int64_t stride = (int64_t)chunk_rows * (D + 3);
     auto part = [&](int k) { return split.partial + (2 * (int64_t)(c + k) + (k == 0 ? 1 : 0)) * stride; };
@@ -673,22 +798,22 @@ __global__ void __launch_bounds__(kKvThreads) kv_join_kernel(KvPool pool, KvAtte
 
 template <int FMT, int NB, int RT>
 struct KvAttendInstance {
-    static constexpr int kSmem = 2 * kKvWarps * 8 * RT * (32 * NB + 3) * 4;
+    using Shape = KvShape<FMT, NB, RT>;
     static cudaError_t init() {
-        return cudaFuncSetAttribute(kv_attend_kernel<FMT, NB, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        return cudaFuncSetAttribute(kv_attend_kernel<FMT, NB, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
     }
     static int launch(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
                       cudaStream_t stream) {
         KvSplit split{};
         split.row_warps = 1;
-        while (split.row_warps < kKvWarps && split.row_warps * 8 * RT < a.group) split.row_warps *= 2;
+        while (split.row_warps < Shape::kWarps && split.row_warps * 8 * RT < a.group) split.row_warps *= 2;
         const int chunk_rows = split.row_warps * 8 * RT;
         split.chunks = (a.group + chunk_rows - 1) / chunk_rows;
         split.unit = work.unit;
         split.more = work.more;
         split.partial = work.partial;
-        kv_attend_kernel<FMT, NB, RT><<<work.ctas, kKvThreads, kSmem, stream>>>(pool, seqs, a, split, status);
-        kv_join_kernel<NB><<<dim3(work.ctas, (chunk_rows * 8 * NB + kKvThreads - 1) / kKvThreads), kKvThreads, 0, stream>>>(
+        kv_attend_kernel<FMT, NB, RT><<<work.ctas, Shape::kThreads, Shape::kSmem, stream>>>(pool, seqs, a, split, status);
+        kv_join_kernel<NB><<<dim3(work.ctas, (chunk_rows * 8 * NB + kKvJoinThreads - 1) / kKvJoinThreads), kKvJoinThreads, 0, stream>>>(
             pool, a, split, chunk_rows);
         return 2;
     }

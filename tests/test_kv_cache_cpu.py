@@ -85,6 +85,66 @@ def test_work_units_cover_every_record_once():
         assert set(done) == want and set(done.values()) <= {1}
 
 
+def test_split_and_join_cover_every_record_once():
+    """The cut of the attention's work: ranges of CTAs and teams, which of their units are whole, begun or continued, and
+    the CTAs that a unit's parts are gathered from."""
+    rng = random.Random(6)
+    for _ in range(300):
+        batch, per_seq = rng.randrange(1, 30), rng.choice([1, 2, 5, 8])
+        n = [rng.choice([0, 0, 1, 2, 7, rng.randrange(0, 400)]) for _ in range(batch)]
+        ctas, teams, least = rng.choice([1, 3, 148]), rng.choice([1, 2, 4, 8]), rng.choice([1, 8])
+        units = [(b, hu) for b in range(batch) if n[b] for hu in range(per_seq)]
+        flat = [(u, r) for u in units for r in range(n[u[0]])]
+        total = len(flat)
+        part = max(-(-total // ctas), least)
+        parts, whole, more = {}, set(), {}
+        for c in range(ctas):
+            c0 = min(c * part, total)
+            c1 = min(c0 + part, total)
+            step = -(-(c1 - c0) // teams)
+            entries = []
+            for t in range(teams):
+                t0 = min(c0 + t * step, c1)
+                t1 = min(t0 + step, c1)
+                while t0 < t1:
+                    u, r = flat[t0]
+                    seg = min(n[u[0]] - r, t1 - t0)
+                    begins, ends = r == 0, r + seg == n[u[0]]
+                    if begins and ends:
+                        assert u not in whole
+                        whole.add(u)
+                    else:
+                        entries.append((2 * t + begins, u, begins + 2 * ends, seg))
+                    t0 += seg
+            assert len({e[0] for e in entries}) == len(entries)          # a slot is used once
+            assert [e[0] for e in entries] == sorted(e[0] for e in entries)
+            i = 0
+            while i < len(entries):                                      # runs of equal units
+                j, ends, count = i, 0, 0
+                while j < len(entries) and entries[j][1] == entries[i][1]:
+                    ends |= entries[j][2]
+                    count += entries[j][3]
+                    j += 1
+                u = entries[i][1]
+                if ends == 3:
+                    assert u not in whole and count == n[u[0]]
+                    whole.add(u)
+                else:
+                    which = ends & 1
+                    assert (c, which) not in parts
+                    parts[c, which] = (u, count)
+                    if which:
+                        end = flat.index((u, 0)) + n[u[0]]
+                        more[c] = (end - 1) // part - c
+                i = j
+        for c, k in more.items():
+            u = parts[c, 1][0]
+            got = [parts[c, 1]] + [parts[c + i, 0] for i in range(1, k + 1)]
+            assert all(g[0] == u for g in got) and sum(g[1] for g in got) == n[u[0]] and u not in whole
+            whole.add(u)
+        assert whole == set(units) and sum(1 + k for k in more.values()) == len(parts)
+
+
 def test_refusals_without_a_device():
     import eos_b200
     from eos_b200 import _lib
