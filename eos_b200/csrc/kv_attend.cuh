@@ -13,8 +13,8 @@
 // records do no rescaling and no shuffles, and weights use f16's range from both ends: they stay below 2^15, and what
 // f16 cannot hold (2^-25) is 2^-31 of the row's largest weight.  A weight and its value's scale are multiplied before the
 // split: w = 2^(x + e - M) with e the largest scale exponent of the token's blocks and M a second lagging maximum, so that
-// the bound holds whatever the scales; the blocks' own exponents (relative to e) are applied to the codes as f16 factors,
-// shifted up as far as the codes allow: what falls below f16 there is 2^-33 of the token's largest value.
+// the bound holds whatever the scales; the blocks' own exponents, relative to e, are f16 factors of the split weights
+// (four multiplications a block where scaling the codes takes eight), so the codes enter the mma as they are.
 #pragma once
 #include "kv_dev.cuh"
 
@@ -23,13 +23,38 @@ namespace eosb {
 constexpr float kKvMaxInit = -1e30f;   // below every score; finite, so that 2^(x - m) of a masked score is 0 and not NaN
 constexpr float kKvHead = 7.f, kKvLag = 15.f;   // m = ceil(largest score) - 7; weights up to 2^15
 constexpr int kKvQueryExp = 13;                  // query rows are scaled to a largest magnitude in [2^13, 2^14)
-// exponent that the blocks' relative scales are shifted up by: the largest code, 448 or 6, times 2^this is below 65504
-__host__ __device__ constexpr int kv_rel_shift(int format) { return format == kKvMx8 ? 6 : 13; }
 
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+        " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&y);
 }
 template <bool kBf>
 __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -90,6 +115,20 @@ __device__ __forceinline__ void load_scales(const uint8_t* p, uint32_t (&a)[(NB 
     } else {
         const uint4 w = *reinterpret_cast<const uint4*>(p);
         a[0] = w.x, a[1] = w.y, b[0] = w.z, b[1] = w.w;
+    }
+}
+// Scale bytes of a token pair's values: block b in byte 2 (b % 2) (first token) and the next (second) of word b / 2
+template <int NB>
+__device__ __forceinline__ void load_pair_scales(const uint8_t* p, uint32_t (&w)[(NB + 1) / 2]) {
+    if constexpr (NB == 1) w[0] = *reinterpret_cast<const uint16_t*>(p);
+    else if constexpr (NB == 2) w[0] = *reinterpret_cast<const uint32_t*>(p);
+    else if constexpr (NB <= 4) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z;
+        if constexpr (NB > 6) w[3] = v.w;
     }
 }
 // exponent field of byte i as a float 2^(byte - 127); 255 becomes infinity, which times the zero codes of such a block is NaN
@@ -154,15 +193,25 @@ struct KvWarp {
         }
     }
 
+    __device__ __forceinline__ void scale_rows(int r, float f) {
+        const float2 f2 = make_float2(f, f);
+#pragma unroll
+        for (int n = 0; n < 4 * NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                const float2 y = mul2(make_float2(o[r][n][i], o[r][n][i + 1]), f2);
+                o[r][n][i] = y.x, o[r][n][i + 1] = y.y;
+            }
+    }
+
     // One record; its tokens [lo, hi) of 0..15 count.
     __device__ __forceinline__ void record(const uint8_t* rec, int lo, int hi, int lane) {
         const int t = lane & 3;
-        float x[RT][4];   // scores of row g: tokens 2t, 2t+1, 2t+8, 2t+9
+        float s[RT][4];   // raw scores of row g: tokens 2t, 2t+1, 2t+8, 2t+9
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             uint32_t k[NB * KP / 4];
             load_lane<NB * KP>(rec + j * 32 * NB * KP, lane, k);
-            float s0[RT], s1[RT];
             if constexpr (!kMx) {
                 float c[RT][4];
 #pragma unroll
@@ -170,18 +219,19 @@ struct KvWarp {
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int s = 0; s < 2; ++s)
+                    for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int r = 0; r < RT; ++r)
-                            mma_16x8x16<kBf>(c[r], q[r][b][2 * s], q[r][b][4 + 2 * s], q[r][b][2 * s + 1],
-                                             q[r][b][4 + 2 * s + 1], k[4 * b + 2 * s], k[4 * b + 2 * s + 1]);
+                            mma_16x8x16<kBf>(c[r], q[r][b][2 * i], q[r][b][4 + 2 * i], q[r][b][2 * i + 1],
+                                             q[r][b][4 + 2 * i + 1], k[4 * b + 2 * i], k[4 * b + 2 * i + 1]);
 #pragma unroll
-                for (int r = 0; r < RT; ++r) s0[r] = c[r][0] + c[r][2], s1[r] = c[r][1] + c[r][3];
+                for (int r = 0; r < RT; ++r) s[r][2 * j] = c[r][0] + c[r][2], s[r][2 * j + 1] = c[r][1] + c[r][3];
             } else {
                 uint32_t sa[(NB + 3) / 4], sb[(NB + 3) / 4];
                 load_scales<NB>(rec + kv_key_scale_offset(FMT, NB) + (8 * j + 2 * t) * kv_scale_stride(NB), sa, sb);
+                float2 sum[RT];
 #pragma unroll
-                for (int r = 0; r < RT; ++r) s0[r] = s1[r] = 0.f;
+                for (int r = 0; r < RT; ++r) sum[r] = make_float2(0.f, 0.f);
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     uint32_t f[4];
@@ -191,19 +241,18 @@ struct KvWarp {
                     } else {
                         f16_of_e2m1x8(k[b], f[0], f[1], f[2], f[3]);
                     }
-                    const float ca = scale_at(sa[b / 4], b & 3), cb = scale_at(sb[b / 4], b & 3);
+                    const float2 scale = make_float2(scale_at(sa[b / 4], b & 3), scale_at(sb[b / 4], b & 3));
 #pragma unroll
                     for (int r = 0; r < RT; ++r) {
                         float c[4] = {0.f, 0.f, 0.f, 0.f};
                         mma_16x8x16<false>(c, q[r][b][0], q[r][b][4], q[r][b][1], q[r][b][5], f[0], f[1]);
                         mma_16x8x16<false>(c, q[r][b][2], q[r][b][6], q[r][b][3], q[r][b][7], f[2], f[3]);
-                        s0[r] = fmaf(c[0] + c[2], ca, s0[r]);
-                        s1[r] = fmaf(c[1] + c[3], cb, s1[r]);
+                        sum[r] = fma2(add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), scale, sum[r]);
                     }
                 }
-            }
 #pragma unroll
-            for (int r = 0; r < RT; ++r) x[r][2 * j] = s0[r] * qs[r], x[r][2 * j + 1] = s1[r] * qs[r];
+                for (int r = 0; r < RT; ++r) s[r][2 * j] = sum[r].x, s[r][2 * j + 1] = sum[r].y;
+            }
         }
         const bool edge = lo > 0 || hi < kKvRecord;
         uint32_t live = 15u;
@@ -213,105 +262,110 @@ struct KvWarp {
             for (int i = 0; i < 4; ++i) {
                 const int tok = 2 * t + (i & 1) + 8 * (i >> 1);
                 if (tok >= lo && tok < hi) live |= 1u << i;
-#pragma unroll
-                for (int r = 0; r < RT; ++r)
-                    if (!(live >> i & 1)) x[r][i] = -INFINITY;
             }
         }
-        // value scales: largest exponent of each token, and every block's exponent relative to it as f16 pairs
+        // value scales: largest exponent of each token, and every block's relative to it as f16 pairs
         float te[4];
         uint32_t rel[2][NB];
         if constexpr (kMx) {
-            uint32_t sc[4][(NB + 3) / 4];
-            const uint8_t* p = rec + kv_value_scale_offset(FMT, NB) + 2 * t * kv_scale_stride(NB);
-            load_scales<NB>(p, sc[0], sc[1]);
-            load_scales<NB>(p + 8 * kv_scale_stride(NB), sc[2], sc[3]);
-            int top[4];
-            uint32_t bad = 0;
+            uint32_t tops[2], odd = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t v = 0;
+            for (int p = 0; p < 2; ++p) {
+                uint32_t w[(NB + 1) / 2];
+                load_pair_scales<NB>(rec + kv_value_scale_offset(FMT, NB) + (t + 4 * p) * 2 * kv_scale_stride(NB), w);
+                tops[p] = *reinterpret_cast<const uint32_t*>(rec + kv_value_top_offset(FMT, NB) + 4 * (t + 4 * p));
+                odd |= tops[p];
+                // bytes 60 - 4 (top - e): with zeros below them, the f16 numbers 2^(e - top), top - e <= 14
+                const uint32_t c = 0x3c3c3c3cu - __byte_perm(tops[p], 0, 0x1010) * 4u;
 #pragma unroll
-                for (int w = 0; w < (NB + 3) / 4; ++w) {
-                    const uint32_t nan = __vcmpeq4(sc[i][w], 0xffffffffu);
-                    bad |= nan;
-                    v = __vmaxu4(v, sc[i][w] & ~nan);
-                }
-                if constexpr (NB > 2) v = __vmaxu4(v, v >> 16);
-                if constexpr (NB > 1) v = __vmaxu4(v, v >> 8);
-                top[i] = max((int)(v & 0xffu), 1);
-                te[i] = (float)(top[i] - 127 - kv_rel_shift(FMT));
+                for (int b = 0; b < NB; ++b) rel[p][b] = __byte_perm(w[b / 2] * 4u + c, 0, b & 1 ? 0x3424 : 0x1404);
+                // the top bytes as floats, by way of the integers behind 2^23
+                te[2 * p] = __uint_as_float(__byte_perm(tops[p], 0x4b000000u, 0x7440)) - 8388735.f;
+                te[2 * p + 1] = __uint_as_float(__byte_perm(tops[p], 0x4b000000u, 0x7441)) - 8388735.f;
             }
+            if (__any_sync(0xffffffffu, (odd & 0xffff0000u) != 0u)) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
+                for (int p = 0; p < 2; ++p) {
+                    uint32_t w[(NB + 1) / 2];
+                    load_pair_scales<NB>(rec + kv_value_scale_offset(FMT, NB) + (t + 4 * p) * 2 * kv_scale_stride(NB), w);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    // 2^(s - top + shift) as f16; 0 where the exponent leaves the float's
-                    const int sa = (int)(sc[2 * i][b / 4] >> (8 * (b & 3)) & 0xffu), sb = (int)(sc[2 * i + 1][b / 4] >> (8 * (b & 3)) & 0xffu);
-                    const float fa = __uint_as_float((uint32_t)max(sa - top[2 * i] + 127 + kv_rel_shift(FMT), 0) << 23);
-                    const float fb = __uint_as_float((uint32_t)max(sb - top[2 * i + 1] + 127 + kv_rel_shift(FMT), 0) << 23);
-                    rel[i][b] = f16x2_of(fa, fb);
+                    for (int b = 0; b < NB; ++b) {
+                        float f[2];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int e = (int)(w[b / 2] >> (16 * (b & 1) + 8 * i) & 0xffu), top = (int)(tops[p] >> (8 * i) & 0xffu);
+                            f[i] = e == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)max(e - top + 127, 0) << 23);
+                        }
+                        rel[p][b] = f16x2_of(f[0], f[1]);   // zero below 2^-25
+                    }
                 }
-            if (bad != 0) {
+            }
+            if (edge) {   // what lies in the places that do not count may be anything
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if ((sc[i][b / 4] >> (8 * (b & 3)) & 0xffu) == 255u) rel[i >> 1][b] |= (i & 1) ? 0x7fff0000u : 0x7fffu;
-            }
-            if (edge) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!(live >> i & 1)) rel[i >> 1][b] &= (i & 1) ? 0x0000ffffu : 0xffff0000u;
+                    for (int p = 0; p < 2; ++p)
+                        rel[p][b] &= (live >> (2 * p) & 1u ? 0xffffu : 0u) | (live >> (2 * p) & 2u ? 0xffff0000u : 0u);
             }
         }
         // softmax
         uint32_t whi[RT][2], wlo[RT][2];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            float top = fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]));
-            if (__any_sync(0xffffffffu, top > m[r] + kKvLag)) {
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float to = top > m[r] + kKvLag ? ceilf(top) - kKvHead : m[r];
-                const float f = ex2(m[r] - to);
+            float x[4];   // exponents of the weights
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = fmaf(s[r][i], qs[r], -m[r]);
+                if (edge && !(live >> i & 1u)) x[i] = -INFINITY;
+            }
+            if (__any_sync(0xffffffffu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > kKvLag)) {
+                // from the scores: the first time, m is far below them and their differences are lost in x
+                float most = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!edge || (live >> i & 1u)) most = fmaxf(most, s[r][i] * qs[r]);
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                const float to = most - m[r] > kKvLag ? ceilf(most) - kKvHead : m[r], f = ex2(m[r] - to);
                 m[r] = to;
                 l[r] *= f;
-                if constexpr (!kMx) {
+                if constexpr (!kMx) scale_rows(r, f);
 #pragma unroll
-                    for (int n = 0; n < 4 * NB; ++n) o[r][n][0] *= f, o[r][n][1] *= f, o[r][n][2] *= f, o[r][n][3] *= f;
-                }
+                for (int i = 0; i < 4; ++i) x[i] = edge && !(live >> i & 1u) ? -INFINITY : fmaf(s[r][i], qs[r], -to);
             }
             float w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = ex2(x[r][i] - m[r]);
+            for (int i = 0; i < 4; ++i) w[i] = ex2(x[i]);
             l[r] += (w[0] + w[1]) + (w[2] + w[3]);
             if constexpr (kMx) {
-                float high = fmaxf(fmaxf(x[r][0] + te[0], x[r][1] + te[1]), fmaxf(x[r][2] + te[2], x[r][3] + te[3]));
-                if (__any_sync(0xffffffffu, high > big[r] + kKvLag)) {
-                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
-                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
-                    const float to = high > big[r] + kKvLag ? ceilf(high) - kKvHead : big[r];
-                    const float f = ex2(big[r] - to);
-                    big[r] = to;
-#pragma unroll
-                    for (int n = 0; n < 4 * NB; ++n) o[r][n][0] *= f, o[r][n][1] *= f, o[r][n][2] *= f, o[r][n][3] *= f;
-                }
-                const float d = m[r] - big[r] + 127.f;
+                float y[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float e = fminf(fmaxf(te[i] + d, 0.f), 254.f);   // an integer
-                    w[i] *= __uint_as_float((uint32_t)(int)e << 23);
+                    y[i] = fmaf(s[r][i], qs[r], te[i] - big[r]);
+                    if (edge && !(live >> i & 1u)) y[i] = -INFINITY;
                 }
+                if (__any_sync(0xffffffffu, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) > kKvLag)) {
+                    float most = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!edge || (live >> i & 1u)) most = fmaxf(most, fmaf(s[r][i], qs[r], te[i]));
+                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                    const float to = most - big[r] > kKvLag ? ceilf(most) - kKvHead : big[r];
+                    scale_rows(r, ex2(big[r] - to));
+                    big[r] = to;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] = edge && !(live >> i & 1u) ? -INFINITY : fmaf(s[r][i], qs[r], te[i] - to);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = ex2(y[i]);
             }
             split_pair<kBf>(w[0], w[1], whi[r][0], wlo[r][0]);
             split_pair<kBf>(w[2], w[3], whi[r][1], wlo[r][1]);
         }
         // values
         uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-        if (!kMx && edge) {   // what lies in the places that do not count may be anything
+        if (!kMx && edge) {
             keep0 = (live & 1 ? 0xffffu : 0u) | (live & 2 ? 0xffff0000u : 0u);
             keep1 = (live & 4 ? 0xffffu : 0u) | (live & 8 ? 0xffff0000u : 0u);
         }
@@ -326,25 +380,23 @@ struct KvWarp {
                     f[2 * e] = v[8 * b + 2 * e], f[2 * e + 1] = v[8 * b + 2 * e + 1];
                     if (edge) f[2 * e] &= keep0, f[2 * e + 1] &= keep1;
                 }
+            } else if constexpr (FMT == kKvMx8) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f16_of_e4m3x4(v[4 * b + e], f[2 * e], f[2 * e + 1]);
             } else {
-                if constexpr (FMT == kKvMx8) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) f16_of_e4m3x4(v[4 * b + e], f[2 * e], f[2 * e + 1]);
-                } else {
-                    f16_of_e2m1x8(v[2 * b], f[0], f[1], f[2], f[3]);
-                    f16_of_e2m1x8(v[2 * b + 1], f[4], f[5], f[6], f[7]);
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&f[e]), *reinterpret_cast<const __half2*>(&rel[e & 1][b]));
-                    f[e] = *reinterpret_cast<const uint32_t*>(&y);
-                }
+                f16_of_e2m1x8(v[2 * b], f[0], f[1], f[2], f[3]);
+                f16_of_e2m1x8(v[2 * b + 1], f[4], f[5], f[6], f[7]);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int r = 0; r < RT; ++r) {
+                uint32_t w0 = whi[r][0], w1 = wlo[r][0], w2 = whi[r][1], w3 = wlo[r][1];
+                if constexpr (kMx) {
+                    w0 = mul_f16x2(w0, rel[0][b]), w1 = mul_f16x2(w1, rel[0][b]);
+                    w2 = mul_f16x2(w2, rel[1][b]), w3 = mul_f16x2(w3, rel[1][b]);
+                }
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
-                    mma_16x8x16<kBf>(o[r][4 * b + e], whi[r][0], wlo[r][0], whi[r][1], wlo[r][1], f[2 * e], f[2 * e + 1]);
+                for (int e = 0; e < 4; ++e) mma_16x8x16<kBf>(o[r][4 * b + e], w0, w1, w2, w3, f[2 * e], f[2 * e + 1]);
+            }
         }
     }
 
@@ -558,39 +610,45 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
         KvWalk ahead = at;
         int64_t to_fetch = t1 - t0;
         const int rpp = pool.records_per_page;
-        int slot = 0, in = 0, page = -1, next_page = -1;   // page slot of the record to fetch, record in the page, page ids
-        auto page_at = [&](int s) { return s < seqs.max_pages ? __ldg(seqs.table + (int64_t)ahead.b * seqs.max_pages + s) : -1; };
+        // the page of the next record: slot in the table, that record (null: a page id out of range), records left there
+        int slot = 0, run = 0, next_page = -1;
+        const uint8_t* src = nullptr;
+        const uint32_t ring_at = smem_u32(smem + team * split.row_warps * Shape::kRing), full_at = smem_u32(&s_full[team][0]);
+        auto page_at = [&](int sl) { return sl < seqs.max_pages ? __ldg(seqs.table + (int64_t)ahead.b * seqs.max_pages + sl) : -1; };
+        auto enter_page = [&](int page, int in) {
+            run = min(rpp - in, ahead.n - ahead.r);
+            src = page < 0 || page >= pool.pages
+                      ? nullptr
+                      : pool.base + (((int64_t)page * pool.heads + ahead.hu / split.chunks) * rpp + in) * Shape::kRecord;
+            next_page = page_at(slot + 1);   // asked for early: its latency passes while this page is read
+        };
         auto enter_unit = [&]() {
             const int rec = ahead.lo / kKvRecord + ahead.r;
             slot = rec / rpp;
-            in = rec - slot * rpp;
-            page = page_at(slot);
-            next_page = page_at(slot + 1);
+            enter_page(page_at(slot), rec - slot * rpp);
         };
         auto fetch = [&](int stage) {   // the next record, if there is one, into `stage`
             if (to_fetch == 0) return;
-            const bool ok = page >= 0 && page < pool.pages;
             if (lane == 0) {
-                const uint32_t bar = smem_u32(&s_full[team][stage]);
-                s_ok[team][stage] = ok;
-                if (ok) {
-                    const int64_t rec = ((int64_t)page * pool.heads + ahead.hu / split.chunks) * rpp + in;
-                    kv_copy_record(smem_u32(smem + team * split.row_warps * Shape::kRing + stage * Shape::kRecord),
-                                   pool.base + rec * Shape::kRecord, Shape::kRecord, bar);
+                s_ok[team][stage] = src != nullptr;
+                if (src != nullptr) {
+                    kv_copy_record(ring_at + stage * Shape::kRecord, src, Shape::kRecord, full_at + 8 * stage);
                 } else {
                     atomicExch(status, kStatusBadPage);
-                    mbar_arrive(bar);
+                    mbar_arrive(full_at + 8 * stage);
                 }
             }
-            if (--to_fetch == 0) return;
-            if (++ahead.r == ahead.n) {
-                ahead.next_unit(pool, seqs, a.window, per_seq);
-                enter_unit();
-            } else if (++in == rpp) {
-                in = 0;
-                ++slot;
-                page = next_page;
-                next_page = page_at(slot + 1);
+            --to_fetch;
+            ++ahead.r;
+            if (src != nullptr) src += Shape::kRecord;
+            if (--run == 0 && to_fetch > 0) {
+                if (ahead.r == ahead.n) {
+                    ahead.next_unit(pool, seqs, a.window, per_seq);
+                    enter_unit();
+                } else {
+                    ++slot;
+                    enter_page(next_page, 0);
+                }
             }
         };
         if (rw == 0) {

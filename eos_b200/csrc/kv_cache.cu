@@ -153,6 +153,7 @@ __global__ void __launch_bounds__(kKvWarps * 32)
     }
     const bool any = mine[0] || mine[1] || mine[2] || mine[3], all = mine[0] && mine[1] && mine[2] && mine[3];
     uint8_t* codes = rec + kv_value_offset(FMT, nb);
+    uint64_t scales[4] = {0, 0, 0, 0};   // of each token: the blocks' scale bytes, 0 for a block of zeros
 #pragma unroll 2
     for (int b = 0; b < nb; ++b) {
         float x[4][4];   // [token][element]
@@ -183,8 +184,7 @@ __global__ void __launch_bounds__(kKvWarps * 32)
                 const float inv = kv_inverse_scale(byte[i]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[i][e] = kv_scaled(x[i][e], byte[i], inv);
-                if (mine[i] && g == 0)
-                    rec[kv_value_scale_offset(FMT, nb) + (2 * t + (i & 1) + 8 * (i >> 1)) * ns + b] = (uint8_t)byte[i];
+                scales[i] |= (uint64_t)(m == 0 ? 0u : byte[i]) << (8 * b);
             }
             if constexpr (FMT == kKvMx8) {
                 const uint32_t k = (mine[0] ? 0u : 0xffu) | (mine[1] ? 0u : 0xff00u) | (mine[2] ? 0u : 0xff0000u) |
@@ -229,6 +229,32 @@ __global__ void __launch_bounds__(kKvWarps * 32)
                     q[3] = (q[3] & ~k[3]) | (old.w & k[3]);
                 }
                 *dst = make_uint4(q[0], q[1], q[2], q[3]);
+            }
+        }
+    }
+    if constexpr (kMx) {   // lane (g, t) stores the scales of block g; the tops by the lanes of block 0
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t top = 1, odd = 0;
+            for (int b = 0; b < nb; ++b) {
+                const uint32_t e = (uint32_t)(scales[i] >> (8 * b)) & 0xffu;
+                if (e == 255u) odd = 1;
+                else top = max(top, e);
+            }
+            for (int b = 0; b < nb; ++b) {
+                const uint32_t e = (uint32_t)(scales[i] >> (8 * b)) & 0xffu;
+                if (e != 0u && e + kKvNear < top) odd = 1;
+            }
+            if (!mine[i]) continue;
+            const int pair = t + 4 * (i >> 1);
+            if (g < nb) {
+                const uint32_t e = (uint32_t)(scales[i] >> (8 * g)) & 0xffu;
+                rec[kv_value_scale_offset(FMT, nb) + (pair * ns + g) * 2 + (i & 1)] = (uint8_t)(e == 0u ? top : e);
+            }
+            if (g == 0) {
+                uint8_t* tops = rec + kv_value_top_offset(FMT, nb) + 4 * pair + (i & 1);
+                tops[0] = (uint8_t)top;
+                tops[2] = (uint8_t)odd;
             }
         }
     }
@@ -314,7 +340,7 @@ __global__ void __launch_bounds__(kKvWarps * 32)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (!mine[i]) continue;
-            const float s = kMx ? kv_scale_value(rec[kv_value_scale_offset(FMT, nb) + (2 * t + (i & 1) + 8 * (i >> 1)) * ns + b]) : 1.f;
+            const float s = kMx ? kv_scale_value(rec[kv_value_scale_offset(FMT, nb) + ((t + 4 * (i >> 1)) * ns + b) * 2 + (i & 1)]) : 1.f;
             float x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {

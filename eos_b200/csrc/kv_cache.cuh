@@ -2,7 +2,7 @@
 //
 // A page holds page_size tokens of every head; the unit of the layout is the RECORD: the keys and values of 16
 // consecutive tokens of one head, contiguous, 16-byte aligned,
-//     key codes | value codes | key scales | value scales           (scales only in the block-scaled formats)
+//     key codes | value codes | key scales | value scales | value tops      (the last three in the block-scaled formats)
 // page p, head h, record r of the page sit at ((p * heads + h) * (page_size / 16) + r) * record_bytes.
 //
 // Inside a record the codes are stored in the order in which the 32 lanes of a warp feed them to mma.sync m16n8k16, so
@@ -13,7 +13,11 @@
 //     values  lane (g, t) holds tokens {2t, 2t+1, 2t+8, 2t+9}, elements 32 b + 4 g + {0..3}, element-major: the two
 //             tokens of one 32-bit operand register are neighbours
 // A lane's bytes are cut into 16-byte pieces (then 8, then 4); piece i of all lanes is one contiguous plane.
-// Scales are one byte per token and block, [16][blocks rounded up to 1, 2, 4 or 8].
+// Scales are one byte per token and block (2^(byte - 127)), blocks rounded up to 1, 2, 4 or 8: keys [16 tokens][blocks],
+// values [8 token pairs][blocks][2], the order in which the attention kernel makes f16 pairs of them.  For every token
+// pair a 32-bit word says what the kernel would otherwise have to find out for each of its loads: the largest scale byte
+// of each token's values (bits 0-7, 8-15) and whether the token is out of the ordinary (bits 16, 24): a block stored as
+// NaN, or one more than 2^14 below the token's largest.  A block of zeros has the token's largest scale.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -38,9 +42,13 @@ __host__ __device__ constexpr int kv_key_scale_offset(int format, int blocks) {
 __host__ __device__ constexpr int kv_value_scale_offset(int format, int blocks) {
     return kv_key_scale_offset(format, blocks) + kv_scale_bytes(format, blocks);
 }
-__host__ __device__ constexpr int kv_record_bytes(int format, int blocks) {
+__host__ __device__ constexpr int kv_value_top_offset(int format, int blocks) {
     return kv_value_scale_offset(format, blocks) + kv_scale_bytes(format, blocks);
 }
+__host__ __device__ constexpr int kv_record_bytes(int format, int blocks) {
+    return kv_value_top_offset(format, blocks) + (format <= kKvBf16 ? 0 : 32);
+}
+constexpr int kKvNear = 14;   // exponents below a token's largest that the attention kernel's ordinary path covers
 // offset of byte p of a lane's `bytes` bytes (planes of 16, then 8, then 4 bytes per lane)
 __host__ __device__ constexpr int kv_lane_offset(int bytes, int lane, int p) {
     const int plane = p >> 4, in = p & 15, rest = bytes - (plane << 4);

@@ -307,6 +307,32 @@ def test_magnitudes_far_apart(fmt):
     s.sync()
 
 
+@pytest.mark.parametrize("fmt", ["mx8", "mx4"])
+@pytest.mark.parametrize("dim", [64, 96, 192, 256])
+def test_blocks_of_one_token_far_apart(fmt, dim):
+    """Value blocks 2^13 to 2^20 below the token's largest, blocks of zeros, and a token whose values are all zero: the
+    small blocks come out with the accuracy of their own size as long as the floor of the split allows."""
+    n, blocks = 70, dim // 32
+    s = Sequences(fmt, dim, 1, 16, [n])
+    g = torch.Generator().manual_seed(dim)
+    k = torch.randn((n, 1, dim), generator=g).cuda()
+    low = torch.randint(0, 21, (n, 1, blocks), generator=g).float()
+    low[:, :, 0] = 0
+    low[: n // 2] = low[: n // 2].clamp(max=13)           # a stretch of ordinary tokens first
+    v = torch.randn((n, 1, blocks, 32), generator=g) * torch.exp2(-low)[..., None]
+    v[5, :, blocks - 1] = 0
+    v[40, :, 0] = 0
+    v[41] = 0
+    v = v.reshape(n, 1, dim).cuda()
+    s.append(k, v, [0], [n])
+    rk, rv = s.read([0], [n])
+    assert same(rv, stored(v, fmt)) and same(rk, stored(k, fmt))
+    q = torch.randn((1, 2, dim), generator=g).cuda()
+    out, lse = s.attend(q, [n], dim ** -0.5)
+    check_attend(q, ([stored(k, fmt)], [stored(v, fmt)]), [n], dim ** -0.5, 0, fmt, out, lse, 2)
+    s.sync()
+
+
 def test_strided_and_unaligned_tensors():
     """Views into one fused projection [tokens, (Hq + 2 Hk) dim], and tensors that start at an odd element."""
     dim, heads, group, n = 64, 2, 3, 50
@@ -390,7 +416,7 @@ def test_refusals():
         with pytest.raises(E, match=what):
             eos_b200.KvCache(rt, *args)
     c = eos_b200.KvCache(rt, 4, 16, 2, 64, "mx8")
-    assert c.page_bytes == 2 * 16 * 2 * (64 + 2)
+    assert c.page_bytes == 2 * 16 * 2 * (64 + 2) + 2 * 32      # codes and scales, and 32 bytes a record of 16 tokens
     x = torch.zeros((4, 2, 64), device="cuda")
     i = torch.zeros(8, dtype=torch.int32, device="cuda")
     p, t = x.data_ptr(), i.data_ptr()

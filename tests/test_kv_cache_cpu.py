@@ -43,7 +43,8 @@ int main() {
                 if (seen[i] != 1) return 4;
             if (format >= kKvMx8) {   // scales of 16 tokens behind the codes
                 if (kv_scale_stride(nb) < nb || kv_scale_bytes(format, nb) != 16 * kv_scale_stride(nb)) return 5;
-                if (kv_value_scale_offset(format, nb) + 16 * kv_scale_stride(nb) != total) return 6;
+                if (kv_value_top_offset(format, nb) != kv_value_scale_offset(format, nb) + 16 * kv_scale_stride(nb)) return 6;
+                if (kv_value_top_offset(format, nb) + 32 != total) return 6;
             } else if (kv_key_scale_offset(format, nb) != total) return 7;
         }
     std::puts("ok");
