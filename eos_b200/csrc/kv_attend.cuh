@@ -158,38 +158,83 @@ struct KvWarp {
         }
     }
 
-    // Query rows [row0, row0 + 8 RT) of a unit, those from `rows` on are zero.  f16 operands: each row is divided by a
-    // power of two first, so that no magnitude leaves f16's range.
+    // Query rows [row0, row0 + 8 RT) of a unit, those from `rows` on are zero: first the raw loads, all of them on their way
+    // at once and waited for in convert_query, ...
     __device__ __forceinline__ void load_query(const KvAttend& a, int64_t at, int row0, int rows, int lane) {
         const int g = lane >> 2, t = lane & 3;
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             const int row = row0 + 8 * r + g;
             const int64_t p = at + (int64_t)row * a.head_stride + 8 * t;
-            float x[NB][8];
+            const uint8_t* base = static_cast<const uint8_t*>(a.query) + p * (a.type == kTypeF32 ? 4 : 2);
+            if (row >= rows) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) q[r][b][i] = 0u;
+            } else if (a.type == kTypeF32) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const uint32_t* w = reinterpret_cast<const uint32_t*>(base) + 32 * b;
+                    if (a.vec) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(w), y = *reinterpret_cast<const uint4*>(w + 4);
+                        q[r][b][0] = x.x, q[r][b][1] = x.y, q[r][b][2] = x.z, q[r][b][3] = x.w;
+                        q[r][b][4] = y.x, q[r][b][5] = y.y, q[r][b][6] = y.z, q[r][b][7] = y.w;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) q[r][b][i] = w[i];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const uint16_t* w = reinterpret_cast<const uint16_t*>(base) + 32 * b;
+                    if (a.vec) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(w);
+                        q[r][b][0] = x.x, q[r][b][1] = x.y, q[r][b][2] = x.z, q[r][b][3] = x.w;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) q[r][b][i] = (uint32_t)w[2 * i] | ((uint32_t)w[2 * i + 1] << 16);
+                    }
+                }
+            }
+        }
+    }
+    // ... then the halves.  f16 operands: each row is divided by a power of two first, so that no magnitude leaves f16's range.
+    __device__ __forceinline__ void convert_query(const KvAttend& a) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            if (a.type == kTypeF32) split_row(a, r, [&](int b, int i) { return make_float2(__uint_as_float(q[r][b][2 * i]), __uint_as_float(q[r][b][2 * i + 1])); });
+            else if (a.type == kTypeF16) split_row(a, r, [&](int b, int i) { return f16x2_floats(q[r][b][i]); });
+            else split_row(a, r, [&](int b, int i) { return bf16x2_floats(q[r][b][i]); });
+        }
+    }
+    template <typename F>
+    __device__ __forceinline__ void split_row(const KvAttend& a, int r, F&& pair) {
+        float inv = 1.f;
+        qs[r] = a.scale_log2;
+        if constexpr (!kBf) {
             uint32_t top = 0;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                if (row < rows) load_row<8>(a.query, p + 32 * b, a.type, a.vec, x[b]);
-                else
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[b][i] = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[b][i]) & 0x7fffffffu);
-            }
-            float inv = 1.f;
-            qs[r] = a.scale_log2;
-            if constexpr (!kBf) {
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const uint32_t e = min(max(top >> 23, kKvQueryExp + 1u), 254u);
-                inv = __uint_as_float((254u + kKvQueryExp - e) << 23);
-                qs[r] *= __uint_as_float((e - kKvQueryExp) << 23);
-            }
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) split_pair<kBf>(x[b][2 * i] * inv, x[b][2 * i + 1] * inv, q[r][b][i], q[r][b][4 + i]);
+                for (int i = 0; i < 4; ++i) {
+                    const float2 x = pair(b, i);
+                    top = max(top, max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu));
+                }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const uint32_t e = min(max(top >> 23, kKvQueryExp + 1u), 254u);
+            inv = __uint_as_float((254u + kKvQueryExp - e) << 23);
+            qs[r] *= __uint_as_float((e - kKvQueryExp) << 23);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float2 x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = pair(b, i);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) split_pair<kBf>(x[i].x * inv, x[i].y * inv, q[r][b][i], q[r][b][4 + i]);
         }
     }
 
@@ -466,12 +511,13 @@ constexpr int kKvMinRecords = 8;    // records of a CTA, at least
 // result of its first unit; that of its last one goes into its ring, which is empty by then.
 template <int FMT, int NB, int RT>
 struct KvShape {
-    static constexpr int kWarps = FMT <= kKvBf16 && NB > 4 ? 4 : 8;
+    // as many warps as registers (and, for 16-bit records of 8 KB and more, rings of three records) allow
+    static constexpr int kWarps = FMT <= kKvBf16 && NB > 4 ? 4 : RT > 1 || NB > 4 ? 8 : NB <= 2 ? 16 : FMT <= kKvBf16 ? 8 : 12;
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kRows = 8 * RT;
     static constexpr int kPartial = kRows * (32 * NB + 3) * 4 + (kRows * 3 * 4 % 16 ? 16 - kRows * 3 * 4 % 16 : 0);
     static constexpr int kRecord = kv_record_bytes(FMT, NB);
-    static constexpr int kSmemMax = 232448 - 5120;               // of a CTA, less the static part
+    static constexpr int kSmemMax = 232448 - 10240;              // of a CTA, less the static part
     static constexpr int kRoom = (kSmemMax / kWarps - kPartial) / kRecord;
     static constexpr int kStages = kRoom > 8 ? 8 : kRoom;        // of one warp's ring
     static constexpr int kRing = kStages * kRecord;
@@ -483,7 +529,7 @@ struct KvSplit {
     int chunks;                     // chunks of query heads per key head
     int row_warps;                  // warps that share a record, each with its own rows (1, 2, 4, 8)
     float* partial;                 // [ctas][2][rows][dim + 3]: numerators of all rows, then (m, big, l) of each
-    int64_t* unit;                  // [ctas][2] unit of each partial, -1: none
+    int64_t* unit;                  // [ctas][2] unit of each partial (sequence << 32 | unit of the sequence), -1: none
     int* more;                      // [ctas] CTAs behind this one that hold parts of its last unit
 };
 
@@ -498,6 +544,10 @@ __device__ __forceinline__ bool kv_span(const KvPool& pool, const KvSeqs& s, int
 __device__ __forceinline__ int kv_records(int lo, int hi) { return hi > lo ? (hi + kKvRecord - 1) / kKvRecord - lo / kKvRecord : 0; }
 
 
+__device__ __forceinline__ int64_t kv_div(int64_t a, int64_t b) {   // not negative; the 32-bit division is far shorter
+    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // A walk over the records of a range, in order: the unit (b, hu) and the record r of its n.
 struct KvWalk {
     int b, hu, r, n, lo, hi;
@@ -505,7 +555,7 @@ struct KvWalk {
     // to the record `at` of all records; i0 / first: a sequence at or before its own, and the records before that
     __device__ __forceinline__ void seek(const KvPool& pool, const KvSeqs& s, int window, int64_t per_seq, int64_t at, int i0,
                                          int64_t first) {
-        const int64_t q = at / per_seq;
+        const int64_t q = kv_div(at, per_seq);
         for (b = i0;; ++b) {
             kv_span(pool, s, window, b, lo, hi);
             n = kv_records(lo, hi);
@@ -513,7 +563,7 @@ struct KvWalk {
             first += n;
         }
         at -= first * per_seq;
-        hu = (int)(at / n);
+        hu = (int)kv_div(at, n);
         r = (int)(at - (int64_t)hu * n);
     }
     // to the first record of the next unit (there is one)
@@ -547,6 +597,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
     __shared__ int64_t s_warp[kWarps];
     __shared__ int64_t s_unit[2 * kWarps];
     __shared__ int s_ends[2 * kWarps];                        // bit 0: the unit begins there, bit 1: it ends there
+    __shared__ int64_t s_until[kWarps];                       // end, among all records, of the unit begun last
     __shared__ __align__(8) uint64_t s_full[kWarps][kMaxStages], s_empty[kWarps][kMaxStages];
     __shared__ uint8_t s_ok[kWarps][kMaxStages];              // whether the record could be fetched
     __shared__ int s_abort, s_drain[kWarps];
@@ -577,6 +628,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
     if (lane == 31) s_warp[warp] = upto;
     if (tid < 2 * kWarps) s_unit[tid] = -1;
     if (tid == 0) s_abort = 0;
+    if (tid < 2) split.unit[2 * (int64_t)blockIdx.x + tid] = -1;
     if (rw == 0 && lane < stages) {
         mbar_init(smem_u32(&s_full[team][lane]), 1);
         mbar_init(smem_u32(&s_empty[team][lane]), split.row_warps);
@@ -592,15 +644,17 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
     s_before[tid] = base + upto - mine;
     __syncthreads();
     total *= per_seq;
-    const int64_t part = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kKvMinRecords);
+    const int64_t part = max(kv_div(total + gridDim.x - 1, gridDim.x), (int64_t)kKvMinRecords);
     const int64_t c0 = min((int64_t)blockIdx.x * part, total), c1 = min(c0 + part, total);
-    const int64_t tpart = (c1 - c0 + teams - 1) / teams;
+    const int64_t tpart = kv_div(c1 - c0 + teams - 1, teams);
     const int64_t t0 = min(c0 + team * tpart, c1), t1 = min(t0 + tpart, c1);
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (t1 > t0) {
         KvWalk at;
         {
-            const int64_t q = t0 / per_seq;
+            const int64_t q = kv_div(t0, per_seq);
             constexpr int kStep = kThreads / 32;
             int i = 31 - __clz(__ballot_sync(0xffffffffu, s_before[lane * kStep] <= q));
             i = i * kStep + 31 - __clz(__ballot_sync(0xffffffffu, lane < kStep && s_before[min(i * kStep + lane, kThreads - 1)] <= q));
@@ -651,6 +705,12 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
                 }
             }
         };
+        KvWarp<FMT, NB, RT> w;
+        auto ask_query = [&]() {
+            const int h = at.hu / split.chunks, row0 = (at.hu - h * split.chunks) * chunk_rows + rw * kRows;
+            w.load_query(a, (int64_t)at.b * a.seq_stride + (int64_t)h * a.group * a.head_stride, row0, a.group, lane);
+        };
+        ask_query();
         if (rw == 0) {
             enter_unit();
             for (int i = 0; i < stages; ++i) fetch(i);
@@ -662,13 +722,12 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
         uint32_t dead_phase = 0;
         int64_t left = t1 - t0;
         const uint8_t* ring = smem + team * split.row_warps * Shape::kRing;
-        KvWarp<FMT, NB, RT> w;
         while (true) {
             const int b = at.b, seg = (int)min((int64_t)(at.n - at.r), left);
             const bool begins = at.r == 0, ends = at.r + seg == at.n;
             const int h = at.hu / split.chunks, row0 = (at.hu - h * split.chunks) * chunk_rows + rw * kRows;
             w.reset();
-            w.load_query(a, (int64_t)b * a.seq_stride + (int64_t)h * a.group * a.head_stride, row0, a.group, lane);
+            w.convert_query(a);
             int first = (at.lo / kKvRecord + at.r) * kKvRecord;   // position of the record's first token
             for (int j = 0; j < seg; ++j, first += kKvRecord) {
                 alive = alive && mbar_wait(smem_u32(&s_full[team][stage]), phase, &s_abort);
@@ -711,13 +770,15 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
                 float* rows = slot_rows(warp, which);
                 w.store_partial(rows, rows + kRows * D, lane);
                 if (lane == 0) {
-                    s_unit[2 * warp + which] = (int64_t)b * per_seq + at.hu;
+                    s_unit[2 * warp + which] = (int64_t)b << 32 | at.hu;
                     s_ends[2 * warp + which] = (begins ? 1 : 0) | (ends ? 2 : 0);
+                    if (begins) s_until[warp] = t1 - seg + at.n;   // (it is the range's last segment)
                 }
             }
             left -= seg;
             if (left == 0) break;
             at.next_unit(pool, seqs, a.window, per_seq);
+            ask_query();
         }
         if (!alive && lane == 0) {
             atomicExch(status, kStatusPipelineTimeout);
@@ -730,77 +791,78 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
     }
     __syncthreads();
 
-    // ---- join of the CTA's partial results: runs of equal units, in order
-    if (tid < 2) split.unit[2 * (int64_t)blockIdx.x + tid] = -1;
-    __syncthreads();
-    const int slots = 2 * teams;
-    auto slot_of = [&](int e, int k) { return 2 * ((e >> 1) * split.row_warps + k) + (e & 1); };   // entry e, row warp k
-    for (int e = 0; e < slots; ++e) {
-        const int64_t u = s_unit[slot_of(e, 0)];
-        if (u < 0) continue;
-        int e1 = e + 1, ends = s_ends[slot_of(e, 0)];
-        for (; e1 < slots; ++e1) {
-            const int64_t v = s_unit[slot_of(e1, 0)];
-            if (v >= 0 && v != u) break;
-            if (v == u) ends |= s_ends[slot_of(e1, 0)];
-        }
-        const int64_t b = u / per_seq;
-        const int hu = (int)(u - b * per_seq), h = hu / split.chunks, row0 = (hu - h * split.chunks) * chunk_rows;
-        const int which = ends & 1;
-        float* po = split.partial + (2 * (int64_t)blockIdx.x + which) * chunk_rows * (D + 3);
-        float* ps = po + chunk_rows * D;
-        for (int i = tid; i < chunk_rows * (D / 4); i += kThreads) {
-            const int row = i / (D / 4), d = 4 * (i - row * (D / 4)), k = row / kRows, in = row - k * kRows;
-            float m = kKvMaxInit, big = kKvMaxInit;
-            for (int f = e; f < e1; ++f) {
-                const int sl = slot_of(f, k);
-                if (s_unit[sl] < 0) continue;
-                const float* st = slot_rows(sl >> 1, sl & 1) + kRows * D + 3 * in;
-                m = fmaxf(m, st[0]);
-                big = fmaxf(big, st[1]);
-            }
-            float l = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int f = e; f < e1; ++f) {
-                const int sl = slot_of(f, k);
-                if (s_unit[sl] < 0) continue;
-                const float* rows = slot_rows(sl >> 1, sl & 1);
-                const float* st = rows + kRows * D + 3 * in;
-                l += st[2] * ex2(st[0] - m);
-                const float c = ex2(st[1] - big);
-                const float4 y = *reinterpret_cast<const float4*>(rows + in * D + d);
-                o.x = fmaf(y.x, c, o.x), o.y = fmaf(y.y, c, o.y), o.z = fmaf(y.z, c, o.z), o.w = fmaf(y.w, c, o.w);
-            }
-            if (ends == 3) {
-                if (row0 + row < a.group) {
-                    const int64_t out_row = b * a.q_heads + (int64_t)h * a.group + row0 + row;
-                    const KvQuotient f(l, big, m);
-                    const float y[4] = {f(o.x), f(o.y), f(o.z), f(o.w)};
-                    store_row<4>(a.out, out_row * D + d, a.type, a.out_vec, y);
-                    if (d == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
+    // ---- join of the CTA's partial results: runs of equal units among the teams' slots, in order.  Lane e looks at slot e
+    // % 2 of team e / 2; one warp joins one row of a run.
+    {
+        auto slot_of = [&](int e, int k) { return 2 * ((e >> 1) * split.row_warps + k) + (e & 1); };   // entry e, row warp k
+        const int mine_at = slot_of(min(lane, 2 * teams - 1), 0);
+        const int64_t unit = lane < 2 * teams ? s_unit[mine_at] : -1;
+        const uint32_t valid = __ballot_sync(0xffffffffu, unit >= 0), before = valid & ((1u << lane) - 1u);
+        const int64_t last = __shfl_sync(0xffffffffu, unit, before ? 31 - __clz(before) : 0);
+        const uint32_t starts = __ballot_sync(0xffffffffu, unit >= 0 && (before == 0 || last != unit));
+        const uint32_t begun = __ballot_sync(0xffffffffu, unit >= 0 && (s_ends[mine_at] & 1)),
+                       ended = __ballot_sync(0xffffffffu, unit >= 0 && (s_ends[mine_at] & 2));
+        const int runs = __popc(starts);
+        for (int item = warp; item < runs * chunk_rows; item += kWarps) {
+            const int run = item / chunk_rows, row = item - run * chunk_rows, k = row / kRows, in = row - k * kRows;
+            uint32_t rest = starts;
+            for (int i = 0; i < run; ++i) rest &= rest - 1;
+            const int e0 = __ffs(rest) - 1;
+            rest &= rest - 1;
+            const uint32_t members = valid & ~((1u << e0) - 1u) & (rest ? (rest & -rest) - 1u : 0xffffffffu);
+            const int64_t u = __shfl_sync(0xffffffffu, unit, e0);
+            const int b = (int)(u >> 32), hu = (int)u, h = hu / split.chunks, row0 = (hu - h * split.chunks) * chunk_rows;
+            const bool whole = (begun & members) && (ended & members);
+            if (whole && row0 + row >= a.group) continue;
+            const bool member = members >> lane & 1u;
+            const int sl = slot_of(member ? lane : e0, k);
+            const float* st = slot_rows(sl >> 1, sl & 1) + kRows * D + 3 * in;
+            const float m = warp_max(st[0]), big = warp_max(st[1]);
+            const float l = warp_sum(member ? st[2] * ex2(st[0] - m) : 0.f);
+            const float c = ex2(st[1] - big);
+            constexpr int kQuads = (D + 127) / 128;
+            float4 o[kQuads];
+#pragma unroll
+            for (int i = 0; i < kQuads; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (uint32_t left = members; left; left &= left - 1) {
+                const int e = __ffs(left) - 1, se = slot_of(e, k);
+                const float f = __shfl_sync(0xffffffffu, c, e);
+                const float* rows = slot_rows(se >> 1, se & 1) + in * D;
+#pragma unroll
+                for (int i = 0; i < kQuads; ++i) {
+                    const int d = 4 * lane + 128 * i;
+                    if (d >= D) continue;
+                    const float4 y = *reinterpret_cast<const float4*>(rows + d);
+                    o[i].x = fmaf(y.x, f, o[i].x), o[i].y = fmaf(y.y, f, o[i].y), o[i].z = fmaf(y.z, f, o[i].z), o[i].w = fmaf(y.w, f, o[i].w);
                 }
+            }
+            if (whole) {
+                const int64_t out_row = (int64_t)b * a.q_heads + (int64_t)h * a.group + row0 + row;
+                const KvQuotient f(l, big, m);
+#pragma unroll
+                for (int i = 0; i < kQuads; ++i) {
+                    const int d = 4 * lane + 128 * i;
+                    const float y[4] = {f(o[i].x), f(o[i].y), f(o[i].z), f(o[i].w)};
+                    if (d < D) store_row<4>(a.out, out_row * D + d, a.type, a.out_vec, y);
+                }
+                if (lane == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
             } else {
-                *reinterpret_cast<float4*>(po + row * D + d) = o;
-                if (d == 0) ps[3 * row] = m, ps[3 * row + 1] = big, ps[3 * row + 2] = l;
-            }
-        }
-        if (ends != 3 && tid == 0) {
-            split.unit[2 * (int64_t)blockIdx.x + which] = u;
-            if (which == 1) {
-                // CTA of the unit's last record
-                int lo, hi;
-                kv_span(pool, seqs, a.window, (int)b, lo, hi);
-                const int n = kv_records(lo, hi);
-                int64_t first = s_before[b / per];
-                for (int64_t i = b / per * per; i < b; ++i) {
-                    int l2, h2;
-                    kv_span(pool, seqs, a.window, (int)i, l2, h2);
-                    first += kv_records(l2, h2);
+                const int which = begun & members ? 1 : 0;
+                float* po = split.partial + (2 * (int64_t)blockIdx.x + which) * chunk_rows * (D + 3);
+#pragma unroll
+                for (int i = 0; i < kQuads; ++i)
+                    if (4 * lane + 128 * i < D) *reinterpret_cast<float4*>(po + row * D + 4 * lane + 128 * i) = o[i];
+                if (lane == 0) {
+                    float* ps = po + chunk_rows * D + 3 * row;
+                    ps[0] = m, ps[1] = big, ps[2] = l;
+                    if (row == 0) {
+                        split.unit[2 * (int64_t)blockIdx.x + which] = u;
+                        // CTA of the unit's last record
+                        if (which) split.more[blockIdx.x] = (int)kv_div(s_until[slot_of(e0, 0) >> 1] - 1, part) - (int)blockIdx.x;
+                    }
                 }
-                split.more[blockIdx.x] = (int)((first * per_seq + (int64_t)(hu + 1) * n - 1) / part) - (int)blockIdx.x;
             }
         }
-        e = e1 - 1;
     }
 
     // ---- sequences with nothing to attend to
@@ -816,42 +878,59 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
     }
 }
 
-// Units that several CTAs hold parts of: block (c, y) joins rows of the unit that begins in CTA c and goes on behind it.
+// Units that several CTAs hold parts of: warp (c, row) joins a row of the unit that begins in CTA c and goes on behind it.
 template <int NB>
 __global__ void __launch_bounds__(kKvJoinThreads) kv_join_kernel(KvPool pool, KvAttend a, KvSplit split, int chunk_rows) {
-    constexpr int D = 32 * NB, kD4 = D / 4;
-    const int c = blockIdx.x;
+    constexpr int D = 32 * NB, kQuads = (D + 127) / 128;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // the attention kernel's results
+    const int c = blockIdx.x, lane = threadIdx.x & 31, row = blockIdx.y * (kKvJoinThreads / 32) + (threadIdx.x >> 5);
     const int64_t u = split.unit[2 * (int64_t)c + 1];
-    if (u < 0) return;
+    if (u < 0 || row >= chunk_rows) return;
     const int more = split.more[c];
-    const int64_t per_seq = (int64_t)pool.heads * split.chunks, b = u / per_seq;
-    const int hu = (int)(u - b * per_seq), h = hu / split.chunks, row0 = (hu - h * split.chunks) * chunk_rows;
-    const int i = blockIdx.y * kKvJoinThreads + threadIdx.x, row = i / kD4, d = 4 * (i - row * kD4);
-    if (row >= chunk_rows || row0 + row >= a.group) return;
+    const int b = (int)(u >> 32), hu = (int)u, h = hu / split.chunks, row0 = (hu - h * split.chunks) * chunk_rows;
+    if (row0 + row >= a.group) return;
     const int64_t stride = (int64_t)chunk_rows * (D + 3);
     auto part = [&](int k) { return split.partial + (2 * (int64_t)(c + k) + (k == 0 ? 1 : 0)) * stride; };
     float m = kKvMaxInit, big = kKvMaxInit;
-#pragma unroll 4
-    for (int k = 0; k <= more; ++k) {
+    for (int k = lane; k <= more; k += 32) {
         const float* s = part(k) + chunk_rows * D + 3 * row;
         m = fmaxf(m, s[0]);
         big = fmaxf(big, s[1]);
     }
+    m = warp_max(m);
+    big = warp_max(big);
     float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int k = 0; k <= more; ++k) {
-        const float* s = part(k) + chunk_rows * D + 3 * row;
-        const float4 y = *reinterpret_cast<const float4*>(part(k) + row * D + d);
-        l += s[2] * ex2(s[0] - m);
+    float4 o[kQuads];
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 <= more; k0 += 32) {
+        const float* s = part(min(k0 + lane, more)) + chunk_rows * D + 3 * row;
         const float f = ex2(s[1] - big);
-        o.x = fmaf(y.x, f, o.x), o.y = fmaf(y.y, f, o.y), o.z = fmaf(y.z, f, o.z), o.w = fmaf(y.w, f, o.w);
+        if (k0 + lane <= more) l += s[2] * ex2(s[0] - m);
+        const int n = min(32, more + 1 - k0);
+#pragma unroll 8
+        for (int k = 0; k < n; ++k) {
+            const float fk = __shfl_sync(0xffffffffu, f, k);
+            const float* rows = part(k0 + k) + row * D;
+#pragma unroll
+            for (int i = 0; i < kQuads; ++i) {
+                const int d = 4 * lane + 128 * i;
+                if (d >= D) continue;
+                const float4 y = *reinterpret_cast<const float4*>(rows + d);
+                o[i].x = fmaf(y.x, fk, o[i].x), o[i].y = fmaf(y.y, fk, o[i].y), o[i].z = fmaf(y.z, fk, o[i].z), o[i].w = fmaf(y.w, fk, o[i].w);
+            }
+        }
     }
-    const int64_t out_row = b * a.q_heads + (int64_t)h * a.group + row0 + row;
+    l = warp_sum(l);
+    const int64_t out_row = (int64_t)b * a.q_heads + (int64_t)h * a.group + row0 + row;
     const KvQuotient f(l, big, m);
-    const float y[4] = {f(o.x), f(o.y), f(o.z), f(o.w)};
-    store_row<4>(a.out, out_row * D + d, a.type, a.out_vec, y);
-    if (d == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+        const int d = 4 * lane + 128 * i;
+        const float y[4] = {f(o[i].x), f(o[i].y), f(o[i].z), f(o[i].w)};
+        if (d < D) store_row<4>(a.out, out_row * D + d, a.type, a.out_vec, y);
+    }
+    if (lane == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
 }
 
 template <int FMT, int NB, int RT>
@@ -871,8 +950,17 @@ struct KvAttendInstance {
         split.more = work.more;
         split.partial = work.partial;
         kv_attend_kernel<FMT, NB, RT><<<work.ctas, Shape::kThreads, Shape::kSmem, stream>>>(pool, seqs, a, split, status);
-        kv_join_kernel<NB><<<dim3(work.ctas, (chunk_rows * 8 * NB + kKvJoinThreads - 1) / kKvJoinThreads), kKvJoinThreads, 0, stream>>>(
-            pool, a, split, chunk_rows);
+        // the join's CTAs start as those of the attention kernel end (programmatic launch), and wait for the last of them
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(work.ctas, (chunk_rows + kKvJoinThreads / 32 - 1) / (kKvJoinThreads / 32));
+        cfg.blockDim = dim3(kKvJoinThreads);
+        cfg.stream = stream;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        cudaLaunchKernelEx(&cfg, kv_join_kernel<NB>, pool, a, split, chunk_rows);
         return 2;
     }
 };
