@@ -3780,6 +3780,7 @@ int eos_b200_kv_cache_create(EosB200Runtime* rt, int64_t pages, int page_size, i
     cudaError_t e = dev_alloc(&p.base, (size_t)(pages * page_bytes));
     c->pool = p;
     if (e == cudaSuccess) e = dev_alloc(&c->work.partial, kv_work_floats(rt->sm_count, head_dim));
+    if (e == cudaSuccess) e = dev_alloc(&c->work.slots, (size_t)rt->sm_count * kKvSlotFloats);
     if (e == cudaSuccess) e = dev_alloc(&c->work.unit, (size_t)2 * rt->sm_count);
     if (e == cudaSuccess) e = dev_alloc(&c->work.more, (size_t)rt->sm_count);
     if (e == cudaSuccess) e = cudaMemsetAsync(p.base, 0, (size_t)(pages * page_bytes), rt->stream);
@@ -3797,6 +3798,7 @@ void eos_b200_kv_cache_destroy(EosB200KvCache* c) {
     if (c == nullptr) return;
     cudaSetDevice(c->rt->device);
     dev_free(c->pool.base);
+    dev_free(c->work.slots);
     dev_free(c->work.partial);
     dev_free(c->work.unit);
     dev_free(c->work.more);

@@ -3,11 +3,16 @@
 //
 //     out = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),   x_j = scale log2(e) q . k_j,   one pass with a running maximum m
 //
-// A warp takes one record (16 tokens of one key head) at a time with mma.sync m16n8k16: the query heads that share the
-// key head are the rows.  At most 8 heads use a tile's 16 rows: rows 0-7 hold the upper half of every fp32 factor
-// (query or weight) and rows 8-15 what the rounding to 16 bits left over, so the products carry 22 bits (f16 operands)
-// at no extra instruction -- each thread finds both halves of its sums in its own registers.  The factor is split, not
-// the cached value, which is exact in its operand type.
+// A warp takes one or two records (16 tokens of one key head each) at a time with mma.sync m16n8k16, and both products are
+// formed transposed: S^T = K q^T with the tokens as the 16 rows and 8 query heads of the key head as the columns, then
+// O^T += V^T P^T with 16 elements of the values as the rows.  The few query heads that share a key head fill the narrow
+// side of the instruction, keys and values its wide one, and the accumulators take half of what heads as rows would.
+// (tcgen05 wants 128 rows of keys in shared memory, in an operand type: the conversion of the codes would have to be
+// written back there first, and the weights once more through it; the kernel is bound by HBM and by the conversions.)
+//
+// Every fp32 factor -- the weights, and a query that does not fit the operand type (fp32, or f16 over a bf16 cache) -- is
+// the sum of two 16-bit operands, so the products carry 22 bits (bf16: 16).  The cached value is never split: it is exact
+// in its operand type.
 //
 // The maxima are integers, and lag: m is set 7 below the largest score and moves only when a score passes m + 15, so most
 // records do no rescaling and no shuffles, and weights use f16's range from both ends: they stay below 2^15, and what
@@ -16,6 +21,8 @@
 // the bound holds whatever the scales; the blocks' own exponents, relative to e, are f16 factors of the split weights
 // (four multiplications a block where scaling the codes takes eight), so the codes enter the mma as they are.
 #pragma once
+#include <algorithm>
+
 #include "kv_dev.cuh"
 
 namespace eosb {
@@ -83,6 +90,13 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint3
     }
 }
 
+// transposes an 8 x 8 matrix of 16-bit values held by a warp (lane 4 g + t: row g, columns 2t and 2t+1)
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+    return r;
+}
+
 // The bytes of one lane at `plane0`, BYTES of them (see kv_lane_offset)
 template <int BYTES>
 __device__ __forceinline__ void load_lane(const uint8_t* plane0, int lane, uint32_t (&w)[BYTES / 4]) {
@@ -100,21 +114,15 @@ __device__ __forceinline__ void load_lane(const uint8_t* plane0, int lane, uint3
         w[BYTES / 4 - 1] = *reinterpret_cast<const uint32_t*>(plane0 + p * 32 + (r >= 8 ? 256 : 0) + lane * 4);
 }
 
-// Scale bytes of two neighbouring tokens, packed four to a word
+// Scale bytes of one token's key, packed four to a word
 template <int NB>
-__device__ __forceinline__ void load_scales(const uint8_t* p, uint32_t (&a)[(NB + 3) / 4], uint32_t (&b)[(NB + 3) / 4]) {
-    if constexpr (NB == 1) {
-        const uint32_t w = *reinterpret_cast<const uint16_t*>(p);
-        a[0] = w & 0xffu, b[0] = w >> 8;
-    } else if constexpr (NB == 2) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
-        a[0] = w & 0xffffu, b[0] = w >> 16;
-    } else if constexpr (NB <= 4) {
+__device__ __forceinline__ void load_scales(const uint8_t* p, uint32_t (&a)[(NB + 3) / 4]) {
+    if constexpr (NB == 1) a[0] = *p;
+    else if constexpr (NB == 2) a[0] = *reinterpret_cast<const uint16_t*>(p);
+    else if constexpr (NB <= 4) a[0] = *reinterpret_cast<const uint32_t*>(p);
+    else {
         const uint2 w = *reinterpret_cast<const uint2*>(p);
-        a[0] = w.x, b[0] = w.y;
-    } else {
-        const uint4 w = *reinterpret_cast<const uint4*>(p);
-        a[0] = w.x, a[1] = w.y, b[0] = w.z, b[1] = w.w;
+        a[0] = w.x, a[1] = w.y;
     }
 }
 // Scale bytes of a token pair's values: block b in byte 2 (b % 2) (first token) and the next (second) of word b / 2
@@ -138,23 +146,27 @@ __device__ __forceinline__ float scale_at(uint32_t word, int i) {
                                             : (i == 1 ? (word << 15) & 0x7f800000u : (word << 23) & 0x7f800000u)));
 }
 
-template <int FMT, int NB, int RT>
+// RT: tiles of 8 query heads; HALVES: operands of the query (1: its type fits the operand type).
+template <int FMT, int NB, int RT, int HALVES>
 struct KvWarp {
     static constexpr bool kMx = FMT >= kKvMx8, kBf = FMT == kKvBf16;
     static constexpr int KP = kv_key_piece(FMT), VP = kv_value_piece(FMT), D = 32 * NB;
 
-    uint32_t q[RT][NB][8];      // per block: 4 upper words, 4 lower words (8 elements of the lane's row)
-    float qs[RT];               // factor of the raw sums: scale log2(e) 2^(query exponent)
-    float m[RT], big[RT], l[RT];   // lagging maxima of x and of x + e (mx formats), this lane's part of the sum of weights
-    float o[RT][4 * NB][4];
+    uint32_t q[RT][NB][4 * HALVES];   // head g of each tile, elements 32 b + 8 t .. + 7: upper halves, then lower ones
+    float qs[RT][2];                  // heads 2t and 2t + 1: factor of the raw sums, scale log2(e) 2^(query exponent)
+    float m[RT][2], big[RT][2];       // lagging maxima of x and of x + e (mx formats)
+    float l[RT][2];                   // this lane's part of the sum of weights
+    float o[RT][NB][2][4];            // [block][i]: elements 32 b + 4 g + 2 i (0, 1) and + 2 i + 1 (2, 3) of heads 2t, 2t + 1
 
     __device__ __forceinline__ void reset() {
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            m[r] = big[r] = kKvMaxInit;
-            l[r] = 0.f;
 #pragma unroll
-            for (int n = 0; n < 4 * NB; ++n) o[r][n][0] = o[r][n][1] = o[r][n][2] = o[r][n][3] = 0.f;
+            for (int i = 0; i < 2; ++i) m[r][i] = big[r][i] = kKvMaxInit, l[r][i] = 0.f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[r][b][i >> 2][i & 3] = 0.f;
         }
     }
 
@@ -162,27 +174,28 @@ struct KvWarp {
     // at once and waited for in convert_query, ...
     __device__ __forceinline__ void load_query(const KvAttend& a, int64_t at, int row0, int rows, int lane) {
         const int g = lane >> 2, t = lane & 3;
+        const bool wide = HALVES == 2 && a.type == kTypeF32;
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             const int row = row0 + 8 * r + g;
-            const int64_t p = at + (int64_t)row * a.head_stride + 8 * t;
-            const uint8_t* base = static_cast<const uint8_t*>(a.query) + p * (a.type == kTypeF32 ? 4 : 2);
-            if (row >= rows) {
+            const uint8_t* base = static_cast<const uint8_t*>(a.query) + (at + (int64_t)row * a.head_stride + 8 * t) * (wide ? 4 : 2);
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) q[r][b][i] = 0u;
-            } else if (a.type == kTypeF32) {
+                for (int i = 0; i < 4 * HALVES; ++i) q[r][b][i] = 0u;
+            if (row >= rows) continue;
+            if (wide) {
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     const uint32_t* w = reinterpret_cast<const uint32_t*>(base) + 32 * b;
-                    if (a.vec) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(w), y = *reinterpret_cast<const uint4*>(w + 4);
-                        q[r][b][0] = x.x, q[r][b][1] = x.y, q[r][b][2] = x.z, q[r][b][3] = x.w;
-                        q[r][b][4] = y.x, q[r][b][5] = y.y, q[r][b][6] = y.z, q[r][b][7] = y.w;
-                    } else {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) q[r][b][i] = w[i];
+                    for (int i = 0; i < 4 * HALVES; i += 4) {
+                        if (a.vec) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(w + i);
+                            q[r][b][i] = x.x, q[r][b][i + 1] = x.y, q[r][b][i + 2] = x.z, q[r][b][i + 3] = x.w;
+                        } else {
+                            q[r][b][i] = w[i], q[r][b][i + 1] = w[i + 1], q[r][b][i + 2] = w[i + 2], q[r][b][i + 3] = w[i + 3];
+                        }
                     }
                 }
             } else {
@@ -200,19 +213,21 @@ struct KvWarp {
             }
         }
     }
-    // ... then the halves.  f16 operands: each row is divided by a power of two first, so that no magnitude leaves f16's range.
-    __device__ __forceinline__ void convert_query(const KvAttend& a) {
+    // ... then the operands.  f16: each row is divided by a power of two first, so that no magnitude leaves f16's range.
+    __device__ __forceinline__ void convert_query(const KvAttend& a, int lane) {
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            if (a.type == kTypeF32) split_row(a, r, [&](int b, int i) { return make_float2(__uint_as_float(q[r][b][2 * i]), __uint_as_float(q[r][b][2 * i + 1])); });
-            else if (a.type == kTypeF16) split_row(a, r, [&](int b, int i) { return f16x2_floats(q[r][b][i]); });
-            else split_row(a, r, [&](int b, int i) { return bf16x2_floats(q[r][b][i]); });
+            if (HALVES == 2 && a.type == kTypeF32)
+                split_row(a, r, lane, [&](int b, int i) {
+                    return make_float2(__uint_as_float(q[r][b][(2 * i) % (4 * HALVES)]), __uint_as_float(q[r][b][(2 * i + 1) % (4 * HALVES)]));
+                });
+            else if (a.type == kTypeF16) split_row(a, r, lane, [&](int b, int i) { return f16x2_floats(q[r][b][i]); });
+            else split_row(a, r, lane, [&](int b, int i) { return bf16x2_floats(q[r][b][i]); });
         }
     }
     template <typename F>
-    __device__ __forceinline__ void split_row(const KvAttend& a, int r, F&& pair) {
-        float inv = 1.f;
-        qs[r] = a.scale_log2;
+    __device__ __forceinline__ void split_row(const KvAttend& a, int r, int lane, F&& pair) {
+        float inv = 1.f, factor = a.scale_log2;
         if constexpr (!kBf) {
             uint32_t top = 0;
 #pragma unroll
@@ -226,259 +241,342 @@ struct KvWarp {
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const uint32_t e = min(max(top >> 23, kKvQueryExp + 1u), 254u);
             inv = __uint_as_float((254u + kKvQueryExp - e) << 23);
-            qs[r] *= __uint_as_float((e - kKvQueryExp) << 23);
+            factor *= __uint_as_float((e - kKvQueryExp) << 23);
         }
+        // the factors of heads 2t and 2t + 1 are those of the lanes with g = 2t and 2t + 1
+        qs[r][0] = __shfl_sync(0xffffffffu, factor, 8 * (lane & 3));
+        qs[r][1] = __shfl_sync(0xffffffffu, factor, 8 * (lane & 3) + 4);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             float2 x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = pair(b, i);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) split_pair<kBf>(x[i].x * inv, x[i].y * inv, q[r][b][i], q[r][b][4 + i]);
+            for (int i = 0; i < 4; ++i) {
+                uint32_t lo;
+                split_pair<kBf>(x[i].x * inv, x[i].y * inv, q[r][b][i], lo);
+                if constexpr (HALVES == 2) q[r][b][4 + i] = lo;
+            }
         }
     }
 
-    __device__ __forceinline__ void scale_rows(int r, float f) {
-        const float2 f2 = make_float2(f, f);
+    __device__ __forceinline__ void scale_rows(int r, float f0, float f1) {
+        const float2 f = make_float2(f0, f1);
 #pragma unroll
-        for (int n = 0; n < 4 * NB; ++n)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-                const float2 y = mul2(make_float2(o[r][n][i], o[r][n][i + 1]), f2);
-                o[r][n][i] = y.x, o[r][n][i + 1] = y.y;
+            for (int i = 0; i < 8; i += 2) {
+                float* c = &o[r][b][i >> 2][i & 3];
+                const float2 y = mul2(make_float2(c[0], c[1]), f);
+                c[0] = y.x, c[1] = y.y;
             }
     }
 
-    // One record; its tokens [lo, hi) of 0..15 count.
-    __device__ __forceinline__ void record(const uint8_t* rec, int lo, int hi, int lane) {
-        const int t = lane & 3;
-        float s[RT][4];   // raw scores of row g: tokens 2t, 2t+1, 2t+8, 2t+9
+    // Raw scores of a record's tokens g (0, 1) and g + 8 (2, 3) with heads 2t, 2t + 1.
+    __device__ __forceinline__ void scores(const uint8_t* rec, float (&s)[RT][4], int lane) const {
+        const int g = lane >> 2;
+        if constexpr (!kMx) {
+            uint32_t k[NB * 8];
+            load_lane<NB * 32>(rec, lane, k);
+            float c[RT][2][4];   // two sums: chains of dependent mma half as long
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            uint32_t k[NB * KP / 4];
-            load_lane<NB * KP>(rec + j * 32 * NB * KP, lane, k);
-            if constexpr (!kMx) {
-                float c[RT][4];
+            for (int r = 0; r < RT; ++r)
 #pragma unroll
-                for (int r = 0; r < RT; ++r) c[r][0] = c[r][1] = c[r][2] = c[r][3] = 0.f;
+                for (int i = 0; i < 8; ++i) c[r][i >> 2][i & 3] = 0.f;
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int r = 0; r < RT; ++r)
-                            mma_16x8x16<kBf>(c[r], q[r][b][2 * i], q[r][b][4 + 2 * i], q[r][b][2 * i + 1],
-                                             q[r][b][4 + 2 * i + 1], k[4 * b + 2 * i], k[4 * b + 2 * i + 1]);
+                            mma_16x8x16<kBf>(c[r][i], k[8 * b + 4 * i], k[8 * b + 4 * i + 1], k[8 * b + 4 * i + 2], k[8 * b + 4 * i + 3],
+                                             q[r][b][4 * h + 2 * i], q[r][b][4 * h + 2 * i + 1]);
 #pragma unroll
-                for (int r = 0; r < RT; ++r) s[r][2 * j] = c[r][0] + c[r][2], s[r][2 * j + 1] = c[r][1] + c[r][3];
-            } else {
-                uint32_t sa[(NB + 3) / 4], sb[(NB + 3) / 4];
-                load_scales<NB>(rec + kv_key_scale_offset(FMT, NB) + (8 * j + 2 * t) * kv_scale_stride(NB), sa, sb);
-                float2 sum[RT];
+            for (int r = 0; r < RT; ++r)
 #pragma unroll
-                for (int r = 0; r < RT; ++r) sum[r] = make_float2(0.f, 0.f);
+                for (int i = 0; i < 4; ++i) s[r][i] = c[r][0][i] + c[r][1][i];
+        } else {
+            uint32_t k0[NB * KP / 4], k1[NB * KP / 4], e0[(NB + 3) / 4], e1[(NB + 3) / 4];
+            load_lane<NB * KP>(rec, lane, k0);
+            load_lane<NB * KP>(rec + 32 * NB * KP, lane, k1);
+            load_scales<NB>(rec + kv_key_scale_offset(FMT, NB) + g * kv_scale_stride(NB), e0);
+            load_scales<NB>(rec + kv_key_scale_offset(FMT, NB) + (g + 8) * kv_scale_stride(NB), e1);
+            float2 sum[RT][2];
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    uint32_t f[4];
-                    if constexpr (FMT == kKvMx8) {
-                        f16_of_e4m3x4(k[2 * b], f[0], f[1]);
-                        f16_of_e4m3x4(k[2 * b + 1], f[2], f[3]);
-                    } else {
-                        f16_of_e2m1x8(k[b], f[0], f[1], f[2], f[3]);
-                    }
-                    const float2 scale = make_float2(scale_at(sa[b / 4], b & 3), scale_at(sb[b / 4], b & 3));
+            for (int r = 0; r < RT; ++r) sum[r][0] = sum[r][1] = make_float2(0.f, 0.f);
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) {
-                        float c[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma_16x8x16<false>(c, q[r][b][0], q[r][b][4], q[r][b][1], q[r][b][5], f[0], f[1]);
-                        mma_16x8x16<false>(c, q[r][b][2], q[r][b][6], q[r][b][3], q[r][b][7], f[2], f[3]);
-                        sum[r] = fma2(add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), scale, sum[r]);
-                    }
+            for (int b = 0; b < NB; ++b) {
+                uint32_t f[4], h[4];   // elements 8 t .. + 7 of tokens g and g + 8
+                if constexpr (FMT == kKvMx8) {
+                    f16_of_e4m3x4(k0[2 * b], f[0], f[1]);
+                    f16_of_e4m3x4(k0[2 * b + 1], f[2], f[3]);
+                    f16_of_e4m3x4(k1[2 * b], h[0], h[1]);
+                    f16_of_e4m3x4(k1[2 * b + 1], h[2], h[3]);
+                } else {
+                    f16_of_e2m1x8(k0[b], f[0], f[1], f[2], f[3]);
+                    f16_of_e2m1x8(k1[b], h[0], h[1], h[2], h[3]);
                 }
+                const float s0 = scale_at(e0[b / 4], b & 3), s1 = scale_at(e1[b / 4], b & 3);
 #pragma unroll
-                for (int r = 0; r < RT; ++r) s[r][2 * j] = sum[r].x, s[r][2 * j + 1] = sum[r].y;
-            }
-        }
-        const bool edge = lo > 0 || hi < kKvRecord;
-        uint32_t live = 15u;
-        if (edge) {
-            live = 0;
+                for (int r = 0; r < RT; ++r) {
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int tok = 2 * t + (i & 1) + 8 * (i >> 1);
-                if (tok >= lo && tok < hi) live |= 1u << i;
+                    for (int u = 0; u < HALVES; ++u) {
+                        mma_16x8x16<false>(c, f[0], h[0], f[1], h[1], q[r][b][4 * u], q[r][b][4 * u + 1]);
+                        mma_16x8x16<false>(c, f[2], h[2], f[3], h[3], q[r][b][4 * u + 2], q[r][b][4 * u + 3]);
+                    }
+                    sum[r][0] = fma2(make_float2(c[0], c[1]), make_float2(s0, s0), sum[r][0]);
+                    sum[r][1] = fma2(make_float2(c[2], c[3]), make_float2(s1, s1), sum[r][1]);
+                }
             }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) s[r][0] = sum[r][0].x, s[r][1] = sum[r][0].y, s[r][2] = sum[r][1].x, s[r][3] = sum[r][1].y;
         }
-        // value scales: largest exponent of each token, and every block's relative to it as f16 pairs
-        float te[4];
-        uint32_t rel[2][NB];
-        if constexpr (kMx) {
-            uint32_t tops[2], odd = 0;
+    }
+
+    // A record's value scales: every block's exponent relative to the largest of its token, as f16 pairs of the tokens 2t,
+    // 2t + 1 and 2t + 8, 2t + 9 (zero for tokens outside [lo, hi)).
+    __device__ __forceinline__ void value_scales(const uint8_t* rec, bool edge, int lo, int hi, uint32_t (&rel)[2][NB], int lane) const {
+        const int t = lane & 3;
+        uint32_t tops[2], odd = 0;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            uint32_t w[(NB + 1) / 2];
+            load_pair_scales<NB>(rec + kv_value_scale_offset(FMT, NB) + (t + 4 * p) * 2 * kv_scale_stride(NB), w);
+            tops[p] = *reinterpret_cast<const uint32_t*>(rec + kv_value_top_offset(FMT, NB) + 4 * (t + 4 * p));
+            odd |= tops[p];
+            // bytes 60 - 4 (top - e): with zeros below them, the f16 numbers 2^(e - top), top - e <= 14
+            const uint32_t c = 0x3c3c3c3cu - __byte_perm(tops[p], 0, 0x1010) * 4u;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) rel[p][b] = __byte_perm(w[b / 2] * 4u + c, 0, b & 1 ? 0x3424 : 0x1404);
+        }
+        if (__any_sync(0xffffffffu, (odd & 0xffff0000u) != 0u)) {
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 uint32_t w[(NB + 1) / 2];
                 load_pair_scales<NB>(rec + kv_value_scale_offset(FMT, NB) + (t + 4 * p) * 2 * kv_scale_stride(NB), w);
-                tops[p] = *reinterpret_cast<const uint32_t*>(rec + kv_value_top_offset(FMT, NB) + 4 * (t + 4 * p));
-                odd |= tops[p];
-                // bytes 60 - 4 (top - e): with zeros below them, the f16 numbers 2^(e - top), top - e <= 14
-                const uint32_t c = 0x3c3c3c3cu - __byte_perm(tops[p], 0, 0x1010) * 4u;
 #pragma unroll
-                for (int b = 0; b < NB; ++b) rel[p][b] = __byte_perm(w[b / 2] * 4u + c, 0, b & 1 ? 0x3424 : 0x1404);
-                // the top bytes as floats, by way of the integers behind 2^23
-                te[2 * p] = __uint_as_float(__byte_perm(tops[p], 0x4b000000u, 0x7440)) - 8388735.f;
-                te[2 * p + 1] = __uint_as_float(__byte_perm(tops[p], 0x4b000000u, 0x7441)) - 8388735.f;
-            }
-            if (__any_sync(0xffffffffu, (odd & 0xffff0000u) != 0u)) {
+                for (int b = 0; b < NB; ++b) {
+                    float f[2];
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    uint32_t w[(NB + 1) / 2];
-                    load_pair_scales<NB>(rec + kv_value_scale_offset(FMT, NB) + (t + 4 * p) * 2 * kv_scale_stride(NB), w);
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        float f[2];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const int e = (int)(w[b / 2] >> (16 * (b & 1) + 8 * i) & 0xffu), top = (int)(tops[p] >> (8 * i) & 0xffu);
-                            f[i] = e == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)max(e - top + 127, 0) << 23);
-                        }
-                        rel[p][b] = f16x2_of(f[0], f[1]);   // zero below 2^-25
+                    for (int i = 0; i < 2; ++i) {
+                        const int e = (int)(w[b / 2] >> (16 * (b & 1) + 8 * i) & 0xffu), top = (int)(tops[p] >> (8 * i) & 0xffu);
+                        f[i] = e == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)max(e - top + 127, 0) << 23);
                     }
+                    rel[p][b] = f16x2_of(f[0], f[1]);   // zero below 2^-25
                 }
             }
-            if (edge) {   // what lies in the places that do not count may be anything
+        }
+        if (edge) {   // what lies in the places that do not count may be anything
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
+            for (int p = 0; p < 2; ++p) {
+                const uint32_t keep = live_pair(t, p, lo, hi);
 #pragma unroll
-                    for (int p = 0; p < 2; ++p)
-                        rel[p][b] &= (live >> (2 * p) & 1u ? 0xffffu : 0u) | (live >> (2 * p) & 2u ? 0xffff0000u : 0u);
+                for (int b = 0; b < NB; ++b) rel[p][b] &= keep;
             }
         }
-        // softmax
-        uint32_t whi[RT][2], wlo[RT][2];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            float x[4];   // exponents of the weights
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[i] = fmaf(s[r][i], qs[r], -m[r]);
-                if (edge && !(live >> i & 1u)) x[i] = -INFINITY;
-            }
-            if (__any_sync(0xffffffffu, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > kKvLag)) {
-                // from the scores: the first time, m is far below them and their differences are lost in x
-                float most = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (!edge || (live >> i & 1u)) most = fmaxf(most, s[r][i] * qs[r]);
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                const float to = most - m[r] > kKvLag ? ceilf(most) - kKvHead : m[r], f = ex2(m[r] - to);
-                m[r] = to;
-                l[r] *= f;
-                if constexpr (!kMx) scale_rows(r, f);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = edge && !(live >> i & 1u) ? -INFINITY : fmaf(s[r][i], qs[r], -to);
-            }
-            float w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = ex2(x[i]);
-            l[r] += (w[0] + w[1]) + (w[2] + w[3]);
-            if constexpr (kMx) {
-                float y[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    y[i] = fmaf(s[r][i], qs[r], te[i] - big[r]);
-                    if (edge && !(live >> i & 1u)) y[i] = -INFINITY;
-                }
-                if (__any_sync(0xffffffffu, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) > kKvLag)) {
-                    float most = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!edge || (live >> i & 1u)) most = fmaxf(most, fmaf(s[r][i], qs[r], te[i]));
-                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                    const float to = most - big[r] > kKvLag ? ceilf(most) - kKvHead : big[r];
-                    scale_rows(r, ex2(big[r] - to));
-                    big[r] = to;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] = edge && !(live >> i & 1u) ? -INFINITY : fmaf(s[r][i], qs[r], te[i] - to);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = ex2(y[i]);
-            }
-            split_pair<kBf>(w[0], w[1], whi[r][0], wlo[r][0]);
-            split_pair<kBf>(w[2], w[3], whi[r][1], wlo[r][1]);
-        }
-        // values
-        uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-        if (!kMx && edge) {
-            keep0 = (live & 1 ? 0xffffu : 0u) | (live & 2 ? 0xffff0000u : 0u);
-            keep1 = (live & 4 ? 0xffffu : 0u) | (live & 8 ? 0xffff0000u : 0u);
-        }
+    }
+    // mask of the f16 pair of tokens 2t + 8 p and the next
+    __device__ static __forceinline__ uint32_t live_pair(int t, int p, int lo, int hi) {
+        const int tok = 2 * t + 8 * p;
+        return (tok >= lo && tok < hi ? 0xffffu : 0u) | (tok + 1 >= lo && tok + 1 < hi ? 0xffff0000u : 0u);
+    }
+
+    // Adds a record's values; weights as pairs of the tokens 2t, 2t + 1 (0) and 2t + 8, 2t + 9 (1) of head g.
+    __device__ __forceinline__ void values(const uint8_t* rec, bool edge, int lo, int hi, const uint32_t (&whi)[RT][2],
+                                           const uint32_t (&wlo)[RT][2], const uint32_t (&rel)[2][NB], int lane) {
+        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+        if (!kMx && edge) keep[0] = live_pair(lane & 3, 0, lo, hi), keep[1] = live_pair(lane & 3, 1, lo, hi);
         uint32_t v[NB * VP / 4];
         load_lane<NB * VP>(rec + kv_value_offset(FMT, NB), lane, v);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            uint32_t f[8];
+            uint32_t f[4][2];   // [element][token pair]
             if constexpr (!kMx) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    f[2 * e] = v[8 * b + 2 * e], f[2 * e + 1] = v[8 * b + 2 * e + 1];
-                    if (edge) f[2 * e] &= keep0, f[2 * e + 1] &= keep1;
-                }
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        f[e][p] = v[8 * b + 4 * (e >> 1) + 2 * p + (e & 1)];
+                        if (edge) f[e][p] &= keep[p];
+                    }
             } else if constexpr (FMT == kKvMx8) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) f16_of_e4m3x4(v[4 * b + e], f[2 * e], f[2 * e + 1]);
+                for (int e = 0; e < 4; ++e) f16_of_e4m3x4(v[4 * b + e], f[e][0], f[e][1]);
             } else {
-                f16_of_e2m1x8(v[2 * b], f[0], f[1], f[2], f[3]);
-                f16_of_e2m1x8(v[2 * b + 1], f[4], f[5], f[6], f[7]);
+                f16_of_e2m1x8(v[2 * b], f[0][0], f[0][1], f[1][0], f[1][1]);
+                f16_of_e2m1x8(v[2 * b + 1], f[2][0], f[2][1], f[3][0], f[3][1]);
             }
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                uint32_t w0 = whi[r][0], w1 = wlo[r][0], w2 = whi[r][1], w3 = wlo[r][1];
+                uint32_t h0 = whi[r][0], h1 = whi[r][1], l0 = wlo[r][0], l1 = wlo[r][1];
                 if constexpr (kMx) {
-                    w0 = mul_f16x2(w0, rel[0][b]), w1 = mul_f16x2(w1, rel[0][b]);
-                    w2 = mul_f16x2(w2, rel[1][b]), w3 = mul_f16x2(w3, rel[1][b]);
+                    h0 = mul_f16x2(h0, rel[0][b]), h1 = mul_f16x2(h1, rel[1][b]);
+                    l0 = mul_f16x2(l0, rel[0][b]), l1 = mul_f16x2(l1, rel[1][b]);
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mma_16x8x16<kBf>(o[r][4 * b + e], w0, w1, w2, w3, f[2 * e], f[2 * e + 1]);
+                for (int i = 0; i < 2; ++i) mma_16x8x16<kBf>(o[r][b][i], f[2 * i][0], f[2 * i + 1][0], f[2 * i][1], f[2 * i + 1][1], h0, h1);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) mma_16x8x16<kBf>(o[r][b][i], f[2 * i][0], f[2 * i + 1][0], f[2 * i][1], f[2 * i + 1][1], l0, l1);
             }
         }
     }
 
-    // numerators of row g of tile r, block b: the 8 elements 32 b + 8 t .. + 7
-    __device__ __forceinline__ void numerators(int r, int b, float (&y)[8]) const {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            y[e] = o[r][4 * b + e][0] + o[r][4 * b + e][2];
-            y[4 + e] = o[r][4 * b + e][1] + o[r][4 * b + e][3];
-        }
+    // the largest over all lanes that hold the same heads
+    static __device__ __forceinline__ float max_over_tokens(float x) {
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
     }
-    __device__ __forceinline__ float denominator(int r) const {
-        float s = l[r];
-        s += __shfl_xor_sync(0xffffffffu, s, 1);
-        return s + __shfl_xor_sync(0xffffffffu, s, 2);
+
+    // N records; of their 16 N tokens [lo, hi) count.  Two at a time keep twice the independent work in flight and share the
+    // tests for a new maximum.
+    template <int N>
+    __device__ __forceinline__ void records(const uint8_t* const (&rec)[N], int lo, int hi, int lane) {
+        const int g = lane >> 2;
+        float s[N][RT][4];
+#pragma unroll
+        for (int n = 0; n < N; ++n) scores(rec[n], s[n], lane);
+        const bool edge = lo > 0 || hi < N * kKvRecord;
+        bool dead[N][2];   // tokens g, g + 8 that do not count
+        float te[N][2];
+        uint32_t rel[N][2][NB];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int tok = n * kKvRecord + g + 8 * i;
+                dead[n][i] = edge && (tok < lo || tok >= hi);
+                // the token's top byte as a float, by way of the integers behind 2^23
+                if constexpr (kMx)
+                    te[n][i] = __uint_as_float(0x4b000000u | rec[n][kv_value_top_offset(FMT, NB) + 4 * (g >> 1) + (g & 1) + 16 * i]) - 8388735.f;
+            }
+            if constexpr (kMx) value_scales(rec[n], edge, lo - n * kKvRecord, hi - n * kKvRecord, rel[n], lane);
+        }
+        // softmax
+        uint32_t whi[N][RT][2], wlo[N][RT][2];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            float x[N][4];   // exponents of the weights
+            float over = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[n][i] = dead[n][i >> 1] ? -INFINITY : fmaf(s[n][r][i], qs[r][i & 1], -m[r][i & 1]);
+                    over = fmaxf(over, x[n][i]);
+                }
+            if (__any_sync(0xffffffffu, over > kKvLag)) {
+                // from the scores: the first time, m is far below them and their differences are lost in x
+                float f[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float most = -INFINITY;
+#pragma unroll
+                    for (int n = 0; n < N; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            if (!dead[n][i]) most = fmaxf(most, s[n][r][2 * i + c] * qs[r][c]);
+                    most = max_over_tokens(most);
+                    const float to = most - m[r][c] > kKvLag ? ceilf(most) - kKvHead : m[r][c];
+                    f[c] = ex2(m[r][c] - to);
+                    m[r][c] = to;
+                    l[r][c] *= f[c];
+                }
+                if constexpr (!kMx) scale_rows(r, f[0], f[1]);
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[n][i] = dead[n][i >> 1] ? -INFINITY : fmaf(s[n][r][i], qs[r][i & 1], -m[r][i & 1]);
+            }
+            float w[N][4];
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[n][i] = ex2(x[n][i]);
+                l[r][0] += w[n][0] + w[n][2];
+                l[r][1] += w[n][1] + w[n][3];
+            }
+            if constexpr (kMx) {
+                float y[N][4], high = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        y[n][i] = dead[n][i >> 1] ? -INFINITY : fmaf(s[n][r][i], qs[r][i & 1], te[n][i >> 1] - big[r][i & 1]);
+                        high = fmaxf(high, y[n][i]);
+                    }
+                if (__any_sync(0xffffffffu, high > kKvLag)) {
+                    float f[2];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float most = -INFINITY;
+#pragma unroll
+                        for (int n = 0; n < N; ++n)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                if (!dead[n][i]) most = fmaxf(most, fmaf(s[n][r][2 * i + c], qs[r][c], te[n][i]));
+                        most = max_over_tokens(most);
+                        const float to = most - big[r][c] > kKvLag ? ceilf(most) - kKvHead : big[r][c];
+                        f[c] = ex2(big[r][c] - to);
+                        big[r][c] = to;
+                    }
+                    scale_rows(r, f[0], f[1]);
+#pragma unroll
+                    for (int n = 0; n < N; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            y[n][i] = dead[n][i >> 1] ? -INFINITY : fmaf(s[n][r][i], qs[r][i & 1], te[n][i >> 1] - big[r][i & 1]);
+                }
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[n][i] = ex2(y[n][i]);
+            }
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t hi16, lo16;
+                    split_pair<kBf>(w[n][2 * i], w[n][2 * i + 1], hi16, lo16);
+                    whi[n][r][i] = transpose8x8(hi16);
+                    wlo[n][r][i] = transpose8x8(lo16);
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) values(rec[n], edge, lo - n * kKvRecord, hi - n * kKvRecord, whi[n], wlo[n], rel[n], lane);
+    }
+
+    // the sum of weights of head 2t + c of tile r
+    __device__ __forceinline__ float denominator(int r, int c) const {
+        float s = l[r][c];
+        s += __shfl_xor_sync(0xffffffffu, s, 4);
+        s += __shfl_xor_sync(0xffffffffu, s, 8);
+        return s + __shfl_xor_sync(0xffffffffu, s, 16);
+    }
+    // its numerators 32 b + 4 g .. + 3
+    __device__ __forceinline__ float4 numerators(int r, int c, int b) const {
+        return make_float4(o[r][b][0][c], o[r][b][0][2 + c], o[r][b][1][c], o[r][b][1][2 + c]);
     }
     // Partial result of this warp's rows: numerators (times 2^big), denominators (times 2^m).
     __device__ __forceinline__ void store_partial(float* o_rows, float* stats, int lane) const {
         const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const float s = denominator(r);
-            const int row = 8 * r + g;
-            if (t == 0) {
-                stats[3 * row] = m[r];
-                stats[3 * row + 1] = kMx ? big[r] : m[r];
-                stats[3 * row + 2] = s;
-            }
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                float y[8];
-                numerators(r, b, y);
-                float* dst = o_rows + row * D + 32 * b + 8 * t;
-                *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
-                *reinterpret_cast<float4*>(dst + 4) = make_float4(y[4], y[5], y[6], y[7]);
+            for (int c = 0; c < 2; ++c) {
+                const float s = denominator(r, c);
+                const int row = 8 * r + 2 * t + c;
+                if (g == 0) {
+                    stats[3 * row] = m[r][c];
+                    stats[3 * row + 1] = kMx ? big[r][c] : m[r][c];
+                    stats[3 * row + 2] = s;
+                }
+#pragma unroll
+                for (int b = 0; b < NB; ++b) *reinterpret_cast<float4*>(o_rows + row * D + 32 * b + 4 * g) = numerators(r, c, b);
             }
-        }
     }
 };
 
@@ -507,28 +605,37 @@ constexpr int kKvJoinThreads = 256;
 constexpr int kKvMinRecords = 8;    // records of a CTA, at least
 
 // Shape of a CTA.  Each warp (or team of warps that share records) has a ring of records in shared memory, filled by
-// bulk copies: one copy a record, since a record is contiguous.  Beside the rings every warp has room for the partial
-// result of its first unit; that of its last one goes into its ring, which is empty by then.
-template <int FMT, int NB, int RT>
+// bulk copies: one copy a record, since a record is contiguous.  The partial result of a warp's first unit goes to the
+// workspace, that of its last one into its ring, which is empty by then.
+template <int FMT, int NB, int RT, int HALVES>
 struct KvShape {
-    // as many warps as registers (and, for 16-bit records of 8 KB and more, rings of three records) allow
-    static constexpr int kWarps = FMT <= kKvBf16 && NB > 4 ? 4 : RT > 1 || NB > 4 ? 8 : NB <= 2 ? 16 : FMT <= kKvBf16 ? 8 : 12;
-    static constexpr int kThreads = 32 * kWarps;
-    static constexpr int kRows = 8 * RT;
-    static constexpr int kPartial = kRows * (32 * NB + 3) * 4 + (kRows * 3 * 4 % 16 ? 16 - kRows * 3 * 4 % 16 : 0);
+    // as many warps as registers and rings allow: accumulators and query take 8 NB RT + 4 NB RT HALVES registers a thread of
+    // the 65536 / (32 warps), and a ring holds two records at least
+    static constexpr int kRegisters = 8 * NB * RT + 4 * NB * RT * HALVES;
+    static constexpr int kWarpsByRegisters = kRegisters <= 48 ? 16 : kRegisters <= 80 ? 12 : 8;
     static constexpr int kRecord = kv_record_bytes(FMT, NB);
     static constexpr int kSmemMax = 232448 - 10240;              // of a CTA, less the static part
-    static constexpr int kRoom = (kSmemMax / kWarps - kPartial) / kRecord;
+    static constexpr int kWarpsByRings = kSmemMax / 16 / kRecord >= 2   ? 16
+                                         : kSmemMax / 12 / kRecord >= 2 ? 12
+                                         : kSmemMax / 8 / kRecord >= 2  ? 8
+                                                                        : 6;
+    static constexpr int kWarps = kWarpsByRegisters < kWarpsByRings ? kWarpsByRegisters : kWarpsByRings;
+    static constexpr int kThreads = 32 * kWarps;
+    static constexpr int kRows = 8 * RT;
+    static constexpr int kPartial = kRows * (32 * NB + 3);       // floats: numerators, then (m, big, l) of each row
+    static constexpr int kRoom = kSmemMax / kWarps / kRecord;
     static constexpr int kStages = kRoom > 8 ? 8 : kRoom;        // of one warp's ring
     static constexpr int kRing = kStages * kRecord;
-    static constexpr int kSmem = kWarps * (kRing + kPartial);
-    static_assert(kStages >= 2 && kRing >= kPartial && kPartial % 16 == 0 && kRing % 16 == 0, "ring");
+    static constexpr bool kPair = NB * RT <= 2 && kStages >= 4;  // two records at a time
+    static constexpr int kSmem = kWarps * kRing;
+    static_assert(kStages >= 2 && kRing >= 4 * kPartial && kRing % 16 == 0 && kWarps * kPartial <= kKvSlotFloats, "ring");
 };
 
 struct KvSplit {
     int chunks;                     // chunks of query heads per key head
     int row_warps;                  // warps that share a record, each with its own rows (1, 2, 4, 8)
-    float* partial;                 // [ctas][2][rows][dim + 3]: numerators of all rows, then (m, big, l) of each
+    float* slots;                   // [ctas][kKvSlotFloats]: partial results of the warps' first units
+    float* partial;                 // [ctas][2][rows][dim + 3]: of the CTAs, numerators of all rows, then (m, big, l) of each
     int64_t* unit;                  // [ctas][2] unit of each partial (sequence << 32 | unit of the sequence), -1: none
     int* more;                      // [ctas] CTAs behind this one that hold parts of its last unit
 };
@@ -586,13 +693,13 @@ __device__ __forceinline__ void kv_copy_record(uint32_t dst, const uint8_t* src,
                  : "memory");
 }
 
-template <int FMT, int NB, int RT>
-__global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
+template <int FMT, int NB, int RT, int HALVES>
+__global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
     kv_attend_kernel(KvPool pool, KvSeqs seqs, KvAttend a, KvSplit split, int* status) {
-    using Shape = KvShape<FMT, NB, RT>;
+    using Shape = KvShape<FMT, NB, RT, HALVES>;
     constexpr int D = 32 * NB, kRows = Shape::kRows, kWarps = Shape::kWarps, kThreads = Shape::kThreads;
     constexpr int kMaxStages = 16;
-    extern __shared__ __align__(128) uint8_t smem[];          // rings, then the warps' partial results
+    extern __shared__ __align__(128) uint8_t smem[];          // rings
     __shared__ int64_t s_before[kThreads];                    // records of the sequences before thread i's
     __shared__ int64_t s_warp[kWarps];
     __shared__ int64_t s_unit[2 * kWarps];
@@ -608,7 +715,8 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
     const int stages = min(kMaxStages, Shape::kStages * split.row_warps);   // of the team's ring
     // partial results: slot 0 (a unit that began before the warp's range), slot 1 (one that goes on behind it)
     auto slot_rows = [&](int w, int which) {
-        return reinterpret_cast<float*>(which ? smem + w * Shape::kRing : smem + kWarps * Shape::kRing + w * Shape::kPartial);
+        return which ? reinterpret_cast<float*>(smem + w * Shape::kRing)
+                     : split.slots + (int64_t)blockIdx.x * kKvSlotFloats + w * Shape::kPartial;
     };
 
     // ---- records of all sequences, scanned by the CTA
@@ -705,7 +813,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
                 }
             }
         };
-        KvWarp<FMT, NB, RT> w;
+        KvWarp<FMT, NB, RT, HALVES> w;
         auto ask_query = [&]() {
             const int h = at.hu / split.chunks, row0 = (at.hu - h * split.chunks) * chunk_rows + rw * kRows;
             w.load_query(a, (int64_t)at.b * a.seq_stride + (int64_t)h * a.group * a.head_stride, row0, a.group, lane);
@@ -727,43 +835,75 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
             const bool begins = at.r == 0, ends = at.r + seg == at.n;
             const int h = at.hu / split.chunks, row0 = (at.hu - h * split.chunks) * chunk_rows + rw * kRows;
             w.reset();
-            w.convert_query(a);
+            w.convert_query(a, lane);
             int first = (at.lo / kKvRecord + at.r) * kKvRecord;   // position of the record's first token
-            for (int j = 0; j < seg; ++j, first += kKvRecord) {
-                alive = alive && mbar_wait(smem_u32(&s_full[team][stage]), phase, &s_abort);
-                if (alive && s_ok[team][stage])
-                    w.record(ring + stage * Shape::kRecord, max(at.lo - first, 0), min(at.hi - first, kKvRecord), lane);
-                __syncwarp();
+            auto arrived = [&](int st, uint32_t ph) { alive = alive && mbar_wait(full_at + 8 * st, ph, &s_abort); };
+            auto release = [&](int st, uint32_t ph) {
                 if (split.row_warps > 1) {
-                    if (lane == 0) mbar_arrive(smem_u32(&s_empty[team][stage]));
-                    if (rw == 0 && to_fetch > 0) alive = alive && mbar_wait(smem_u32(&s_empty[team][stage]), phase, &s_abort);
+                    if (lane == 0) mbar_arrive(smem_u32(&s_empty[team][st]));
+                    if (rw == 0 && to_fetch > 0) alive = alive && mbar_wait(smem_u32(&s_empty[team][st]), ph, &s_abort);
                 }
                 if (alive) {
-                    if (rw == 0) fetch(stage);
-                    dead_stage = stage, dead_phase = phase;
+                    if (rw == 0) fetch(st);
+                    dead_stage = st, dead_phase = ph;
                 }
-                if (++stage == stages) stage = 0, phase ^= 1;
+            };
+            for (int j = 0; j < seg;) {
+                const int next = stage + 1 == stages ? 0 : stage + 1;
+                const uint32_t next_phase = next == 0 ? phase ^ 1u : phase;
+                const uint8_t* here = ring + stage * Shape::kRecord;
+                const int lo = max(at.lo - first, 0), hi = at.hi - first;
+                arrived(stage, phase);
+                if (Shape::kPair && j + 1 < seg) {
+                    arrived(next, next_phase);
+                    const uint8_t* there = ring + next * Shape::kRecord;
+                    const bool ok0 = s_ok[team][stage], ok1 = s_ok[team][next];
+                    if (alive && ok0 && ok1) {
+                        const uint8_t* const both[2] = {here, there};
+                        w.template records<2>(both, lo, min(hi, 2 * kKvRecord), lane);
+                    } else if (alive && (ok0 || ok1)) {
+                        // the tokens of the record that is missing are left out
+                        const uint8_t* const one[1] = {ok0 ? here : there};
+                        w.template records<1>(one, ok0 ? lo : 0, min(ok0 ? hi : hi - kKvRecord, kKvRecord), lane);
+                    }
+                    __syncwarp();
+                    release(stage, phase);
+                    release(next, next_phase);
+                    stage = next + 1 == stages ? 0 : next + 1;
+                    phase = stage == 0 ? next_phase ^ 1u : next_phase;
+                    j += 2;
+                    first += 2 * kKvRecord;
+                } else {
+                    if (alive && s_ok[team][stage]) {
+                        const uint8_t* const one[1] = {here};
+                        w.template records<1>(one, lo, min(hi, kKvRecord), lane);
+                    }
+                    __syncwarp();
+                    release(stage, phase);
+                    stage = next, phase = next_phase;
+                    ++j;
+                    first += kKvRecord;
+                }
             }
             if (begins && ends) {
                 const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-                for (int k = 0; k < RT; ++k) {
-                    const float l = w.denominator(k);
-                    const int row = row0 + 8 * k + g;
-                    if (row >= a.group) continue;
-                    const int64_t out_row = (int64_t)b * a.q_heads + (int64_t)h * a.group + row;
-                    const float big = FMT >= kKvMx8 ? w.big[k] : w.m[k];
-                    const KvQuotient f(l, big, w.m[k]);
-                    if (t == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
+                for (int k = 0; k < RT; ++k)
 #pragma unroll
-                    for (int blk = 0; blk < NB; ++blk) {
-                        float y[8];
-                        w.numerators(k, blk, y);
+                    for (int c = 0; c < 2; ++c) {
+                        const float l = w.denominator(k, c);   // (all lanes)
+                        const int row = row0 + 8 * k + 2 * t + c;
+                        if (row >= a.group) continue;
+                        const int64_t out_row = (int64_t)b * a.q_heads + (int64_t)h * a.group + row;
+                        const KvQuotient f(l, FMT >= kKvMx8 ? w.big[k][c] : w.m[k][c], w.m[k][c]);
+                        if (g == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = f(y[e]);
-                        store_row<8>(a.out, out_row * D + 32 * blk + 8 * t, a.type, a.out_vec, y);
+                        for (int blk = 0; blk < NB; ++blk) {
+                            const float4 o = w.numerators(k, c, blk);
+                            const float y[4] = {f(o.x), f(o.y), f(o.z), f(o.w)};
+                            store_row<4>(a.out, out_row * D + 32 * blk + 4 * g, a.type, a.out_vec, y);
+                        }
                     }
-                }
             } else {
                 const int which = begins ? 1 : 0;
                 if (begins && split.row_warps > 1) named_bar_sync(1 + team, 32 * split.row_warps);   // the ring is free
@@ -802,9 +942,9 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT>::kThreads)
         const uint32_t starts = __ballot_sync(0xffffffffu, unit >= 0 && (before == 0 || last != unit));
         const uint32_t begun = __ballot_sync(0xffffffffu, unit >= 0 && (s_ends[mine_at] & 1)),
                        ended = __ballot_sync(0xffffffffu, unit >= 0 && (s_ends[mine_at] & 2));
-        const int runs = __popc(starts);
-        for (int item = warp; item < runs * chunk_rows; item += kWarps) {
-            const int run = item / chunk_rows, row = item - run * chunk_rows, k = row / kRows, in = row - k * kRows;
+        const int rows_used = min(chunk_rows, a.group), items = __popc(starts) * rows_used;
+        for (int item = warp; item < items; item += kWarps) {
+            const int run = item / rows_used, row = item - run * rows_used, k = row / kRows, in = row - k * kRows;
             uint32_t rest = starts;
             for (int i = 0; i < run; ++i) rest &= rest - 1;
             const int e0 = __ffs(rest) - 1;
@@ -933,29 +1073,32 @@ __global__ void __launch_bounds__(kKvJoinThreads) kv_join_kernel(KvPool pool, Kv
     if (lane == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
 }
 
-template <int FMT, int NB, int RT>
+template <int FMT, int NB, int RT, int HALVES>
 struct KvAttendInstance {
-    using Shape = KvShape<FMT, NB, RT>;
+    using Shape = KvShape<FMT, NB, RT, HALVES>;
     static cudaError_t init() {
-        return cudaFuncSetAttribute(kv_attend_kernel<FMT, NB, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
+        return cudaFuncSetAttribute(kv_attend_kernel<FMT, NB, RT, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
     }
     static int launch(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
                       cudaStream_t stream) {
         KvSplit split{};
+        // warps for the rows of a key head: the smallest divisor of the CTA's warps that covers them, at most 128 rows
         split.row_warps = 1;
-        while (split.row_warps < Shape::kWarps && split.row_warps * 8 * RT < a.group) split.row_warps *= 2;
+        for (int d = 2; d <= 8 && split.row_warps * 8 * RT < a.group; ++d)
+            if (Shape::kWarps % d == 0) split.row_warps = d;
         const int chunk_rows = split.row_warps * 8 * RT;
         split.chunks = (a.group + chunk_rows - 1) / chunk_rows;
         split.unit = work.unit;
         split.more = work.more;
+        split.slots = work.slots;
         split.partial = work.partial;
-        kv_attend_kernel<FMT, NB, RT><<<work.ctas, Shape::kThreads, Shape::kSmem, stream>>>(pool, seqs, a, split, status);
+        kv_attend_kernel<FMT, NB, RT, HALVES><<<work.ctas, Shape::kThreads, Shape::kSmem, stream>>>(pool, seqs, a, split, status);
         // the join's CTAs start as those of the attention kernel end (programmatic launch), and wait for the last of them
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr.val.programmaticStreamSerializationAllowed = 1;
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(work.ctas, (chunk_rows + kKvJoinThreads / 32 - 1) / (kKvJoinThreads / 32));
+        cfg.gridDim = dim3(work.ctas, (std::min(chunk_rows, a.group) + kKvJoinThreads / 32 - 1) / (kKvJoinThreads / 32));
         cfg.blockDim = dim3(kKvJoinThreads);
         cfg.stream = stream;
         cfg.attrs = &attr;
@@ -965,20 +1108,34 @@ struct KvAttendInstance {
     }
 };
 
-// Two row tiles (16 heads) a warp where a key head serves more than 8 query heads and the accumulators of two tiles fit
-// the registers (head sizes up to 128).
+// Two tiles (16 heads) a warp where a key head serves more than 8 query heads -- the codes are converted once for both --
+// and accumulators and query leave enough of 255 registers.
+constexpr bool kv_two_tiles(int nb, int halves) { return nb * (16 + 8 * halves) <= 144; }
+template <int FMT, int NB, int HALVES>
+int kv_attend_tiles(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status, cudaStream_t stream) {
+    if constexpr (kv_two_tiles(NB, HALVES))
+        if (a.group > 8) return KvAttendInstance<FMT, NB, 2, HALVES>::launch(pool, seqs, a, work, status, stream);
+    return KvAttendInstance<FMT, NB, 1, HALVES>::launch(pool, seqs, a, work, status, stream);
+}
+// The query is one operand where its type fits it exactly.
 template <int FMT, int NB>
 int kv_attend_rows(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status, cudaStream_t stream) {
-    if constexpr (NB <= 4)
-        if (a.group > 8) return KvAttendInstance<FMT, NB, 2>::launch(pool, seqs, a, work, status, stream);
-    return KvAttendInstance<FMT, NB, 1>::launch(pool, seqs, a, work, status, stream);
+    return a.type == kTypeBf16 || (a.type == kTypeF16 && FMT != kKvBf16)
+               ? kv_attend_tiles<FMT, NB, 1>(pool, seqs, a, work, status, stream)
+               : kv_attend_tiles<FMT, NB, 2>(pool, seqs, a, work, status, stream);
+}
+template <int FMT, int NB, int HALVES>
+cudaError_t kv_attend_tiles_init() {
+    if constexpr (kv_two_tiles(NB, HALVES)) {
+        const cudaError_t e = KvAttendInstance<FMT, NB, 2, HALVES>::init();
+        if (e != cudaSuccess) return e;
+    }
+    return KvAttendInstance<FMT, NB, 1, HALVES>::init();
 }
 template <int FMT, int NB>
 cudaError_t kv_attend_rows_init() {
-    cudaError_t e = KvAttendInstance<FMT, NB, 1>::init();
-    if constexpr (NB <= 4)
-        if (e == cudaSuccess) e = KvAttendInstance<FMT, NB, 2>::init();
-    return e;
+    const cudaError_t e = kv_attend_tiles_init<FMT, NB, 1>();
+    return e == cudaSuccess ? kv_attend_tiles_init<FMT, NB, 2>() : e;
 }
 
 template <int FMT>

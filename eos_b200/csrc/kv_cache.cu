@@ -104,19 +104,19 @@ __global__ void __launch_bounds__(kKvWarps * 32)
         const bool mine = pos >= un.lo && pos < un.hi;
         if (!__any_sync(0xffffffffu, mine)) continue;
         const int64_t at = (un.row0 + pos) * key.token_stride + (int64_t)h * key.head_stride + 8 * t;
-        uint8_t* codes = rec + j * 32 * nb * KP;
+        uint8_t* codes = rec + (kMx ? j * 32 * nb * KP : 0);
 #pragma unroll 4
         for (int b = 0; b < nb; ++b) {
             float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             if (mine) load_row<8>(key.p, at + 32 * b, type, key.vec, x);
             uint8_t* dst = codes + kv_lane_offset(nb * KP, lane, b * KP);
             if constexpr (!kMx) {
-                uint4 v;
-                v.x = FMT == kKvF16 ? f16x2_of(x[0], x[1]) : bf16x2_of(x[0], x[1]);
-                v.y = FMT == kKvF16 ? f16x2_of(x[2], x[3]) : bf16x2_of(x[2], x[3]);
-                v.z = FMT == kKvF16 ? f16x2_of(x[4], x[5]) : bf16x2_of(x[4], x[5]);
-                v.w = FMT == kKvF16 ? f16x2_of(x[6], x[7]) : bf16x2_of(x[6], x[7]);
-                if (mine) *reinterpret_cast<uint4*>(dst) = v;
+                // words 0, 1 and 2, 3 of the token go to words j, j + 2 of the block's first and second 16 bytes
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t v = FMT == kKvF16 ? f16x2_of(x[2 * i], x[2 * i + 1]) : bf16x2_of(x[2 * i], x[2 * i + 1]);
+                    if (mine) *reinterpret_cast<uint32_t*>(codes + kv_lane_offset(2 * nb * KP, lane, 32 * b + 16 * (i >> 1) + 8 * (i & 1) + 4 * j)) = v;
+                }
             } else {
                 uint32_t m = 0;   // as integers: an infinity or a NaN stays the largest
 #pragma unroll
@@ -169,8 +169,9 @@ __global__ void __launch_bounds__(kKvWarps * 32)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float a = x[2 * i][e], c = x[2 * i + 1][e];
-                    v[2 * e + i] = FMT == kKvF16 ? f16x2_of(a, c) : bf16x2_of(a, c);
-                    keep[2 * e + i] = (mine[2 * i] ? 0u : 0x0000ffffu) | (mine[2 * i + 1] ? 0u : 0xffff0000u);
+                    const int at_word = 4 * (e >> 1) + 2 * i + (e & 1);
+                    v[at_word] = FMT == kKvF16 ? f16x2_of(a, c) : bf16x2_of(a, c);
+                    keep[at_word] = (mine[2 * i] ? 0u : 0x0000ffffu) | (mine[2 * i + 1] ? 0u : 0xffff0000u);
                 }
         } else {
             uint32_t byte[4];
@@ -283,15 +284,16 @@ __global__ void __launch_bounds__(kKvWarps * 32)
         const int pos = base + 8 * j + g;
         if (pos < un.lo || pos >= un.hi) continue;
         const int64_t at = (un.row0 + pos) * key.token_stride + (int64_t)h * key.head_stride + 8 * t;
-        const uint8_t* codes = rec + j * 32 * nb * KP;
+        const uint8_t* codes = rec + (kMx ? j * 32 * nb * KP : 0);
 #pragma unroll 4
         for (int b = 0; b < nb; ++b) {
             const uint8_t* src = codes + kv_lane_offset(nb * KP, lane, b * KP);
             float x[8];
             uint32_t c[4];
             if constexpr (!kMx) {
-                const uint4 v = *reinterpret_cast<const uint4*>(src);
-                c[0] = v.x, c[1] = v.y, c[2] = v.z, c[3] = v.w;
+                const uint4 v = *reinterpret_cast<const uint4*>(codes + kv_lane_offset(2 * nb * KP, lane, 32 * b));
+                const uint4 y = *reinterpret_cast<const uint4*>(codes + kv_lane_offset(2 * nb * KP, lane, 32 * b + 16));
+                c[0] = j ? v.y : v.x, c[1] = j ? v.w : v.z, c[2] = j ? y.y : y.x, c[3] = j ? y.w : y.z;
             } else if constexpr (FMT == kKvMx8) {
                 const uint2 v = *reinterpret_cast<const uint2*>(src);
                 f16_of_e4m3x4(v.x, c[0], c[1]);
@@ -325,7 +327,7 @@ __global__ void __launch_bounds__(kKvWarps * 32)
         if constexpr (!kMx) {
             const uint4 a = *reinterpret_cast<const uint4*>(codes + kv_lane_offset(nb * VP, lane, b * VP));
             const uint4 d = *reinterpret_cast<const uint4*>(codes + kv_lane_offset(nb * VP, lane, b * VP + 16));
-            c[0] = a.x, c[1] = a.y, c[2] = a.z, c[3] = a.w, c[4] = d.x, c[5] = d.y, c[6] = d.z, c[7] = d.w;
+            c[0] = a.x, c[2] = a.y, c[1] = a.z, c[3] = a.w, c[4] = d.x, c[6] = d.y, c[5] = d.z, c[7] = d.w;
         } else if constexpr (FMT == kKvMx8) {
             const uint4 a = *reinterpret_cast<const uint4*>(codes + kv_lane_offset(nb * VP, lane, b * VP));
             f16_of_e4m3x4(a.x, c[0], c[1]);

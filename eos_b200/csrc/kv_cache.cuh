@@ -8,10 +8,13 @@
 // Inside a record the codes are stored in the order in which the 32 lanes of a warp feed them to mma.sync m16n8k16, so
 // that the attention kernel reads them with conflict-free 16-byte loads and no shuffle.  With lane = 4 g + t
 // (g = 0..7, t = 0..3) and blocks b of 32 elements:
-//     keys    two tiles j of 8 tokens; lane (g, t) holds token 8 j + g, elements 32 b + 8 t .. + 7 of every block b
-//             (an mma sums over elements, so any order of them serves as long as the query uses the same one)
-//     values  lane (g, t) holds tokens {2t, 2t+1, 2t+8, 2t+9}, elements 32 b + 4 g + {0..3}, element-major: the two
-//             tokens of one 32-bit operand register are neighbours
+//     keys    lane (g, t) holds elements 32 b + 8 t .. + 7 of every block b of the tokens g and g + 8 (an mma sums over
+//             elements, so any order of them serves as long as the query uses the same one): first all of token g, then
+//             all of token g + 8 -- but in the 16-bit formats, whose words are operands as they are, the two tokens' words
+//             in turn, so that the four operands of an mma are one 16-byte load
+//     values  lane (g, t) holds tokens {2t, 2t+1, 2t+8, 2t+9}, elements 32 b + 4 g + {0..3}; the two tokens of one 32-bit
+//             operand are neighbours.  mx: element by element; 16 bits: words of the pairs (2t, 2t+1) and (2t+8, 2t+9) in the
+//             order of the operands, elements (0, 1) with the first pair, (0, 1) with the second, (2, 3) likewise
 // A lane's bytes are cut into 16-byte pieces (then 8, then 4); piece i of all lanes is one contiguous plane.
 // Scales are one byte per token and block (2^(byte - 127)), blocks rounded up to 1, 2, 4 or 8: keys [16 tokens][blocks],
 // values [8 token pairs][blocks][2], the order in which the attention kernel makes f16 pairs of them.  For every token
@@ -28,7 +31,7 @@ constexpr int kKvF16 = 0, kKvBf16 = 1, kKvMx8 = 2, kKvMx4 = 3;        // EOS_B20
 constexpr int kTypeF32 = 0, kTypeF16 = 1, kTypeBf16 = 2;              // EOS_B200_TYPE_*
 constexpr int kKvRecord = 16;                                         // tokens of a record
 
-// bytes of one lane and one 32-element block: keys (one token tile) and values (all 16 tokens)
+// bytes of one lane and one 32-element block: keys (one token) and values (four)
 __host__ __device__ constexpr int kv_key_piece(int format) { return format <= kKvBf16 ? 16 : format == kKvMx8 ? 8 : 4; }
 __host__ __device__ constexpr int kv_value_piece(int format) { return 2 * kv_key_piece(format); }
 __host__ __device__ constexpr int kv_scale_stride(int blocks) { return blocks <= 2 ? blocks : blocks <= 4 ? 4 : 8; }
@@ -100,11 +103,13 @@ struct KvAttend {
 // Workspace of a cache's attention calls, of a fixed size: captured graphs keep its addresses.
 struct KvWork {
     int ctas;               // one per SM
+    float* slots;           // [ctas][kKvSlotFloats]
     float* partial;         // kv_work_floats(ctas, dim)
     int64_t* unit;          // [ctas][2]
     int* more;              // [ctas]
 };
-constexpr int kKvMaxRows = 128;   // query heads of one unit, at most
+constexpr int kKvMaxRows = 128;        // query heads of one unit, at most
+constexpr int kKvSlotFloats = 33280;   // partial results of a CTA's warps
 inline size_t kv_work_floats(int ctas, int dim) { return (size_t)ctas * 2 * kKvMaxRows * (dim + 3); }
 
 // cudaSuccess once the kernels of this format and dim are ready on the current device

@@ -33,8 +33,14 @@ int main() {
             };
             for (int lane = 0; lane < 32; ++lane)
                 for (int b = 0; b < nb; ++b) {
-                    for (int j = 0; j < 2; ++j)
-                        if (!piece(j * 32 * nb * kp, nb * kp, lane, b * kp, kp)) return 2;
+                    if (format <= kKvBf16) {   // both tokens' words in turn
+                        for (int j = 0; j < 2; ++j)
+                            for (int i = 0; i < 4; ++i)
+                                if (!piece(0, 2 * nb * kp, lane, 32 * b + 16 * (i >> 1) + 8 * (i & 1) + 4 * j, 4)) return 2;
+                    } else {
+                        for (int j = 0; j < 2; ++j)
+                            if (!piece(j * 32 * nb * kp, nb * kp, lane, b * kp, kp)) return 2;
+                    }
                     const int step = vp < 16 ? vp : 16;
                     for (int p = 0; p < vp; p += step)
                         if (!piece(kv_value_offset(format, nb), nb * vp, lane, b * vp + p, step)) return 3;
