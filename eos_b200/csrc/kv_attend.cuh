@@ -605,19 +605,19 @@ constexpr int kKvJoinThreads = 256;
 constexpr int kKvMinRecords = 8;    // records of a CTA, at least
 
 // Shape of a CTA.  Each warp (or team of warps that share records) has a ring of records in shared memory, filled by
-// bulk copies: one copy a record, since a record is contiguous.  The partial result of a warp's first unit goes to the
-// workspace, that of its last one into its ring, which is empty by then.
+// bulk copies: one copy a record, since a record is contiguous.  The partial result of a warp's last unit goes into its
+// ring, which is empty by then; that of its first one, if it is another, to the workspace.
 template <int FMT, int NB, int RT, int HALVES>
 struct KvShape {
     // as many warps as registers and rings allow: accumulators and query take 8 NB RT + 4 NB RT HALVES registers a thread of
-    // the 65536 / (32 warps), and a ring holds two records at least
+    // the 65536 / (32 warps), and a ring holds three records (two of 16 KB)
     static constexpr int kRegisters = 8 * NB * RT + 4 * NB * RT * HALVES;
     static constexpr int kWarpsByRegisters = kRegisters <= 48 ? 16 : kRegisters <= 80 ? 12 : 8;
     static constexpr int kRecord = kv_record_bytes(FMT, NB);
     static constexpr int kSmemMax = 232448 - 10240;              // of a CTA, less the static part
-    static constexpr int kWarpsByRings = kSmemMax / 16 / kRecord >= 2   ? 16
-                                         : kSmemMax / 12 / kRecord >= 2 ? 12
-                                         : kSmemMax / 8 / kRecord >= 2  ? 8
+    static constexpr int kWarpsByRings = kSmemMax / 16 / kRecord >= 3   ? 16
+                                         : kSmemMax / 12 / kRecord >= 3 ? 12
+                                         : kSmemMax / 8 / kRecord >= 3  ? 8
                                                                         : 6;
     static constexpr int kWarps = kWarpsByRegisters < kWarpsByRings ? kWarpsByRegisters : kWarpsByRings;
     static constexpr int kThreads = 32 * kWarps;
@@ -631,9 +631,29 @@ struct KvShape {
     static_assert(kStages >= 2 && kRing >= 4 * kPartial && kRing % 16 == 0 && kWarps * kPartial <= kKvSlotFloats, "ring");
 };
 
+// Division of a number that is not negative by a constant of the launch: below 2^31 floor(a / d) = a m >> s with
+// s = 31 + ceil(log2 d), m = ceil(2^s / d) -- the excess a (m d - 2^s) / (d 2^s) is below 2^31 / 2^s <= 1 / d.
+struct KvDiv {
+    uint32_t d, m;
+    int s;
+    KvDiv() = default;
+    explicit KvDiv(uint32_t by) : d(by), s(31) {
+        while ((1ull << (s - 31)) < by) ++s;
+        m = (uint32_t)(((s < 63 ? 1ull << s : 0) + by - 1) / by);
+    }
+    __device__ __forceinline__ int64_t operator()(int64_t a) const {
+        return a >> 31 ? a / d : (int64_t)((uint64_t)(uint32_t)a * m >> s);
+    }
+};
+__device__ __forceinline__ int64_t kv_div(int64_t a, int64_t b) {   // not negative; the 32-bit division is far shorter
+    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 struct KvSplit {
     int chunks;                     // chunks of query heads per key head
-    int row_warps;                  // warps that share a record, each with its own rows (1, 2, 4, 8)
+    int row_warps;                  // warps that share a record, each with its own rows
+    int per_seq, teams;             // units of a sequence; warps of a CTA / row_warps
+    KvDiv by_ctas, by_per_seq, by_teams, by_page, by_chunks;   // (by_page: records of a page)
     float* slots;                   // [ctas][kKvSlotFloats]: partial results of the warps' first units
     float* partial;                 // [ctas][2][rows][dim + 3]: of the CTAs, numerators of all rows, then (m, big, l) of each
     int64_t* unit;                  // [ctas][2] unit of each partial (sequence << 32 | unit of the sequence), -1: none
@@ -651,18 +671,14 @@ __device__ __forceinline__ bool kv_span(const KvPool& pool, const KvSeqs& s, int
 __device__ __forceinline__ int kv_records(int lo, int hi) { return hi > lo ? (hi + kKvRecord - 1) / kKvRecord - lo / kKvRecord : 0; }
 
 
-__device__ __forceinline__ int64_t kv_div(int64_t a, int64_t b) {   // not negative; the 32-bit division is far shorter
-    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
-}
 
 // A walk over the records of a range, in order: the unit (b, hu) and the record r of its n.
 struct KvWalk {
     int b, hu, r, n, lo, hi;
 
     // to the record `at` of all records; i0 / first: a sequence at or before its own, and the records before that
-    __device__ __forceinline__ void seek(const KvPool& pool, const KvSeqs& s, int window, int64_t per_seq, int64_t at, int i0,
+    __device__ __forceinline__ void seek(const KvPool& pool, const KvSeqs& s, int window, int per_seq, int64_t q, int64_t at, int i0,
                                          int64_t first) {
-        const int64_t q = kv_div(at, per_seq);
         for (b = i0;; ++b) {
             kv_span(pool, s, window, b, lo, hi);
             n = kv_records(lo, hi);
@@ -670,7 +686,7 @@ struct KvWalk {
             first += n;
         }
         at -= first * per_seq;
-        hu = (int)kv_div(at, n);
+        hu = per_seq > 1 ? (int)kv_div(at, n) : 0;
         r = (int)(at - (int64_t)hu * n);
     }
     // to the first record of the next unit (there is one)
@@ -703,20 +719,21 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
     __shared__ int64_t s_before[kThreads];                    // records of the sequences before thread i's
     __shared__ int64_t s_warp[kWarps];
     __shared__ int64_t s_unit[2 * kWarps];
-    __shared__ int s_ends[2 * kWarps];                        // bit 0: the unit begins there, bit 1: it ends there
+    __shared__ int s_ends[2 * kWarps];                        // bit 0: the unit begins there, 1: it ends there, 2: in the ring
     __shared__ int64_t s_until[kWarps];                       // end, among all records, of the unit begun last
     __shared__ __align__(8) uint64_t s_full[kWarps][kMaxStages], s_empty[kWarps][kMaxStages];
     __shared__ uint8_t s_ok[kWarps][kMaxStages];              // whether the record could be fetched
     __shared__ int s_abort, s_drain[kWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int per_seq = pool.heads * split.chunks;            // units of a sequence
+    const int per_seq = split.per_seq;
     const int chunk_rows = kRows * split.row_warps;
-    const int teams = kWarps / split.row_warps, team = warp / split.row_warps, rw = warp % split.row_warps;
+    const int teams = split.teams, team = split.row_warps == 1 ? warp : warp / split.row_warps, rw = warp - team * split.row_warps;
     const int stages = min(kMaxStages, Shape::kStages * split.row_warps);   // of the team's ring
-    // partial results: slot 0 (a unit that began before the warp's range), slot 1 (one that goes on behind it)
-    auto slot_rows = [&](int w, int which) {
-        return which ? reinterpret_cast<float*>(smem + w * Shape::kRing)
-                     : split.slots + (int64_t)blockIdx.x * kKvSlotFloats + w * Shape::kPartial;
+    // partial results: slot 0 (a unit that began before the warp's range), slot 1 (one that goes on behind it); `last`: of
+    // the warp's last unit
+    auto slot_rows = [&](int w, bool last) {
+        return last ? reinterpret_cast<float*>(smem + w * Shape::kRing)
+                    : split.slots + (int64_t)blockIdx.x * kKvSlotFloats + w * Shape::kPartial;
     };
 
     // ---- records of all sequences, scanned by the CTA
@@ -752,9 +769,9 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
     s_before[tid] = base + upto - mine;
     __syncthreads();
     total *= per_seq;
-    const int64_t part = max(kv_div(total + gridDim.x - 1, gridDim.x), (int64_t)kKvMinRecords);
+    const int64_t part = max(split.by_ctas(total + gridDim.x - 1), (int64_t)kKvMinRecords);
     const int64_t c0 = min((int64_t)blockIdx.x * part, total), c1 = min(c0 + part, total);
-    const int64_t tpart = kv_div(c1 - c0 + teams - 1, teams);
+    const int64_t tpart = split.by_teams(c1 - c0 + teams - 1);
     const int64_t t0 = min(c0 + team * tpart, c1), t1 = min(t0 + tpart, c1);
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -762,11 +779,11 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
     if (t1 > t0) {
         KvWalk at;
         {
-            const int64_t q = kv_div(t0, per_seq);
+            const int64_t q = split.by_per_seq(t0);   // all units of a sequence have as many records
             constexpr int kStep = kThreads / 32;
             int i = 31 - __clz(__ballot_sync(0xffffffffu, s_before[lane * kStep] <= q));
             i = i * kStep + 31 - __clz(__ballot_sync(0xffffffffu, lane < kStep && s_before[min(i * kStep + lane, kThreads - 1)] <= q));
-            at.seek(pool, seqs, a.window, per_seq, t0, i * per, s_before[i]);
+            at.seek(pool, seqs, a.window, per_seq, q, t0, i * per, s_before[i]);
         }
         // ---- the copies: the walk of the records to fetch runs `stages` ahead of the one below
         KvWalk ahead = at;
@@ -781,12 +798,12 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
             run = min(rpp - in, ahead.n - ahead.r);
             src = page < 0 || page >= pool.pages
                       ? nullptr
-                      : pool.base + (((int64_t)page * pool.heads + ahead.hu / split.chunks) * rpp + in) * Shape::kRecord;
+                      : pool.base + (((int64_t)page * pool.heads + (int)split.by_chunks(ahead.hu)) * rpp + in) * Shape::kRecord;
             next_page = page_at(slot + 1);   // asked for early: its latency passes while this page is read
         };
         auto enter_unit = [&]() {
             const int rec = ahead.lo / kKvRecord + ahead.r;
-            slot = rec / rpp;
+            slot = (int)split.by_page(rec);
             enter_page(page_at(slot), rec - slot * rpp);
         };
         auto fetch = [&](int stage) {   // the next record, if there is one, into `stage`
@@ -815,7 +832,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
         };
         KvWarp<FMT, NB, RT, HALVES> w;
         auto ask_query = [&]() {
-            const int h = at.hu / split.chunks, row0 = (at.hu - h * split.chunks) * chunk_rows + rw * kRows;
+            const int h = (int)split.by_chunks(at.hu), row0 = (at.hu - h * split.chunks) * chunk_rows + rw * kRows;
             w.load_query(a, (int64_t)at.b * a.seq_stride + (int64_t)h * a.group * a.head_stride, row0, a.group, lane);
         };
         ask_query();
@@ -833,7 +850,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
         while (true) {
             const int b = at.b, seg = (int)min((int64_t)(at.n - at.r), left);
             const bool begins = at.r == 0, ends = at.r + seg == at.n;
-            const int h = at.hu / split.chunks, row0 = (at.hu - h * split.chunks) * chunk_rows + rw * kRows;
+            const int h = (int)split.by_chunks(at.hu), row0 = (at.hu - h * split.chunks) * chunk_rows + rw * kRows;
             w.reset();
             w.convert_query(a, lane);
             int first = (at.lo / kKvRecord + at.r) * kKvRecord;   // position of the record's first token
@@ -906,12 +923,13 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
                     }
             } else {
                 const int which = begins ? 1 : 0;
-                if (begins && split.row_warps > 1) named_bar_sync(1 + team, 32 * split.row_warps);   // the ring is free
-                float* rows = slot_rows(warp, which);
+                const bool last = left == seg;
+                if (last && split.row_warps > 1) named_bar_sync(1 + team, 32 * split.row_warps);   // the ring is free
+                float* rows = slot_rows(warp, last);
                 w.store_partial(rows, rows + kRows * D, lane);
                 if (lane == 0) {
                     s_unit[2 * warp + which] = (int64_t)b << 32 | at.hu;
-                    s_ends[2 * warp + which] = (begins ? 1 : 0) | (ends ? 2 : 0);
+                    s_ends[2 * warp + which] = (begins ? 1 : 0) | (ends ? 2 : 0) | (last ? 4 : 0);
                     if (begins) s_until[warp] = t1 - seg + at.n;   // (it is the range's last segment)
                 }
             }
@@ -956,25 +974,35 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
             if (whole && row0 + row >= a.group) continue;
             const bool member = members >> lane & 1u;
             const int sl = slot_of(member ? lane : e0, k);
-            const float* st = slot_rows(sl >> 1, sl & 1) + kRows * D + 3 * in;
+            const float* rows = slot_rows(sl >> 1, s_ends[sl] & 4);   // lane e: the partial result of slot e
+            const float* st = rows + kRows * D + 3 * in;
             const float m = warp_max(st[0]), big = warp_max(st[1]);
             const float l = warp_sum(member ? st[2] * ex2(st[0] - m) : 0.f);
-            const float c = ex2(st[1] - big);
+            const float c = member ? ex2(st[1] - big) : 0.f;
             constexpr int kQuads = (D + 127) / 128;
             float4 o[kQuads];
 #pragma unroll
             for (int i = 0; i < kQuads; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (uint32_t left = members; left; left &= left - 1) {
-                const int e = __ffs(left) - 1, se = slot_of(e, k);
-                const float f = __shfl_sync(0xffffffffu, c, e);
-                const float* rows = slot_rows(se >> 1, se & 1) + in * D;
+            for (uint32_t left = members; left;) {
+                float4 y[4][kQuads];
+                float f[4];
 #pragma unroll
-                for (int i = 0; i < kQuads; ++i) {
-                    const int d = 4 * lane + 128 * i;
-                    if (d >= D) continue;
-                    const float4 y = *reinterpret_cast<const float4*>(rows + d);
-                    o[i].x = fmaf(y.x, f, o[i].x), o[i].y = fmaf(y.y, f, o[i].y), o[i].z = fmaf(y.z, f, o[i].z), o[i].w = fmaf(y.w, f, o[i].w);
+                for (int x = 0; x < 4; ++x) {   // four loads on their way at once; the last slot again, times 0, at the end
+                    const int e = left ? __ffs(left) - 1 : e0;
+                    f[x] = left ? __shfl_sync(0xffffffffu, c, e) : 0.f;
+                    const float* from = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(rows), e)) + in * D;
+                    left &= left - 1;
+#pragma unroll
+                    for (int i = 0; i < kQuads; ++i)
+                        y[x][i] = *reinterpret_cast<const float4*>(from + min(4 * lane + 128 * i, D - 4));
                 }
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int i = 0; i < kQuads; ++i) {
+                        o[i].x = fmaf(y[x][i].x, f[x], o[i].x), o[i].y = fmaf(y[x][i].y, f[x], o[i].y);
+                        o[i].z = fmaf(y[x][i].z, f[x], o[i].z), o[i].w = fmaf(y[x][i].w, f[x], o[i].w);
+                    }
             }
             if (whole) {
                 const int64_t out_row = (int64_t)b * a.q_heads + (int64_t)h * a.group + row0 + row;
@@ -1088,6 +1116,13 @@ struct KvAttendInstance {
             if (Shape::kWarps % d == 0) split.row_warps = d;
         const int chunk_rows = split.row_warps * 8 * RT;
         split.chunks = (a.group + chunk_rows - 1) / chunk_rows;
+        split.per_seq = pool.heads * split.chunks;
+        split.teams = Shape::kWarps / split.row_warps;
+        split.by_ctas = KvDiv(work.ctas);
+        split.by_per_seq = KvDiv(split.per_seq);
+        split.by_teams = KvDiv(split.teams);
+        split.by_page = KvDiv(pool.records_per_page);
+        split.by_chunks = KvDiv(split.chunks);
         split.unit = work.unit;
         split.more = work.more;
         split.slots = work.slots;

@@ -98,30 +98,33 @@ __device__ __forceinline__ void load_row(const void* p, int64_t at, int type, in
         x[2 * i] = v.x, x[2 * i + 1] = v.y;
     }
 }
+// elements one by one, out of line: for rows that are not aligned
+__device__ __noinline__ inline void store_elements(void* p, int type, int n, float a, float b, float c, float d) {
+    for (int i = 0; i < n; ++i) {
+        const float y = i == 0 ? a : i == 1 ? b : i == 2 ? c : d;
+        if (type == kTypeF32) static_cast<float*>(p)[i] = y;
+        else static_cast<uint16_t*>(p)[i] = (uint16_t)(type == kTypeF16 ? f16x2_of(y, 0.f) : bf16x2_of(y, 0.f));
+    }
+}
 template <int N>
 __device__ __forceinline__ void store_row(void* p, int64_t at, int type, int vec, const float (&x)[N]) {
-    if (type == kTypeF32) {
-        float* f = static_cast<float*>(p) + at;
-        if (vec) {
+    uint8_t* dst = static_cast<uint8_t*>(p) + at * (type == kTypeF32 ? 4 : 2);
+    if (!vec) {
 #pragma unroll
-            for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(f + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) f[i] = x[i];
-        }
+        for (int i = 0; i < N; i += 4)
+            store_elements(dst + i * (type == kTypeF32 ? 4 : 2), type, 4, x[i], x[i + 1], x[i + 2], x[i + 3]);
         return;
     }
-    uint16_t* h = static_cast<uint16_t*>(p) + at;
+    if (type == kTypeF32) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(dst + 4 * i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+        return;
+    }
     uint32_t w[N / 2];
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) w[i] = type == kTypeF16 ? f16x2_of(x[2 * i], x[2 * i + 1]) : bf16x2_of(x[2 * i], x[2 * i + 1]);
-    if (vec) {
-        if constexpr (N == 8) *reinterpret_cast<uint4*>(h) = make_uint4(w[0], w[1], w[2], w[3]);
-        else *reinterpret_cast<uint2*>(h) = make_uint2(w[0], w[1]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) h[2 * i] = (uint16_t)w[i], h[2 * i + 1] = (uint16_t)(w[i] >> 16);
-    }
+    if constexpr (N == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
 }
 
 }  // namespace eosb
