@@ -3781,8 +3781,8 @@ int eos_b200_kv_cache_create(EosB200Runtime* rt, int64_t pages, int page_size, i
     c->pool = p;
     if (e == cudaSuccess) e = dev_alloc(&c->work.partial, kv_work_floats(rt->sm_count, head_dim));
     if (e == cudaSuccess) e = dev_alloc(&c->work.slots, (size_t)rt->sm_count * kKvSlotFloats);
-    if (e == cudaSuccess) e = dev_alloc(&c->work.unit, (size_t)2 * rt->sm_count);
-    if (e == cudaSuccess) e = dev_alloc(&c->work.more, (size_t)rt->sm_count);
+    if (e == cudaSuccess) e = dev_alloc(&c->work.count, (size_t)3 * rt->sm_count);
+    if (e == cudaSuccess) e = cudaMemsetAsync(c->work.count, 0, (size_t)3 * rt->sm_count * sizeof(int), rt->stream);
     if (e == cudaSuccess) e = cudaMemsetAsync(p.base, 0, (size_t)(pages * page_bytes), rt->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(rt->stream);
     if (e != cudaSuccess) {
@@ -3800,8 +3800,7 @@ void eos_b200_kv_cache_destroy(EosB200KvCache* c) {
     dev_free(c->pool.base);
     dev_free(c->work.slots);
     dev_free(c->work.partial);
-    dev_free(c->work.unit);
-    dev_free(c->work.more);
+    dev_free(c->work.count);
     delete c;
 }
 
@@ -3866,8 +3865,8 @@ int eos_b200_kv_cache_attend_device(EosB200KvCache* c, const void* d_query, int 
     if (d_query == nullptr || d_page_table == nullptr || d_lengths == nullptr || d_out == nullptr)
         return fail(err, "kv_cache_attend: null argument");
     if (max_pages <= 0) return fail(err, "kv_cache_attend: max_pages must be positive");
-    if (reinterpret_cast<uintptr_t>(d_query) % type_bytes(type) != 0 || reinterpret_cast<uintptr_t>(d_out) % type_bytes(type) != 0)
-        return fail(err, "kv_cache_attend: query or out is not aligned to its element type");
+    if (reinterpret_cast<uintptr_t>(d_query) % type_bytes(type) != 0) return fail(err, "kv_cache_attend: query is not aligned to its element type");
+    if (reinterpret_cast<uintptr_t>(d_out) % 16 != 0) return fail(err, "kv_cache_attend: out must be 16-byte aligned");
     KvSeqs seqs = {d_page_table, max_pages, batch, nullptr, nullptr, d_lengths};
     KvAttend a{};
     a.query = d_query;
@@ -3878,7 +3877,6 @@ int eos_b200_kv_cache_attend_device(EosB200KvCache* c, const void* d_query, int 
     a.q_heads = q_heads;
     a.group = q_heads / c->pool.heads;
     a.out = d_out;
-    a.out_vec = reinterpret_cast<uintptr_t>(d_out) % 16 == 0 ? 1 : 0;
     a.lse = d_lse;
     a.scale_log2 = (float)((double)scale * 1.4426950408889634);
     a.window = window;

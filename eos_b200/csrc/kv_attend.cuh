@@ -27,6 +27,13 @@
 
 namespace eosb {
 
+// A value that the compiler takes for a new one each time: a condition on it inside a loop does not double the loop.  The
+// code that runs once or seldom is most of the kernel, and comes from the L2 while the records do.
+__device__ __forceinline__ int opaque(int x) {
+    asm volatile("" : "+r"(x));
+    return x;
+}
+
 constexpr float kKvMaxInit = -1e30f;   // below every score; finite, so that 2^(x - m) of a masked score is 0 and not NaN
 constexpr float kKvHead = 7.f, kKvLag = 15.f;   // m = ceil(largest score) - 7; weights up to 2^15
 constexpr int kKvQueryExp = 13;                  // query rows are scaled to a largest magnitude in [2^13, 2^14)
@@ -174,7 +181,8 @@ struct KvWarp {
     // at once and waited for in convert_query, ...
     __device__ __forceinline__ void load_query(const KvAttend& a, int64_t at, int row0, int rows, int lane) {
         const int g = lane >> 2, t = lane & 3;
-        const bool wide = HALVES == 2 && a.type == kTypeF32;
+        const bool wide = HALVES == 2 && opaque(a.type) == kTypeF32;   // two 16-byte loads a block, else one
+        const int vec = opaque(a.vec);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             const int row = row0 + 8 * r + g;
@@ -182,48 +190,37 @@ struct KvWarp {
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int i = 0; i < 4 * HALVES; ++i) q[r][b][i] = 0u;
-            if (row >= rows) continue;
-            if (wide) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const uint32_t* w = reinterpret_cast<const uint32_t*>(base) + 32 * b;
-#pragma unroll
-                    for (int i = 0; i < 4 * HALVES; i += 4) {
-                        if (a.vec) {
-                            const uint4 x = *reinterpret_cast<const uint4*>(w + i);
-                            q[r][b][i] = x.x, q[r][b][i + 1] = x.y, q[r][b][i + 2] = x.z, q[r][b][i + 3] = x.w;
-                        } else {
-                            q[r][b][i] = w[i], q[r][b][i + 1] = w[i + 1], q[r][b][i + 2] = w[i + 2], q[r][b][i + 3] = w[i + 3];
-                        }
+                for (int i = 0; i < 4 * HALVES; i += 4) {
+                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                    const uint8_t* from = base + b * (wide ? 128 : 64) + 4 * i;
+                    if (row < rows && (i == 0 || wide)) {
+                        if (vec) x = *reinterpret_cast<const uint4*>(from);
+                        else x = load16_unaligned(from);
                     }
+                    q[r][b][i] = x.x, q[r][b][i + 1] = x.y, q[r][b][i + 2] = x.z, q[r][b][i + 3] = x.w;
                 }
-            } else {
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const uint16_t* w = reinterpret_cast<const uint16_t*>(base) + 32 * b;
-                    if (a.vec) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(w);
-                        q[r][b][0] = x.x, q[r][b][1] = x.y, q[r][b][2] = x.z, q[r][b][3] = x.w;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) q[r][b][i] = (uint32_t)w[2 * i] | ((uint32_t)w[2 * i + 1] << 16);
-                    }
-                }
-            }
         }
     }
     // ... then the operands.  f16: each row is divided by a power of two first, so that no magnitude leaves f16's range.
+    // One operand: the type is f16 or bf16 (over a bf16 cache bf16); two: f32 (or f16).
     __device__ __forceinline__ void convert_query(const KvAttend& a, int lane) {
+        const int type = opaque(a.type);
+        const bool f16 = type == kTypeF16, wide = type == kTypeF32;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            if (HALVES == 2 && a.type == kTypeF32)
-                split_row(a, r, lane, [&](int b, int i) {
-                    return make_float2(__uint_as_float(q[r][b][(2 * i) % (4 * HALVES)]), __uint_as_float(q[r][b][(2 * i + 1) % (4 * HALVES)]));
-                });
-            else if (a.type == kTypeF16) split_row(a, r, lane, [&](int b, int i) { return f16x2_floats(q[r][b][i]); });
-            else split_row(a, r, lane, [&](int b, int i) { return bf16x2_floats(q[r][b][i]); });
-        }
+        for (int r = 0; r < RT; ++r)
+            split_row(a, r, lane, [&](int b, int i) {
+                if constexpr (HALVES == 1) {
+                    const uint32_t w = q[r][b][i];
+                    if constexpr (kBf) return bf16x2_floats(w);
+                    const float2 x = f16x2_floats(w), y = bf16x2_floats(w);
+                    return make_float2(f16 ? x.x : y.x, f16 ? x.y : y.y);
+                } else {
+                    const float2 y = make_float2(__uint_as_float(q[r][b][2 * i]), __uint_as_float(q[r][b][2 * i + 1]));
+                    if constexpr (!kBf) return y;
+                    const float2 x = f16x2_floats(q[r][b][i]);
+                    return make_float2(wide ? y.x : x.x, wide ? y.y : x.y);
+                }
+            });
     }
     template <typename F>
     __device__ __forceinline__ void split_row(const KvAttend& a, int r, int lane, F&& pair) {
@@ -586,10 +583,10 @@ struct KvQuotient {
     float inv, p, q, lse;
     __device__ __forceinline__ KvQuotient(float l, float big, float m) {
         const int k = (int)fminf(fmaxf(big - m, -252.f), 252.f), half = k / 2;   // an integer
-        inv = l == 0.f ? 0.f : 1.f / l;
+        inv = l == 0.f ? 0.f : __fdividef(1.f, l);   // (l stays below 2^126: 2^15 for each of fewer than 2^31 tokens)
         p = __uint_as_float((uint32_t)(half + 127) << 23);
         q = __uint_as_float((uint32_t)(k - half + 127) << 23);
-        lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
+        lse = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.693147180559945309f;
     }
     __device__ __forceinline__ float operator()(float o) const { return o * inv * p * q; }
 };
@@ -599,9 +596,10 @@ struct KvQuotient {
 // the other, are cut into equal ranges, one for each CTA and within it for each warp, wherever the cuts fall: lengths may
 // differ as they like.  A warp writes what it holds of units that lie in its range altogether; at most its first and its
 // last unit are partial.  Partial results are joined in shared memory by the CTA, and what is still partial then (at most
-// two units a CTA) through the workspace by the join kernel.  All joins run in a fixed order: same bits every time.
+// two units a CTA) through the workspace by whichever of the unit's CTAs is done last.  All joins run in a fixed order:
+// same bits every time.  (A second kernel for that join cost 4 to 7 us a call.)
 // ------------------------------------------------------------------------------------------------
-constexpr int kKvJoinThreads = 256;
+constexpr int kKvGroup = 12;        // neighbouring CTAs whose parts are joined first (at most 31 groups of it, for 372 SMs)
 constexpr int kKvMinRecords = 8;    // records of a CTA, at least
 
 // Shape of a CTA.  Each warp (or team of warps that share records) has a ring of records in shared memory, filled by
@@ -628,8 +626,10 @@ struct KvShape {
     static constexpr int kRing = kStages * kRecord;
     static constexpr bool kPair = NB * RT <= 2 && kStages >= 4;  // two records at a time
     static constexpr int kSmem = kWarps * kRing;
-    static_assert(kStages >= 2 && kRing >= 4 * kPartial && kRing % 16 == 0 && kWarps * kPartial <= kKvSlotFloats, "ring");
+    static_assert(kStages >= 2 && kStages <= 16 && kRing >= 4 * kPartial && kRing % 16 == 0 && kWarps * kPartial <= kKvSlotFloats, "ring");
 };
+
+__device__ __noinline__ inline int64_t kv_div64(int64_t a, int64_t b) { return a / b; }
 
 // Division of a number that is not negative by a constant of the launch: below 2^31 floor(a / d) = a m >> s with
 // s = 31 + ceil(log2 d), m = ceil(2^s / d) -- the excess a (m d - 2^s) / (d 2^s) is below 2^31 / 2^s <= 1 / d.
@@ -642,11 +642,11 @@ struct KvDiv {
         m = (uint32_t)(((s < 63 ? 1ull << s : 0) + by - 1) / by);
     }
     __device__ __forceinline__ int64_t operator()(int64_t a) const {
-        return a >> 31 ? a / d : (int64_t)((uint64_t)(uint32_t)a * m >> s);
+        return a >> 31 ? kv_div64(a, d) : (int64_t)((uint64_t)(uint32_t)a * m >> s);
     }
 };
 __device__ __forceinline__ int64_t kv_div(int64_t a, int64_t b) {   // not negative; the 32-bit division is far shorter
-    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : kv_div64(a, b);
 }
 
 struct KvSplit {
@@ -656,8 +656,7 @@ struct KvSplit {
     KvDiv by_ctas, by_per_seq, by_teams, by_page, by_chunks;   // (by_page: records of a page)
     float* slots;                   // [ctas][kKvSlotFloats]: partial results of the warps' first units
     float* partial;                 // [ctas][2][rows][dim + 3]: of the CTAs, numerators of all rows, then (m, big, l) of each
-    int64_t* unit;                  // [ctas][2] unit of each partial (sequence << 32 | unit of the sequence), -1: none
-    int* more;                      // [ctas] CTAs behind this one that hold parts of its last unit
+    int* count;                     // [ctas][2], [ctas]: parts of a group, groups of a unit that are done; zero between calls
 };
 
 // positions of sequence b that are attended to: [lo, hi)
@@ -701,12 +700,31 @@ struct KvWalk {
     }
 };
 
-// One bulk copy of a record into shared memory, its bytes counted on the mbarrier.
-__device__ __forceinline__ void kv_copy_record(uint32_t dst, const uint8_t* src, uint32_t bytes, uint32_t bar) {
+// Where a team's copies are: the walk stands behind the records that are fetched or about to be from the current page.
+struct KvAhead {
+    KvWalk walk;
+    int to_fetch, slot, in;   // records left behind them, slot of the page in the table, first record of the next page
+};
+
+// One bulk copy of a record into shared memory, its bytes counted on the mbarrier.  The records are read once: they make
+// way in the L2 first, so that page tables, partial results and the program itself stay there (2 to 3 us of 60 to 180).
+__device__ __forceinline__ void kv_copy_record(uint32_t dst, const uint8_t* src, uint32_t bytes, uint32_t bar, uint64_t policy) {
     mbar_arrive_expect_tx(bar, bytes);
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(policy)
                  : "memory");
+}
+
+// 16 bytes of a partial result, in shared memory or (other CTAs' too, so not from the L1) in global memory
+__device__ __forceinline__ float4 load_part4(const float* p) {
+    float4 v;
+    asm volatile("ld.relaxed.gpu.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float load_part(const float* p) {
+    float v;
+    asm volatile("ld.relaxed.gpu.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+    return v;
 }
 
 template <int FMT, int NB, int RT, int HALVES>
@@ -720,10 +738,13 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
     __shared__ int64_t s_warp[kWarps];
     __shared__ int64_t s_unit[2 * kWarps];
     __shared__ int s_ends[2 * kWarps];                        // bit 0: the unit begins there, 1: it ends there, 2: in the ring
-    __shared__ int64_t s_until[kWarps];                       // end, among all records, of the unit begun last
+    __shared__ int64_t s_from[2 * kWarps];                    // first record, among all, of the slot's unit, and
+    __shared__ int s_long[2 * kWarps];                        // its records
+    __shared__ int s_turn[2];                                 // whether this CTA joins its first / last unit's parts
     __shared__ __align__(8) uint64_t s_full[kWarps][kMaxStages], s_empty[kWarps][kMaxStages];
     __shared__ uint8_t s_ok[kWarps][kMaxStages];              // whether the record could be fetched
     __shared__ int s_abort, s_drain[kWarps];
+    __shared__ KvAhead s_ahead[kWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per_seq = split.per_seq;
     const int chunk_rows = kRows * split.row_warps;
@@ -739,6 +760,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
     // ---- records of all sequences, scanned by the CTA
     const int per = (seqs.batch + kThreads - 1) / kThreads;
     int64_t mine = 0;
+#pragma unroll 1
     for (int b = tid * per; b < min((tid + 1) * per, seqs.batch); ++b) {
         int lo, hi;
         if (!kv_span(pool, seqs, a.window, b, lo, hi) && blockIdx.x == 0) atomicExch(status, kStatusBadSequence);
@@ -753,7 +775,6 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
     if (lane == 31) s_warp[warp] = upto;
     if (tid < 2 * kWarps) s_unit[tid] = -1;
     if (tid == 0) s_abort = 0;
-    if (tid < 2) split.unit[2 * (int64_t)blockIdx.x + tid] = -1;
     if (rw == 0 && lane < stages) {
         mbar_init(smem_u32(&s_full[team][lane]), 1);
         mbar_init(smem_u32(&s_empty[team][lane]), split.row_warps);
@@ -772,11 +793,10 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
     const int64_t part = max(split.by_ctas(total + gridDim.x - 1), (int64_t)kKvMinRecords);
     const int64_t c0 = min((int64_t)blockIdx.x * part, total), c1 = min(c0 + part, total);
     const int64_t tpart = split.by_teams(c1 - c0 + teams - 1);
-    const int64_t t0 = min(c0 + team * tpart, c1), t1 = min(t0 + tpart, c1);
+    const int64_t t0 = min(c0 + team * tpart, c1);
+    int left = (int)(min(t0 + tpart, c1) - t0);   // records of the team that are not yet done with
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-    if (t1 > t0) {
+    if (left > 0) {
         KvWalk at;
         {
             const int64_t q = split.by_per_seq(t0);   // all units of a sequence have as many records
@@ -785,172 +805,174 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
             i = i * kStep + 31 - __clz(__ballot_sync(0xffffffffu, lane < kStep && s_before[min(i * kStep + lane, kThreads - 1)] <= q));
             at.seek(pool, seqs, a.window, per_seq, q, t0, i * per, s_before[i]);
         }
-        // ---- the copies: the walk of the records to fetch runs `stages` ahead of the one below
-        KvWalk ahead = at;
-        int64_t to_fetch = t1 - t0;
-        const int rpp = pool.records_per_page;
-        // the page of the next record: slot in the table, that record (null: a page id out of range), records left there
-        int slot = 0, run = 0, next_page = -1;
-        const uint8_t* src = nullptr;
-        const uint32_t ring_at = smem_u32(smem + team * split.row_warps * Shape::kRing), full_at = smem_u32(&s_full[team][0]);
-        auto page_at = [&](int sl) { return sl < seqs.max_pages ? __ldg(seqs.table + (int64_t)ahead.b * seqs.max_pages + sl) : -1; };
-        auto enter_page = [&](int page, int in) {
-            run = min(rpp - in, ahead.n - ahead.r);
+        // The copies, by the team's first warp: the walk of the records to fetch runs a ring ahead of the one below.  What it
+        // needs at the end of a page only waits in shared memory.
+        const uint8_t* src = nullptr;   // the next record (null: a page id out of range)
+        int run = 0;                    // records to fetch from there on the page
+        int next_page = -1;             // page id of the next slot of the page table, asked for early
+        KvAhead& ahead = s_ahead[warp];
+        if (rw == 0) {
+            const int rec = at.lo / kKvRecord + at.r, slot = (int)split.by_page(rec);
+            next_page = __ldg(seqs.table + (int64_t)at.b * seqs.max_pages + slot);   // (kv_span cuts at max_pages)
+            if (lane == 0) ahead = {at, left, slot - 1, rec - slot * pool.records_per_page};
+            __syncwarp();
+        }
+        auto another_page = [&]() {     // false: nothing left to fetch
+            KvWalk x = ahead.walk;
+            int to_fetch = ahead.to_fetch, slot = ahead.slot + 1, in = ahead.in, page = next_page;
+            if (to_fetch == 0) return false;
+            if (x.r == x.n) {
+                x.next_unit(pool, seqs, a.window, per_seq);
+                slot = (int)split.by_page(x.lo / kKvRecord);
+                in = x.lo / kKvRecord - slot * pool.records_per_page;
+                page = __ldg(seqs.table + (int64_t)x.b * seqs.max_pages + slot);
+            }
+            run = min(min(pool.records_per_page - in, x.n - x.r), to_fetch);
             src = page < 0 || page >= pool.pages
                       ? nullptr
-                      : pool.base + (((int64_t)page * pool.heads + (int)split.by_chunks(ahead.hu)) * rpp + in) * Shape::kRecord;
-            next_page = page_at(slot + 1);   // asked for early: its latency passes while this page is read
+                      : pool.base + (((int64_t)page * pool.heads + (int)split.by_chunks(x.hu)) * pool.records_per_page + in) * Shape::kRecord;
+            if (slot + 1 < seqs.max_pages) next_page = __ldg(seqs.table + (int64_t)x.b * seqs.max_pages + slot + 1);
+            x.r += run;
+            __syncwarp();
+            if (lane == 0) ahead = {x, to_fetch - run, slot, 0};
+            __syncwarp();
+            return true;
         };
-        auto enter_unit = [&]() {
-            const int rec = ahead.lo / kKvRecord + ahead.r;
-            slot = (int)split.by_page(rec);
-            enter_page(page_at(slot), rec - slot * rpp);
-        };
-        auto fetch = [&](int stage) {   // the next record, if there is one, into `stage`
-            if (to_fetch == 0) return;
-            if (lane == 0) {
-                s_ok[team][stage] = src != nullptr;
-                if (src != nullptr) {
-                    kv_copy_record(ring_at + stage * Shape::kRecord, src, Shape::kRecord, full_at + 8 * stage);
-                } else {
-                    atomicExch(status, kStatusBadPage);
-                    mbar_arrive(full_at + 8 * stage);
-                }
-            }
-            --to_fetch;
-            ++ahead.r;
-            if (src != nullptr) src += Shape::kRecord;
-            if (--run == 0 && to_fetch > 0) {
-                if (ahead.r == ahead.n) {
-                    ahead.next_unit(pool, seqs, a.window, per_seq);
-                    enter_unit();
-                } else {
-                    ++slot;
-                    enter_page(next_page, 0);
-                }
-            }
-        };
+        const uint32_t ring_at = smem_u32(smem + team * split.row_warps * Shape::kRing), full_at = smem_u32(&s_full[team][0]),
+                       empty_at = smem_u32(&s_empty[team][0]);
+        uint64_t policy;
+        asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+
         KvWarp<FMT, NB, RT, HALVES> w;
-        auto ask_query = [&]() {
+        int stage = 0, fill = 0, empty = rw == 0 ? stages : 0;   // stage to read next; stage to fill next, stages to fill
+        uint32_t phase = 0, fill_phase = 1;
+        bool alive = true;   // no wait has run out
+#pragma unroll 1
+        while (true) {
+            int seg = min(at.n - at.r, left);   // records of the unit here
             const int h = (int)split.by_chunks(at.hu), row0 = (at.hu - h * split.chunks) * chunk_rows + rw * kRows;
             w.load_query(a, (int64_t)at.b * a.seq_stride + (int64_t)h * a.group * a.head_stride, row0, a.group, lane);
-        };
-        ask_query();
-        if (rw == 0) {
-            enter_unit();
-            for (int i = 0; i < stages; ++i) fetch(i);
-        }
-        int stage = 0;
-        uint32_t phase = 0;
-        bool alive = true;          // no wait has run out
-        int dead_stage = -1;         // the last stage that a wait was good for, and its phase
-        uint32_t dead_phase = 0;
-        int64_t left = t1 - t0;
-        const uint8_t* ring = smem + team * split.row_warps * Shape::kRing;
-        while (true) {
-            const int b = at.b, seg = (int)min((int64_t)(at.n - at.r), left);
-            const bool begins = at.r == 0, ends = at.r + seg == at.n;
-            const int h = (int)split.by_chunks(at.hu), row0 = (at.hu - h * split.chunks) * chunk_rows + rw * kRows;
-            w.reset();
             w.convert_query(a, lane);
-            int first = (at.lo / kKvRecord + at.r) * kKvRecord;   // position of the record's first token
-            auto arrived = [&](int st, uint32_t ph) { alive = alive && mbar_wait(full_at + 8 * st, ph, &s_abort); };
-            auto release = [&](int st, uint32_t ph) {
-                if (split.row_warps > 1) {
-                    if (lane == 0) mbar_arrive(smem_u32(&s_empty[team][st]));
-                    if (rw == 0 && to_fetch > 0) alive = alive && mbar_wait(smem_u32(&s_empty[team][st]), ph, &s_abort);
+            w.reset();
+            // the unit's span relative to the next record's first token
+            int lo = at.lo - (at.lo / kKvRecord + at.r) * kKvRecord, hi = lo + at.hi - at.lo;
+            const int row_warps = opaque(split.row_warps);
+#pragma unroll 1
+            for (int j = seg; j > 0;) {
+#pragma unroll 1
+                while (empty > 0 && alive) {
+                    if (run == 0 && !another_page()) {
+                        empty = -0x40000000;   // never again
+                        break;
+                    }
+                    // every warp of the team is done with what the stage held (true at once the first time round)
+                    if (row_warps > 1) alive = mbar_wait(empty_at + 8 * fill, fill_phase, &s_abort);
+                    if (!alive) break;
+                    if (lane == 0) {
+                        s_ok[team][fill] = src != nullptr;
+                        if (src != nullptr) {
+                            kv_copy_record(ring_at + fill * Shape::kRecord, src, Shape::kRecord, full_at + 8 * fill, policy);
+                        } else {
+                            atomicExch(status, kStatusBadPage);
+                            mbar_arrive(full_at + 8 * fill);
+                        }
+                    }
+                    if (src != nullptr) src += Shape::kRecord;
+                    --run;
+                    --empty;
+                    if (++fill == stages) fill = 0, fill_phase ^= 1u;
                 }
-                if (alive) {
-                    if (rw == 0) fetch(st);
-                    dead_stage = st, dead_phase = ph;
-                }
-            };
-            for (int j = 0; j < seg;) {
+                const int take = Shape::kPair && j > 1 ? 2 : 1;
                 const int next = stage + 1 == stages ? 0 : stage + 1;
-                const uint32_t next_phase = next == 0 ? phase ^ 1u : phase;
-                const uint8_t* here = ring + stage * Shape::kRecord;
-                const int lo = max(at.lo - first, 0), hi = at.hi - first;
-                arrived(stage, phase);
-                if (Shape::kPair && j + 1 < seg) {
-                    arrived(next, next_phase);
-                    const uint8_t* there = ring + next * Shape::kRecord;
-                    const bool ok0 = s_ok[team][stage], ok1 = s_ok[team][next];
-                    if (alive && ok0 && ok1) {
-                        const uint8_t* const both[2] = {here, there};
-                        w.template records<2>(both, lo, min(hi, 2 * kKvRecord), lane);
-                    } else if (alive && (ok0 || ok1)) {
-                        // the tokens of the record that is missing are left out
-                        const uint8_t* const one[1] = {ok0 ? here : there};
-                        w.template records<1>(one, ok0 ? lo : 0, min(ok0 ? hi : hi - kKvRecord, kKvRecord), lane);
+                alive = alive && mbar_wait(full_at + 8 * stage, phase, &s_abort);
+                const uint8_t* here = smem + team * split.row_warps * Shape::kRing + stage * Shape::kRecord;
+                const bool ok = alive && s_ok[team][stage];
+                bool one = ok;
+                int shift = 0;
+                if constexpr (Shape::kPair) {
+                    if (take == 2) {
+                        alive = alive && mbar_wait(full_at + 8 * next, next == 0 ? phase ^ 1u : phase, &s_abort);
+                        const uint8_t* there = smem + team * split.row_warps * Shape::kRing + next * Shape::kRecord;
+                        const bool ok2 = alive && s_ok[team][next];
+                        one = ok != ok2;   // a record that is missing is left out
+                        if (ok && ok2) {
+                            const uint8_t* const both[2] = {here, there};
+                            w.template records<2>(both, max(lo, 0), min(hi, 2 * kKvRecord), lane);
+                        } else if (ok2) {
+                            here = there;
+                            shift = kKvRecord;
+                        }
                     }
-                    __syncwarp();
-                    release(stage, phase);
-                    release(next, next_phase);
-                    stage = next + 1 == stages ? 0 : next + 1;
-                    phase = stage == 0 ? next_phase ^ 1u : next_phase;
-                    j += 2;
-                    first += 2 * kKvRecord;
-                } else {
-                    if (alive && s_ok[team][stage]) {
-                        const uint8_t* const one[1] = {here};
-                        w.template records<1>(one, lo, min(hi, kKvRecord), lane);
-                    }
-                    __syncwarp();
-                    release(stage, phase);
-                    stage = next, phase = next_phase;
-                    ++j;
-                    first += kKvRecord;
                 }
+                if (one) {
+                    const uint8_t* const single[1] = {here};
+                    w.template records<1>(single, max(lo - shift, 0), min(hi - shift, kKvRecord), lane);
+                }
+                __syncwarp();
+                if (row_warps > 1 && lane == 0) {
+                    mbar_arrive(empty_at + 8 * stage);
+                    if (take == 2) mbar_arrive(empty_at + 8 * next);
+                }
+                j -= take;
+                if (rw == 0) empty += take;
+                lo -= take * kKvRecord;
+                hi -= take * kKvRecord;
+                stage += take;
+                if (stage >= stages) stage -= stages, phase ^= 1u;
             }
+            const bool begins = at.r == 0, ends = at.r + seg == at.n;
             if (begins && ends) {
                 const int g = lane >> 2, t = lane & 3;
+                const int64_t out0 = (int64_t)at.b * a.q_heads + split.by_chunks(at.hu) * a.group;
 #pragma unroll
                 for (int k = 0; k < RT; ++k)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        const float l = w.denominator(k, c);   // (all lanes)
+                        const float l = w.denominator(k, c);
                         const int row = row0 + 8 * k + 2 * t + c;
-                        if (row >= a.group) continue;
-                        const int64_t out_row = (int64_t)b * a.q_heads + (int64_t)h * a.group + row;
-                        const KvQuotient f(l, FMT >= kKvMx8 ? w.big[k][c] : w.m[k][c], w.m[k][c]);
-                        if (g == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
+                        if (row < a.group) {
+                            const KvQuotient f(l, FMT >= kKvMx8 ? w.big[k][c] : w.m[k][c], w.m[k][c]);
+                            if (g == 0 && a.lse != nullptr) a.lse[out0 + row] = f.lse;
 #pragma unroll
-                        for (int blk = 0; blk < NB; ++blk) {
-                            const float4 o = w.numerators(k, c, blk);
-                            const float y[4] = {f(o.x), f(o.y), f(o.z), f(o.w)};
-                            store_row<4>(a.out, out_row * D + 32 * blk + 4 * g, a.type, a.out_vec, y);
+                            for (int blk = 0; blk < NB; ++blk) {
+                                const float4 o = w.numerators(k, c, blk);
+                                const float y[4] = {f(o.x), f(o.y), f(o.z), f(o.w)};
+                                store_row<4>(a.out, (out0 + row) * D + 32 * blk + 4 * g, a.type, 1, y);
+                            }
                         }
                     }
             } else {
                 const int which = begins ? 1 : 0;
                 const bool last = left == seg;
-                if (last && split.row_warps > 1) named_bar_sync(1 + team, 32 * split.row_warps);   // the ring is free
+                if (last && row_warps > 1) named_bar_sync(1 + team, 32 * row_warps);   // the ring is free
                 float* rows = slot_rows(warp, last);
                 w.store_partial(rows, rows + kRows * D, lane);
                 if (lane == 0) {
-                    s_unit[2 * warp + which] = (int64_t)b << 32 | at.hu;
+                    s_unit[2 * warp + which] = (int64_t)at.b << 32 | at.hu;
                     s_ends[2 * warp + which] = (begins ? 1 : 0) | (ends ? 2 : 0) | (last ? 4 : 0);
-                    if (begins) s_until[warp] = t1 - seg + at.n;   // (it is the range's last segment)
+                    s_from[2 * warp + which] = min(t0 + tpart, c1) - left - at.r;
+                    s_long[2 * warp + which] = at.n;
                 }
             }
             left -= seg;
             if (left == 0) break;
             at.next_unit(pool, seqs, a.window, per_seq);
-            ask_query();
         }
         if (!alive && lane == 0) {
             atomicExch(status, kStatusPipelineTimeout);
-            // the copies still under way (of the stages behind the last good one) must land before the CTA leaves
+            // the copies still under way must land before the CTA leaves: the last fill of every stage
             for (int i = 0; rw == 0 && i < stages; ++i) {
                 s_drain[warp] = 0;
-                mbar_wait_limit(smem_u32(&s_full[team][i]), i > dead_stage ? dead_phase : dead_phase ^ 1u, &s_drain[warp], 100000000LL);
+                mbar_wait_limit(full_at + 8 * i, i < fill ? fill_phase ^ 1u : fill_phase, &s_drain[warp], 100000000LL);
             }
         }
     }
     __syncthreads();
 
-    // ---- join of the CTA's partial results: runs of equal units among the teams' slots, in order.  Lane e looks at slot e
-    // % 2 of team e / 2; one warp joins one row of a run.
+    // ---- Joins.  Phase 0: the partial results of the CTA's warps, runs of equal units among the teams' slots, in order (lane e
+    // looks at slot e % 2 of team e / 2).  What is whole then is final.  Units that several CTAs hold parts of: of every 12
+    // neighbours the one that is done last joins their parts (phase 1), and of these the last one joins the unit's groups
+    // (phase 2).  What is joined, and in which order, is fixed.  One warp joins one row of a task.
     {
         auto slot_of = [&](int e, int k) { return 2 * ((e >> 1) * split.row_warps + k) + (e & 1); };   // entry e, row warp k
         const int mine_at = slot_of(min(lane, 2 * teams - 1), 0);
@@ -960,73 +982,149 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
         const uint32_t starts = __ballot_sync(0xffffffffu, unit >= 0 && (before == 0 || last != unit));
         const uint32_t begun = __ballot_sync(0xffffffffu, unit >= 0 && (s_ends[mine_at] & 1)),
                        ended = __ballot_sync(0xffffffffu, unit >= 0 && (s_ends[mine_at] & 2));
-        const int rows_used = min(chunk_rows, a.group), items = __popc(starts) * rows_used;
-        for (int item = warp; item < items; item += kWarps) {
-            const int run = item / rows_used, row = item - run * rows_used, k = row / kRows, in = row - k * kRows;
-            uint32_t rest = starts;
-            for (int i = 0; i < run; ++i) rest &= rest - 1;
-            const int e0 = __ffs(rest) - 1;
-            rest &= rest - 1;
-            const uint32_t members = valid & ~((1u << e0) - 1u) & (rest ? (rest & -rest) - 1u : 0xffffffffu);
-            const int64_t u = __shfl_sync(0xffffffffu, unit, e0);
-            const int b = (int)(u >> 32), hu = (int)u, h = hu / split.chunks, row0 = (hu - h * split.chunks) * chunk_rows;
-            const bool whole = (begun & members) && (ended & members);
-            if (whole && row0 + row >= a.group) continue;
-            const bool member = members >> lane & 1u;
-            const int sl = slot_of(member ? lane : e0, k);
-            const float* rows = slot_rows(sl >> 1, s_ends[sl] & 4);   // lane e: the partial result of slot e
-            const float* st = rows + kRows * D + 3 * in;
-            const float m = warp_max(st[0]), big = warp_max(st[1]);
-            const float l = warp_sum(member ? st[2] * ex2(st[0] - m) : 0.f);
-            const float c = member ? ex2(st[1] - big) : 0.f;
-            constexpr int kQuads = (D + 127) / 128;
-            float4 o[kQuads];
+        const int rows_used = min(chunk_rows, a.group);
+        auto run_from = [&](int e0) {   // the slots of the run that starts at e0
+            const uint32_t later = starts & ~((2u << e0) - 1u);
+            return valid & ~((1u << e0) - 1u) & (later ? (later & -later) - 1u : 0xffffffffu);
+        };
+        // the CTA's partial result of a unit that began before it (0) or goes on behind it (1)
+        auto partial_of = [&](int64_t cta, int which) { return split.partial + (2 * cta + which) * chunk_rows * (D + 3); };
+        // the CTA's units that are not whole in it: the first run's, if it began before the CTA, and the last run's, if it goes on
+        const int e_first = starts ? __ffs(starts) - 1 : 0, e_last = starts ? 31 - __clz(starts) : 0;
+        const uint32_t m_first = starts ? run_from(e_first) : 0u, m_last = starts ? run_from(e_last) : 0u;
+        const bool open_first = m_first && !(begun & m_first), open_last = m_last && (begun & m_last) && !(ended & m_last);
+        int owner[2], parts[2];         // the CTA that such a unit begins in, and how many hold parts of it
+        bool turn[2];                   // whether this CTA joins them
+#pragma unroll 1
+        for (int phase_no = 0; phase_no < 3; ++phase_no) {
+            if (phase_no == 1) {
+                if (!open_first && !open_last) break;
 #pragma unroll
-            for (int i = 0; i < kQuads; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (uint32_t left = members; left;) {
-                float4 y[4][kQuads];
-                float f[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {   // four loads on their way at once; the last slot again, times 0, at the end
-                    const int e = left ? __ffs(left) - 1 : e0;
-                    f[x] = left ? __shfl_sync(0xffffffffu, c, e) : 0.f;
-                    const float* from = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(rows), e)) + in * D;
-                    left &= left - 1;
-#pragma unroll
-                    for (int i = 0; i < kQuads; ++i)
-                        y[x][i] = *reinterpret_cast<const float4*>(from + min(4 * lane + 128 * i, D - 4));
+                for (int i = 0; i < 2; ++i) {
+                    const int at_slot = slot_of(i ? e_last : e_first, 0);
+                    owner[i] = (int)kv_div(s_from[at_slot], part);
+                    parts[i] = (int)kv_div(s_from[at_slot] + s_long[at_slot] - 1, part) - owner[i] + 1;
                 }
+            }
+            if (phase_no > 0) {
+                __syncthreads();   // the CTA's parts are written
+                if (tid < 64 && lane == 0) {   // warp 0 for the first unit, warp 1 for the last
+                    const int i = tid >> 5;
+                    const int group = ((int)blockIdx.x - owner[i]) / kKvGroup, groups = (parts[i] + kKvGroup - 1) / kKvGroup;
+                    const int lead = owner[i] + group * kKvGroup;
+                    int* count = phase_no == 1 ? split.count + 2 * lead + (lead == owner[i] ? 1 : 0) : split.count + 2 * gridDim.x + owner[i];
+                    const int of = phase_no == 1 ? min(kKvGroup, parts[i] - group * kKvGroup) : groups;
+                    bool mine_now = false;
+                    if (phase_no == 1 ? (i ? open_last : open_first) : (s_turn[i] && groups > 1)) {
+                        __threadfence();
+                        mine_now = atomicAdd(count, 1) == of - 1;
+                        if (mine_now) *count = 0;   // for the next call
+                        __threadfence();
+                    }
+                    s_turn[i] = mine_now;
+                }
+                __syncthreads();
+                turn[0] = s_turn[0], turn[1] = s_turn[1];
+                if (!turn[0] && !turn[1]) break;
+            }
+            const int tasks = phase_no == 0 ? __popc(starts) : 2;
+#pragma unroll 1
+            for (int item = warp; item < tasks * rows_used; item += kWarps) {
+                const int task = item / rows_used, row = item - task * rows_used;
+                // where the results to join lie, one a lane, and where the joined one goes
+                const float *from, *from_stats;
+                float* to;
+                uint32_t members;
+                int64_t u;
+                bool final_row;
+                if (phase_no == 0) {
+                    const int k = row / kRows, in = row - k * kRows;
+                    uint32_t rest = starts;
+                    for (int i = 0; i < task; ++i) rest &= rest - 1;
+                    const int e0 = __ffs(rest) - 1;
+                    members = run_from(e0);
+                    const int sl = slot_of(members >> lane & 1u ? lane : e0, k);
+                    const float* rows = slot_rows(sl >> 1, s_ends[sl] & 4);
+                    from = rows + in * D;
+                    from_stats = rows + kRows * D + 3 * in;
+                    u = __shfl_sync(0xffffffffu, unit, e0);
+                    final_row = (begun & members) && (ended & members);
+                    to = partial_of(blockIdx.x, begun & members ? 1 : 0);
+                } else {
+                    if (!(task ? turn[1] : turn[0])) continue;
+                    const int own = task ? owner[1] : owner[0], all = task ? parts[1] : parts[0];
+                    const int group = ((int)blockIdx.x - own) / kKvGroup, groups = (all + kKvGroup - 1) / kKvGroup;
+                    const int lead = phase_no == 1 ? own + group * kKvGroup : own;
+                    const int n = phase_no == 1 ? min(kKvGroup, all - group * kKvGroup) : groups;
+                    const int cta = lead + (phase_no == 1 ? 1 : kKvGroup) * min(lane, n - 1);
+                    const float* rows = partial_of(cta, cta == own ? 1 : 0);
+                    from = rows + row * D;
+                    from_stats = rows + chunk_rows * D + 3 * row;
+                    members = (1u << n) - 1u;
+                    u = __shfl_sync(0xffffffffu, unit, task ? e_last : e_first);
+                    final_row = phase_no == 2 || groups == 1;
+                    to = partial_of(lead, lead == own ? 1 : 0);
+                }
+                constexpr int kQuads = (D + 127) / 128;   // lane: elements 4 lane + 128 i .. + 3
+                const bool member = members >> lane & 1u;
+                float s[3] = {kKvMaxInit, kKvMaxInit, 0.f};
+                if (member) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
+                    for (int i = 0; i < 3; ++i) s[i] = load_part(from_stats + i);
+                }
+                float4 o[kQuads];
+#pragma unroll
+                for (int i = 0; i < kQuads; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                float m = 0.f, big = 0.f, l = 0.f, c = 0.f;
+                const int any = __ffs(members) - 1;
+                for (uint32_t rest = members, round = 0; rest; ++round) {
+                    float4 y[4][kQuads];
+                    int e[4];
+                    bool real[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {   // four on their way at once; the first result again, times 0, at the end
+                        real[x] = rest != 0;
+                        e[x] = rest ? __ffs(rest) - 1 : any;
+                        rest &= rest - 1;
+                        const float* row_at = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(from), e[x]));
+#pragma unroll
+                        for (int i = 0; i < kQuads; ++i) y[x][i] = load_part4(row_at + min(4 * lane + 128 * i, D - 4));
+                    }
+                    if (round == 0) {   // (while the first rows are on their way)
+                        m = warp_max(s[0]);
+                        big = warp_max(s[1]);
+                        l = warp_sum(s[2] * ex2(s[0] - m));
+                        c = member ? ex2(s[1] - big) : 0.f;
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        float f = __shfl_sync(0xffffffffu, c, e[x]);
+                        if (!real[x]) f = 0.f;
+#pragma unroll
+                        for (int i = 0; i < kQuads; ++i) {
+                            o[i].x = fmaf(y[x][i].x, f, o[i].x), o[i].y = fmaf(y[x][i].y, f, o[i].y);
+                            o[i].z = fmaf(y[x][i].z, f, o[i].z), o[i].w = fmaf(y[x][i].w, f, o[i].w);
+                        }
+                    }
+                }
+                if (final_row) {
+                    const int hu = (int)u, h = (int)split.by_chunks(hu), at_row = (hu - h * split.chunks) * chunk_rows + row;
+                    if (at_row >= a.group) continue;   // a row behind the key head's last query head
+                    const int64_t out_row = (u >> 32) * a.q_heads + (int64_t)h * a.group + at_row;
+                    const KvQuotient f(l, big, m);
 #pragma unroll
                     for (int i = 0; i < kQuads; ++i) {
-                        o[i].x = fmaf(y[x][i].x, f[x], o[i].x), o[i].y = fmaf(y[x][i].y, f[x], o[i].y);
-                        o[i].z = fmaf(y[x][i].z, f[x], o[i].z), o[i].w = fmaf(y[x][i].w, f[x], o[i].w);
+                        const float y[4] = {f(o[i].x), f(o[i].y), f(o[i].z), f(o[i].w)};
+                        if (4 * lane + 128 * i < D) store_row<4>(a.out, out_row * D + 4 * lane + 128 * i, a.type, 1, y);
                     }
-            }
-            if (whole) {
-                const int64_t out_row = (int64_t)b * a.q_heads + (int64_t)h * a.group + row0 + row;
-                const KvQuotient f(l, big, m);
+                    if (lane == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
+                } else {
 #pragma unroll
-                for (int i = 0; i < kQuads; ++i) {
-                    const int d = 4 * lane + 128 * i;
-                    const float y[4] = {f(o[i].x), f(o[i].y), f(o[i].z), f(o[i].w)};
-                    if (d < D) store_row<4>(a.out, out_row * D + d, a.type, a.out_vec, y);
-                }
-                if (lane == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
-            } else {
-                const int which = begun & members ? 1 : 0;
-                float* po = split.partial + (2 * (int64_t)blockIdx.x + which) * chunk_rows * (D + 3);
-#pragma unroll
-                for (int i = 0; i < kQuads; ++i)
-                    if (4 * lane + 128 * i < D) *reinterpret_cast<float4*>(po + row * D + 4 * lane + 128 * i) = o[i];
-                if (lane == 0) {
-                    float* ps = po + chunk_rows * D + 3 * row;
-                    ps[0] = m, ps[1] = big, ps[2] = l;
-                    if (row == 0) {
-                        split.unit[2 * (int64_t)blockIdx.x + which] = u;
-                        // CTA of the unit's last record
-                        if (which) split.more[blockIdx.x] = (int)kv_div(s_until[slot_of(e0, 0) >> 1] - 1, part) - (int)blockIdx.x;
+                    for (int i = 0; i < kQuads; ++i)
+                        if (4 * lane + 128 * i < D) *reinterpret_cast<float4*>(to + row * D + 4 * lane + 128 * i) = o[i];
+                    if (lane == 0) {
+                        float* to_stats = to + chunk_rows * D + 3 * row;
+                        to_stats[0] = m, to_stats[1] = big, to_stats[2] = l;
                     }
                 }
             }
@@ -1034,71 +1132,19 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
     }
 
     // ---- sequences with nothing to attend to
+#pragma unroll 1
     for (int64_t b = blockIdx.x; b < seqs.batch; b += gridDim.x) {
         int lo, hi;
         kv_span(pool, seqs, a.window, (int)b, lo, hi);
         if (hi > lo) continue;
         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
         for (int i = tid; i < a.q_heads * (D / 4); i += kThreads)
-            store_row<4>(a.out, b * a.q_heads * D + 4 * i, a.type, a.out_vec, zero);
+            store_row<4>(a.out, b * a.q_heads * D + 4 * i, a.type, 1, zero);
         if (a.lse != nullptr)
+#pragma unroll 1
             for (int i = tid; i < a.q_heads; i += kThreads) a.lse[b * a.q_heads + i] = -INFINITY;
     }
-}
-
-// Units that several CTAs hold parts of: warp (c, row) joins a row of the unit that begins in CTA c and goes on behind it.
-template <int NB>
-__global__ void __launch_bounds__(kKvJoinThreads) kv_join_kernel(KvPool pool, KvAttend a, KvSplit split, int chunk_rows) {
-    constexpr int D = 32 * NB, kQuads = (D + 127) / 128;
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // the attention kernel's results
-    const int c = blockIdx.x, lane = threadIdx.x & 31, row = blockIdx.y * (kKvJoinThreads / 32) + (threadIdx.x >> 5);
-    const int64_t u = split.unit[2 * (int64_t)c + 1];
-    if (u < 0 || row >= chunk_rows) return;
-    const int more = split.more[c];
-    const int b = (int)(u >> 32), hu = (int)u, h = hu / split.chunks, row0 = (hu - h * split.chunks) * chunk_rows;
-    if (row0 + row >= a.group) return;
-    const int64_t stride = (int64_t)chunk_rows * (D + 3);
-    auto part = [&](int k) { return split.partial + (2 * (int64_t)(c + k) + (k == 0 ? 1 : 0)) * stride; };
-    float m = kKvMaxInit, big = kKvMaxInit;
-    for (int k = lane; k <= more; k += 32) {
-        const float* s = part(k) + chunk_rows * D + 3 * row;
-        m = fmaxf(m, s[0]);
-        big = fmaxf(big, s[1]);
-    }
-    m = warp_max(m);
-    big = warp_max(big);
-    float l = 0.f;
-    float4 o[kQuads];
-#pragma unroll
-    for (int i = 0; i < kQuads; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = 0; k0 <= more; k0 += 32) {
-        const float* s = part(min(k0 + lane, more)) + chunk_rows * D + 3 * row;
-        const float f = ex2(s[1] - big);
-        if (k0 + lane <= more) l += s[2] * ex2(s[0] - m);
-        const int n = min(32, more + 1 - k0);
-#pragma unroll 8
-        for (int k = 0; k < n; ++k) {
-            const float fk = __shfl_sync(0xffffffffu, f, k);
-            const float* rows = part(k0 + k) + row * D;
-#pragma unroll
-            for (int i = 0; i < kQuads; ++i) {
-                const int d = 4 * lane + 128 * i;
-                if (d >= D) continue;
-                const float4 y = *reinterpret_cast<const float4*>(rows + d);
-                o[i].x = fmaf(y.x, fk, o[i].x), o[i].y = fmaf(y.y, fk, o[i].y), o[i].z = fmaf(y.z, fk, o[i].z), o[i].w = fmaf(y.w, fk, o[i].w);
-            }
-        }
-    }
-    l = warp_sum(l);
-    const int64_t out_row = (int64_t)b * a.q_heads + (int64_t)h * a.group + row0 + row;
-    const KvQuotient f(l, big, m);
-#pragma unroll
-    for (int i = 0; i < kQuads; ++i) {
-        const int d = 4 * lane + 128 * i;
-        const float y[4] = {f(o[i].x), f(o[i].y), f(o[i].z), f(o[i].w)};
-        if (d < D) store_row<4>(a.out, out_row * D + d, a.type, a.out_vec, y);
-    }
-    if (lane == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
 }
 
 template <int FMT, int NB, int RT, int HALVES>
@@ -1123,23 +1169,11 @@ struct KvAttendInstance {
         split.by_teams = KvDiv(split.teams);
         split.by_page = KvDiv(pool.records_per_page);
         split.by_chunks = KvDiv(split.chunks);
-        split.unit = work.unit;
-        split.more = work.more;
+        split.count = work.count;
         split.slots = work.slots;
         split.partial = work.partial;
         kv_attend_kernel<FMT, NB, RT, HALVES><<<work.ctas, Shape::kThreads, Shape::kSmem, stream>>>(pool, seqs, a, split, status);
-        // the join's CTAs start as those of the attention kernel end (programmatic launch), and wait for the last of them
-        cudaLaunchAttribute attr{};
-        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr.val.programmaticStreamSerializationAllowed = 1;
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(work.ctas, (std::min(chunk_rows, a.group) + kKvJoinThreads / 32 - 1) / (kKvJoinThreads / 32));
-        cfg.blockDim = dim3(kKvJoinThreads);
-        cfg.stream = stream;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        cudaLaunchKernelEx(&cfg, kv_join_kernel<NB>, pool, a, split, chunk_rows);
-        return 2;
+        return 1;
     }
 };
 

@@ -93,8 +93,7 @@ struct KvAttend {
     int vec;                // 16-byte loads of the query are aligned
     int type;               // of query and out
     int q_heads, group;
-    void* out;              // [batch, q_heads, dim]
-    int out_vec;            // 16-byte stores of out are aligned
+    void* out;              // [batch, q_heads, dim], 16-byte aligned
     float* lse;             // [batch, q_heads] or null
     float scale_log2;       // score scale times log2(e)
     int window;             // 0: all positions
@@ -105,8 +104,7 @@ struct KvWork {
     int ctas;               // one per SM
     float* slots;           // [ctas][kKvSlotFloats]
     float* partial;         // kv_work_floats(ctas, dim)
-    int64_t* unit;          // [ctas][2]
-    int* more;              // [ctas]
+    int* count;             // [3 ctas], zero between calls
 };
 constexpr int kKvMaxRows = 128;        // query heads of one unit, at most
 constexpr int kKvSlotFloats = 33280;   // partial results of a CTA's warps

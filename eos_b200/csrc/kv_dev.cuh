@@ -98,6 +98,14 @@ __device__ __forceinline__ void load_row(const void* p, int64_t at, int type, in
         x[2 * i] = v.x, x[2 * i + 1] = v.y;
     }
 }
+// 16 bytes from an address that is aligned to 2 bytes only, out of line
+__device__ __noinline__ inline uint4 load16_unaligned(const uint8_t* p) {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+    uint4 v;
+    v.x = (uint32_t)h[0] | (uint32_t)h[1] << 16, v.y = (uint32_t)h[2] | (uint32_t)h[3] << 16;
+    v.z = (uint32_t)h[4] | (uint32_t)h[5] << 16, v.w = (uint32_t)h[6] | (uint32_t)h[7] << 16;
+    return v;
+}
 // elements one by one, out of line: for rows that are not aligned
 __device__ __noinline__ inline void store_elements(void* p, int type, int n, float a, float b, float c, float d) {
     for (int i = 0; i < n; ++i) {
