@@ -728,7 +728,7 @@ __device__ __forceinline__ float load_part(const float* p) {
 }
 
 template <int FMT, int NB, int RT, int HALVES>
-__global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads)
+__global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads, 1)
     kv_attend_kernel(KvPool pool, KvSeqs seqs, KvAttend a, KvSplit split, int* status) {
     using Shape = KvShape<FMT, NB, RT, HALVES>;
     constexpr int D = 32 * NB, kRows = Shape::kRows, kWarps = Shape::kWarps, kThreads = Shape::kThreads;

@@ -18,11 +18,10 @@ PAGE_UNIT = 16
 
 
 def _type(t: Union[str, int]) -> int:
-    if isinstance(t, str):
-        if t not in TYPES:
-            raise ValueError(f"unsupported element type {t!r}; supported values are {', '.join(TYPES)}")
-        return TYPES[t]
-    return int(t)
+    code = TYPES.get(t, t)
+    if isinstance(code, str):
+        raise ValueError(f"unsupported element type {t!r}; supported values are {', '.join(TYPES)}")
+    return code
 
 
 def _stream(stream: Optional[int]) -> Optional[int]:
@@ -48,6 +47,19 @@ class KvCache:
         _lib.call("eos_b200_kv_cache_create", rt.handle, int(pages), int(page_size), int(kv_heads), int(head_dim),
                   FORMATS[format], C.byref(self.handle))
         rt._adopt(self)
+        # one call in flight per handle: the result structures are made once, which a call of a few microseconds notices
+        lib = _lib.lib()
+        self._append, self._read = lib.eos_b200_kv_cache_append_device, lib.eos_b200_kv_cache_read_device
+        self._attend = lib.eos_b200_kv_cache_attend_device
+        self._stats, self._err = Stats(), C.c_char_p()
+        self._stats_ref, self._err_ref = C.byref(self._stats), C.byref(self._err)
+
+    def _done(self, rc: int) -> int:
+        if rc:
+            err, self._err = self._err, C.c_char_p()
+            self._err_ref = C.byref(self._err)
+            _lib.check(rc, err)
+        return self._stats.kernel_launches
 
     @property
     def page_bytes(self) -> int:
@@ -60,22 +72,18 @@ class KvCache:
         """Writes new tokens: d_key, d_value [tokens, kv_heads, head_dim]; sequence b owns the rows d_cu_tokens[b] up to
         d_cu_tokens[b + 1] and writes them from position d_starts[b] on (None: one token per sequence).  strides: elements
         between (key tokens, key heads, value tokens, value heads).  Returns kernels launched."""
-        st = Stats()
-        _lib.call("eos_b200_kv_cache_append_device", self.handle, d_key, d_value, _type(type), tokens,
-                  None if strides is None else C.byref(KvStrides(*strides)), batch, d_page_table, max_pages, d_starts,
-                  d_cu_tokens, _stream(stream), C.byref(st))
-        return st.kernel_launches
+        return self._done(self._append(self.handle, d_key, d_value, _type(type), tokens,
+                                       None if strides is None else C.byref(KvStrides(*strides)), batch, d_page_table,
+                                       max_pages, d_starts, d_cu_tokens, _stream(stream), self._stats_ref, self._err_ref))
 
     def read_device(self, d_key: int, d_value: int, type: Union[str, int], tokens: int, batch: int, d_page_table: int,
                     max_pages: int, d_starts: int, d_cu_tokens: Optional[int] = None,
                     strides: Optional[Tuple[int, int, int, int]] = None, stream: Optional[int] = None) -> int:
         """The inverse of append_device with the same arguments: d_key, d_value receive the cached values.  Rows behind
         the last sequence are left as they were."""
-        st = Stats()
-        _lib.call("eos_b200_kv_cache_read_device", self.handle, d_key, d_value, _type(type), tokens,
-                  None if strides is None else C.byref(KvStrides(*strides)), batch, d_page_table, max_pages, d_starts,
-                  d_cu_tokens, _stream(stream), C.byref(st))
-        return st.kernel_launches
+        return self._done(self._read(self.handle, d_key, d_value, _type(type), tokens,
+                                     None if strides is None else C.byref(KvStrides(*strides)), batch, d_page_table, max_pages,
+                                     d_starts, d_cu_tokens, _stream(stream), self._stats_ref, self._err_ref))
 
     def attend_device(self, d_query: int, type: Union[str, int], q_heads: int, batch: int, d_page_table: int, max_pages: int,
                       d_lengths: int, d_out: int, scale: float, window: int = 0, d_lse: Optional[int] = None,
@@ -84,11 +92,9 @@ class KvCache:
         d_lengths[b] cached positions; out [batch, q_heads, head_dim] of the query's type, d_lse [batch, q_heads] fp32 the
         logarithm of the softmax denominators.  Query head i reads key head i // (q_heads // kv_heads).  query_strides:
         elements between sequences and between heads, 0: contiguous.  Returns kernels launched."""
-        st = Stats()
-        _lib.call("eos_b200_kv_cache_attend_device", self.handle, d_query, _type(type), q_heads, query_strides[0],
-                  query_strides[1], batch, d_page_table, max_pages, d_lengths, scale, window, d_out, d_lse, _stream(stream),
-                  C.byref(st))
-        return st.kernel_launches
+        return self._done(self._attend(self.handle, d_query, _type(type), q_heads, query_strides[0], query_strides[1], batch,
+                                       d_page_table, max_pages, d_lengths, scale, window, d_out, d_lse, _stream(stream),
+                                       self._stats_ref, self._err_ref))
 
     def sync(self, stream: Optional[int] = None) -> None:
         """Waits for the stream; raises EosB200DeviceStatusError if a kernel met a page, position or length out of range."""
