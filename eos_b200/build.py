@@ -10,7 +10,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libeos_b200.so")
 SOURCES = ["gemm_tc.cu", "attention_tc.cu", "encoder_kernels.cu", "turboquant.cu", "turboquant_tc.cu", "turboquant_tc256.cu", "sparse_attention.cu", "token_pool.cu",
-           "kv_cache.cu", "kv_attend_f16.cu", "kv_attend_bf16.cu", "kv_attend_mx8.cu", "kv_attend_mx4.cu", "capi.cu"]
+           "kv_cache.cu", "kv_io_f16.cu", "kv_io_bf16.cu", "kv_io_mx8.cu", "kv_io_mx4.cu",
+           "kv_attend_f16.cu", "kv_attend_bf16.cu", "kv_attend_mx8.cu", "kv_attend_mx4.cu", "capi.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--extended-lambda",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",

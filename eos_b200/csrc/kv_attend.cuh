@@ -104,48 +104,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
     return r;
 }
 
-// The bytes of one lane at `plane0`, BYTES of them (see kv_lane_offset)
-template <int BYTES>
-__device__ __forceinline__ void load_lane(const uint8_t* plane0, int lane, uint32_t (&w)[BYTES / 4]) {
-#pragma unroll
-    for (int p = 0; p + 16 <= BYTES; p += 16) {
-        const uint4 v = *reinterpret_cast<const uint4*>(plane0 + p * 32 + lane * 16);
-        w[p / 4] = v.x, w[p / 4 + 1] = v.y, w[p / 4 + 2] = v.z, w[p / 4 + 3] = v.w;
-    }
-    constexpr int r = BYTES & 15, p = BYTES - r;
-    if constexpr (r >= 8) {
-        const uint2 v = *reinterpret_cast<const uint2*>(plane0 + p * 32 + lane * 8);
-        w[p / 4] = v.x, w[p / 4 + 1] = v.y;
-    }
-    if constexpr ((r & 7) != 0)
-        w[BYTES / 4 - 1] = *reinterpret_cast<const uint32_t*>(plane0 + p * 32 + (r >= 8 ? 256 : 0) + lane * 4);
-}
-
-// Scale bytes of one token's key, packed four to a word
-template <int NB>
-__device__ __forceinline__ void load_scales(const uint8_t* p, uint32_t (&a)[(NB + 3) / 4]) {
-    if constexpr (NB == 1) a[0] = *p;
-    else if constexpr (NB == 2) a[0] = *reinterpret_cast<const uint16_t*>(p);
-    else if constexpr (NB <= 4) a[0] = *reinterpret_cast<const uint32_t*>(p);
-    else {
-        const uint2 w = *reinterpret_cast<const uint2*>(p);
-        a[0] = w.x, a[1] = w.y;
-    }
-}
-// Scale bytes of a token pair's values: block b in byte 2 (b % 2) (first token) and the next (second) of word b / 2
-template <int NB>
-__device__ __forceinline__ void load_pair_scales(const uint8_t* p, uint32_t (&w)[(NB + 1) / 2]) {
-    if constexpr (NB == 1) w[0] = *reinterpret_cast<const uint16_t*>(p);
-    else if constexpr (NB == 2) w[0] = *reinterpret_cast<const uint32_t*>(p);
-    else if constexpr (NB <= 4) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        w[0] = v.x, w[1] = v.y;
-    } else {
-        const uint4 v = *reinterpret_cast<const uint4*>(p);
-        w[0] = v.x, w[1] = v.y, w[2] = v.z;
-        if constexpr (NB > 6) w[3] = v.w;
-    }
-}
 // exponent field of byte i as a float 2^(byte - 127); 255 becomes infinity, which times the zero codes of such a block is NaN
 __device__ __forceinline__ float scale_at(uint32_t word, int i) {
     return __uint_as_float(i == 3 ? (word >> 1) & 0x7f800000u
@@ -937,7 +895,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads, 1)
                             for (int blk = 0; blk < NB; ++blk) {
                                 const float4 o = w.numerators(k, c, blk);
                                 const float y[4] = {f(o.x), f(o.y), f(o.z), f(o.w)};
-                                store_row<4>(a.out, (out0 + row) * D + 32 * blk + 4 * g, a.type, 1, y);
+                                store_row(a.out, (out0 + row) * D + 32 * blk + 4 * g, a.type, y);
                             }
                         }
                     }
@@ -1115,7 +1073,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < kQuads; ++i) {
                         const float y[4] = {f(o[i].x), f(o[i].y), f(o[i].z), f(o[i].w)};
-                        if (4 * lane + 128 * i < D) store_row<4>(a.out, out_row * D + 4 * lane + 128 * i, a.type, 1, y);
+                        if (4 * lane + 128 * i < D) store_row(a.out, out_row * D + 4 * lane + 128 * i, a.type, y);
                     }
                     if (lane == 0 && a.lse != nullptr) a.lse[out_row] = f.lse;
                 } else {
@@ -1140,7 +1098,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads, 1)
         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (int i = tid; i < a.q_heads * (D / 4); i += kThreads)
-            store_row<4>(a.out, b * a.q_heads * D + 4 * i, a.type, 1, zero);
+            store_row(a.out, b * a.q_heads * D + 4 * i, a.type, zero);
         if (a.lse != nullptr)
 #pragma unroll 1
             for (int i = tid; i < a.q_heads; i += kThreads) a.lse[b * a.q_heads + i] = -INFINITY;

@@ -1,0 +1,574 @@
+// Paged key-value cache: quantising tokens as they are written, and reading them back (kernel templates, one instance per
+// format, head size and element type; kv_io_*.cu compile them).
+//
+// Formats.  f16 / bf16 hold each element rounded to nearest.  mx8 (e4m3) and mx4 (e2m1) hold, for every 32 consecutive
+// elements of a head's vector, one scale 2^e with the smallest e >= -126 for which max|x| <= top 2^e (top = 448 or 6,
+// the type's largest value, so nothing saturates) and the codes x / 2^e rounded to nearest, ties to even.  The scale is
+// a power of two: the division is exact, every code has one right answer, and a code times its scale is exact in fp32.
+// A block that holds an infinity or a NaN is stored as NaN (scale byte 255, codes zero).
+//
+// One warp per (record, head): it owns all 16 tokens of the record that the call writes, so a record that is completed
+// by several calls needs no atomics, and neighbouring tokens' codes are merged by a plain read-modify-write.  All of a
+// warp's loads are issued before the first is used, and codes are built in registers in the order of the record.
+#pragma once
+#include "kv_dev.cuh"
+
+namespace eosb {
+
+constexpr int kKvIoWarps = 8;
+
+// The sequence and record that work unit u of a call stands for.  Sequence b starts at unit cu[b] / 16 + 2 b: n tokens
+// that start anywhere in a record touch at most floor((n + 30) / 16) records, and the gap to sequence b + 1 is at least
+// that.  Warp-wide search, 32 probes a step; lanes agree on the result.
+struct KvUnit {
+    int b, rec;       // sequence, record index within the sequence
+    int lo, hi;       // positions [lo, hi) of the record that the call covers
+    int64_t row0;     // row of position 0 of the sequence (may be negative: rows are row0 + position)
+    bool ok;
+};
+__device__ __forceinline__ KvUnit kv_unit(const KvSeqs& s, int64_t tokens, int64_t u, int lane, int* status) {
+    KvUnit r;
+    r.ok = false;
+    int64_t row, n, first = 0;
+    if (s.cu == nullptr) {
+        r.b = (int)u, row = u, n = 1;
+    } else {
+        int lo = 0, hi = s.batch;
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 31) >> 5;
+            const int probe = lo + lane * step;
+            const bool below = lane == 0 || (probe < hi && (int64_t)(__ldg(s.cu + probe) >> 4) + 2 * (int64_t)probe <= u);
+            const int top = 31 - __clz(__ballot_sync(0xffffffffu, below));
+            lo += top * step;
+            hi = min(hi, lo + step);
+        }
+        r.b = lo;
+        row = __ldg(s.cu + lo);
+        n = (int64_t)__ldg(s.cu + lo + 1) - row;
+        first = u - ((int64_t)(row >> 4) + 2 * (int64_t)lo);
+    }
+    if (n == 0) return r;
+    const int64_t start = __ldg(s.starts + r.b);
+    if (n < 0 || row < 0 || row + n > tokens || start < 0 || start + n > 0x7fffffffLL) {
+        if (lane == 0) atomicExch(status, kStatusBadSequence);
+        return r;
+    }
+    const int64_t rec = (start >> 4) + first;
+    if (first < 0 || rec * kKvRecord >= start + n) return r;
+    r.rec = (int)rec;
+    r.lo = (int)max(start, rec * kKvRecord);
+    r.hi = (int)min(start + n, (rec + 1) * kKvRecord);
+    r.row0 = row - start;
+    r.ok = true;
+    return r;
+}
+
+// ---------------------------------------------------------------- elements
+// N (4 or 8) consecutive elements of a call's tensor, as they lie in memory
+template <int TYPE, int N>
+struct KvRow {
+    static constexpr int kWords = TYPE == kTypeF32 ? N : N / 2;
+    uint32_t w[kWords];
+
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0u;
+    }
+    __device__ __forceinline__ void load(const uint8_t* p, int vec) {
+        if (vec) {
+            if constexpr (kWords == 2) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+                w[0] = v.x, w[1] = v.y;
+            } else {
+#pragma unroll
+                for (int i = 0; i < kWords; i += 4) {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+                    w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+                }
+            }
+        } else {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = (uint32_t)h[2 * i] | (uint32_t)h[2 * i + 1] << 16;
+        }
+    }
+    __device__ __forceinline__ float2 pair(int i) const {   // elements 2i, 2i + 1
+        if constexpr (TYPE == kTypeF32) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        else if constexpr (TYPE == kTypeF16) return f16x2_floats(w[i]);
+        else return bf16x2_floats(w[i]);
+    }
+    // Largest magnitude, as bits that compare like it with infinities and NaN on top: of fp32, or two 16-bit halves
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0u;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i)
+            m = TYPE == kTypeF32 ? max(m, w[i] & 0x7fffffffu) : __vmaxu2(m, w[i] & 0x7fff7fffu);
+        return m;
+    }
+};
+// the larger half of a 16-bit pair's, as its fp32 bits
+template <int TYPE>
+__device__ __forceinline__ uint32_t top_bits(uint32_t h) {   // h < 2^16
+    if constexpr (TYPE == kTypeF16) return __float_as_uint(f16x2_floats(h).x);
+    return h << 16;
+}
+
+// scale byte of a block with the largest magnitude amax (its fp32 bits)
+template <int FMT>
+__device__ __forceinline__ uint32_t kv_scale_byte(uint32_t amax_bits) {
+    const uint32_t e = amax_bits >> 23, m = amax_bits & 0x7fffffu;
+    const int byte = FMT == kKvMx8 ? (int)e - 8 + (m > 0x600000u) : (int)e - 2 + (m > 0x400000u);   // 448 = 1.75 2^8, 6 = 1.5 2^2
+    return e == 255u ? 255u : (uint32_t)max(byte, 1);
+}
+// 2^-e of a scale byte; 0 for a block stored as NaN
+__device__ __forceinline__ float kv_inverse_scale(uint32_t byte) { return __uint_as_float(byte == 255u ? 0u : (254u - byte) << 23); }
+// (a NaN or infinity times 0 is a NaN; its code is to be zero)
+__device__ __forceinline__ float2 kv_scaled(float2 x, float inv) {
+    const float2 y = make_float2(x.x * inv, x.y * inv);
+    return make_float2(inv == 0.f ? 0.f : y.x, inv == 0.f ? 0.f : y.y);
+}
+
+__device__ __forceinline__ uint32_t e4m3x4_of(float a, float b, float c, float d) {
+    uint32_t r;
+    asm("{\n .reg .b16 l, h;\n cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n cvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n mov.b32 %0, {l, h};\n}"
+        : "=r"(r)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+    return r;
+}
+__device__ __forceinline__ uint32_t e2m1x8_of(float a, float b, float c, float d, float e, float f, float g, float h) {
+    uint32_t r;
+    asm("{\n .reg .b8 p, q, r, s;\n cvt.rn.satfinite.e2m1x2.f32 p, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 q, %4, %3;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 r, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 s, %8, %7;\n mov.b32 %0, {p, q, r, s};\n}"
+        : "=r"(r)
+        : "f"(a), "f"(b), "f"(c), "f"(d), "f"(e), "f"(f), "f"(g), "f"(h));
+    return r;
+}
+
+// The bytes of one lane (see kv_lane_offset)
+template <int BYTES>
+__device__ __forceinline__ void store_lane(uint8_t* plane0, int lane, const uint32_t (&w)[BYTES / 4]) {
+#pragma unroll
+    for (int p = 0; p + 16 <= BYTES; p += 16)
+        *reinterpret_cast<uint4*>(plane0 + p * 32 + lane * 16) = make_uint4(w[p / 4], w[p / 4 + 1], w[p / 4 + 2], w[p / 4 + 3]);
+    constexpr int r = BYTES & 15, p = BYTES - r;
+    if constexpr (r >= 8) *reinterpret_cast<uint2*>(plane0 + p * 32 + lane * 8) = make_uint2(w[p / 4], w[p / 4 + 1]);
+    if constexpr ((r & 7) != 0) *reinterpret_cast<uint32_t*>(plane0 + p * 32 + (r >= 8 ? 256 : 0) + lane * 4) = w[BYTES / 4 - 1];
+}
+
+// ---------------------------------------------------------------- append
+template <int FMT, int NB, int TYPE>
+__global__ void __launch_bounds__(kKvIoWarps * 32)
+    kv_append_kernel(KvPool pool, KvSeqs seqs, KvRows key, KvRows value, int64_t tokens, int64_t units, int* status) {
+    constexpr bool kMx = FMT >= kKvMx8;
+    constexpr int KP = kv_key_piece(FMT), VP = kv_value_piece(FMT), NS = kv_scale_stride(NB), ES = TYPE == kTypeF32 ? 4 : 2;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int64_t w = (int64_t)blockIdx.x * kKvIoWarps + (threadIdx.x >> 5);
+    const int64_t u = w / pool.heads;
+    if (u >= units) return;
+    const int h = (int)(w - u * pool.heads);
+    const KvUnit un = kv_unit(seqs, tokens, u, lane, status);
+    if (!un.ok) return;
+    uint8_t* rec = kv_record(pool, seqs, un.b, un.rec, h);
+    if (rec == nullptr) {
+        if (lane == 0) atomicExch(status, kStatusBadPage);
+        return;
+    }
+    const int base = un.rec * kKvRecord;
+    // ---- keys: lane (g, t) owns 8 elements of the tokens g and g + 8 in every block
+    bool kmine[2];
+    KvRow<TYPE, 8> kx[2][NB];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int pos = base + 8 * j + g;
+        kmine[j] = pos >= un.lo && pos < un.hi;
+        const uint8_t* p = static_cast<const uint8_t*>(key.p) + ((un.row0 + pos) * key.token_stride + (int64_t)h * key.head_stride + 8 * t) * ES;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            kx[j][b].zero();
+            if (kmine[j]) kx[j][b].load(p + 32 * b * ES, key.vec);
+        }
+    }
+    // ---- values: lane (g, t) owns elements 4 g .. + 3 of every block for the tokens 2t, 2t+1, 2t+8, 2t+9
+    bool vmine[4];
+    const uint8_t* vp[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int pos = base + 2 * t + (i & 1) + 8 * (i >> 1);
+        vmine[i] = pos >= un.lo && pos < un.hi;
+        vp[i] = static_cast<const uint8_t*>(value.p) + ((un.row0 + pos) * value.token_stride + (int64_t)h * value.head_stride + 4 * g) * ES;
+    }
+    KvRow<TYPE, 4> vx[4][NB];
+    auto load_values = [&]() {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                vx[i][b].zero();
+                if (vmine[i]) vx[i][b].load(vp[i] + 32 * b * ES, value.vec);
+            }
+    };
+    // (fp32 rows of 192 elements and more do not fit the registers beside the keys)
+    constexpr bool kLate = TYPE == kTypeF32 && NB >= 6;
+    if constexpr (!kLate) load_values();
+    // the values' codes that this call leaves alone
+    const bool any = vmine[0] || vmine[1] || vmine[2] || vmine[3], all = vmine[0] && vmine[1] && vmine[2] && vmine[3];
+    uint32_t old[NB * VP / 4];
+    if (any && !all) load_lane<NB * VP>(rec + kv_value_offset(FMT, NB), lane, old);
+
+    if constexpr (!kMx) {
+        // words of the two tokens in turn
+        uint32_t kw[NB * 8];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float2 x = kx[j][b].pair(i);
+                    kw[8 * b + 4 * (i >> 1) + 2 * (i & 1) + j] = TYPE == FMT + 1 ? kx[j][b].w[i % KvRow<TYPE, 8>::kWords]   // (f16 to f16, bf16 to bf16)
+                                                                 : FMT == kKvF16 ? f16x2_of(x.x, x.y) : bf16x2_of(x.x, x.y);
+                }
+        if (kmine[0] && kmine[1]) {
+            store_lane<NB * 32>(rec, lane, kw);
+        } else if (kmine[0] || kmine[1]) {
+#pragma unroll
+            for (int i = 0; i < NB * 8; i += 2)
+                *reinterpret_cast<uint32_t*>(rec + kv_lane_offset(NB * 32, lane, 4 * i + (kmine[1] ? 4 : 0))) = kmine[1] ? kw[i + 1] : kw[i];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            uint32_t codes[NB * KP / 4];
+            uint64_t bytes = 0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                uint32_t m = kx[j][b].top();
+                if constexpr (TYPE == kTypeF32) {
+                    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                } else {
+                    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                    m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                    m = top_bits<TYPE>(max(m & 0xffffu, m >> 16));
+                }
+                const uint32_t byte = kv_scale_byte<FMT>(m);
+                const float inv = kv_inverse_scale(byte);
+                bytes |= (uint64_t)byte << (8 * b);
+                float2 x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = kv_scaled(kx[j][b].pair(i), inv);
+                if constexpr (FMT == kKvMx8) {
+                    codes[2 * b] = e4m3x4_of(x[0].x, x[0].y, x[1].x, x[1].y);
+                    codes[2 * b + 1] = e4m3x4_of(x[2].x, x[2].y, x[3].x, x[3].y);
+                } else {
+                    codes[b] = e2m1x8_of(x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y);
+                }
+            }
+            if (kmine[j]) {
+                store_lane<NB * KP>(rec + j * 32 * NB * KP, lane, codes);
+                if (t == 0) {
+                    uint8_t* p = rec + kv_key_scale_offset(FMT, NB) + (8 * j + g) * NS;
+                    if constexpr (NS == 1) *p = (uint8_t)bytes;
+                    else if constexpr (NS == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)bytes;
+                    else if constexpr (NS == 4) *reinterpret_cast<uint32_t*>(p) = (uint32_t)bytes;
+                    else *reinterpret_cast<uint2*>(p) = make_uint2((uint32_t)bytes, (uint32_t)(bytes >> 32));
+                }
+            }
+        }
+    }
+
+    // ---- values
+    if constexpr (kLate) load_values();
+    uint32_t v[NB * VP / 4], keep[4];   // keep: bits of a block's words that belong to tokens of other calls
+    uint64_t scales[4] = {0, 0, 0, 0};  // of each token: the blocks' scale bytes, 0 for a block of zeros
+    if constexpr (!kMx) {
+        keep[0] = (vmine[0] ? 0u : 0x0000ffffu) | (vmine[1] ? 0u : 0xffff0000u);
+        keep[1] = (vmine[2] ? 0u : 0x0000ffffu) | (vmine[3] ? 0u : 0xffff0000u);
+    } else if constexpr (FMT == kKvMx8) {
+        keep[0] = (vmine[0] ? 0u : 0xffu) | (vmine[1] ? 0u : 0xff00u) | (vmine[2] ? 0u : 0xff0000u) | (vmine[3] ? 0u : 0xff000000u);
+    } else {
+        keep[0] = ((vmine[0] ? 0u : 0xfu) | (vmine[1] ? 0u : 0xf0u) | (vmine[2] ? 0u : 0xf00u) | (vmine[3] ? 0u : 0xf000u)) * 0x10001u;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        float x[4][4];   // [token][element]
+        if constexpr (kMx) {
+            uint32_t m[4];   // fp32 bits of the tokens' largest magnitudes
+            if constexpr (TYPE == kTypeF32) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    m[i] = vx[i][b].top();
+                    m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], 4));
+                    m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], 8));
+                    m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], 16));
+                }
+            } else {
+                // two tokens a word
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const uint32_t a = vx[2 * p][b].top(), c = vx[2 * p + 1][b].top();
+                    uint32_t y = __vmaxu2(__byte_perm(a, c, 0x5410), __byte_perm(a, c, 0x7632));
+                    y = __vmaxu2(y, __shfl_xor_sync(0xffffffffu, y, 4));
+                    y = __vmaxu2(y, __shfl_xor_sync(0xffffffffu, y, 8));
+                    y = __vmaxu2(y, __shfl_xor_sync(0xffffffffu, y, 16));
+                    m[2 * p] = top_bits<TYPE>(y & 0xffffu), m[2 * p + 1] = top_bits<TYPE>(y >> 16);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t byte = kv_scale_byte<FMT>(m[i]);
+                const float inv = kv_inverse_scale(byte);
+                scales[i] |= (uint64_t)(m[i] == 0u ? 0u : byte) << (8 * b);
+                const float2 y = kv_scaled(vx[i][b].pair(0), inv), z = kv_scaled(vx[i][b].pair(1), inv);
+                x[i][0] = y.x, x[i][1] = y.y, x[i][2] = z.x, x[i][3] = z.y;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 y = vx[i][b].pair(0), z = vx[i][b].pair(1);
+                x[i][0] = y.x, x[i][1] = y.y, x[i][2] = z.x, x[i][3] = z.y;
+            }
+        }
+        if constexpr (!kMx) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const int at = 8 * b + 4 * (e >> 1) + 2 * p + (e & 1);
+                    if constexpr (TYPE == FMT + 1)
+                        v[at] = __byte_perm(vx[2 * p][b].w[e >> 1], vx[2 * p + 1][b].w[e >> 1], e & 1 ? 0x7632 : 0x5410);
+                    else
+                        v[at] = FMT == kKvF16 ? f16x2_of(x[2 * p][e], x[2 * p + 1][e]) : bf16x2_of(x[2 * p][e], x[2 * p + 1][e]);
+                }
+        } else if constexpr (FMT == kKvMx8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * b + e] = e4m3x4_of(x[0][e], x[1][e], x[2][e], x[3][e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                v[2 * b + e] = e2m1x8_of(x[0][2 * e], x[1][2 * e], x[2][2 * e], x[3][2 * e], x[0][2 * e + 1], x[1][2 * e + 1],
+                                         x[2][2 * e + 1], x[3][2 * e + 1]);
+        }
+    }
+    if (any) {
+        if (!all) {
+#pragma unroll
+            for (int i = 0; i < NB * VP / 4; ++i) {
+                const uint32_t k = kMx ? keep[0] : keep[i >> 1 & 1];
+                v[i] = (v[i] & ~k) | (old[i] & k);
+            }
+        }
+        store_lane<NB * VP>(rec + kv_value_offset(FMT, NB), lane, v);
+    }
+    if constexpr (kMx) {   // scales and tops: two token pairs a lane t, lanes g = 0 and 1 one each
+        uint32_t top[4], odd[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            top[i] = 1, odd[i] = 0;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const uint32_t e = (uint32_t)(scales[i] >> (8 * b)) & 0xffu;
+                if (e == 255u) odd[i] = 1;
+                else top[i] = max(top[i], e);
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const uint32_t e = (uint32_t)(scales[i] >> (8 * b)) & 0xffu;
+                if (e != 0u && e + kKvNear < top[i]) odd[i] = 1;
+                if (e == 0u) scales[i] |= (uint64_t)top[i] << (8 * b);
+            }
+        }
+        if (g < 2) {
+            const bool second = g == 1;
+            const uint64_t sa = second ? scales[2] : scales[0], sb = second ? scales[3] : scales[1];
+            const bool ma = second ? vmine[2] : vmine[0], mb = second ? vmine[3] : vmine[1];
+            const uint32_t word = (second ? top[2] : top[0]) | (second ? top[3] : top[1]) << 8 | (second ? odd[2] : odd[0]) << 16 |
+                                  (second ? odd[3] : odd[1]) << 24;
+            uint8_t* sp = rec + kv_value_scale_offset(FMT, NB) + (t + 4 * g) * 2 * NS;
+            uint8_t* tp = rec + kv_value_top_offset(FMT, NB) + 4 * (t + 4 * g);
+            if (ma && mb) {
+                uint32_t out[(NB + 1) / 2];
+#pragma unroll
+                for (int i = 0; i < (NB + 1) / 2; ++i)   // bytes (a, b) of blocks 2i and 2i + 1
+                    out[i] = __byte_perm((uint32_t)(sa >> (16 * i)) & 0xffffu, (uint32_t)(sb >> (16 * i)) & 0xffffu, 0x5140);
+                if constexpr (NB == 1) *reinterpret_cast<uint16_t*>(sp) = (uint16_t)out[0];
+                else {
+#pragma unroll
+                    for (int i = 0; i < (NB + 1) / 2; ++i) *reinterpret_cast<uint32_t*>(sp + 4 * i) = out[i];
+                }
+                *reinterpret_cast<uint32_t*>(tp) = word;
+            } else if (ma || mb) {
+                const uint64_t s = ma ? sa : sb;
+                const int at = ma ? 0 : 1;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) sp[2 * b + at] = (uint8_t)(s >> (8 * b));
+                tp[at] = (uint8_t)(word >> (8 * at));
+                tp[2 + at] = (uint8_t)(word >> (16 + 8 * at));
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- read
+template <int TYPE, int N>
+__device__ __forceinline__ void store_out(uint8_t* p, int vec, const float (&x)[N]) {
+    constexpr int kWords = TYPE == kTypeF32 ? N : N / 2;
+    uint32_t w[kWords];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        if constexpr (TYPE == kTypeF32) w[2 * i] = __float_as_uint(x[2 * i]), w[2 * i + 1] = __float_as_uint(x[2 * i + 1]);
+        else w[i] = TYPE == kTypeF16 ? f16x2_of(x[2 * i], x[2 * i + 1]) : bf16x2_of(x[2 * i], x[2 * i + 1]);
+    }
+    if (vec) {
+        if constexpr (kWords == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        else {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) *(reinterpret_cast<uint4*>(p) + i / 4) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        }
+    } else {
+        uint16_t* h = reinterpret_cast<uint16_t*>(p);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) h[2 * i] = (uint16_t)w[i], h[2 * i + 1] = (uint16_t)(w[i] >> 16);
+    }
+}
+
+template <int FMT, int NB, int TYPE>
+__global__ void __launch_bounds__(kKvIoWarps * 32)
+    kv_read_kernel(KvPool pool, KvSeqs seqs, KvRows key, KvRows value, int64_t tokens, int64_t units, int* status) {
+    constexpr bool kMx = FMT >= kKvMx8;
+    constexpr int KP = kv_key_piece(FMT), VP = kv_value_piece(FMT), NS = kv_scale_stride(NB), ES = TYPE == kTypeF32 ? 4 : 2;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int64_t w = (int64_t)blockIdx.x * kKvIoWarps + (threadIdx.x >> 5);
+    const int64_t u = w / pool.heads;
+    if (u >= units) return;
+    const int h = (int)(w - u * pool.heads);
+    const KvUnit un = kv_unit(seqs, tokens, u, lane, status);
+    if (!un.ok) return;
+    const uint8_t* rec = kv_record(pool, seqs, un.b, un.rec, h);
+    if (rec == nullptr) {
+        if (lane == 0) atomicExch(status, kStatusBadPage);
+        return;
+    }
+    const int base = un.rec * kKvRecord;
+    // all loads first
+    constexpr int kKeyWords = kMx ? NB * KP / 4 : NB * 8;
+    uint32_t k0[kKeyWords], k1[kMx ? NB * KP / 4 : 1], v[NB * VP / 4], e0[(NB + 3) / 4], e1[(NB + 3) / 4], f0[(NB + 1) / 2], f1[(NB + 1) / 2];
+    if constexpr (kMx) {
+        load_lane<NB * KP>(rec, lane, k0);
+        load_lane<NB * KP>(rec + 32 * NB * KP, lane, k1);
+        load_scales<NB>(rec + kv_key_scale_offset(FMT, NB) + g * NS, e0);
+        load_scales<NB>(rec + kv_key_scale_offset(FMT, NB) + (g + 8) * NS, e1);
+        load_pair_scales<NB>(rec + kv_value_scale_offset(FMT, NB) + t * 2 * NS, f0);
+        load_pair_scales<NB>(rec + kv_value_scale_offset(FMT, NB) + (t + 4) * 2 * NS, f1);
+    } else {
+        load_lane<NB * 32>(rec, lane, k0);
+    }
+    load_lane<NB * VP>(rec + kv_value_offset(FMT, NB), lane, v);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int pos = base + 8 * j + g;
+        if (pos < un.lo || pos >= un.hi) continue;
+        uint8_t* p = static_cast<uint8_t*>(key.p) + ((un.row0 + pos) * key.token_stride + (int64_t)h * key.head_stride + 8 * t) * ES;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            uint32_t c[4];
+            if constexpr (!kMx) {
+                c[0] = k0[8 * b + j], c[1] = k0[8 * b + 2 + j], c[2] = k0[8 * b + 4 + j], c[3] = k0[8 * b + 6 + j];
+            } else if constexpr (FMT == kKvMx8) {
+                f16_of_e4m3x4(j ? k1[2 * b] : k0[2 * b], c[0], c[1]);
+                f16_of_e4m3x4(j ? k1[2 * b + 1] : k0[2 * b + 1], c[2], c[3]);
+            } else {
+                f16_of_e2m1x8(j ? k1[b] : k0[b], c[0], c[1], c[2], c[3]);
+            }
+            const float s = kMx ? kv_scale_value((j ? e1[b / 4] : e0[b / 4]) >> (8 * (b & 3)) & 0xffu) : 1.f;
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = FMT == kKvBf16 ? bf16x2_floats(c[i]) : f16x2_floats(c[i]);
+                x[2 * i] = kMx ? f.x * s : f.x;
+                x[2 * i + 1] = kMx ? f.y * s : f.y;
+            }
+            store_out<TYPE, 8>(p + 32 * b * ES, key.vec, x);
+        }
+    }
+    bool mine[4];
+    uint8_t* p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int pos = base + 2 * t + (i & 1) + 8 * (i >> 1);
+        mine[i] = pos >= un.lo && pos < un.hi;
+        p[i] = static_cast<uint8_t*>(value.p) + ((un.row0 + pos) * value.token_stride + (int64_t)h * value.head_stride + 4 * g) * ES;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        uint32_t c[8];   // [element][token pair]
+        if constexpr (!kMx) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[2 * e] = v[8 * b + 4 * (e >> 1) + (e & 1)], c[2 * e + 1] = v[8 * b + 4 * (e >> 1) + 2 + (e & 1)];
+        } else if constexpr (FMT == kKvMx8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f16_of_e4m3x4(v[4 * b + e], c[2 * e], c[2 * e + 1]);
+        } else {
+            f16_of_e2m1x8(v[2 * b], c[0], c[1], c[2], c[3]);
+            f16_of_e2m1x8(v[2 * b + 1], c[4], c[5], c[6], c[7]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (!mine[i]) continue;
+            const float s = kMx ? kv_scale_value(((i >> 1) ? f1[b / 2] : f0[b / 2]) >> (16 * (b & 1) + 8 * (i & 1)) & 0xffu) : 1.f;
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = FMT == kKvBf16 ? bf16x2_floats(c[2 * e + (i >> 1)]) : f16x2_floats(c[2 * e + (i >> 1)]);
+                const float y = (i & 1) ? f.y : f.x;
+                x[e] = kMx ? y * s : y;
+            }
+            store_out<TYPE, 4>(p[i] + 32 * b * ES, value.vec, x);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- launches
+// Work units of a call: see kv_unit.  The rows behind the last sequence belong to no unit.
+inline int64_t kv_units(const KvSeqs& s, int64_t tokens) { return s.cu == nullptr ? tokens : (tokens >> 4) + 2 * (int64_t)s.batch; }
+
+template <bool READ, int FMT, int NB, int TYPE>
+void kv_io_launch(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int64_t tokens, int* status,
+                  cudaStream_t stream) {
+    const int64_t units = kv_units(seqs, tokens);
+    const unsigned blocks = (unsigned)((units * pool.heads + kKvIoWarps - 1) / kKvIoWarps);
+    if constexpr (READ) kv_read_kernel<FMT, NB, TYPE><<<blocks, kKvIoWarps * 32, 0, stream>>>(pool, seqs, key, value, tokens, units, status);
+    else kv_append_kernel<FMT, NB, TYPE><<<blocks, kKvIoWarps * 32, 0, stream>>>(pool, seqs, key, value, tokens, units, status);
+}
+template <bool READ, int FMT, int NB>
+void kv_io_type(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
+                int* status, cudaStream_t stream) {
+    switch (type) {
+        case kTypeF32: return kv_io_launch<READ, FMT, NB, kTypeF32>(pool, seqs, key, value, tokens, status, stream);
+        case kTypeF16: return kv_io_launch<READ, FMT, NB, kTypeF16>(pool, seqs, key, value, tokens, status, stream);
+        default: return kv_io_launch<READ, FMT, NB, kTypeBf16>(pool, seqs, key, value, tokens, status, stream);
+    }
+}
+template <bool READ, int FMT>
+void kv_io_format(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
+                  int* status, cudaStream_t stream) {
+    switch (pool.blocks) {
+        case 1: return kv_io_type<READ, FMT, 1>(pool, seqs, key, value, type, tokens, status, stream);
+        case 2: return kv_io_type<READ, FMT, 2>(pool, seqs, key, value, type, tokens, status, stream);
+        case 3: return kv_io_type<READ, FMT, 3>(pool, seqs, key, value, type, tokens, status, stream);
+        case 4: return kv_io_type<READ, FMT, 4>(pool, seqs, key, value, type, tokens, status, stream);
+        case 6: return kv_io_type<READ, FMT, 6>(pool, seqs, key, value, type, tokens, status, stream);
+        default: return kv_io_type<READ, FMT, 8>(pool, seqs, key, value, type, tokens, status, stream);
+    }
+}
+
+#define EOSB_KV_IO(name)                                                                                                   \
+    void kv_append_##name(const KvPool&, const KvSeqs&, const KvRows&, const KvRows&, int, int64_t, int*, cudaStream_t);   \
+    void kv_read_##name(const KvPool&, const KvSeqs&, const KvRows&, const KvRows&, int, int64_t, int*, cudaStream_t);
+EOSB_KV_IO(f16)
+EOSB_KV_IO(bf16)
+EOSB_KV_IO(mx8)
+EOSB_KV_IO(mx4)
+#undef EOSB_KV_IO
+
+}  // namespace eosb
