@@ -20,7 +20,7 @@
 // values [8 token pairs][blocks][2], the order in which the attention kernel makes f16 pairs of them.  For every token
 // pair a 32-bit word says what the kernel would otherwise have to find out for each of its loads: the largest scale byte
 // of each token's values (bits 0-7, 8-15) and whether the token is out of the ordinary (bits 16, 24): a block stored as
-// NaN, or one more than 2^14 below the token's largest.  A block of zeros has the token's largest scale.
+// NaN, or one more than 2^14 below the token's largest (a block of zeros too).
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -113,20 +113,15 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t h) {   // h < 2^16
     return h << 16;
 }
 
-// scale byte of a block with the largest magnitude amax (its fp32 bits)
+// scale byte of a block with the largest magnitude amax (its fp32 bits): its exponent less that of the largest code, one
+// more where the mantissa passes that code's (448 = 1.75 2^8, 6 = 1.5 2^2); 255 for infinities and NaN
 template <int FMT>
 __device__ __forceinline__ uint32_t kv_scale_byte(uint32_t amax_bits) {
-    const uint32_t e = amax_bits >> 23, m = amax_bits & 0x7fffffu;
-    const int byte = FMT == kKvMx8 ? (int)e - 8 + (m > 0x600000u) : (int)e - 2 + (m > 0x400000u);   // 448 = 1.75 2^8, 6 = 1.5 2^2
-    return e == 255u ? 255u : (uint32_t)max(byte, 1);
+    const int byte = (int)((amax_bits + (FMT == kKvMx8 ? 0x1fffffu : 0x3fffffu)) >> 23) - (FMT == kKvMx8 ? 8 : 2);
+    return amax_bits >= 0x7f800000u ? 255u : (uint32_t)max(byte, 1);
 }
 // 2^-e of a scale byte; 0 for a block stored as NaN
 __device__ __forceinline__ float kv_inverse_scale(uint32_t byte) { return __uint_as_float(byte == 255u ? 0u : (254u - byte) << 23); }
-// (a NaN or infinity times 0 is a NaN; its code is to be zero)
-__device__ __forceinline__ float2 kv_scaled(float2 x, float inv) {
-    const float2 y = make_float2(x.x * inv, x.y * inv);
-    return make_float2(inv == 0.f ? 0.f : y.x, inv == 0.f ? 0.f : y.y);
-}
 
 __device__ __forceinline__ uint32_t e4m3x4_of(float a, float b, float c, float d) {
     uint32_t r;
@@ -174,6 +169,7 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
         return;
     }
     const int base = un.rec * kKvRecord;
+    const bool full = un.hi - un.lo == kKvRecord && key.vec && value.vec;   // the usual record of a prompt: no conditions on the loads
     // ---- keys: lane (g, t) owns 8 elements of the tokens g and g + 8 in every block
     bool kmine[2];
     KvRow<TYPE, 8> kx[2][NB];
@@ -182,10 +178,15 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
         const int pos = base + 8 * j + g;
         kmine[j] = pos >= un.lo && pos < un.hi;
         const uint8_t* p = static_cast<const uint8_t*>(key.p) + ((un.row0 + pos) * key.token_stride + (int64_t)h * key.head_stride + 8 * t) * ES;
+        if (full) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            kx[j][b].zero();
-            if (kmine[j]) kx[j][b].load(p + 32 * b * ES, key.vec);
+            for (int b = 0; b < NB; ++b) kx[j][b].load(p + 32 * b * ES, 1);
+        } else {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                kx[j][b].zero();
+                if (kmine[j]) kx[j][b].load(p + 32 * b * ES, key.vec);
+            }
         }
     }
     // ---- values: lane (g, t) owns elements 4 g .. + 3 of every block for the tokens 2t, 2t+1, 2t+8, 2t+9
@@ -199,13 +200,20 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
     }
     KvRow<TYPE, 4> vx[4][NB];
     auto load_values = [&]() {
+        if (full) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                vx[i][b].zero();
-                if (vmine[i]) vx[i][b].load(vp[i] + 32 * b * ES, value.vec);
-            }
+                for (int i = 0; i < 4; ++i) vx[i][b].load(vp[i] + 32 * b * ES, 1);
+        } else {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    vx[i][b].zero();
+                    if (vmine[i]) vx[i][b].load(vp[i] + 32 * b * ES, value.vec);
+                }
+        }
     };
     // (fp32 rows of 192 elements and more do not fit the registers beside the keys)
     constexpr bool kLate = TYPE == kTypeF32 && NB >= 6;
@@ -239,7 +247,7 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             uint32_t codes[NB * KP / 4];
-            uint64_t bytes = 0;
+            uint32_t bytes[2] = {0u, 0u};
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 uint32_t m = kx[j][b].top();
@@ -253,10 +261,15 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
                 }
                 const uint32_t byte = kv_scale_byte<FMT>(m);
                 const float inv = kv_inverse_scale(byte);
-                bytes |= (uint64_t)byte << (8 * b);
+                bytes[b / 4] |= byte << (8 * (b & 3));
                 float2 x[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = kv_scaled(kx[j][b].pair(i), inv);
+                for (int i = 0; i < 4; ++i) x[i] = mul2(kx[j][b].pair(i), make_float2(inv, inv));
+                if (__any_sync(0xffffffffu, inv == 0.f)) {   // (a NaN or infinity times 0 is a NaN; its code is to be zero)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (inv == 0.f) x[i] = make_float2(0.f, 0.f);
+                }
                 if constexpr (FMT == kKvMx8) {
                     codes[2 * b] = e4m3x4_of(x[0].x, x[0].y, x[1].x, x[1].y);
                     codes[2 * b + 1] = e4m3x4_of(x[2].x, x[2].y, x[3].x, x[3].y);
@@ -268,10 +281,10 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
                 store_lane<NB * KP>(rec + j * 32 * NB * KP, lane, codes);
                 if (t == 0) {
                     uint8_t* p = rec + kv_key_scale_offset(FMT, NB) + (8 * j + g) * NS;
-                    if constexpr (NS == 1) *p = (uint8_t)bytes;
-                    else if constexpr (NS == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)bytes;
-                    else if constexpr (NS == 4) *reinterpret_cast<uint32_t*>(p) = (uint32_t)bytes;
-                    else *reinterpret_cast<uint2*>(p) = make_uint2((uint32_t)bytes, (uint32_t)(bytes >> 32));
+                    if constexpr (NS == 1) *p = (uint8_t)bytes[0];
+                    else if constexpr (NS == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)bytes[0];
+                    else if constexpr (NS == 4) *reinterpret_cast<uint32_t*>(p) = bytes[0];
+                    else *reinterpret_cast<uint2*>(p) = make_uint2(bytes[0], bytes[1]);
                 }
             }
         }
@@ -280,7 +293,8 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
     // ---- values
     if constexpr (kLate) load_values();
     uint32_t v[NB * VP / 4], keep[4];   // keep: bits of a block's words that belong to tokens of other calls
-    uint64_t scales[4] = {0, 0, 0, 0};  // of each token: the blocks' scale bytes, 0 for a block of zeros
+    uint32_t scales[4][2] = {};         // of each token: the blocks' scale bytes, and the largest and smallest of them
+    uint32_t top[4] = {0u, 0u, 0u, 0u}, least[4] = {255u, 255u, 255u, 255u};
     if constexpr (!kMx) {
         keep[0] = (vmine[0] ? 0u : 0x0000ffffu) | (vmine[1] ? 0u : 0xffff0000u);
         keep[1] = (vmine[2] ? 0u : 0x0000ffffu) | (vmine[3] ? 0u : 0xffff0000u);
@@ -318,9 +332,16 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
             for (int i = 0; i < 4; ++i) {
                 const uint32_t byte = kv_scale_byte<FMT>(m[i]);
                 const float inv = kv_inverse_scale(byte);
-                scales[i] |= (uint64_t)(m[i] == 0u ? 0u : byte) << (8 * b);
-                const float2 y = kv_scaled(vx[i][b].pair(0), inv), z = kv_scaled(vx[i][b].pair(1), inv);
+                scales[i][b / 4] |= byte << (8 * (b & 3));
+                top[i] = max(top[i], byte);
+                least[i] = min(least[i], byte);
+                const float2 y = mul2(vx[i][b].pair(0), make_float2(inv, inv)), z = mul2(vx[i][b].pair(1), make_float2(inv, inv));
                 x[i][0] = y.x, x[i][1] = y.y, x[i][2] = z.x, x[i][3] = z.y;
+            }
+            if (__any_sync(0xffffffffu, max(max(top[0], top[1]), max(top[2], top[3])) == 255u)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if ((scales[i][b / 4] >> (8 * (b & 3)) & 0xffu) == 255u) x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
             }
         } else {
 #pragma unroll
@@ -361,26 +382,27 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
         store_lane<NB * VP>(rec + kv_value_offset(FMT, NB), lane, v);
     }
     if constexpr (kMx) {   // scales and tops: two token pairs a lane t, lanes g = 0 and 1 one each
-        uint32_t top[4], odd[4];
+        uint32_t odd[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            top[i] = 1, odd[i] = 0;
+        for (int i = 0; i < 4; ++i) odd[i] = least[i] + kKvNear < top[i] ? 1u : 0u;
+        if (__any_sync(0xffffffffu, max(max(top[0], top[1]), max(top[2], top[3])) == 255u)) {   // a block stored as NaN
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const uint32_t e = (uint32_t)(scales[i] >> (8 * b)) & 0xffu;
-                if (e == 255u) odd[i] = 1;
-                else top[i] = max(top[i], e);
-            }
+            for (int i = 0; i < 4; ++i) {
+                if (top[i] != 255u) continue;
+                odd[i] = 1u;
+                top[i] = 1u;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const uint32_t e = (uint32_t)(scales[i] >> (8 * b)) & 0xffu;
-                if (e != 0u && e + kKvNear < top[i]) odd[i] = 1;
-                if (e == 0u) scales[i] |= (uint64_t)top[i] << (8 * b);
+                for (int b = 0; b < NB; ++b) {
+                    const uint32_t e = scales[i][b / 4] >> (8 * (b & 3)) & 0xffu;
+                    if (e != 255u) top[i] = max(top[i], e);
+                }
             }
         }
         if (g < 2) {
             const bool second = g == 1;
-            const uint64_t sa = second ? scales[2] : scales[0], sb = second ? scales[3] : scales[1];
+            uint32_t sa[2], sb[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) sa[i] = second ? scales[2][i] : scales[0][i], sb[i] = second ? scales[3][i] : scales[1][i];
             const bool ma = second ? vmine[2] : vmine[0], mb = second ? vmine[3] : vmine[1];
             const uint32_t word = (second ? top[2] : top[0]) | (second ? top[3] : top[1]) << 8 | (second ? odd[2] : odd[0]) << 16 |
                                   (second ? odd[3] : odd[1]) << 24;
@@ -390,7 +412,7 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
                 uint32_t out[(NB + 1) / 2];
 #pragma unroll
                 for (int i = 0; i < (NB + 1) / 2; ++i)   // bytes (a, b) of blocks 2i and 2i + 1
-                    out[i] = __byte_perm((uint32_t)(sa >> (16 * i)) & 0xffffu, (uint32_t)(sb >> (16 * i)) & 0xffffu, 0x5140);
+                    out[i] = __byte_perm(sa[i / 2], sb[i / 2], i & 1 ? 0x7362 : 0x5140);
                 if constexpr (NB == 1) *reinterpret_cast<uint16_t*>(sp) = (uint16_t)out[0];
                 else {
 #pragma unroll
@@ -398,10 +420,9 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
                 }
                 *reinterpret_cast<uint32_t*>(tp) = word;
             } else if (ma || mb) {
-                const uint64_t s = ma ? sa : sb;
                 const int at = ma ? 0 : 1;
 #pragma unroll
-                for (int b = 0; b < NB; ++b) sp[2 * b + at] = (uint8_t)(s >> (8 * b));
+                for (int b = 0; b < NB; ++b) sp[2 * b + at] = (uint8_t)((ma ? sa[b / 4] : sb[b / 4]) >> (8 * (b & 3)));
                 tp[at] = (uint8_t)(word >> (8 * at));
                 tp[2 + at] = (uint8_t)(word >> (16 + 8 * at));
             }
