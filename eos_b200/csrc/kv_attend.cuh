@@ -270,7 +270,8 @@ struct KvWarp {
 
     // A record's value scales: every block's exponent relative to the largest of its token, as f16 pairs of the tokens 2t,
     // 2t + 1 and 2t + 8, 2t + 9 (zero for tokens outside [lo, hi)).
-    __device__ __forceinline__ void value_scales(const uint8_t* rec, bool edge, int lo, int hi, uint32_t (&rel)[2][NB], int lane) const {
+    template <bool EDGE>
+    __device__ __forceinline__ void value_scales(const uint8_t* rec, int lo, int hi, uint32_t (&rel)[2][NB], int lane) const {
         const int t = lane & 3;
         uint32_t tops[2], odd = 0;
 #pragma unroll
@@ -301,7 +302,7 @@ struct KvWarp {
                 }
             }
         }
-        if (edge) {   // what lies in the places that do not count may be anything
+        if constexpr (EDGE) {   // what lies in the places that do not count may be anything
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const uint32_t keep = live_pair(t, p, lo, hi);
@@ -317,10 +318,11 @@ struct KvWarp {
     }
 
     // Adds a record's values; weights as pairs of the tokens 2t, 2t + 1 (0) and 2t + 8, 2t + 9 (1) of head g.
-    __device__ __forceinline__ void values(const uint8_t* rec, bool edge, int lo, int hi, const uint32_t (&whi)[RT][2],
+    template <bool EDGE>
+    __device__ __forceinline__ void values(const uint8_t* rec, int lo, int hi, const uint32_t (&whi)[RT][2],
                                            const uint32_t (&wlo)[RT][2], const uint32_t (&rel)[2][NB], int lane) {
         uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-        if (!kMx && edge) keep[0] = live_pair(lane & 3, 0, lo, hi), keep[1] = live_pair(lane & 3, 1, lo, hi);
+        if constexpr (!kMx && EDGE) keep[0] = live_pair(lane & 3, 0, lo, hi), keep[1] = live_pair(lane & 3, 1, lo, hi);
         uint32_t v[NB * VP / 4];
         load_lane<NB * VP>(rec + kv_value_offset(FMT, NB), lane, v);
 #pragma unroll
@@ -332,7 +334,7 @@ struct KvWarp {
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
                         f[e][p] = v[8 * b + 4 * (e >> 1) + 2 * p + (e & 1)];
-                        if (edge) f[e][p] &= keep[p];
+                        if constexpr (EDGE) f[e][p] &= keep[p];
                     }
             } else if constexpr (FMT == kKvMx8) {
 #pragma unroll
@@ -363,15 +365,14 @@ struct KvWarp {
         return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
     }
 
-    // N records; of their 16 N tokens [lo, hi) count.  Two at a time keep twice the independent work in flight and share the
-    // tests for a new maximum.
-    template <int N>
+    // N records; EDGE: of their 16 N tokens [lo, hi) count, else all.  Two at a time keep twice the independent work in
+    // flight and share the tests for a new maximum and the work around the ring.
+    template <int N, bool EDGE>
     __device__ __forceinline__ void records(const uint8_t* const (&rec)[N], int lo, int hi, int lane) {
         const int g = lane >> 2;
         float s[N][RT][4];
 #pragma unroll
         for (int n = 0; n < N; ++n) scores(rec[n], s[n], lane);
-        const bool edge = lo > 0 || hi < N * kKvRecord;
         bool dead[N][2];   // tokens g, g + 8 that do not count
         float te[N][2];
         uint32_t rel[N][2][NB];
@@ -380,12 +381,12 @@ struct KvWarp {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int tok = n * kKvRecord + g + 8 * i;
-                dead[n][i] = edge && (tok < lo || tok >= hi);
+                dead[n][i] = EDGE && (tok < lo || tok >= hi);
                 // the token's top byte as a float, by way of the integers behind 2^23
                 if constexpr (kMx)
                     te[n][i] = __uint_as_float(0x4b000000u | rec[n][kv_value_top_offset(FMT, NB) + 4 * (g >> 1) + (g & 1) + 16 * i]) - 8388735.f;
             }
-            if constexpr (kMx) value_scales(rec[n], edge, lo - n * kKvRecord, hi - n * kKvRecord, rel[n], lane);
+            if constexpr (kMx) value_scales<EDGE>(rec[n], lo - n * kKvRecord, hi - n * kKvRecord, rel[n], lane);
         }
         // softmax
         uint32_t whi[N][RT][2], wlo[N][RT][2];
@@ -478,7 +479,7 @@ struct KvWarp {
                 }
         }
 #pragma unroll
-        for (int n = 0; n < N; ++n) values(rec[n], edge, lo - n * kKvRecord, hi - n * kKvRecord, whi[n], wlo[n], rel[n], lane);
+        for (int n = 0; n < N; ++n) values<EDGE>(rec[n], lo - n * kKvRecord, hi - n * kKvRecord, whi[n], wlo[n], rel[n], lane);
     }
 
     // the sum of weights of head 2t + c of tile r
@@ -542,26 +543,20 @@ constexpr int kKvMinRecords = 8;    // records of a CTA, at least
 // ring, which is empty by then; that of its first one, if it is another, to the workspace.
 template <int FMT, int NB, int RT, int HALVES>
 struct KvShape {
-    // as many warps as registers and rings allow: accumulators and query take 8 NB RT + 4 NB RT HALVES registers a thread of
-    // the 65536 / (32 warps), and a ring holds three records (two of 16 KB)
+    // at most as many warps as registers allow: accumulators and query take 8 NB RT + 4 NB RT HALVES registers a thread of the
+    // 65536 / (32 warps)
     static constexpr int kRegisters = 8 * NB * RT + 4 * NB * RT * HALVES;
-    static constexpr int kWarpsByRegisters = kRegisters <= 48 ? 16 : kRegisters <= 80 ? 12 : 8;
+    // two records at a time where a record is much arithmetic for few bytes
+    static constexpr bool kPair = FMT >= kKvMx8 && NB * RT <= 4;
+    static constexpr int kMaxWarps = kRegisters <= (FMT == kKvMx4 ? 48 : 32) ? 16 : kRegisters <= 80 ? 12 : 8;
+    static constexpr int kMaxThreads = 32 * kMaxWarps;
     static constexpr int kRecord = kv_record_bytes(FMT, NB);
-    static constexpr int kSmemMax = 232448 - 10240;              // of a CTA, less the static part
-    static constexpr int kWarpsByRings = kSmemMax / 16 / kRecord >= 3   ? 16
-                                         : kSmemMax / 12 / kRecord >= 3 ? 12
-                                         : kSmemMax / 8 / kRecord >= 3  ? 8
-                                                                        : 6;
-    static constexpr int kWarps = kWarpsByRegisters < kWarpsByRings ? kWarpsByRegisters : kWarpsByRings;
-    static constexpr int kThreads = 32 * kWarps;
+    static constexpr int kMaxStages = 16;                        // of a ring
+    static constexpr int kSmemMax = 232448 - 12288;              // of a CTA, less the static part
     static constexpr int kRows = 8 * RT;
     static constexpr int kPartial = kRows * (32 * NB + 3);       // floats: numerators, then (m, big, l) of each row
-    static constexpr int kRoom = kSmemMax / kWarps / kRecord;
-    static constexpr int kStages = kRoom > 8 ? 8 : kRoom;        // of one warp's ring
-    static constexpr int kRing = kStages * kRecord;
-    static constexpr bool kPair = NB * RT <= 2 && kStages >= 4;  // two records at a time
-    static constexpr int kSmem = kWarps * kRing;
-    static_assert(kStages >= 2 && kStages <= 16 && kRing >= 4 * kPartial && kRing % 16 == 0 && kWarps * kPartial <= kKvSlotFloats, "ring");
+    static_assert(kMaxWarps * kPartial <= kKvSlotFloats && kMaxWarps * kPartial * 4 <= kSmemMax && kSmemMax / 4 / kRecord >= 3 &&
+                      kPartial * 4 % 32 == 0 && kRecord % 16 == 0, "rings, slots");
 };
 
 __device__ __noinline__ inline int64_t kv_div64(int64_t a, int64_t b) { return a / b; }
@@ -587,7 +582,8 @@ __device__ __forceinline__ int64_t kv_div(int64_t a, int64_t b) {   // not negat
 struct KvSplit {
     int chunks;                     // chunks of query heads per key head
     int row_warps;                  // warps that share a record, each with its own rows
-    int per_seq, teams;             // units of a sequence; warps of a CTA / row_warps
+    int per_seq, teams, stages;     // units of a sequence; warps of a CTA / row_warps; records of a team's ring
+    int ring_bytes;                 // of a team: its records, and room for its warps' partial results
     KvDiv by_ctas, by_per_seq, by_teams, by_page, by_chunks;   // (by_page: records of a page)
     float* slots;                   // [ctas][kKvSlotFloats]: partial results of the warps' first units
     float* partial;                 // [ctas][2][rows][dim + 3]: of the CTAs, numerators of all rows, then (m, big, l) of each
@@ -663,37 +659,39 @@ __device__ __forceinline__ float load_part(const float* p) {
 }
 
 template <int FMT, int NB, int RT, int HALVES>
-__global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads, 1)
+__global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
     kv_attend_kernel(KvPool pool, KvSeqs seqs, KvAttend a, KvSplit split, int* status) {
     using Shape = KvShape<FMT, NB, RT, HALVES>;
-    constexpr int D = 32 * NB, kRows = Shape::kRows, kWarps = Shape::kWarps, kThreads = Shape::kThreads;
-    constexpr int kMaxStages = 16;
+    constexpr int D = 32 * NB, kRows = Shape::kRows, kMaxWarps = Shape::kMaxWarps, kMaxStages = Shape::kMaxStages;
     extern __shared__ __align__(128) uint8_t smem[];          // rings
-    __shared__ int64_t s_before[kThreads];                    // records of the sequences before thread i's
-    __shared__ int64_t s_warp[kWarps];
-    __shared__ int64_t s_unit[2 * kWarps];
-    __shared__ int s_ends[2 * kWarps];                        // bit 0: the unit begins there, 1: it ends there, 2: in the ring
-    __shared__ int64_t s_from[2 * kWarps];                    // first record, among all, of the slot's unit, and
-    __shared__ int s_long[2 * kWarps];                        // its records
+    __shared__ int64_t s_before[32 * kMaxWarps];                  // records of the sequences before thread i's
+    __shared__ int64_t s_warp[kMaxWarps];
+    __shared__ int64_t s_unit[2 * kMaxWarps];
+    __shared__ int s_ends[2 * kMaxWarps];                        // bit 0: the unit begins there, 1: it ends there, 2: in the ring
+    __shared__ int64_t s_from[2 * kMaxWarps];                    // first record, among all, of the slot's unit, and
+    __shared__ int s_long[2 * kMaxWarps];                        // its records
     __shared__ int s_turn[2];                                 // whether this CTA joins its first / last unit's parts
-    __shared__ __align__(8) uint64_t s_full[kWarps][kMaxStages], s_empty[kWarps][kMaxStages];
-    __shared__ uint8_t s_ok[kWarps][kMaxStages];              // whether the record could be fetched
-    __shared__ int s_abort, s_drain[kWarps];
-    __shared__ KvAhead s_ahead[kWarps];
+    __shared__ __align__(8) uint64_t s_full[kMaxWarps][kMaxStages], s_empty[kMaxWarps][kMaxStages];
+    __shared__ uint8_t s_ok[kMaxWarps][kMaxStages];              // whether the record could be fetched
+    __shared__ int s_abort, s_drain[kMaxWarps];
+    __shared__ KvAhead s_ahead[kMaxWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int threads = blockDim.x, warps = threads >> 5;
     const int per_seq = split.per_seq;
     const int chunk_rows = kRows * split.row_warps;
     const int teams = split.teams, team = split.row_warps == 1 ? warp : warp / split.row_warps, rw = warp - team * split.row_warps;
-    const int stages = min(kMaxStages, Shape::kStages * split.row_warps);   // of the team's ring
+    const int stages = split.stages;
+    uint8_t* ring = smem + team * split.ring_bytes;
     // partial results: slot 0 (a unit that began before the warp's range), slot 1 (one that goes on behind it); `last`: of
     // the warp's last unit
     auto slot_rows = [&](int w, bool last) {
-        return last ? reinterpret_cast<float*>(smem + w * Shape::kRing)
+        const int of = split.row_warps == 1 ? w : w / split.row_warps;   // team
+        return last ? reinterpret_cast<float*>(smem + of * split.ring_bytes) + (w - of * split.row_warps) * Shape::kPartial
                     : split.slots + (int64_t)blockIdx.x * kKvSlotFloats + w * Shape::kPartial;
     };
 
     // ---- records of all sequences, scanned by the CTA
-    const int per = (seqs.batch + kThreads - 1) / kThreads;
+    const int per = (seqs.batch + threads - 1) / threads;
     int64_t mine = 0;
 #pragma unroll 1
     for (int b = tid * per; b < min((tid + 1) * per, seqs.batch); ++b) {
@@ -708,7 +706,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads, 1)
         if (lane >= o) upto += v;
     }
     if (lane == 31) s_warp[warp] = upto;
-    if (tid < 2 * kWarps) s_unit[tid] = -1;
+    if (tid < 2 * warps) s_unit[tid] = -1;
     if (tid == 0) s_abort = 0;
     if (rw == 0 && lane < stages) {
         mbar_init(smem_u32(&s_full[team][lane]), 1);
@@ -717,8 +715,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads, 1)
     mbar_fence_init();
     __syncthreads();
     int64_t base = 0, total = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
+    for (int i = 0; i < warps; ++i) {
         if (i < warp) base += s_warp[i];
         total += s_warp[i];
     }
@@ -735,9 +732,8 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads, 1)
         KvWalk at;
         {
             const int64_t q = split.by_per_seq(t0);   // all units of a sequence have as many records
-            constexpr int kStep = kThreads / 32;
-            int i = 31 - __clz(__ballot_sync(0xffffffffu, s_before[lane * kStep] <= q));
-            i = i * kStep + 31 - __clz(__ballot_sync(0xffffffffu, lane < kStep && s_before[min(i * kStep + lane, kThreads - 1)] <= q));
+            int i = 31 - __clz(__ballot_sync(0xffffffffu, s_before[lane * warps] <= q));
+            i = i * warps + 31 - __clz(__ballot_sync(0xffffffffu, lane < warps && s_before[min(i * warps + lane, threads - 1)] <= q));
             at.seek(pool, seqs, a.window, per_seq, q, t0, i * per, s_before[i]);
         }
         // The copies, by the team's first warp: the walk of the records to fetch runs a ring ahead of the one below.  What it
@@ -773,7 +769,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads, 1)
             __syncwarp();
             return true;
         };
-        const uint32_t ring_at = smem_u32(smem + team * split.row_warps * Shape::kRing), full_at = smem_u32(&s_full[team][0]),
+        const uint32_t ring_at = smem_u32(ring), full_at = smem_u32(&s_full[team][0]),
                        empty_at = smem_u32(&s_empty[team][0]);
         uint64_t policy;
         asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
@@ -792,6 +788,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads, 1)
             // the unit's span relative to the next record's first token
             int lo = at.lo - (at.lo / kKvRecord + at.r) * kKvRecord, hi = lo + at.hi - at.lo;
             const int row_warps = opaque(split.row_warps);
+            const bool pair = opaque(stages) >= 4;   // (else two would leave nothing under way)
 #pragma unroll 1
             for (int j = seg; j > 0;) {
 #pragma unroll 1
@@ -800,48 +797,53 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads, 1)
                         empty = -0x40000000;   // never again
                         break;
                     }
-                    // every warp of the team is done with what the stage held (true at once the first time round)
-                    if (row_warps > 1) alive = mbar_wait(empty_at + 8 * fill, fill_phase, &s_abort);
-                    if (!alive) break;
-                    if (lane == 0) {
-                        s_ok[team][fill] = src != nullptr;
-                        if (src != nullptr) {
-                            kv_copy_record(ring_at + fill * Shape::kRecord, src, Shape::kRecord, full_at + 8 * fill, policy);
-                        } else {
-                            atomicExch(status, kStatusBadPage);
-                            mbar_arrive(full_at + 8 * fill);
+                    // as many at once as there are in a row, one a lane
+                    const int k = min(min(empty, run), stages - fill);
+                    if (lane < k) {
+                        const int st = fill + lane;
+                        // every warp of the team is done with what the stage held (true at once the first time round)
+                        if (row_warps > 1) alive = mbar_wait(empty_at + 8 * st, fill_phase, &s_abort);
+                        if (alive) {
+                            s_ok[team][st] = src != nullptr;
+                            if (src != nullptr) {
+                                kv_copy_record(ring_at + st * Shape::kRecord, src + lane * Shape::kRecord, Shape::kRecord, full_at + 8 * st, policy);
+                            } else {
+                                atomicExch(status, kStatusBadPage);
+                                mbar_arrive(full_at + 8 * st);
+                            }
                         }
                     }
-                    if (src != nullptr) src += Shape::kRecord;
-                    --run;
-                    --empty;
-                    if (++fill == stages) fill = 0, fill_phase ^= 1u;
+                    if (row_warps > 1) alive = __all_sync(0xffffffffu, alive);
+                    if (src != nullptr) src += k * Shape::kRecord;
+                    run -= k;
+                    empty -= k;
+                    fill += k;
+                    if (fill == stages) fill = 0, fill_phase ^= 1u;
                 }
-                const int take = Shape::kPair && j > 1 ? 2 : 1;
+                const int take = Shape::kPair && j > 1 && lo <= 0 && hi >= 2 * kKvRecord && pair ? 2 : 1;
                 const int next = stage + 1 == stages ? 0 : stage + 1;
                 alive = alive && mbar_wait(full_at + 8 * stage, phase, &s_abort);
-                const uint8_t* here = smem + team * split.row_warps * Shape::kRing + stage * Shape::kRecord;
+                const uint8_t* here = ring + stage * Shape::kRecord;
                 const bool ok = alive && s_ok[team][stage];
                 bool one = ok;
-                int shift = 0;
                 if constexpr (Shape::kPair) {
-                    if (take == 2) {
+                    if (take == 2) {   // (all tokens of both count)
                         alive = alive && mbar_wait(full_at + 8 * next, next == 0 ? phase ^ 1u : phase, &s_abort);
-                        const uint8_t* there = smem + team * split.row_warps * Shape::kRing + next * Shape::kRecord;
+                        const uint8_t* there = ring + next * Shape::kRecord;
                         const bool ok2 = alive && s_ok[team][next];
                         one = ok != ok2;   // a record that is missing is left out
                         if (ok && ok2) {
                             const uint8_t* const both[2] = {here, there};
-                            w.template records<2>(both, max(lo, 0), min(hi, 2 * kKvRecord), lane);
+                            w.template records<2, false>(both, 0, 2 * kKvRecord, lane);
                         } else if (ok2) {
                             here = there;
-                            shift = kKvRecord;
                         }
                     }
                 }
                 if (one) {
                     const uint8_t* const single[1] = {here};
-                    w.template records<1>(single, max(lo - shift, 0), min(hi - shift, kKvRecord), lane);
+                    if (!Shape::kPair && lo <= 0 && hi >= kKvRecord) w.template records<1, false>(single, 0, kKvRecord, lane);
+                    else w.template records<1, true>(single, max(lo, 0), min(hi, kKvRecord), lane);
                 }
                 __syncwarp();
                 if (row_warps > 1 && lane == 0) {
@@ -964,7 +966,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads, 1)
             }
             const int tasks = phase_no == 0 ? __popc(starts) : 2;
 #pragma unroll 1
-            for (int item = warp; item < tasks * rows_used; item += kWarps) {
+            for (int item = warp; item < tasks * rows_used; item += warps) {
                 const int task = item / rows_used, row = item - task * rows_used;
                 // where the results to join lie, one a lane, and where the joined one goes
                 const float *from, *from_stats;
@@ -1074,11 +1076,11 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kThreads, 1)
         if (hi > lo) continue;
         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-        for (int i = tid; i < a.q_heads * (D / 4); i += kThreads)
+        for (int i = tid; i < a.q_heads * (D / 4); i += threads)
             store_row(a.out, b * a.q_heads * D + 4 * i, a.type, zero);
         if (a.lse != nullptr)
 #pragma unroll 1
-            for (int i = tid; i < a.q_heads; i += kThreads) a.lse[b * a.q_heads + i] = -INFINITY;
+            for (int i = tid; i < a.q_heads; i += threads) a.lse[b * a.q_heads + i] = -INFINITY;
     }
 }
 
@@ -1086,19 +1088,29 @@ template <int FMT, int NB, int RT, int HALVES>
 struct KvAttendInstance {
     using Shape = KvShape<FMT, NB, RT, HALVES>;
     static cudaError_t init() {
-        return cudaFuncSetAttribute(kv_attend_kernel<FMT, NB, RT, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
+        return cudaFuncSetAttribute(kv_attend_kernel<FMT, NB, RT, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmemMax);
     }
     static int launch(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
                       cudaStream_t stream) {
         KvSplit split{};
-        // warps for the rows of a key head: the smallest divisor of the CTA's warps that covers them, at most 128 rows
+        // warps for the rows of a key head: as many as it takes to cover them, a power of two, at most 8 (64 or 128 rows)
         split.row_warps = 1;
-        for (int d = 2; d <= 8 && split.row_warps * 8 * RT < a.group; ++d)
-            if (Shape::kWarps % d == 0) split.row_warps = d;
+        while (split.row_warps < 8 && split.row_warps * 8 * RT < a.group) split.row_warps *= 2;
+        // as many warps as registers allow and rings of three records (of four where two records are taken at a time)
+        int warps = Shape::kMaxWarps;
+        for (;; warps -= 4) {
+            split.teams = warps / split.row_warps;
+            split.stages = std::min(Shape::kSmemMax / split.teams / Shape::kRecord, Shape::kMaxStages);
+            if (warps % split.row_warps == 0 && (split.stages >= (Shape::kPair ? 4 : 3) || warps <= 8)) break;
+        }
+        if (split.stages < 3) {   // 16-bit records of 12 KB and more, one row warp
+            warps = split.teams = 4;
+            split.stages = Shape::kSmemMax / split.teams / Shape::kRecord;
+        }
+        split.ring_bytes = std::max(split.stages * Shape::kRecord, split.row_warps * Shape::kPartial * 4);
         const int chunk_rows = split.row_warps * 8 * RT;
         split.chunks = (a.group + chunk_rows - 1) / chunk_rows;
         split.per_seq = pool.heads * split.chunks;
-        split.teams = Shape::kWarps / split.row_warps;
         split.by_ctas = KvDiv(work.ctas);
         split.by_per_seq = KvDiv(split.per_seq);
         split.by_teams = KvDiv(split.teams);
@@ -1107,7 +1119,7 @@ struct KvAttendInstance {
         split.count = work.count;
         split.slots = work.slots;
         split.partial = work.partial;
-        kv_attend_kernel<FMT, NB, RT, HALVES><<<work.ctas, Shape::kThreads, Shape::kSmem, stream>>>(pool, seqs, a, split, status);
+        kv_attend_kernel<FMT, NB, RT, HALVES><<<work.ctas, 32 * warps, split.teams * split.ring_bytes, stream>>>(pool, seqs, a, split, status);
         return 1;
     }
 };
