@@ -81,12 +81,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
     return r;
 }
 
-// exponent field of byte i as a float 2^(byte - 127); 255 becomes infinity, which times the zero codes of such a block is NaN
-__device__ __forceinline__ float scale_at(uint32_t word, int i) {
-    return __uint_as_float(i == 3 ? (word >> 1) & 0x7f800000u
-                                  : (i == 2 ? (word << 7) & 0x7f800000u
-                                            : (i == 1 ? (word << 15) & 0x7f800000u : (word << 23) & 0x7f800000u)));
-}
+// byte i of a word as a float 2^(byte - 127); 255 becomes infinity, which times the zero codes of such a block is NaN
+__device__ __forceinline__ float scale_at(uint32_t word, int i) { return __uint_as_float(__byte_perm(word, 0, 0x4440 | i) << 23); }
 
 // RT: tiles of 8 query heads; HALVES: operands of the query (1: its type fits the operand type).
 template <int FMT, int NB, int RT, int HALVES>
@@ -235,9 +231,8 @@ struct KvWarp {
             load_lane<NB * KP>(rec + 32 * NB * KP, lane, k1);
             load_scales<NB>(rec + kv_key_scale_offset(FMT, NB) + g * kv_scale_stride(NB), e0);
             load_scales<NB>(rec + kv_key_scale_offset(FMT, NB) + (g + 8) * kv_scale_stride(NB), e1);
-            float2 sum[RT][2];
 #pragma unroll
-            for (int r = 0; r < RT; ++r) sum[r][0] = sum[r][1] = make_float2(0.f, 0.f);
+            for (int r = 0; r < RT; ++r) s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.f;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 uint32_t f[4], h[4];   // elements 8 t .. + 7 of tokens g and g + 8
@@ -259,12 +254,10 @@ struct KvWarp {
                         mma_16x8x16<false>(c, f[0], h[0], f[1], h[1], q[r][b][4 * u], q[r][b][4 * u + 1]);
                         mma_16x8x16<false>(c, f[2], h[2], f[3], h[3], q[r][b][4 * u + 2], q[r][b][4 * u + 3]);
                     }
-                    sum[r][0] = fma2(make_float2(c[0], c[1]), make_float2(s0, s0), sum[r][0]);
-                    sum[r][1] = fma2(make_float2(c[2], c[3]), make_float2(s1, s1), sum[r][1]);
+                    s[r][0] = fmaf(c[0], s0, s[r][0]), s[r][1] = fmaf(c[1], s0, s[r][1]);
+                    s[r][2] = fmaf(c[2], s1, s[r][2]), s[r][3] = fmaf(c[3], s1, s[r][3]);
                 }
             }
-#pragma unroll
-            for (int r = 0; r < RT; ++r) s[r][0] = sum[r][0].x, s[r][1] = sum[r][0].y, s[r][2] = sum[r][1].x, s[r][3] = sum[r][1].y;
         }
     }
 
@@ -788,11 +781,12 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
             // the unit's span relative to the next record's first token
             int lo = at.lo - (at.lo / kKvRecord + at.r) * kKvRecord, hi = lo + at.hi - at.lo;
             const int row_warps = opaque(split.row_warps);
+            const int batch = stages >> 1;
             const bool pair = opaque(stages) >= 4;   // (else two would leave nothing under way)
 #pragma unroll 1
             for (int j = seg; j > 0;) {
 #pragma unroll 1
-                while (empty > 0 && alive) {
+                while (empty >= batch && alive) {   // half a ring at a time
                     if (run == 0 && !another_page()) {
                         empty = -0x40000000;   // never again
                         break;
@@ -955,8 +949,10 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
                     if (phase_no == 1 ? (i ? open_last : open_first) : (s_turn[i] && groups > 1)) {
                         __threadfence();
                         mine_now = atomicAdd(count, 1) == of - 1;
-                        if (mine_now) *count = 0;   // for the next call
-                        __threadfence();
+                        if (mine_now) {
+                            *count = 0;   // for the next call
+                            __threadfence();
+                        }
                     }
                     s_turn[i] = mine_now;
                 }
