@@ -3772,18 +3772,23 @@ int eos_b200_kv_cache_create(EosB200Runtime* rt, int64_t pages, int page_size, i
         return fail(err, "kv_cache_create: " + std::to_string(pages) + " pages of " + std::to_string(page_bytes) +
                              " bytes exceed the device's memory");
     CUDA_TRY(cudaSetDevice(rt->device));
-    CUDA_TRY(kv_attend_init(format, p.blocks));
+    CUDA_TRY(kv_init(format, p.blocks));
     EosB200KvCache* c = new (std::nothrow) EosB200KvCache();
     if (c == nullptr) return fail(err, "kv_cache_create: out of host memory");
     c->rt = rt;
-    c->work.ctas = rt->sm_count;
-    cudaError_t e = dev_alloc(&p.base, (size_t)(pages * page_bytes));
+    // one allocation: the pages, then the workspace (its counts first), each part 256-byte aligned
+    const auto part = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
+    const size_t ctas = (size_t)rt->sm_count, pool_bytes = part((size_t)(pages * page_bytes)), count_bytes = part(3 * ctas * sizeof(int)),
+                 slot_bytes = part(ctas * kv_slot_floats(head_dim) * sizeof(float));
+    cudaError_t e = dev_alloc(&p.base, pool_bytes + count_bytes + slot_bytes + ctas * 2 * kKvMaxRows * (head_dim + 3) * sizeof(float));
     c->pool = p;
-    if (e == cudaSuccess) e = dev_alloc(&c->work.partial, kv_work_floats(rt->sm_count, head_dim));
-    if (e == cudaSuccess) e = dev_alloc(&c->work.slots, (size_t)rt->sm_count * kKvSlotFloats);
-    if (e == cudaSuccess) e = dev_alloc(&c->work.count, (size_t)3 * rt->sm_count);
-    if (e == cudaSuccess) e = cudaMemsetAsync(c->work.count, 0, (size_t)3 * rt->sm_count * sizeof(int), rt->stream);
-    if (e == cudaSuccess) e = cudaMemsetAsync(p.base, 0, (size_t)(pages * page_bytes), rt->stream);
+    c->work.ctas = rt->sm_count;
+    if (e == cudaSuccess) {
+        c->work.count = reinterpret_cast<int*>(p.base + pool_bytes);
+        c->work.slots = reinterpret_cast<float*>(p.base + pool_bytes + count_bytes);
+        c->work.partial = reinterpret_cast<float*>(p.base + pool_bytes + count_bytes + slot_bytes);
+        e = cudaMemsetAsync(p.base, 0, pool_bytes + count_bytes, rt->stream);
+    }
     if (e == cudaSuccess) e = cudaStreamSynchronize(rt->stream);
     if (e != cudaSuccess) {
         cudaGetLastError();
@@ -3798,9 +3803,6 @@ void eos_b200_kv_cache_destroy(EosB200KvCache* c) {
     if (c == nullptr) return;
     cudaSetDevice(c->rt->device);
     dev_free(c->pool.base);
-    dev_free(c->work.slots);
-    dev_free(c->work.partial);
-    dev_free(c->work.count);
     delete c;
 }
 

@@ -548,7 +548,7 @@ struct KvShape {
     static constexpr int kSmemMax = 232448 - 12288;              // of a CTA, less the static part
     static constexpr int kRows = 8 * RT;
     static constexpr int kPartial = kRows * (32 * NB + 3);       // floats: numerators, then (m, big, l) of each row
-    static_assert(kMaxWarps * kPartial <= kKvSlotFloats && kMaxWarps * kPartial * 4 <= kSmemMax && kSmemMax / 4 / kRecord >= 3 &&
+    static_assert(kMaxWarps * kPartial <= kv_slot_floats(32 * NB) && kMaxWarps * kPartial * 4 <= kSmemMax && kSmemMax / 4 / kRecord >= 3 &&
                       kPartial * 4 % 32 == 0 && kRecord % 16 == 0, "rings, slots");
 };
 
@@ -578,7 +578,7 @@ struct KvSplit {
     int per_seq, teams, stages;     // units of a sequence; warps of a CTA / row_warps; records of a team's ring
     int ring_bytes;                 // of a team: its records, and room for its warps' partial results
     KvDiv by_ctas, by_per_seq, by_teams, by_page, by_chunks;   // (by_page: records of a page)
-    float* slots;                   // [ctas][kKvSlotFloats]: partial results of the warps' first units
+    float* slots;                   // [ctas][kv_slot_floats]: partial results of the warps' first units
     float* partial;                 // [ctas][2][rows][dim + 3]: of the CTAs, numerators of all rows, then (m, big, l) of each
     int* count;                     // [ctas][2], [ctas]: parts of a group, groups of a unit that are done; zero between calls
 };
@@ -680,7 +680,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
     auto slot_rows = [&](int w, bool last) {
         const int of = split.row_warps == 1 ? w : w / split.row_warps;   // team
         return last ? reinterpret_cast<float*>(smem + of * split.ring_bytes) + (w - of * split.row_warps) * Shape::kPartial
-                    : split.slots + (int64_t)blockIdx.x * kKvSlotFloats + w * Shape::kPartial;
+                    : split.slots + (int64_t)blockIdx.x * kv_slot_floats(D) + w * Shape::kPartial;
     };
 
     // ---- records of all sequences, scanned by the CTA
@@ -719,7 +719,8 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
     const int64_t c0 = min((int64_t)blockIdx.x * part, total), c1 = min(c0 + part, total);
     const int64_t tpart = split.by_teams(c1 - c0 + teams - 1);
     const int64_t t0 = min(c0 + team * tpart, c1);
-    int left = (int)(min(t0 + tpart, c1) - t0);   // records of the team that are not yet done with
+    int left = (int)min(min(t0 + tpart, c1) - t0, (int64_t)0x7fffffff);   // records of the team that are not yet done with
+    if (tpart > 0x7fffffff && tid == 0) atomicExch(status, kStatusBadSequence);   // (2^31 records a warp: lengths gone wrong)
 
     if (left > 0) {
         KvWalk at;

@@ -36,12 +36,13 @@ int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, 
     }
 }
 
-cudaError_t kv_attend_init(int format, int blocks) {
+cudaError_t kv_init(int format, int blocks) {
+    cudaError_t e;
     switch (format) {
-        case kKvF16: return kv_attend_f16_init(blocks);
-        case kKvBf16: return kv_attend_bf16_init(blocks);
-        case kKvMx8: return kv_attend_mx8_init(blocks);
-        default: return kv_attend_mx4_init(blocks);
+        case kKvF16: e = kv_io_f16_init(blocks); return e == cudaSuccess ? kv_attend_f16_init(blocks) : e;
+        case kKvBf16: e = kv_io_bf16_init(blocks); return e == cudaSuccess ? kv_attend_bf16_init(blocks) : e;
+        case kKvMx8: e = kv_io_mx8_init(blocks); return e == cudaSuccess ? kv_attend_mx8_init(blocks) : e;
+        default: e = kv_io_mx4_init(blocks); return e == cudaSuccess ? kv_attend_mx4_init(blocks) : e;
     }
 }
 

@@ -102,16 +102,15 @@ struct KvAttend {
 // Workspace of a cache's attention calls, of a fixed size: captured graphs keep its addresses.
 struct KvWork {
     int ctas;               // one per SM
-    float* slots;           // [ctas][kKvSlotFloats]
-    float* partial;         // kv_work_floats(ctas, dim)
+    float* slots;           // [ctas][kv_slot_floats(dim)]: partial results of the CTAs' warps
+    float* partial;         // [ctas][2][kKvMaxRows][dim + 3]: of the CTAs
     int* count;             // [3 ctas], zero between calls
 };
 constexpr int kKvMaxRows = 128;        // query heads of one unit, at most
-constexpr int kKvSlotFloats = 33280;   // partial results of a CTA's warps
-inline size_t kv_work_floats(int ctas, int dim) { return (size_t)ctas * 2 * kKvMaxRows * (dim + 3); }
+__host__ __device__ constexpr int kv_slot_floats(int dim) { return kKvMaxRows * (dim + 3) + (dim <= 96 ? 128 * (dim + 3) : 0); }   // 128 or (small heads, 16 warps) 256 rows
 
 // cudaSuccess once the kernels of this format and dim are ready on the current device
-cudaError_t kv_attend_init(int format, int blocks);
+cudaError_t kv_init(int format, int blocks);
 int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
                      cudaStream_t stream);
 

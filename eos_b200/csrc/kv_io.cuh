@@ -583,9 +583,34 @@ void kv_io_format(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, con
     }
 }
 
+// Loads the kernels of a cache (their first launch may be inside a stream capture, which loading does not get along with).
+template <int FMT, int NB>
+cudaError_t kv_io_blocks_init() {
+    cudaFuncAttributes at;
+    cudaError_t e = cudaFuncGetAttributes(&at, kv_append_kernel<FMT, NB, kTypeF32>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, kv_append_kernel<FMT, NB, kTypeF16>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, kv_append_kernel<FMT, NB, kTypeBf16>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, kv_read_kernel<FMT, NB, kTypeF32>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, kv_read_kernel<FMT, NB, kTypeF16>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, kv_read_kernel<FMT, NB, kTypeBf16>);
+    return e;
+}
+template <int FMT>
+cudaError_t kv_io_format_init(int blocks) {
+    switch (blocks) {
+        case 1: return kv_io_blocks_init<FMT, 1>();
+        case 2: return kv_io_blocks_init<FMT, 2>();
+        case 3: return kv_io_blocks_init<FMT, 3>();
+        case 4: return kv_io_blocks_init<FMT, 4>();
+        case 6: return kv_io_blocks_init<FMT, 6>();
+        default: return kv_io_blocks_init<FMT, 8>();
+    }
+}
+
 #define EOSB_KV_IO(name)                                                                                                   \
     void kv_append_##name(const KvPool&, const KvSeqs&, const KvRows&, const KvRows&, int, int64_t, int*, cudaStream_t);   \
-    void kv_read_##name(const KvPool&, const KvSeqs&, const KvRows&, const KvRows&, int, int64_t, int*, cudaStream_t);
+    void kv_read_##name(const KvPool&, const KvSeqs&, const KvRows&, const KvRows&, int, int64_t, int*, cudaStream_t);     \
+    cudaError_t kv_io_##name##_init(int blocks);
 EOSB_KV_IO(f16)
 EOSB_KV_IO(bf16)
 EOSB_KV_IO(mx8)

@@ -12,4 +12,6 @@ void kv_read_bf16(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, con
     kv_io_format<true, kKvBf16>(pool, seqs, key, value, type, tokens, status, stream);
 }
 
+cudaError_t kv_io_bf16_init(int blocks) { return kv_io_format_init<kKvBf16>(blocks); }
+
 }  // namespace eosb

@@ -12,4 +12,6 @@ void kv_read_f16(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, cons
     kv_io_format<true, kKvF16>(pool, seqs, key, value, type, tokens, status, stream);
 }
 
+cudaError_t kv_io_f16_init(int blocks) { return kv_io_format_init<kKvF16>(blocks); }
+
 }  // namespace eosb

@@ -12,4 +12,6 @@ void kv_read_mx4(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, cons
     kv_io_format<true, kKvMx4>(pool, seqs, key, value, type, tokens, status, stream);
 }
 
+cudaError_t kv_io_mx4_init(int blocks) { return kv_io_format_init<kKvMx4>(blocks); }
+
 }  // namespace eosb

@@ -12,4 +12,6 @@ void kv_read_mx8(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, cons
     kv_io_format<true, kKvMx8>(pool, seqs, key, value, type, tokens, status, stream);
 }
 
+cudaError_t kv_io_mx8_init(int blocks) { return kv_io_format_init<kKvMx8>(blocks); }
+
 }  // namespace eosb

@@ -603,7 +603,7 @@ EOS_B200_API int eos_b200_kv_cache_read_device(EosB200KvCache* cache, void* d_ke
  * (contiguous, 16-byte aligned); d_lse (nullable) [batch, q_heads] fp32 receives ln sum_j exp(scale q . k_j).  A sequence with n = 0 gives zeros
  * and -infinity.  query_seq_stride / query_head_stride in elements, 0: contiguous.  The new token's own key and value
  * are appended before the call when it attends to itself.
- * Positions on a page that is out of range are left out and eos_b200_kv_cache_sync reports it; a length that is negative
+ * batch is at most 65535.  Positions on a page that is out of range are left out and eos_b200_kv_cache_sync reports it; a length that is negative
  * or longer than the page table is cut, and reported too.  Rows that meet an infinity or a NaN are not finite; other rows are not touched by it.
  * Enqueued, allocation-free and capturable as above; calls of one cache share its workspace and must be ordered (one
  * stream, or events between streams). */

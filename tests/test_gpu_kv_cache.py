@@ -357,6 +357,93 @@ def test_strided_and_unaligned_tensors():
         s.sync()
 
 
+def test_odd_strides_both_ways():
+    """Rows at odd distances, written from and read back into larger buffers; what lies between the rows stays."""
+    dim, heads, n = 96, 2, 37
+    for type_ in ("f16", "f32"):
+        token, head = heads * (dim + 3) + 5, dim + 3
+        buf = torch.randn(n * token + 8, generator=torch.Generator().manual_seed(4)).to(DTYPES[type_]).cuda()
+        view = torch.as_strided(buf, (n, heads, dim), (token, head, 1), 1)
+        s = Sequences("mx8", dim, heads, 16, [n + 3])
+        cu, st = s._ints([0, n]), s._ints([3])
+        at = buf.data_ptr() + buf.element_size()
+        stream = torch.cuda.current_stream().cuda_stream
+        s.cache.append_device(at, at, type_, n, 1, s.table.data_ptr(), s.max_pages, st.data_ptr(), cu.data_ptr(), (token, head) * 2, stream)
+        out = torch.full_like(buf, 5.0)
+        val = torch.full_like(buf, 6.0)
+        es = buf.element_size()
+        s.cache.read_device(out.data_ptr() + es, val.data_ptr() + es, type_, n, 1, s.table.data_ptr(), s.max_pages, st.data_ptr(),
+                            cu.data_ptr(), (token, head) * 2, stream)
+        torch.cuda.synchronize()
+        want = stored(view, "mx8").float().to(DTYPES[type_])
+        for got, fill in ((out, 5.0), (val, 6.0)):
+            assert same(torch.as_strided(got, (n, heads, dim), (token, head, 1), 1), want)
+            torch.as_strided(got, (n, heads, dim), (token, head, 1), 1).fill_(fill)
+            assert (got == fill).all()
+        s.sync()
+
+
+def test_scales_of_any_sign_no_lse_and_rows_that_are_not_finite():
+    dim, heads, group, lengths = 64, 2, 12, [50, 17, 200]
+    for fmt in ("f16", "mx4"):
+        s = Sequences(fmt, dim, heads, 16, lengths)
+        k, v = tensors(sum(lengths), heads, dim, "f32", 8)
+        s.append(k, v, [0] * 3, lengths)
+        cut = lambda x: torch.split(stored(x, fmt), lengths)  # noqa: E731
+        q = tensors(3, heads * group, dim, "f32", 9)[0]
+        for scale in (0.0, -0.2, 0.5):
+            out, lse = s.attend(q, lengths, scale)
+            check_attend(q, (cut(k), cut(v)), lengths, scale, 0, fmt, out, lse, group)
+        n = s._ints(lengths)
+        again = torch.empty_like(out)
+        s.cache.attend_device(q.data_ptr(), "f32", heads * group, 3, s.table.data_ptr(), s.max_pages, n.data_ptr(),
+                              again.data_ptr(), 0.5, stream=torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        assert torch.equal(again, out)
+        # a query that is not finite spoils its own row only
+        bad = q.clone()
+        bad[1, 3, 7] = float("nan")
+        bad[2, 15, 0] = float("inf")
+        got, _ = s.attend(bad, lengths, 0.5)
+        hit = torch.zeros(got.shape[:2], dtype=torch.bool, device="cuda")
+        hit[1, 3] = hit[2, 15] = True
+        assert not torch.isfinite(got[hit]).any() and torch.equal(got[~hit], out[~hit])
+        s.sync()
+
+
+def test_many_sequences_and_units():
+    """More sequences than threads of a CTA, most of them empty or one token long."""
+    dim, heads, batch = 32, 2, 1500
+    rng = np.random.default_rng(3)
+    lengths = [int(x) for x in rng.choice([0, 0, 1, 2, 16, 17, 40], size=batch)]
+    s = Sequences("mx8", dim, heads, 16, lengths)
+    k, v = tensors(sum(lengths), heads, dim, "f16", 13)
+    s.append(k, v, [0] * batch, lengths)
+    q = tensors(batch, heads * 2, dim, "f16", 14)[0]
+    out, lse = s.attend(q, lengths, 0.25)
+    s.sync()
+    cut = lambda x: torch.split(stored(x, "mx8"), lengths)  # noqa: E731
+    check_attend(q, (cut(k), cut(v)), lengths, 0.25, 0, "mx8", out, lse, 2)
+
+
+@pytest.mark.parametrize("fmt,type_,dim,heads,group", [("f16", "f16", 128, 1, 4), ("bf16", "bf16", 256, 1, 16), ("mx8", "f32", 128, 2, 1),
+                                                       ("mx4", "bf16", 64, 1, 33)])
+def test_one_long_sequence_over_all_ctas(fmt, type_, dim, heads, group):
+    """Units that every CTA holds a part of: joined by neighbours first, then over the groups."""
+    n = 40000 + 13
+    s = Sequences(fmt, dim, heads, 64, [n, 5], seed=2)
+    k, v = tensors(n + 5, heads, dim, type_, 15)
+    s.append(k, v, [0, 0], [n, 5])
+    q = tensors(2, heads * group, dim, type_, 16)[0]
+    scale = 3 * dim ** -0.5
+    out, lse = s.attend(q, [n, 5], scale)
+    s.sync()
+    cut = lambda x: torch.split(stored(x, fmt), [n, 5])  # noqa: E731
+    check_attend(q, (cut(k), cut(v)), [n, 5], scale, 0, fmt, out, lse, group)
+    again, lse2 = s.attend(q, [n, 5], scale)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
 def test_bad_pages_and_lengths_are_reported_and_left_out():
     import eos_b200
     dim, heads, n = 64, 2, 64
