@@ -3714,9 +3714,10 @@ namespace {
 
 int type_bytes(int type) { return type == EOS_B200_TYPE_F32 ? 4 : 2; }
 
-bool aligned16(const void* p, int64_t stride_a, int64_t stride_b, int type) {
-    const int64_t es = type_bytes(type);
-    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride_a * es % 16 == 0 && stride_b * es % 16 == 0;
+// 2: rows at these strides start on 32-byte boundaries, 1: on 16-byte ones, 0: neither
+int row_alignment(const void* p, int64_t stride_a, int64_t stride_b, int type) {
+    const uint64_t all = reinterpret_cast<uintptr_t>(p) | (uint64_t)(stride_a * type_bytes(type)) | (uint64_t)(stride_b * type_bytes(type));
+    return all % 32 == 0 ? 2 : all % 16 == 0 ? 1 : 0;
 }
 
 // What append and read check alike; fills the kernels' views.
@@ -3739,8 +3740,8 @@ std::string kv_rows_check(const EosB200KvCache* c, const void* key, const void* 
     // blocks of eight warps, one (record, head) each
     if ((tokens / kKvRecord + 2 * (int64_t)batch + 1) * c->pool.heads / 8 >= 0x7fffffffLL) return "too many tokens x heads in one call";
     *seqs = {table, max_pages, batch, starts, cu, nullptr};
-    *k = {const_cast<void*>(key), s.key_token, s.key_head, aligned16(key, s.key_token, s.key_head, type) ? 1 : 0};
-    *v = {const_cast<void*>(value), s.value_token, s.value_head, aligned16(value, s.value_token, s.value_head, type) ? 1 : 0};
+    *k = {const_cast<void*>(key), s.key_token, s.key_head, row_alignment(key, s.key_token, s.key_head, type)};
+    *v = {const_cast<void*>(value), s.value_token, s.value_head, row_alignment(value, s.value_token, s.value_head, type)};
     return "";
 }
 
@@ -3874,7 +3875,7 @@ int eos_b200_kv_cache_attend_device(EosB200KvCache* c, const void* d_query, int 
     a.query = d_query;
     a.head_stride = query_head_stride > 0 ? query_head_stride : c->pool.dim;
     a.seq_stride = query_seq_stride > 0 ? query_seq_stride : (int64_t)q_heads * c->pool.dim;
-    a.vec = aligned16(d_query, a.seq_stride, a.head_stride, type) ? 1 : 0;
+    a.vec = row_alignment(d_query, a.seq_stride, a.head_stride, type);
     a.type = type;
     a.q_heads = q_heads;
     a.group = q_heads / c->pool.heads;

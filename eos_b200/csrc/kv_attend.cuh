@@ -777,12 +777,11 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
             int seg = min(at.n - at.r, left);   // records of the unit here
             const int h = (int)split.by_chunks(at.hu), row0 = (at.hu - h * split.chunks) * chunk_rows + rw * kRows;
             w.load_query(a, (int64_t)at.b * a.seq_stride + (int64_t)h * a.group * a.head_stride, row0, a.group, lane);
-            w.convert_query(a, lane);
-            w.reset();
             // the unit's span relative to the next record's first token
             int lo = at.lo - (at.lo / kKvRecord + at.r) * kKvRecord, hi = lo + at.hi - at.lo;
             const int row_warps = opaque(split.row_warps);
             const int batch = stages >> 1;
+            int fresh = opaque(1);                       // the query is on its way
             const bool pair = opaque(stages) >= 4;   // (else two would leave nothing under way)
 #pragma unroll 1
             for (int j = seg; j > 0;) {
@@ -814,6 +813,11 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
                     empty -= k;
                     fill += k;
                     if (fill == stages) fill = 0, fill_phase ^= 1u;
+                }
+                if (fresh) {   // (the first copies' latency and the query's pass together)
+                    w.convert_query(a, lane);
+                    w.reset();
+                    fresh = opaque(0);
                 }
                 const int take = Shape::kPair && j > 1 && lo <= 0 && hi >= 2 * kKvRecord && pair ? 2 : 1;
                 const int next = stage + 1 == stages ? 0 : stage + 1;

@@ -79,7 +79,7 @@ struct KvSeqs {
 struct KvRows {             // keys or values of a call, [tokens, heads, dim] with strides in elements
     void* p;
     int64_t token_stride, head_stride;
-    int vec;                // 16-byte accesses are aligned
+    int vec;                // accesses of 16 bytes (1), of 32 bytes (2) are aligned
 };
 
 void launch_kv_append(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type,

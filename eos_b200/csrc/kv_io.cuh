@@ -79,12 +79,19 @@ struct KvRow {
             if constexpr (kWords == 2) {
                 const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
                 w[0] = v.x, w[1] = v.y;
-            } else {
+            } else if constexpr (kWords == 8) {   // a lane's 32 bytes are a whole sector
+                if (vec > 1) {
+                    ld_global_v8(p, w);
+                } else {
 #pragma unroll
-                for (int i = 0; i < kWords; i += 4) {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
-                    w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+                    for (int i = 0; i < kWords; i += 4) {
+                        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+                        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+                    }
                 }
+            } else {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+                w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
             }
         } else {
             const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
@@ -180,7 +187,7 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
         const uint8_t* p = static_cast<const uint8_t*>(key.p) + ((un.row0 + pos) * key.token_stride + (int64_t)h * key.head_stride + 8 * t) * ES;
         if (full) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) kx[j][b].load(p + 32 * b * ES, 1);
+            for (int b = 0; b < NB; ++b) kx[j][b].load(p + 32 * b * ES, key.vec);
         } else {
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -442,9 +449,11 @@ __device__ __forceinline__ void store_out(uint8_t* p, int vec, const float (&x)[
     }
     if (vec) {
         if constexpr (kWords == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        else if constexpr (kWords == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        else if (vec > 1) st_global_v8(p, w);
         else {
-#pragma unroll
-            for (int i = 0; i < kWords; i += 4) *(reinterpret_cast<uint4*>(p) + i / 4) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+            *(reinterpret_cast<uint4*>(p) + 1) = make_uint4(w[4], w[5], w[6], w[7]);
         }
     } else {
         uint16_t* h = reinterpret_cast<uint16_t*>(p);
