@@ -8,8 +8,8 @@
 // A block that holds an infinity or a NaN is stored as NaN (scale byte 255, codes zero).
 //
 // One warp per (record, head): it owns all 16 tokens of the record that the call writes, so a record that is completed
-// by several calls needs no atomics, and neighbouring tokens' codes are merged by a plain read-modify-write.  All of a
-// warp's loads are issued before the first is used, and codes are built in registers in the order of the record.
+// by several calls needs no atomics, and neighbouring tokens' codes are merged by a plain read-modify-write.  Loads are
+// issued together before the first is used, and codes are built in registers in the order of the record.
 #pragma once
 #include "kv_dev.cuh"
 
@@ -158,8 +158,16 @@ __device__ __forceinline__ void store_lane(uint8_t* plane0, int lane, const uint
 }
 
 // ---------------------------------------------------------------- append
+// Raw words that a lane holds of the keys, or of the values.  The block-scaled formats are bound by latency, so the values
+// are loaded when the keys are done with, and the registers that saves go to more warps (16-bit rows of 128 to mx8: 32
+// warps an SM 159 us with the read back, 24 warps 168, 16 warps with all loads first 176); the plain formats run at HBM's
+// rate with all loads first.
+__host__ __device__ constexpr int kv_raw_words(int nb, int type) { return type == kTypeF32 ? 16 * nb : 8 * nb; }
+__host__ __device__ constexpr int kv_append_blocks(int fmt, int nb, int type) {
+    return fmt < kKvMx8 ? 1 : kv_raw_words(nb, type) <= 32 ? 4 : kv_raw_words(nb, type) <= 48 ? 3 : kv_raw_words(nb, type) <= 64 ? 2 : 1;
+}
 template <int FMT, int NB, int TYPE>
-__global__ void __launch_bounds__(kKvIoWarps * 32)
+__global__ void __launch_bounds__(kKvIoWarps * 32, kv_append_blocks(FMT, NB, TYPE))
     kv_append_kernel(KvPool pool, KvSeqs seqs, KvRows key, KvRows value, int64_t tokens, int64_t units, int* status) {
     constexpr bool kMx = FMT >= kKvMx8;
     constexpr int KP = kv_key_piece(FMT), VP = kv_value_piece(FMT), NS = kv_scale_stride(NB), ES = TYPE == kTypeF32 ? 4 : 2;
@@ -222,8 +230,7 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
                 }
         }
     };
-    // (fp32 rows of 192 elements and more do not fit the registers beside the keys)
-    constexpr bool kLate = TYPE == kTypeF32 && NB >= 6;
+    constexpr bool kLate = kMx || kv_raw_words(NB, TYPE) >= 96;   // (fp32 rows of 192 elements do not fit the registers beside the keys)
     if constexpr (!kLate) load_values();
     // the values' codes that this call leaves alone
     const bool any = vmine[0] || vmine[1] || vmine[2] || vmine[3], all = vmine[0] && vmine[1] && vmine[2] && vmine[3];
