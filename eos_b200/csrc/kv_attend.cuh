@@ -17,8 +17,8 @@
 // The maxima are integers, and lag: m is set 7 below the largest score and moves only when a score passes m + 15, so most
 // records do no rescaling and no shuffles, and weights use f16's range from both ends: they stay below 2^15, and what
 // f16 cannot hold (2^-25) is 2^-31 of the row's largest weight.  A weight and its value's scale are multiplied before the
-// split: w = 2^(x + e - M) with e the largest scale exponent of the token's blocks and M a second lagging maximum, so that
-// the bound holds whatever the scales; the blocks' own exponents, relative to e, are f16 factors of the split weights
+// split: w = 2^(x - m + e - d) with e the largest scale exponent of the token's blocks and d a second lagging maximum,
+// relative to the first, so that the bound holds whatever the scales; the blocks' own exponents, relative to e, are f16 factors of the split weights
 // (four multiplications a block where scaling the codes takes eight), so the codes enter the mma as they are.
 #pragma once
 #include <algorithm>
@@ -34,7 +34,7 @@ __device__ __forceinline__ int opaque(int x) {
     return x;
 }
 
-constexpr float kKvMaxInit = -1e30f;   // below every score; finite, so that 2^(x - m) of a masked score is 0 and not NaN
+constexpr float kKvMaxInit = -1.5e38f;   // below every score; finite, so that 2^(x - m) of a masked score is 0 and not NaN
 constexpr float kKvHead = 7.f, kKvLag = 15.f;   // m = ceil(largest score) - 7; weights up to 2^15
 constexpr int kKvQueryExp = 13;                  // query rows are scaled to a largest magnitude in [2^13, 2^14)
 
@@ -91,8 +91,8 @@ struct KvWarp {
     static constexpr int KP = kv_key_piece(FMT), VP = kv_value_piece(FMT), D = 32 * NB;
 
     uint32_t q[RT][NB][4 * HALVES];   // head g of each tile, elements 32 b + 8 t .. + 7: upper halves, then lower ones
-    float qs[RT][2];                  // heads 2t and 2t + 1: factor of the raw sums, scale log2(e) 2^(query exponent)
-    float m[RT][2], big[RT][2];       // lagging maxima of x and of x + e (mx formats)
+    float2 qs[RT];                    // heads 2t and 2t + 1: factor of the raw sums, scale log2(e) 2^(query exponent)
+    float2 nm[RT], nd[RT];            // heads 2t, 2t + 1: minus the lagging maxima of x; of x + e relative to those (mx formats)
     float l[RT][2];                   // this lane's part of the sum of weights
     float o[RT][NB][2][4];            // [block][i]: elements 32 b + 4 g + 2 i (0, 1) and + 2 i + 1 (2, 3) of heads 2t, 2t + 1
 
@@ -100,7 +100,9 @@ struct KvWarp {
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) m[r][i] = big[r][i] = kKvMaxInit, l[r][i] = 0.f;
+            for (int i = 0; i < 2; ++i) l[r][i] = 0.f;
+            nm[r] = make_float2(-kKvMaxInit, -kKvMaxInit);
+            nd[r] = make_float2(0.f, 0.f);
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -172,8 +174,8 @@ struct KvWarp {
             factor *= __uint_as_float((e - kKvQueryExp) << 23);
         }
         // the factors of heads 2t and 2t + 1 are those of the lanes with g = 2t and 2t + 1
-        qs[r][0] = __shfl_sync(0xffffffffu, factor, 8 * (lane & 3));
-        qs[r][1] = __shfl_sync(0xffffffffu, factor, 8 * (lane & 3) + 4);
+        qs[r].x = __shfl_sync(0xffffffffu, factor, 8 * (lane & 3));
+        qs[r].y = __shfl_sync(0xffffffffu, factor, 8 * (lane & 3) + 4);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             float2 x[4];
@@ -188,8 +190,7 @@ struct KvWarp {
         }
     }
 
-    __device__ __forceinline__ void scale_rows(int r, float f0, float f1) {
-        const float2 f = make_float2(f0, f1);
+    __device__ __forceinline__ void scale_rows(int r, float2 f) {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -358,6 +359,22 @@ struct KvWarp {
         return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
     }
 
+    // Moves a lagging maximum (held negated) to 7 below the largest of p if that passes it by more than the lag; returns the
+    // factor for what was summed relative to the old one, applies it to l, and moves the second maximum, which is relative.
+    template <int N, typename F>
+    static __device__ __forceinline__ float raise(const float2 (&p)[N][2], float& neg, float& neg_relative, float& l, F&& head) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < N; ++n) most = fmaxf(most, fmaxf(head(p[n][0]), head(p[n][1])));
+        most = max_over_tokens(most);
+        const float to = most + neg > kKvLag ? kKvHead - ceilf(most) : neg, shift = to - neg;   // old - new
+        neg = to;
+        neg_relative -= shift;
+        const float f = ex2(shift);
+        l *= f;
+        return f;
+    }
+
     // N records; EDGE: of their 16 N tokens [lo, hi) count, else all.  Two at a time keep twice the independent work in
     // flight and share the tests for a new maximum and the work around the ring.
     template <int N, bool EDGE>
@@ -385,81 +402,65 @@ struct KvWarp {
         uint32_t whi[N][RT][2], wlo[N][RT][2];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            float x[N][4];   // exponents of the weights
+            // tokens g (0) and g + 8 (1): scores, and exponents of the weights.  A score is rounded before m is taken from it
+            // (no fma): what m was made of and what it is compared with are the same number, however large
+            float2 p[N][2], x[N][2];
             float over = -INFINITY;
 #pragma unroll
             for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[n][i] = dead[n][i >> 1] ? -INFINITY : fmaf(s[n][r][i], qs[r][i & 1], -m[r][i & 1]);
-                    over = fmaxf(over, x[n][i]);
+                for (int i = 0; i < 2; ++i) {
+                    p[n][i] = mul2(make_float2(s[n][r][2 * i], s[n][r][2 * i + 1]), qs[r]);
+                    if (dead[n][i]) p[n][i] = make_float2(-INFINITY, -INFINITY);
+                    x[n][i] = add2(p[n][i], nm[r]);
+                    over = fmaxf(over, fmaxf(x[n][i].x, x[n][i].y));
                 }
             if (__any_sync(0xffffffffu, over > kKvLag)) {
                 // from the scores: the first time, m is far below them and their differences are lost in x
-                float f[2];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float most = -INFINITY;
-#pragma unroll
-                    for (int n = 0; n < N; ++n)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            if (!dead[n][i]) most = fmaxf(most, s[n][r][2 * i + c] * qs[r][c]);
-                    most = max_over_tokens(most);
-                    const float to = most - m[r][c] > kKvLag ? ceilf(most) - kKvHead : m[r][c];
-                    f[c] = ex2(m[r][c] - to);
-                    m[r][c] = to;
-                    l[r][c] *= f[c];
-                }
-                if constexpr (!kMx) scale_rows(r, f[0], f[1]);
+                const float2 f = make_float2(raise(p, nm[r].x, nd[r].x, l[r][0], [](float2 v) { return v.x; }),
+                                             raise(p, nm[r].y, nd[r].y, l[r][1], [](float2 v) { return v.y; }));
+                if constexpr (!kMx) scale_rows(r, f);
 #pragma unroll
                 for (int n = 0; n < N; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[n][i] = dead[n][i >> 1] ? -INFINITY : fmaf(s[n][r][i], qs[r][i & 1], -m[r][i & 1]);
+                    for (int i = 0; i < 2; ++i) x[n][i] = add2(p[n][i], nm[r]);
             }
             float w[N][4];
 #pragma unroll
             for (int n = 0; n < N; ++n) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[n][i] = ex2(x[n][i]);
+                for (int i = 0; i < 2; ++i) w[n][2 * i] = ex2(x[n][i].x), w[n][2 * i + 1] = ex2(x[n][i].y);
                 l[r][0] += w[n][0] + w[n][2];
                 l[r][1] += w[n][1] + w[n][3];
             }
             if constexpr (kMx) {
-                float y[N][4], high = -INFINITY;
+                float2 y[N][2];
+                float high = -INFINITY;
 #pragma unroll
                 for (int n = 0; n < N; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        y[n][i] = dead[n][i >> 1] ? -INFINITY : fmaf(s[n][r][i], qs[r][i & 1], te[n][i >> 1] - big[r][i & 1]);
-                        high = fmaxf(high, y[n][i]);
+                    for (int i = 0; i < 2; ++i) {
+                        y[n][i] = add2(x[n][i], add2(make_float2(te[n][i], te[n][i]), nd[r]));
+                        high = fmaxf(high, fmaxf(y[n][i].x, y[n][i].y));
                     }
                 if (__any_sync(0xffffffffu, high > kKvLag)) {
-                    float f[2];
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float most = -INFINITY;
-#pragma unroll
-                        for (int n = 0; n < N; ++n)
-#pragma unroll
-                            for (int i = 0; i < 2; ++i)
-                                if (!dead[n][i]) most = fmaxf(most, fmaf(s[n][r][2 * i + c], qs[r][c], te[n][i]));
-                        most = max_over_tokens(most);
-                        const float to = most - big[r][c] > kKvLag ? ceilf(most) - kKvHead : big[r][c];
-                        f[c] = ex2(big[r][c] - to);
-                        big[r][c] = to;
-                    }
-                    scale_rows(r, f[0], f[1]);
+                    float2 sum[N][2];
 #pragma unroll
                     for (int n = 0; n < N; ++n)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            y[n][i] = dead[n][i >> 1] ? -INFINITY : fmaf(s[n][r][i], qs[r][i & 1], te[n][i >> 1] - big[r][i & 1]);
+                        for (int i = 0; i < 2; ++i) sum[n][i] = add2(x[n][i], make_float2(te[n][i], te[n][i]));
+                    float none = 0.f, nothing = 0.f;
+                    scale_rows(r, make_float2(raise(sum, nd[r].x, none, nothing, [](float2 v) { return v.x; }),
+                                              raise(sum, nd[r].y, none, nothing, [](float2 v) { return v.y; })));
+#pragma unroll
+                    for (int n = 0; n < N; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) y[n][i] = add2(x[n][i], add2(make_float2(te[n][i], te[n][i]), nd[r]));
                 }
 #pragma unroll
                 for (int n = 0; n < N; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[n][i] = ex2(y[n][i]);
+                    for (int i = 0; i < 2; ++i) w[n][2 * i] = ex2(y[n][i].x), w[n][2 * i + 1] = ex2(y[n][i].y);
             }
 #pragma unroll
             for (int n = 0; n < N; ++n)
@@ -486,7 +487,9 @@ struct KvWarp {
     __device__ __forceinline__ float4 numerators(int r, int c, int b) const {
         return make_float4(o[r][b][0][c], o[r][b][0][2 + c], o[r][b][1][c], o[r][b][1][2 + c]);
     }
-    // Partial result of this warp's rows: numerators (times 2^big), denominators (times 2^m).
+    __device__ __forceinline__ float maximum(int r, int c) const { return -(c ? nm[r].y : nm[r].x); }
+    __device__ __forceinline__ float relative(int r, int c) const { return kMx ? -(c ? nd[r].y : nd[r].x) : 0.f; }
+    // Partial result of this warp's rows: denominators (times 2^m), numerators (times 2^(m + d)); m, d, denominators last.
     __device__ __forceinline__ void store_partial(float* o_rows, float* stats, int lane) const {
         const int g = lane >> 2, t = lane & 3;
 #pragma unroll
@@ -496,8 +499,8 @@ struct KvWarp {
                 const float s = denominator(r, c);
                 const int row = 8 * r + 2 * t + c;
                 if (g == 0) {
-                    stats[3 * row] = m[r][c];
-                    stats[3 * row + 1] = kMx ? big[r][c] : m[r][c];
+                    stats[3 * row] = maximum(r, c);
+                    stats[3 * row + 1] = relative(r, c);
                     stats[3 * row + 2] = s;
                 }
 #pragma unroll
@@ -506,12 +509,12 @@ struct KvWarp {
     }
 };
 
-// The quotient of a numerator 2^big o and a denominator 2^m l.  The power of two is applied in two halves: the scales of
+// The quotient of a numerator 2^(m + d) o and a denominator 2^m l.  The power of two is applied in two halves: the scales of
 // the values span fp32's exponents, and their product with 1 / l alone could leave them.  Nothing attended to gives 0.
 struct KvQuotient {
     float inv, p, q, lse;
-    __device__ __forceinline__ KvQuotient(float l, float big, float m) {
-        const int k = (int)fminf(fmaxf(big - m, -252.f), 252.f), half = k / 2;   // an integer
+    __device__ __forceinline__ KvQuotient(float l, float d, float m) {
+        const int k = (int)fminf(fmaxf(d, -252.f), 252.f), half = k / 2;   // an integer
         inv = l == 0.f ? 0.f : __fdividef(1.f, l);   // (l stays below 2^126: 2^15 for each of fewer than 2^31 tokens)
         p = __uint_as_float((uint32_t)(half + 127) << 23);
         q = __uint_as_float((uint32_t)(k - half + 127) << 23);
@@ -547,7 +550,7 @@ struct KvShape {
     static constexpr int kMaxStages = 16;                        // of a ring
     static constexpr int kSmemMax = 232448 - 12288;              // of a CTA, less the static part
     static constexpr int kRows = 8 * RT;
-    static constexpr int kPartial = kRows * (32 * NB + 3);       // floats: numerators, then (m, big, l) of each row
+    static constexpr int kPartial = kRows * (32 * NB + 3);       // floats: numerators, then (m, d, l) of each row
     static_assert(kMaxWarps * kPartial <= kv_slot_floats(32 * NB) && kMaxWarps * kPartial * 4 <= kSmemMax && kSmemMax / 4 / kRecord >= 3 &&
                       kPartial * 4 % 32 == 0 && kRecord % 16 == 0, "rings, slots");
 };
@@ -579,7 +582,7 @@ struct KvSplit {
     int ring_bytes;                 // of a team: its records, and room for its warps' partial results
     KvDiv by_ctas, by_per_seq, by_teams, by_page, by_chunks;   // (by_page: records of a page)
     float* slots;                   // [ctas][kv_slot_floats]: partial results of the warps' first units
-    float* partial;                 // [ctas][2][rows][dim + 3]: of the CTAs, numerators of all rows, then (m, big, l) of each
+    float* partial;                 // [ctas][2][rows][dim + 3]: of the CTAs, numerators of all rows, then (m, d, l) of each
     int* count;                     // [ctas][2], [ctas]: parts of a group, groups of a unit that are done; zero between calls
 };
 
@@ -867,7 +870,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
                         const float l = w.denominator(k, c);
                         const int row = row0 + 8 * k + 2 * t + c;
                         if (row < a.group) {
-                            const KvQuotient f(l, FMT >= kKvMx8 ? w.big[k][c] : w.m[k][c], w.m[k][c]);
+                            const KvQuotient f(l, w.relative(k, c), w.maximum(k, c));
                             if (g == 0 && a.lse != nullptr) a.lse[out0 + row] = f.lse;
 #pragma unroll
                             for (int blk = 0; blk < NB; ++blk) {
@@ -1005,7 +1008,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
                 }
                 constexpr int kQuads = (D + 127) / 128;   // lane: elements 4 lane + 128 i .. + 3
                 const bool member = members >> lane & 1u;
-                float s[3] = {kKvMaxInit, kKvMaxInit, 0.f};
+                float s[3] = {kKvMaxInit, 0.f, 0.f};   // m, d, l
                 if (member) {
 #pragma unroll
                     for (int i = 0; i < 3; ++i) s[i] = load_part(from_stats + i);
@@ -1013,7 +1016,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
                 float4 o[kQuads];
 #pragma unroll
                 for (int i = 0; i < kQuads; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                float m = 0.f, big = 0.f, l = 0.f, c = 0.f;
+                float m = 0.f, d = 0.f, l = 0.f, c = 0.f;
                 const int any = __ffs(members) - 1;
                 for (uint32_t rest = members, round = 0; rest; ++round) {
                     float4 y[4][kQuads];
@@ -1030,9 +1033,10 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
                     }
                     if (round == 0) {   // (while the first rows are on their way)
                         m = warp_max(s[0]);
-                        big = warp_max(s[1]);
-                        l = warp_sum(s[2] * ex2(s[0] - m));
-                        c = member ? ex2(s[1] - big) : 0.f;
+                        const float shift = s[0] - m, e = member ? s[1] + shift : kKvMaxInit;
+                        if constexpr (FMT >= kKvMx8) d = warp_max(e);
+                        l = warp_sum(s[2] * ex2(shift));
+                        c = member ? ex2(e - d) : 0.f;
                     }
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
@@ -1049,7 +1053,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
                     const int hu = (int)u, h = (int)split.by_chunks(hu), at_row = (hu - h * split.chunks) * chunk_rows + row;
                     if (at_row >= a.group) continue;   // a row behind the key head's last query head
                     const int64_t out_row = (u >> 32) * a.q_heads + (int64_t)h * a.group + at_row;
-                    const KvQuotient f(l, big, m);
+                    const KvQuotient f(l, d, m);
 #pragma unroll
                     for (int i = 0; i < kQuads; ++i) {
                         const float y[4] = {f(o[i].x), f(o[i].y), f(o[i].z), f(o[i].w)};
@@ -1062,7 +1066,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
                         if (4 * lane + 128 * i < D) *reinterpret_cast<float4*>(to + row * D + 4 * lane + 128 * i) = o[i];
                     if (lane == 0) {
                         float* to_stats = to + chunk_rows * D + 3 * row;
-                        to_stats[0] = m, to_stats[1] = big, to_stats[2] = l;
+                        to_stats[0] = m, to_stats[1] = d, to_stats[2] = l;
                     }
                 }
             }

@@ -7,6 +7,8 @@
                                                  # the four projections of a layer, weights resident as f16
     python -m eos_b200.profile_cases scan        # TurboQuant scan, 2,000,000 x 768 4-bit codes (776 MB), 8 / 16 / 32 queries per pass
     python -m eos_b200.profile_cases score_tc    # TurboQuant tensor-core batch scoring, 1,250,000 x 768 4-bit codes (485 MB), 512 queries
+    python -m eos_b200.profile_cases kv_cache    # paged key-value cache: write, read, attend over 131,072 tokens x 8 heads x 128, e4m3
+    python -m eos_b200.profile_cases kv_cache_mx4 / kv_cache_f16   # the same in e2m1 / f16
     python -m eos_b200.profile_cases attention   # 2-layer encoder forward, 128 x 512 tokens (attention + LN kernels)
 
 Each case touches more than the 126 MB L2 but holds well under a few GB on the device.
@@ -213,10 +215,56 @@ def case_sparse_attention(batches: int = 8, q_len: int = 2048, k_len: int = 8192
     rt.close()
 
 
+def case_kv_cache(fmt: str = "mx8", tokens: int = 131072, heads: int = 8, group: int = 4, dim: int = 128, page: int = 64) -> None:
+    import torch
+
+    import eos_b200
+    rt = eos_b200.Runtime(0)
+    pages = tokens // page
+    cache = eos_b200.KvCache(rt, pages, page, heads, dim, fmt)
+    ts = torch.cuda.Stream()
+    torch.cuda.set_stream(ts)
+    stream = ts.cuda_stream
+    k = torch.randn((tokens, heads, dim), device="cuda").half()
+    v = torch.randn((tokens, heads, dim), device="cuda").half()
+    q = torch.randn((1, heads * group, dim), device="cuda").half()
+    table = torch.randperm(pages, device="cuda").to(torch.int32)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    start, cu, n = ints(0), ints(0, tokens), ints(tokens)
+    out = torch.empty_like(q)
+    rk, rv = torch.empty_like(k), torch.empty_like(v)
+    calls = {
+        "append": lambda: cache.append_device(k.data_ptr(), v.data_ptr(), "f16", tokens, 1, table.data_ptr(), pages,
+                                              start.data_ptr(), cu.data_ptr(), stream=stream),
+        "read": lambda: cache.read_device(rk.data_ptr(), rv.data_ptr(), "f16", tokens, 1, table.data_ptr(), pages,
+                                          start.data_ptr(), cu.data_ptr(), stream=stream),
+        "attend": lambda: cache.attend_device(q.data_ptr(), "f16", heads * group, 1, table.data_ptr(), pages, n.data_ptr(),
+                                              out.data_ptr(), dim ** -0.5, stream=stream),
+    }
+    stored = pages * cache.page_bytes
+    plain = 2 * tokens * heads * dim * 2
+    moved = {"append": plain + stored, "read": plain + stored, "attend": stored}
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    for name, call in calls.items():
+        for _ in range(3):
+            call()
+        e0.record(ts)
+        for _ in range(10):
+            call()
+        e1.record(ts)
+        torch.cuda.synchronize()
+        us = e0.elapsed_time(e1) * 100
+        print(f"kv {name} {fmt}: {tokens} tokens x {heads} heads x {dim}: {us:.1f} us, {moved[name] / us / 1e3:.0f} GB/s")
+    cache.sync(stream)
+    cache.close()
+    rt.close()
+
+
 if __name__ == "__main__":
     name = sys.argv[1] if len(sys.argv) > 1 else "gemm"
     {"gemm": case_gemm, "gemm_res": lambda: case_gemm(True), "scan": case_scan, "score_tc": case_score_tc, "score_tc256": lambda: case_score_tc(per_pass=256), "attention": case_attention,
      "layernorm": lambda: case_attention(512),   # the same two-layer forward at 512 sequences: rows larger than L2
+     "kv_cache": case_kv_cache, "kv_cache_mx4": lambda: case_kv_cache("mx4"), "kv_cache_f16": lambda: case_kv_cache("f16"),
      "maxsim": case_maxsim, "pack": case_pack, "sparse_attention": case_sparse_attention,
      "gemm_f16w": lambda: case_gemm(False, 1), "gemm_res_f16w": lambda: case_gemm(True, 1),
      "gemm_big": lambda: case_gemm(False, 0, 131072), "gemm_res_big": lambda: case_gemm(True, 0, 131072),

@@ -333,6 +333,34 @@ def test_blocks_of_one_token_far_apart(fmt, dim):
     s.sync()
 
 
+@pytest.mark.parametrize("fmt", ["f16", "bf16", "mx8", "mx4"])
+@pytest.mark.parametrize("size", [1e9, 1e12, 1e30])
+def test_scores_past_the_integers_of_fp32(fmt, size):
+    """Scores of 1e9 and more are further apart than their weights' range, or the same: two tokens, in different parts of
+    the work, share all of the weight, and the others have none.  Equal keys give equal scores and weights, so what is
+    left is the split of the weights (2^-22, bf16 2^-16, in numerator and denominator) and a few roundings of fp32.  The
+    score itself carries the query's split (1e9 is not a sum of two 8-bit numbers: 2^-17 for bf16) and fp32's roundings."""
+    dim, n = 64, 300
+    _, v = tensors(n, 1, dim, "f16", 5)
+    v = stored(v, fmt).half()
+    for sign in (1.0, -1.0):
+        k = torch.zeros((n, 1, dim), device="cuda", dtype=torch.float16)
+        k[:, 0, 0] = 3.0
+        k[[5, 290], 0, 0] = 6.0 if sign > 0 else 1.5   # (exact in every format)
+        s = Sequences(fmt, dim, 1, 16, [n])
+        s.append(k, v, [0], [n])
+        q = torch.zeros((1, 2, dim), device="cuda")
+        q[0, :, 0] = torch.tensor([sign * size, 0.0])
+        out, lse = s.attend(q, [n], 1.0)
+        s.sync()
+        two = v[[5, 290], 0].double()
+        tol = (2.0 ** -14 if fmt == "bf16" else 2.0 ** -20) * two.abs().mean(0) + 2.0 ** -24 * two.abs().amax()
+        assert ((out[0, 0].double() - two.mean(0)).abs() <= tol).all()
+        top = (6.0 if sign > 0 else -1.5) * size
+        assert abs(float(lse[0, 0]) - (top + np.log(2.0))) <= (2.0 ** -16 if fmt == "bf16" else 2.0 ** -21) * abs(top)
+        check_attend(q[:, 1:], [k[None], v[None]], [n], 1.0, 0, fmt, out[:, 1:], lse[:, 1:], 1)
+
+
 def test_strided_and_unaligned_tensors():
     """Views into one fused projection [tokens, (Hq + 2 Hk) dim], and tensors that start at an odd element."""
     dim, heads, group, n = 64, 2, 3, 50
