@@ -526,13 +526,16 @@ struct KvQuotient {
 // ------------------------------------------------------------------------------------------------
 // Split of the work.  Units are (sequence, key head, chunk of query heads); the records of all units, one unit after
 // the other, are cut into equal ranges, one for each CTA and within it for each warp, wherever the cuts fall: lengths may
-// differ as they like.  A warp writes what it holds of units that lie in its range altogether; at most its first and its
+// differ as they like.  (Where whole units make ranges that are hardly longer, the CTAs' cuts are between units: nothing is
+// left to join across CTAs, which takes 3 to 4 us.  96 sequences of 32 to 64 records, one unit each: 35 -> 30 us; 128 units of 7
+// to 44: 14.8 -> 11.9; 8 of 32, on 8 CTAs instead of 32: 11.2, the same.)  A warp writes what it holds of units that lie in its range altogether; at most its first and its
 // last unit are partial.  Partial results are joined in shared memory by the CTA, and what is still partial then (at most
 // two units a CTA) through the workspace by whichever of the unit's CTAs is done last.  All joins run in a fixed order:
 // same bits every time.  (A second kernel for that join cost 4 to 7 us a call.)
 // ------------------------------------------------------------------------------------------------
-constexpr int kKvGroup = 12;        // neighbouring CTAs whose parts are joined first (at most 31 groups of it, for 372 SMs)
+constexpr int kKvGroup = 24;        // neighbouring CTAs whose parts are joined first (at most 31 groups of it, for 744 SMs)
 constexpr int kKvMinRecords = 8;    // records of a CTA, at least
+constexpr int kKvWhole = 24;        // records more than an equal range that a CTA may take to keep its units whole
 
 // Shape of a CTA.  Each warp (or team of warps that share records) has a ring of records in shared memory, filled by
 // bulk copies: one copy a record, since a record is contiguous.  The partial result of a warp's last unit goes into its
@@ -716,10 +719,21 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
         total += s_warp[i];
     }
     s_before[tid] = base + upto - mine;
-    __syncthreads();
     total *= per_seq;
     const int64_t part = max(split.by_ctas(total + gridDim.x - 1), (int64_t)kKvMinRecords);
-    const int64_t c0 = min((int64_t)blockIdx.x * part, total), c1 = min(c0 + part, total);
+    // Whole units, as many for each CTA, where no range gets much longer by it
+    const int64_t units = (int64_t)seqs.batch * per_seq, whole = split.by_ctas(units + gridDim.x - 1);
+    const bool cut = __syncthreads_or(per > 1 || whole * mine > part + kKvWhole);
+    auto range_begin = [&](int64_t cta) -> int64_t {
+        if (cut) return min(cta * part, total);
+        const int64_t u = cta * whole;
+        if (u >= units) return total;
+        const int b = (int)split.by_per_seq(u);
+        int lo, hi;
+        kv_span(pool, seqs, a.window, b, lo, hi);
+        return s_before[b] * per_seq + (u - (int64_t)b * per_seq) * kv_records(lo, hi);
+    };
+    const int64_t c0 = range_begin(blockIdx.x), c1 = range_begin((int64_t)blockIdx.x + 1);
     const int64_t tpart = split.by_teams(c1 - c0 + teams - 1);
     const int64_t t0 = min(c0 + team * tpart, c1);
     int left = (int)min(min(t0 + tpart, c1) - t0, (int64_t)0x7fffffff);   // records of the team that are not yet done with
@@ -909,7 +923,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
     __syncthreads();
 
     // ---- Joins.  Phase 0: the partial results of the CTA's warps, runs of equal units among the teams' slots, in order (lane e
-    // looks at slot e % 2 of team e / 2).  What is whole then is final.  Units that several CTAs hold parts of: of every 12
+    // looks at slot e % 2 of team e / 2).  What is whole then is final.  Units that several CTAs hold parts of: of every 24
     // neighbours the one that is done last joins their parts (phase 1), and of these the last one joins the unit's groups
     // (phase 2).  What is joined, and in which order, is fixed.  One warp joins one row of a task.
     {
@@ -955,12 +969,10 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
                     const int of = phase_no == 1 ? min(kKvGroup, parts[i] - group * kKvGroup) : groups;
                     bool mine_now = false;
                     if (phase_no == 1 ? (i ? open_last : open_first) : (s_turn[i] && groups > 1)) {
-                        __threadfence();
-                        mine_now = atomicAdd(count, 1) == of - 1;
-                        if (mine_now) {
-                            *count = 0;   // for the next call
-                            __threadfence();
-                        }
+                        int done;
+                        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(done) : "l"(count) : "memory");
+                        mine_now = done == of - 1;
+                        if (mine_now) *count = 0;   // for the next call
                     }
                     s_turn[i] = mine_now;
                 }
@@ -1129,12 +1141,14 @@ struct KvAttendInstance {
     }
 };
 
-// Two tiles (16 heads) a warp where a key head serves more than 8 query heads -- the codes are converted once for both --
-// and accumulators and query leave enough of 255 registers.
-constexpr bool kv_two_tiles(int nb, int halves) { return nb * (16 + 8 * halves) <= 144; }
+// Two tiles (16 heads) a warp where a key head serves more than 8 query heads, codes are to be converted -- once for both --
+// and accumulators and query leave enough of 255 registers.  16 sequences of 8000 to 16384 tokens, 4 key heads of 192 with
+// 16 query heads each: mx8 92 us against 100 with two warps that share the records, mx4 89 against 95; f16, with nothing
+// to convert, 113 against 108 (of 128: 82 against 80).
+constexpr bool kv_two_tiles(int fmt, int nb, int halves) { return fmt >= kKvMx8 && nb * (16 + 8 * halves) <= 144; }
 template <int FMT, int NB, int HALVES>
 int kv_attend_tiles(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status, cudaStream_t stream) {
-    if constexpr (kv_two_tiles(NB, HALVES))
+    if constexpr (kv_two_tiles(FMT, NB, HALVES))
         if (a.group > 8) return KvAttendInstance<FMT, NB, 2, HALVES>::launch(pool, seqs, a, work, status, stream);
     return KvAttendInstance<FMT, NB, 1, HALVES>::launch(pool, seqs, a, work, status, stream);
 }
@@ -1147,7 +1161,7 @@ int kv_attend_rows(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, co
 }
 template <int FMT, int NB, int HALVES>
 cudaError_t kv_attend_tiles_init() {
-    if constexpr (kv_two_tiles(NB, HALVES)) {
+    if constexpr (kv_two_tiles(FMT, NB, HALVES)) {
         const cudaError_t e = KvAttendInstance<FMT, NB, 2, HALVES>::init();
         if (e != cudaSuccess) return e;
     }

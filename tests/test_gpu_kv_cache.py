@@ -454,6 +454,26 @@ def test_many_sequences_and_units():
     check_attend(q, (cut(k), cut(v)), lengths, 0.25, 0, "mx8", out, lse, 2)
 
 
+@pytest.mark.parametrize("batch,heads,lengths", [(1, 8, [300]), (37, 8, [200, 0, 193, 208]), (296, 1, [17, 1, 0, 32]),
+                                                 (10, 8, [700, 1, 40]), (96, 1, [1000, 64])])
+def test_units_left_whole_and_cut(batch, heads, lengths):
+    """Batches on both sides of the choice of where the work is cut, with windows that cut them shorter again."""
+    dim, group = 64, 3
+    lengths = [lengths[i % len(lengths)] for i in range(batch)]
+    s = Sequences("f16", dim, heads, 32, lengths)
+    k, v = tensors(sum(lengths), heads, dim, "f16", 17)
+    s.append(k, v, [0] * batch, lengths)
+    q = tensors(batch, heads * group, dim, "f16", 18)[0]
+    cut = lambda x: torch.split(stored(x, "f16"), lengths)  # noqa: E731
+    kv = cut(k), cut(v)
+    for window in (0, 90):
+        out, lse = s.attend(q, lengths, 0.1, window)
+        s.sync()
+        check_attend(q, kv, lengths, 0.1, window, "f16", out, lse, group)
+        again, lse2 = s.attend(q, lengths, 0.1, window)
+        assert same(out, again) and same(lse, lse2)
+
+
 @pytest.mark.parametrize("fmt,type_,dim,heads,group", [("f16", "f16", 128, 1, 4), ("bf16", "bf16", 256, 1, 16), ("mx8", "f32", 128, 2, 1),
                                                        ("mx4", "bf16", 64, 1, 33)])
 def test_one_long_sequence_over_all_ctas(fmt, type_, dim, heads, group):

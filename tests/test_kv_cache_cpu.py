@@ -152,6 +152,30 @@ def test_split_and_join_cover_every_record_once():
         assert whole == set(units) and sum(1 + k for k in more.values()) == len(parts)
 
 
+def test_cuts_between_units_cover_every_unit_once():
+    """The cut where units are left whole: CTA i begins with the first record of unit i * whole."""
+    rng = random.Random(8)
+    for _ in range(500):
+        batch, per_seq, ctas = rng.randrange(1, 60), rng.choice([1, 2, 5, 8]), rng.choice([1, 3, 148])
+        n = [rng.choice([0, 1, rng.randrange(0, 60)]) for _ in range(batch)]
+        before = [sum(n[:b]) for b in range(batch)]
+        total, units = sum(n) * per_seq, batch * per_seq
+        whole = -(-units // ctas)
+
+        def begin(cta):
+            u = cta * whole
+            return total if u >= units else before[u // per_seq] * per_seq + u % per_seq * n[u // per_seq]
+
+        starts, at = set(), 0
+        for b in range(batch):
+            for _ in range(per_seq):
+                starts.add(at)
+                at += n[b]
+        cuts = [begin(c) for c in range(ctas + 1)]
+        assert cuts[0] == 0 and cuts[-1] == total and cuts == sorted(cuts) and set(cuts) <= starts | {total}
+        assert all(b - a <= whole * max(n) for a, b in zip(cuts, cuts[1:]))
+
+
 def test_refusals_without_a_device():
     import eos_b200
     from eos_b200 import _lib
