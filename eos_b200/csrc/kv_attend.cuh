@@ -20,6 +20,14 @@
 // split: w = 2^(x - m + e - d) with e the largest scale exponent of the token's blocks and d a second lagging maximum,
 // relative to the first, so that the bound holds whatever the scales; the blocks' own exponents, relative to e, are f16 factors of the split weights
 // (four multiplications a block where scaling the codes takes eight), so the codes enter the mma as they are.
+//
+// What bounds it (GPU time of a call, heads of 128 unless said; floor: the records' bytes at 6540 GB/s).  f16, 32 sequences of
+// 8192 tokens, 8 key heads with 8 query heads each: 174 to 179 us, 6.0 to 6.2 TB/s, floor 164: HBM.  mx8, one sequence of
+// 131071 tokens, 8 key heads with 4 query heads each: 55 us, 5.0 TB/s, floor 42: the loop runs at HBM's rate, and the rest is
+// a call's constant part -- launch and exit 2.5 us, lengths, page ids and the first records one after the other 4 us, joins
+// 4 to 5 us, of which 3 to 4 are those across CTAs.  mx4, 16 sequences of 4000 to 32768 tokens, 8 key heads with 8 query
+// heads each: 90 us, 3.4 TB/s, floor 47: the conversion of the codes and the split of the weights, some 400 instructions
+// a warp and record, of which 170 run at half rate.  One short sequence: 7 us, launch and latencies.
 #pragma once
 #include <algorithm>
 
@@ -533,6 +541,8 @@ struct KvQuotient {
 // two units a CTA) through the workspace by whichever of the unit's CTAs is done last.  All joins run in a fixed order:
 // same bits every time.  (A second kernel for that join cost 4 to 7 us a call.)
 // ------------------------------------------------------------------------------------------------
+// (Groups of 12: one sequence of 2000 tokens and 8 heads, 16 CTAs a unit, 14.4 us instead of 12.9, of 131071 56.5 instead of
+// 55.3.  Ranges of at least 16 records: 1000 tokens 14.6 us instead of 12.2.)
 constexpr int kKvGroup = 24;        // neighbouring CTAs whose parts are joined first (at most 31 groups of it, for 744 SMs)
 constexpr int kKvMinRecords = 8;    // records of a CTA, at least
 constexpr int kKvWhole = 24;        // records more than an equal range that a CTA may take to keep its units whole
@@ -545,7 +555,10 @@ struct KvShape {
     // at most as many warps as registers allow: accumulators and query take 8 NB RT + 4 NB RT HALVES registers a thread of the
     // 65536 / (32 warps)
     static constexpr int kRegisters = 8 * NB * RT + 4 * NB * RT * HALVES;
-    // two records at a time where a record is much arithmetic for few bytes
+    // (16 instead of 12 for mx8 and heads of 128: a batch of up to 4097 tokens 68 us instead of 63; 12 instead of 16 for mx4:
+    // 96 instead of 90, whose spills of some 80 bytes cost less than the warps bring.)
+    // Two records at a time where a record is much arithmetic for few bytes: mx8, 131071 tokens, 56.5 us instead of 61.3 one
+    // at a time, mx4 89.6 instead of 96.8; 16-bit formats lose by it, heads of 64 under fp32 queries 38.4 instead of 32.8.
     static constexpr bool kPair = FMT >= kKvMx8 && NB * RT <= 4;
     static constexpr int kMaxWarps = kRegisters <= (FMT == kKvMx4 ? 48 : 32) ? 16 : kRegisters <= 80 ? 12 : 8;
     static constexpr int kMaxThreads = 32 * kMaxWarps;
@@ -598,7 +611,6 @@ __device__ __forceinline__ bool kv_span(const KvPool& pool, const KvSeqs& s, int
     return n >= 0 && n <= room;
 }
 __device__ __forceinline__ int kv_records(int lo, int hi) { return hi > lo ? (hi + kKvRecord - 1) / kKvRecord - lo / kKvRecord : 0; }
-
 
 
 // A walk over the records of a range, in order: the unit (b, hu) and the record r of its n.

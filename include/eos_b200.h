@@ -581,7 +581,8 @@ typedef struct {
  * position p is token p % page_size of page d_page_table[b * max_pages + p / page_size].  d_cu_tokens is [batch + 1],
  * ascending, its last entry at most `tokens`; NULL: one token per sequence (tokens == batch).  Rows behind the last
  * sequence are not read.  Nothing else of a page changes.  The positions written by one call must be distinct (no page
- * twice among the pages written); tokens of other positions may be read by other calls meanwhile.
+ * twice among the pages written), and calls that run at the same time must write different pages (16 tokens share words);
+ * other positions may be read by other calls meanwhile.
  * Enqueued on `stream` (NULL: the runtime's stream) without synchronising, allocation-free, and may be captured into a
  * graph; all arrays are device memory and are read when the kernel runs.  Sequences whose entries are out of range
  * (negative, behind the page table, a page id outside the cache) are skipped as far as they are, and
@@ -606,7 +607,8 @@ EOS_B200_API int eos_b200_kv_cache_read_device(EosB200KvCache* cache, void* d_ke
  * batch is at most 65535.  Positions on a page that is out of range are left out and eos_b200_kv_cache_sync reports it; a length that is negative
  * or longer than the page table is cut, and reported too.  Rows that meet an infinity or a NaN are not finite; other rows are not touched by it.
  * Enqueued, allocation-free and capturable as above; calls of one cache share its workspace and must be ordered (one
- * stream, or events between streams). */
+ * stream, or events between streams; replays of graphs that hold them likewise): overlapping ones give wrong results, and may
+ * go on giving them.  Two caches are independent. */
 EOS_B200_API int eos_b200_kv_cache_attend_device(EosB200KvCache* cache, const void* d_query, int type, int q_heads,
                                                  int64_t query_seq_stride, int64_t query_head_stride, int batch,
                                                  const int32_t* d_page_table, int max_pages, const int32_t* d_lengths, float scale,
