@@ -104,6 +104,7 @@ def check_attend(q, kv, lengths, scale, window, fmt, out, lse, group):
         d = S (2 split + (dim + 8) u),  split = 2^-22 (f16 operands: 11 + 11 bits) or 2^-16 (bf16: 8 + 8),
     a weight by the factor 2 d + 2^-20 (exp2, and its argument's rounding), and n weighted values add n u and the
     weights' split; the result is rounded once more to its type.  Numerator and denominator each carry this once.
+    Weights of bf16 results are one f16 number (unless the cache is bf16), in the numerator alone: half a step, 2^-11.
     Below f16's normal numbers a split factor is off by 2^-25 absolutely instead.  Query rows are scaled to a largest
     magnitude of at least 2^13, so that is 2^-38 of it.  Weights, times their value's scale s_j, are scaled to a largest of
     at least 2^6, so that is 2^-31 max(p s): 2^-31 sum_j |v_j| for f16 (s = 1); for the block-scaled formats s_j is at most
@@ -128,6 +129,8 @@ def check_attend(q, kv, lengths, scale, window, fmt, out, lse, group):
             d += abs(scale) * 2.0 ** -38 * float(qq.abs().max()) * float(kh.abs().sum(-1).max())
             err = 2 * (2 * d + 2.0 ** -20) + (n - lo + 16) * u + 2 * split
             tol = err * (p @ vh.abs()) + half * want.abs() + 1e-30
+            if out.dtype == torch.bfloat16 and fmt != "bf16":
+                tol += 2.0 ** -11 * (p @ vh.abs())
             if fmt == "f16":
                 tol += 2.0 ** -31 * vh.abs().sum(0)
             elif fmt != "bf16":
