@@ -12,8 +12,8 @@
 // issued together before the first is used, and codes are built in registers in the order of the record.
 //
 // What bounds them (131072 tokens of 8 heads of 128, 16-bit rows): the 16-bit formats HBM -- append and read 163 us each, 6.6
-// TB/s.  mx8 append 137 us, 5.9 TB/s: a warp's two rounds of loads with the quantisation between them; read 131 us, 6.2 TB/s.
-// mx4 append 131 us, 5.2 TB/s, read 111 us, 6.1 TB/s.  (DRAM moves the rows and the records once: 537 + 249 MB and 279 + 484 MB
+// TB/s.  mx8 append 131 us, 6.2 TB/s: a warp's two rounds of loads with the quantisation between them (137 when the page was
+// looked up before the first); read 131 us, 6.2 TB/s.  mx4 append 124 us, 5.5 TB/s, read 111 us, 6.1 TB/s.  (DRAM moves the rows and the records once: 537 + 249 MB and 279 + 484 MB
 // at mx8, what an append leaves in the L2 of its 278 MB aside.)  One token for each of 64 sequences, the read back included:
 // 11 us, two launches and the latency of starts, page table, rows and the record's old bytes one after the other.
 #pragma once
@@ -36,8 +36,10 @@ __device__ __forceinline__ KvUnit kv_unit(const KvSeqs& s, int64_t tokens, int64
     KvUnit r;
     r.ok = false;
     int64_t row, n, first = 0;
+    int64_t start;   // (asked for together with the row offsets)
     if (s.cu == nullptr) {
         r.b = (int)u, row = u, n = 1;
+        start = __ldg(s.starts + r.b);
     } else {
         int lo = 0, hi = s.batch;
         while (hi - lo > 1) {
@@ -50,11 +52,11 @@ __device__ __forceinline__ KvUnit kv_unit(const KvSeqs& s, int64_t tokens, int64
         }
         r.b = lo;
         row = __ldg(s.cu + lo);
+        start = __ldg(s.starts + lo);
         n = (int64_t)__ldg(s.cu + lo + 1) - row;
         first = u - ((int64_t)(row >> 4) + 2 * (int64_t)lo);
     }
     if (n == 0) return r;
-    const int64_t start = __ldg(s.starts + r.b);
     if (n < 0 || row < 0 || row + n > tokens || start < 0 || start + n > 0x7fffffffLL) {
         if (lane == 0) atomicExch(status, kStatusBadSequence);
         return r;
@@ -166,7 +168,8 @@ __device__ __forceinline__ void store_lane(uint8_t* plane0, int lane, const uint
 // ---------------------------------------------------------------- append
 // Raw words that a lane holds of the keys, or of the values.  The block-scaled formats are bound by latency, so the values
 // are loaded when the keys are done with, and the registers that saves go to more warps (16-bit rows of 128 to mx8: 32
-// warps an SM 159 us with the read back, 24 warps 168, 16 warps with all loads first 176); the plain formats run at HBM's
+// warps an SM 159 us with the read back (155 now), 24 warps 168, 16 warps with all loads first 176; fetching the values' rows into
+// the L2 meanwhile brings nothing); the plain formats run at HBM's
 // rate with all loads first.
 __host__ __device__ constexpr int kv_raw_words(int nb, int type) { return type == kTypeF32 ? 16 * nb : 8 * nb; }
 __host__ __device__ constexpr int kv_append_blocks(int fmt, int nb, int type) {
@@ -184,11 +187,6 @@ __global__ void __launch_bounds__(kKvIoWarps * 32, kv_append_blocks(FMT, NB, TYP
     const int h = (int)(w - u * pool.heads);
     const KvUnit un = kv_unit(seqs, tokens, u, lane, status);
     if (!un.ok) return;
-    uint8_t* rec = kv_record(pool, seqs, un.b, un.rec, h);
-    if (rec == nullptr) {
-        if (lane == 0) atomicExch(status, kStatusBadPage);
-        return;
-    }
     const int base = un.rec * kKvRecord;
     const bool full = un.hi - un.lo == kKvRecord && key.vec && value.vec;   // the usual record of a prompt: no conditions on the loads
     // ---- keys: lane (g, t) owns 8 elements of the tokens g and g + 8 in every block
@@ -209,6 +207,12 @@ __global__ void __launch_bounds__(kKvIoWarps * 32, kv_append_blocks(FMT, NB, TYP
                 if (kmine[j]) kx[j][b].load(p + 32 * b * ES, key.vec);
             }
         }
+    }
+    // the rows are on their way while the page is looked up
+    uint8_t* rec = kv_record(pool, seqs, un.b, un.rec, h);
+    if (rec == nullptr) {
+        if (lane == 0) atomicExch(status, kStatusBadPage);
+        return;
     }
     // ---- values: lane (g, t) owns elements 4 g .. + 3 of every block for the tokens 2t, 2t+1, 2t+8, 2t+9
     bool vmine[4];
