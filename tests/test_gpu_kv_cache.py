@@ -654,3 +654,93 @@ def test_shared_pages():
     second = stored(torch.cat([k[:32], k[32:] * 2]), "mx4")
     check_attend(q, ([stored(k, "mx4"), second], [stored(v, "mx4")] * 2), [64, 60], 0.2, 0, "mx4", out, lse, 2)
     s.sync()
+
+
+@pytest.mark.parametrize("fmt", ["f16", "mx4"])
+def test_offsets_past_32_bits(fmt):
+    """A cache of 5 GiB whose last pages are used, and rows and queries 2^28 and 2^30 elements apart."""
+    import eos_b200
+    dim, heads, page, n = 128, 2, 64, 17
+    rt = eos_b200.Runtime(0)
+    probe = eos_b200.KvCache(rt, 1, page, heads, dim, fmt)
+    pages = (5 << 30) // probe.page_bytes
+    probe.close()
+    cache = eos_b200.KvCache(rt, pages, page, heads, dim, fmt)
+    far = torch.zeros((1 << 32) + (1 << 16), dtype=torch.float16, device="cuda")
+    step = 1 << 28
+    key = torch.as_strided(far, (n, heads, dim), (step - 8, dim, 1), 0)
+    value = torch.as_strided(far, (n, heads, dim), (step - 8, dim, 1), heads * dim)
+    k, v = tensors(n, heads, dim, "f16", 31)
+    key.copy_(k)
+    value.copy_(v)
+    table = torch.tensor([[pages - 1], [pages - 3], [1], [pages - 2]], dtype=torch.int32, device="cuda")
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    cu, starts, lengths = ints(0, 5, 5, 11, 17), ints(0, 0, 0, 0), ints(5, 0, 6, 6)
+    st = torch.cuda.current_stream().cuda_stream
+    strides = (step - 8, dim, step - 8, dim)
+    cache.append_device(key.data_ptr(), value.data_ptr(), "f16", n, 4, table.data_ptr(), 1, starts.data_ptr(), cu.data_ptr(),
+                        strides, st)
+    far.zero_()
+    cache.read_device(key.data_ptr(), value.data_ptr(), "f16", n, 4, table.data_ptr(), 1, starts.data_ptr(), cu.data_ptr(),
+                      strides, st)
+    sk, sv = stored(k, fmt), stored(v, fmt)
+    assert same(key, sk.half()) and same(value, sv.half())
+    far.zero_()
+    q0 = tensors(4, heads * 3, dim, "f16", 32)[0]
+    q = torch.as_strided(far, q0.shape, ((1 << 30) + 8, dim, 1), 0)
+    q.copy_(q0)
+    out, lse = torch.empty_like(q0), torch.empty(q0.shape[:2], device="cuda")
+    cache.attend_device(q.data_ptr(), "f16", heads * 3, 4, table.data_ptr(), 1, lengths.data_ptr(), out.data_ptr(), 0.1, 0,
+                        lse.data_ptr(), ((1 << 30) + 8, dim), st)
+    cache.sync(st)
+    cut = lambda x: torch.split(x, [5, 0, 6, 6])  # noqa: E731
+    check_attend(q0, (cut(sk), cut(sv)), [5, 0, 6, 6], 0.1, 0, fmt, out, lse, 3)
+    cache.close()
+
+
+def test_two_caches_at_once():
+    """Attends, appends and reads of two caches, eager and replayed, on two streams that nothing orders."""
+    import eos_b200
+    rt = eos_b200.Runtime(0)
+    dim, heads, lengths = 64, 2, [5000, 700, 33]
+    made = []
+    for i in range(2):
+        s = Sequences("mx8", dim, heads, 32, [x + 1 for x in lengths], seed=i, runtime=rt)
+        k, v = tensors(sum(lengths), heads, dim, "f16", 40 + i)
+        s.append(k, v, [0, 0, 0], lengths)
+        q = tensors(3, heads * 4, dim, "bf16", 50 + i)[0]
+        want, lse = s.attend(q, lengths, 0.125)
+        made.append((s, k, v, q, want, lse, torch.cuda.Stream(), s._ints(lengths), s._ints([0, 0, 0]), s._ints(np.cumsum([0] + lengths))))
+    results = []
+    graphs = []
+
+    def step(m, out, lse, rk, rv):
+        s, k, v, q, _, _, stream, n, zero, cu = m
+        at = torch.cuda.current_stream().cuda_stream
+        s.cache.append_device(k.data_ptr(), v.data_ptr(), "f16", k.shape[0], 3, s.table.data_ptr(), s.max_pages, zero.data_ptr(),
+                              cu.data_ptr(), stream=at)
+        s.cache.attend_device(q.data_ptr(), "bf16", heads * 4, 3, s.table.data_ptr(), s.max_pages, n.data_ptr(), out.data_ptr(),
+                              0.125, 0, lse.data_ptr(), stream=at)
+        s.cache.read_device(rk.data_ptr(), rv.data_ptr(), "f16", k.shape[0], 3, s.table.data_ptr(), s.max_pages, zero.data_ptr(),
+                            cu.data_ptr(), stream=at)
+
+    for m in made:
+        outs = [(torch.zeros_like(m[4]), torch.zeros_like(m[5]), torch.zeros_like(m[1]), torch.zeros_like(m[2])) for _ in range(2)]
+        results.append(outs)
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=m[6]):
+            step(m, *outs[1])
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for m, outs, g in zip(made, results, graphs):
+            with torch.cuda.stream(m[6]):
+                step(m, *outs[0])
+                g.replay()
+    torch.cuda.synchronize()
+    for m, outs in zip(made, results):
+        for out, lse, rk, rv in outs:
+            assert same(out, m[4]) and same(lse, m[5])
+            assert same(rk, stored(m[1], "mx8").half()) and same(rv, stored(m[2], "mx8").half())
+        m[0].sync()
