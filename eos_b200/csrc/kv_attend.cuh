@@ -539,10 +539,10 @@ struct KvQuotient {
 // the other, are cut into equal ranges, one for each CTA and within it for each warp, wherever the cuts fall: lengths may
 // differ as they like.  (Where whole units make ranges that are hardly longer, the CTAs' cuts are between units: nothing is
 // left to join across CTAs, which takes 3 to 4 us.  96 sequences of 32 to 64 records, one unit each: 35 -> 30 us; 128 units of 7
-// to 44: 14.8 -> 11.9; 8 of 32, on 8 CTAs instead of 32: 11.2, the same.)  A warp writes what it holds of units that lie in its range altogether; at most its first and its
-// last unit are partial.  Partial results are joined in shared memory by the CTA, and what is still partial then (at most
-// two units a CTA) through the workspace by whichever of the unit's CTAs is done last.  All joins run in a fixed order:
-// same bits every time.  (A second kernel for that join cost 4 to 7 us a call.)
+// to 44: 14.8 -> 11.9; 8 of 32, on 8 CTAs instead of 32: 11.2, the same.)  A warp writes what it holds of units that lie in
+// its range altogether; at most its first and its last unit are partial.  Partial results are joined in shared memory by the
+// CTA, and what is still partial then (at most two units a CTA) through the workspace by whichever of the unit's CTAs is done
+// last.  All joins run in a fixed order: same bits every time.  (A second kernel for that join cost 4 to 7 us a call.)
 // ------------------------------------------------------------------------------------------------
 // (Groups of 12: one sequence of 2000 tokens and 8 heads, 16 CTAs a unit, 14.4 us instead of 12.9, of 131071 56.5 instead of
 // 55.3.  Ranges of at least 16 records: 1000 tokens 14.6 us instead of 12.2.)
@@ -561,7 +561,8 @@ struct KvShape {
     // (16 instead of 12 for mx8 and heads of 128: a batch of up to 4097 tokens 68 us instead of 63; 12 instead of 16 for mx4:
     // 96 instead of 90, whose spills of some 80 bytes cost less than the warps bring.)
     // Two records at a time where a record is much arithmetic for few bytes: mx8, 131071 tokens, 56.5 us instead of 61.3 one
-    // at a time, mx4 89.6 instead of 96.8 (weights in two operands); 16-bit formats lose by it, heads of 64 under fp32 queries 38.4 instead of 32.8.
+    // at a time, mx4 89.6 instead of 96.8 (weights in two operands); 16-bit formats lose by it, heads of 64 under fp32 queries
+    // 38.4 instead of 32.8.
     static constexpr bool kPair = FMT >= kKvMx8 && NB * RT <= 4;
     static constexpr int kMaxWarps = kRegisters <= (FMT == kKvMx4 ? 48 : 32) ? 16 : kRegisters <= 80 ? 12 : 8;
     static constexpr int kMaxThreads = 32 * kMaxWarps;

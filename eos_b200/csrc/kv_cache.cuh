@@ -107,7 +107,8 @@ struct KvWork {
     int* count;             // [3 ctas], zero between calls
 };
 constexpr int kKvMaxRows = 128;        // query heads of one unit, at most
-__host__ __device__ constexpr int kv_slot_floats(int dim) { return kKvMaxRows * (dim + 3) + (dim <= 96 ? 128 * (dim + 3) : 0); }   // 128 or (small heads, 16 warps) 256 rows
+// 128 rows, or (small heads, 16 warps) 256
+__host__ __device__ constexpr int kv_slot_floats(int dim) { return kKvMaxRows * (dim + 3) + (dim <= 96 ? 128 * (dim + 3) : 0); }
 
 // cudaSuccess once the kernels of this format and dim are ready on the current device
 cudaError_t kv_init(int format, int blocks);

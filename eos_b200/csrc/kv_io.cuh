@@ -13,9 +13,10 @@
 //
 // What bounds them (131072 tokens of 8 heads of 128, 16-bit rows): the 16-bit formats HBM -- append and read 163 us each, 6.6
 // TB/s.  mx8 append 131 us, 6.2 TB/s: a warp's two rounds of loads with the quantisation between them (137 when the page was
-// looked up before the first); read 131 us, 6.2 TB/s.  mx4 append 124 us, 5.5 TB/s, read 111 us, 6.1 TB/s.  (DRAM moves the rows and the records once: 537 + 249 MB and 279 + 484 MB
-// at mx8, what an append leaves in the L2 of its 278 MB aside.)  One token for each of 64 sequences, the read back included:
-// 11 us, two launches and the latency of starts, page table, rows and the record's old bytes one after the other.
+// looked up before the first); read 131 us, 6.2 TB/s.  mx4 append 124 us, 5.5 TB/s, read 111 us, 6.1
+// TB/s.  (DRAM moves the rows and the records once: 537 + 249 MB and 279 + 484 MB at mx8, what an append leaves in the L2 of
+// its 279 MB aside.)  One token for each of 64 sequences, the read back included: 10 to 11 us, two launches and the latency of
+// starts, rows and page table, and the record's old bytes one after the other.
 #pragma once
 #include "kv_dev.cuh"
 

@@ -601,11 +601,12 @@ EOS_B200_API int eos_b200_kv_cache_read_device(EosB200KvCache* cache, void* d_ke
 /* Attention of one new token per sequence: query [batch, q_heads, head_dim] of `type`, query head i reads key head
  * i / (q_heads / kv_heads).  Sequence b attends to positions [max(0, n - window), n), n = d_lengths[b] (window 0: all
  * of them):  out = sum_j softmax_j(scale q . k_j) v_j, sums in fp32, rounded to `type` into d_out [batch, q_heads, head_dim]
- * (contiguous, 16-byte aligned, apart from the query); d_lse (nullable) [batch, q_heads] fp32 receives ln sum_j exp(scale q . k_j).  A sequence with n = 0 gives zeros
- * and -infinity.  query_seq_stride / query_head_stride in elements, 0: contiguous.  The new token's own key and value
+ * (contiguous, 16-byte aligned, apart from the query); d_lse (nullable) [batch, q_heads] fp32 receives
+ * ln sum_j exp(scale q . k_j).  A sequence with n = 0 gives zeros and -infinity.  query_seq_stride / query_head_stride in elements, 0: contiguous.  The new token's own key and value
  * are appended before the call when it attends to itself.
- * batch is at most 65535.  Positions on a page that is out of range are left out and eos_b200_kv_cache_sync reports it; a length that is negative
- * or longer than the page table is cut, and reported too.  Rows that meet an infinity or a NaN are not finite; other rows are not touched by it.
+ * batch is at most 65535.  Positions on a page that is out of range are left out and eos_b200_kv_cache_sync reports it; a
+ * length that is negative or longer than the page table is cut, and reported too.  Rows that meet an infinity or a NaN are
+ * not finite; other rows are not touched by it.
  * Enqueued, allocation-free and capturable as above; calls of one cache share its workspace and must be ordered (one
  * stream, or events between streams; replays of graphs that hold them likewise): overlapping ones give wrong results, and may
  * go on giving them.  Two caches are independent. */
