@@ -12,9 +12,8 @@
 //
 // Every fp32 factor -- the weights, and a query that does not fit the operand type (fp32, or f16 over a bf16 cache) -- is
 // the sum of two 16-bit operands, so the products carry 22 bits (bf16: 16).  The cached value is never split: it is exact
-// in its operand type.  Where the result is rounded to bf16 (half a step: 2^-8 of it) the weights are one f16 operand (2^-11 of
-// each, of either sign) unless the operand type is bf16; their sum stays fp32, of the weights before that rounding.  The error
-// against 64 bits of a batch over mx4 is the same to two digits, 1.7e-3, and its time 82 us instead of 89.5.
+// in its operand type.  (Weights in one f16 operand where the result is bf16 saved 7 us of 90 over mx4 and 1 of 64 over mx8, and
+// moved one result in twenty to a neighbouring bf16 number: results are the rounding of one in 32 bits, whatever their type.)
 //
 // The maxima are integers, and lag: m is set 7 below the largest score and moves only when a score passes m + 15, so most
 // records do no rescaling and no shuffles, and weights use f16's range from both ends: they stay below 2^15, and what
@@ -28,8 +27,8 @@
 // 131071 tokens, 8 key heads with 4 query heads each: 55 us, 5.0 TB/s, floor 42: the loop runs at HBM's rate, and the rest is
 // a call's constant part -- launch and exit 2.5 us, lengths, page ids and the first records one after the other 4 us, joins
 // 4 to 5 us, of which 3 to 4 are those across CTAs.  mx4, 16 sequences of 4000 to 32768 tokens, 8 key heads with 8 query
-// heads each, bf16 queries: 82 us, 3.7 TB/s, floor 47: the conversion of the codes and the weights, some 400 instructions a
-// warp and record where the weights are two operands, of which 170 run at half rate.  One short sequence: 7 us, launch and latencies.
+// heads each: 90 us, 3.4 TB/s, floor 47: the conversion of the codes and the split of the weights, some 400 instructions
+// a warp and record, of which 170 run at half rate.  One short sequence: 7 us, launch and latencies.
 #pragma once
 #include <algorithm>
 
@@ -94,8 +93,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
 // byte i of a word as a float 2^(byte - 127); 255 becomes infinity, which times the zero codes of such a block is NaN
 __device__ __forceinline__ float scale_at(uint32_t word, int i) { return __uint_as_float(__byte_perm(word, 0, 0x4440 | i) << 23); }
 
-// RT: tiles of 8 query heads; HALVES: operands of the query (1: its type fits the operand type); PARTS: operands of the weights.
-template <int FMT, int NB, int RT, int HALVES, int PARTS>
+// RT: tiles of 8 query heads; HALVES: operands of the query (1: its type fits the operand type).
+template <int FMT, int NB, int RT, int HALVES>
 struct KvWarp {
     static constexpr bool kMx = FMT >= kKvMx8, kBf = FMT == kKvBf16;
     static constexpr int KP = kv_key_piece(FMT), VP = kv_value_piece(FMT), D = 32 * NB;
@@ -352,13 +351,12 @@ struct KvWarp {
                 uint32_t h0 = whi[r][0], h1 = whi[r][1], l0 = wlo[r][0], l1 = wlo[r][1];
                 if constexpr (kMx) {
                     h0 = mul_f16x2(h0, rel[0][b]), h1 = mul_f16x2(h1, rel[1][b]);
-                    if constexpr (PARTS == 2) l0 = mul_f16x2(l0, rel[0][b]), l1 = mul_f16x2(l1, rel[1][b]);
+                    l0 = mul_f16x2(l0, rel[0][b]), l1 = mul_f16x2(l1, rel[1][b]);
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) mma_16x8x16<kBf>(o[r][b][i], f[2 * i][0], f[2 * i + 1][0], f[2 * i][1], f[2 * i + 1][1], h0, h1);
-                if constexpr (PARTS == 2)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) mma_16x8x16<kBf>(o[r][b][i], f[2 * i][0], f[2 * i + 1][0], f[2 * i][1], f[2 * i + 1][1], l0, l1);
+                for (int i = 0; i < 2; ++i) mma_16x8x16<kBf>(o[r][b][i], f[2 * i][0], f[2 * i + 1][0], f[2 * i][1], f[2 * i + 1][1], l0, l1);
             }
         }
     }
@@ -480,7 +478,7 @@ struct KvWarp {
                     uint32_t hi16, lo16;
                     split_pair<kBf>(w[n][2 * i], w[n][2 * i + 1], hi16, lo16);
                     whi[n][r][i] = transpose8x8(hi16);
-                    wlo[n][r][i] = PARTS == 2 ? transpose8x8(lo16) : 0u;
+                    wlo[n][r][i] = transpose8x8(lo16);
                 }
         }
 #pragma unroll
@@ -553,7 +551,7 @@ constexpr int kKvWhole = 24;        // records more than an equal range that a C
 // Shape of a CTA.  Each warp (or team of warps that share records) has a ring of records in shared memory, filled by
 // bulk copies: one copy a record, since a record is contiguous.  The partial result of a warp's last unit goes into its
 // ring, which is empty by then; that of its first one, if it is another, to the workspace.
-template <int FMT, int NB, int RT, int HALVES, int PARTS>
+template <int FMT, int NB, int RT, int HALVES>
 struct KvShape {
     // at most as many warps as registers allow: accumulators and query take 8 NB RT + 4 NB RT HALVES registers a thread of the
     // 65536 / (32 warps)
@@ -561,8 +559,7 @@ struct KvShape {
     // (16 instead of 12 for mx8 and heads of 128: a batch of up to 4097 tokens 68 us instead of 63; 12 instead of 16 for mx4:
     // 96 instead of 90, whose spills of some 80 bytes cost less than the warps bring.)
     // Two records at a time where a record is much arithmetic for few bytes: mx8, 131071 tokens, 56.5 us instead of 61.3 one
-    // at a time, mx4 89.6 instead of 96.8 (weights in two operands); 16-bit formats lose by it, heads of 64 under fp32 queries
-    // 38.4 instead of 32.8.
+    // at a time, mx4 89.6 instead of 96.8; 16-bit formats lose by it, heads of 64 under fp32 queries 38.4 instead of 32.8.
     static constexpr bool kPair = FMT >= kKvMx8 && NB * RT <= 4;
     static constexpr int kMaxWarps = kRegisters <= (FMT == kKvMx4 ? 48 : 32) ? 16 : kRegisters <= 80 ? 12 : 8;
     static constexpr int kMaxThreads = 32 * kMaxWarps;
@@ -673,10 +670,10 @@ __device__ __forceinline__ float load_part(const float* p) {
     return v;
 }
 
-template <int FMT, int NB, int RT, int HALVES, int PARTS>
-__global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES, PARTS>::kMaxThreads, 1)
+template <int FMT, int NB, int RT, int HALVES>
+__global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
     kv_attend_kernel(KvPool pool, KvSeqs seqs, KvAttend a, KvSplit split, int* status) {
-    using Shape = KvShape<FMT, NB, RT, HALVES, PARTS>;
+    using Shape = KvShape<FMT, NB, RT, HALVES>;
     constexpr int D = 32 * NB, kRows = Shape::kRows, kMaxWarps = Shape::kMaxWarps, kMaxStages = Shape::kMaxStages;
     extern __shared__ __align__(128) uint8_t smem[];          // rings
     __shared__ int64_t s_before[32 * kMaxWarps];                  // records of the sequences before thread i's
@@ -801,7 +798,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES, PARTS>::kMaxThrea
         uint64_t policy;
         asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
 
-        KvWarp<FMT, NB, RT, HALVES, PARTS> w;
+        KvWarp<FMT, NB, RT, HALVES> w;
         int stage = 0, fill = 0, empty = rw == 0 ? stages : 0;   // stage to read next; stage to fill next, stages to fill
         uint32_t phase = 0, fill_phase = 1;
         bool alive = true;   // no wait has run out
@@ -1117,11 +1114,11 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES, PARTS>::kMaxThrea
     }
 }
 
-template <int FMT, int NB, int RT, int HALVES, int PARTS>
+template <int FMT, int NB, int RT, int HALVES>
 struct KvAttendInstance {
-    using Shape = KvShape<FMT, NB, RT, HALVES, PARTS>;
+    using Shape = KvShape<FMT, NB, RT, HALVES>;
     static cudaError_t init() {
-        return cudaFuncSetAttribute(kv_attend_kernel<FMT, NB, RT, HALVES, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmemMax);
+        return cudaFuncSetAttribute(kv_attend_kernel<FMT, NB, RT, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmemMax);
     }
     static int launch(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
                       cudaStream_t stream) {
@@ -1152,7 +1149,7 @@ struct KvAttendInstance {
         split.count = work.count;
         split.slots = work.slots;
         split.partial = work.partial;
-        kv_attend_kernel<FMT, NB, RT, HALVES, PARTS><<<work.ctas, 32 * warps, split.teams * split.ring_bytes, stream>>>(pool, seqs, a, split, status);
+        kv_attend_kernel<FMT, NB, RT, HALVES><<<work.ctas, 32 * warps, split.teams * split.ring_bytes, stream>>>(pool, seqs, a, split, status);
         return 1;
     }
 };
@@ -1161,36 +1158,32 @@ struct KvAttendInstance {
 // and accumulators and query leave enough of 255 registers.  16 sequences of 8000 to 16384 tokens, 4 key heads of 192 with
 // 16 query heads each: mx8 92 us against 100 with two warps that share the records, mx4 89 against 95; f16, with nothing
 // to convert, 113 against 108 (of 128: 82 against 80).
-constexpr int kv_bf16_parts(int fmt) { return fmt == kKvBf16 ? 2 : 1; }
 constexpr bool kv_two_tiles(int fmt, int nb, int halves) { return fmt >= kKvMx8 && nb * (16 + 8 * halves) <= 144; }
-template <int FMT, int NB, int HALVES, int PARTS>
+template <int FMT, int NB, int HALVES>
 int kv_attend_tiles(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status, cudaStream_t stream) {
     if constexpr (kv_two_tiles(FMT, NB, HALVES))
-        if (a.group > 8) return KvAttendInstance<FMT, NB, 2, HALVES, PARTS>::launch(pool, seqs, a, work, status, stream);
-    return KvAttendInstance<FMT, NB, 1, HALVES, PARTS>::launch(pool, seqs, a, work, status, stream);
+        if (a.group > 8) return KvAttendInstance<FMT, NB, 2, HALVES>::launch(pool, seqs, a, work, status, stream);
+    return KvAttendInstance<FMT, NB, 1, HALVES>::launch(pool, seqs, a, work, status, stream);
 }
-// The query is one operand where its type fits it exactly; the weights are where 11 bits are more than the result keeps.
+// The query is one operand where its type fits it exactly.
 template <int FMT, int NB>
 int kv_attend_rows(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status, cudaStream_t stream) {
-    if (a.type == kTypeBf16) return kv_attend_tiles<FMT, NB, 1, kv_bf16_parts(FMT)>(pool, seqs, a, work, status, stream);
-    if constexpr (FMT != kKvBf16)
-        if (a.type == kTypeF16) return kv_attend_tiles<FMT, NB, 1, 2>(pool, seqs, a, work, status, stream);
-    return kv_attend_tiles<FMT, NB, 2, 2>(pool, seqs, a, work, status, stream);
+    return a.type == kTypeBf16 || (a.type == kTypeF16 && FMT != kKvBf16)
+               ? kv_attend_tiles<FMT, NB, 1>(pool, seqs, a, work, status, stream)
+               : kv_attend_tiles<FMT, NB, 2>(pool, seqs, a, work, status, stream);
 }
-template <int FMT, int NB, int HALVES, int PARTS>
+template <int FMT, int NB, int HALVES>
 cudaError_t kv_attend_tiles_init() {
     if constexpr (kv_two_tiles(FMT, NB, HALVES)) {
-        const cudaError_t e = KvAttendInstance<FMT, NB, 2, HALVES, PARTS>::init();
+        const cudaError_t e = KvAttendInstance<FMT, NB, 2, HALVES>::init();
         if (e != cudaSuccess) return e;
     }
-    return KvAttendInstance<FMT, NB, 1, HALVES, PARTS>::init();
+    return KvAttendInstance<FMT, NB, 1, HALVES>::init();
 }
 template <int FMT, int NB>
 cudaError_t kv_attend_rows_init() {
-    cudaError_t e = kv_attend_tiles_init<FMT, NB, 1, kv_bf16_parts(FMT)>();
-    if constexpr (FMT != kKvBf16)
-        if (e == cudaSuccess) e = kv_attend_tiles_init<FMT, NB, 1, 2>();
-    return e == cudaSuccess ? kv_attend_tiles_init<FMT, NB, 2, 2>() : e;
+    const cudaError_t e = kv_attend_tiles_init<FMT, NB, 1>();
+    return e == cudaSuccess ? kv_attend_tiles_init<FMT, NB, 2>() : e;
 }
 
 template <int FMT>

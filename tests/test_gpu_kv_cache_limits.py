@@ -1,0 +1,51 @@
+"""Paged key-value cache on the device, at the limits of what its calls allow: the bits that results carry, the range of
+scores and lengths, errors and workspaces of caches that live side by side."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from tests.test_gpu_kv_cache import DTYPES, Sequences, stored, tensors  # noqa: E402
+
+
+def formula(q, k, v, scale, group):
+    """out, lse in 64 bits of one sequence, p @ |v| and the largest |score| of every row: q [heads * group, dim];
+    k, v [n, heads, dim]."""
+    q, k, v = (x.double().cpu() for x in (q, k, v))
+    rows = []
+    for h in range(q.shape[0]):
+        kh, vh = k[:, h // group], v[:, h // group]
+        x = scale * (kh @ q[h])
+        p = torch.softmax(x, 0)
+        rows.append((p @ vh, torch.logsumexp(x, 0), p @ vh.abs(), x.abs().max()))
+    return [torch.stack([r[i] for r in rows]) for i in range(4)]
+
+
+def whole(shape, type_, seed):
+    """Whole numbers from -2 to 2, exact in every type and format: their products' sums are exact too."""
+    return torch.randint(-2, 3, shape, generator=torch.Generator().manual_seed(seed)).to(DTYPES[type_]).cuda()
+
+
+@pytest.mark.parametrize("fmt,dim,group,n", [("f16", 64, 2, 16), ("f16", 128, 9, 5), ("mx8", 128, 4, 16), ("mx8", 96, 12, 33),
+                                             ("mx4", 128, 8, 16), ("mx4", 256, 3, 5)])
+def test_bf16_results_are_the_rounding_of_a_result_in_32_bits(fmt, dim, group, n):
+    """The weights of bf16 results carry the 22 bits that all others do.  The dot products here are exact, so a score is off
+    by the roundings of its scale, of its product with it and of its distance from the maximum, 2^-22 |x| with room, a
+    weight by twice that and 2^-20 (exp2), n additions by u = 2^-23 each and the weights' split by 2^-22, in numerator and
+    denominator.  The split's floor, 2^-25 below f16's normal numbers, is 2^-31 sum |v| (f16) or n 2^-29 max|v|
+    (block scales).  What is left is the one rounding to bf16."""
+    heads, scale, u = 2, 2.0 ** -4, 2.0 ** -23
+    s = Sequences(fmt, dim, heads, 32, [n])
+    k, v = whole((n, heads, dim), "bf16", 61), tensors(n, heads, dim, "bf16", 62)[1]
+    s.append(k, v, [0], [n])
+    q = whole((1, heads * group, dim), "bf16", 63)
+    out, _ = s.attend(q, [n], scale)
+    s.sync()
+    sv = stored(v, fmt)
+    want, _, size, top = formula(q[0], k, sv, scale, group)
+    tol = (2 * (2 * 2.0 ** -22 * top + 2.0 ** -20) + (n + 16) * u + 2 * 2.0 ** -22)[:, None] * size
+    tol += 2.0 ** -31 * n * sv.abs().max().item() * (1 if fmt == "f16" else 4)
+    got = out[0].double().cpu()
+    low, high = ((want - tol).float().bfloat16().double(), (want + tol).float().bfloat16().double())
+    assert ((got >= low) & (got <= high)).all(), float(((got < low) | (got > high)).double().mean())
