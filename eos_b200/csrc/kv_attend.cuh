@@ -11,8 +11,9 @@
 // written back there first, and the weights once more through it; the kernel is bound by HBM and by the conversions.)
 //
 // Every fp32 factor -- the weights, and a query that does not fit the operand type (fp32, or f16 over a bf16 cache) -- is
-// the sum of two 16-bit operands, so the products carry 22 bits (bf16: 16).  The cached value is never split: it is exact
-// in its operand type.  (Weights in one f16 operand where the result is bf16 saved 7 us of 90 over mx4 and 1 of 64 over mx8, and
+// the sum of two 16-bit operands, so the products carry 22 bits.  Over a bf16 cache, whose operands hold 8, it is the sum of
+// three for fp32 queries and results, 24 bits, and of two, 16, for 16-bit ones, which keep 11 at most (an f16 query is exact in
+// two; its lse stays that of 32 bits, for it is taken before the split).  The cached value is never split: it is exact in its operand type.  (Weights in one f16 operand where the result is bf16 saved 7 us of 90 over mx4 and 1 of 64 over mx8, and
 // moved one result in twenty to a neighbouring bf16 number: results are the rounding of one in 32 bits, whatever their type.)
 //
 // The maxima are integers, and lag: m is set 7 below the largest score and moves only when a score passes m + 15, so most
@@ -69,17 +70,14 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// a pair of fp32 values as the sum of two 16-bit pairs
-template <bool kBf>
-__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
-    if constexpr (kBf) {
-        hi = bf16x2_of(a, b);
-        const float2 f = bf16x2_floats(hi);
-        lo = bf16x2_of(a - f.x, b - f.y);
-    } else {
-        hi = f16x2_of(a, b);
-        const float2 f = f16x2_floats(hi);
-        lo = f16x2_of(a - f.x, b - f.y);
+// a pair of fp32 values as the sum of PARTS 16-bit pairs, the largest first
+template <bool kBf, int PARTS>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&part)[PARTS]) {
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+        part[i] = kBf ? bf16x2_of(a, b) : f16x2_of(a, b);
+        const float2 f = kBf ? bf16x2_floats(part[i]) : f16x2_floats(part[i]);
+        a -= f.x, b -= f.y;
     }
 }
 
@@ -93,13 +91,16 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
 // byte i of a word as a float 2^(byte - 127); 255 becomes infinity, which times the zero codes of such a block is NaN
 __device__ __forceinline__ float scale_at(uint32_t word, int i) { return __uint_as_float(__byte_perm(word, 0, 0x4440 | i) << 23); }
 
-// RT: tiles of 8 query heads; HALVES: operands of the query (1: its type fits the operand type).
+// RT: tiles of 8 query heads; HALVES: operands of the query (1: its type fits the operand type; 3: f32 over a bf16 cache).
 template <int FMT, int NB, int RT, int HALVES>
 struct KvWarp {
     static constexpr bool kMx = FMT >= kKvMx8, kBf = FMT == kKvBf16;
     static constexpr int KP = kv_key_piece(FMT), VP = kv_value_piece(FMT), D = 32 * NB;
+    static constexpr int kParts = HALVES == 3 ? 3 : 2;           // operands of the weights
+    static constexpr bool kWide = HALVES == (kBf ? 3 : 2);       // the query is fp32
+    using Weights = uint32_t[RT][kParts][2];
 
-    uint32_t q[RT][NB][4 * HALVES];   // head g of each tile, elements 32 b + 8 t .. + 7: upper halves, then lower ones
+    uint32_t q[RT][NB][4 * HALVES];   // head g of each tile, elements 32 b + 8 t .. + 7: the largest parts, then the next
     float2 qs[RT];                    // heads 2t and 2t + 1: factor of the raw sums, scale log2(e) 2^(query exponent)
     float2 nm[RT], nd[RT];            // heads 2t, 2t + 1: minus the lagging maxima of x; of x + e relative to those (mx formats)
     float l[RT][2];                   // this lane's part of the sum of weights
@@ -123,19 +124,18 @@ struct KvWarp {
     // at once and waited for in convert_query, ...
     __device__ __forceinline__ void load_query(const KvAttend& a, int64_t at, int row0, int rows, int lane) {
         const int g = lane >> 2, t = lane & 3;
-        const bool wide = HALVES == 2 && opaque(a.type) == kTypeF32;   // two 16-byte loads a block, else one
         const int vec = opaque(a.vec);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             const int row = row0 + 8 * r + g;
-            const uint8_t* base = static_cast<const uint8_t*>(a.query) + (at + (int64_t)row * a.head_stride + 8 * t) * (wide ? 4 : 2);
+            const uint8_t* base = static_cast<const uint8_t*>(a.query) + (at + (int64_t)row * a.head_stride + 8 * t) * (kWide ? 4 : 2);
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int i = 0; i < 4 * HALVES; i += 4) {
+                for (int i = 0; i < (kWide ? 8 : 4); i += 4) {   // two 16-byte loads a block, or one
                     uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                    const uint8_t* from = base + b * (wide ? 128 : 64) + 4 * i;
-                    if (row < rows && (i == 0 || wide)) {
+                    const uint8_t* from = base + b * (kWide ? 128 : 64) + 4 * i;
+                    if (row < rows) {
                         if (vec) x = *reinterpret_cast<const uint4*>(from);
                         else x = load16_unaligned(from);
                     }
@@ -144,23 +144,19 @@ struct KvWarp {
         }
     }
     // ... then the operands.  f16: each row is divided by a power of two first, so that no magnitude leaves f16's range.
-    // One operand: the type is f16 or bf16 (over a bf16 cache bf16); two: f32 (or f16).
+    // One operand: the type is f16 or bf16 (over a bf16 cache bf16); more: f32 (over a bf16 cache two: f16).
     __device__ __forceinline__ void convert_query(const KvAttend& a, int lane) {
-        const int type = opaque(a.type);
-        const bool f16 = type == kTypeF16, wide = type == kTypeF32;
+        const bool f16 = opaque(a.type) == kTypeF16;
 #pragma unroll
         for (int r = 0; r < RT; ++r)
             split_row(a, r, lane, [&](int b, int i) {
-                if constexpr (HALVES == 1) {
+                if constexpr (!kWide) {
                     const uint32_t w = q[r][b][i];
-                    if constexpr (kBf) return bf16x2_floats(w);
+                    if constexpr (kBf) return HALVES == 1 ? bf16x2_floats(w) : f16x2_floats(w);
                     const float2 x = f16x2_floats(w), y = bf16x2_floats(w);
                     return make_float2(f16 ? x.x : y.x, f16 ? x.y : y.y);
                 } else {
-                    const float2 y = make_float2(__uint_as_float(q[r][b][2 * i]), __uint_as_float(q[r][b][2 * i + 1]));
-                    if constexpr (!kBf) return y;
-                    const float2 x = f16x2_floats(q[r][b][i]);
-                    return make_float2(wide ? y.x : x.x, wide ? y.y : x.y);
+                    return make_float2(__uint_as_float(q[r][b][2 * i]), __uint_as_float(q[r][b][2 * i + 1]));
                 }
             });
     }
@@ -192,9 +188,10 @@ struct KvWarp {
             for (int i = 0; i < 4; ++i) x[i] = pair(b, i);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                uint32_t lo;
-                split_pair<kBf>(x[i].x * inv, x[i].y * inv, q[r][b][i], lo);
-                if constexpr (HALVES == 2) q[r][b][4 + i] = lo;
+                uint32_t part[HALVES];
+                split_pair<kBf>(x[i].x * inv, x[i].y * inv, part);
+#pragma unroll
+                for (int u = 0; u < HALVES; ++u) q[r][b][4 * u + i] = part[u];
             }
         }
     }
@@ -322,8 +319,8 @@ struct KvWarp {
 
     // Adds a record's values; weights as pairs of the tokens 2t, 2t + 1 (0) and 2t + 8, 2t + 9 (1) of head g.
     template <bool EDGE>
-    __device__ __forceinline__ void values(const uint8_t* rec, int lo, int hi, const uint32_t (&whi)[RT][2],
-                                           const uint32_t (&wlo)[RT][2], const uint32_t (&rel)[2][NB], int lane) {
+    __device__ __forceinline__ void values(const uint8_t* rec, int lo, int hi, const Weights& weights, const uint32_t (&rel)[2][NB],
+                                           int lane) {
         uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
         if constexpr (!kMx && EDGE) keep[0] = live_pair(lane & 3, 0, lo, hi), keep[1] = live_pair(lane & 3, 1, lo, hi);
         uint32_t v[NB * VP / 4];
@@ -348,15 +345,16 @@ struct KvWarp {
             }
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                uint32_t h0 = whi[r][0], h1 = whi[r][1], l0 = wlo[r][0], l1 = wlo[r][1];
-                if constexpr (kMx) {
-                    h0 = mul_f16x2(h0, rel[0][b]), h1 = mul_f16x2(h1, rel[1][b]);
-                    l0 = mul_f16x2(l0, rel[0][b]), l1 = mul_f16x2(l1, rel[1][b]);
-                }
+                uint32_t w[kParts][2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) mma_16x8x16<kBf>(o[r][b][i], f[2 * i][0], f[2 * i + 1][0], f[2 * i][1], f[2 * i + 1][1], h0, h1);
+                for (int u = 0; u < kParts; ++u)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) mma_16x8x16<kBf>(o[r][b][i], f[2 * i][0], f[2 * i + 1][0], f[2 * i][1], f[2 * i + 1][1], l0, l1);
+                    for (int p = 0; p < 2; ++p) w[u][p] = kMx ? mul_f16x2(weights[r][u][p], rel[p][b]) : weights[r][u][p];
+#pragma unroll
+                for (int u = 0; u < kParts; ++u)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        mma_16x8x16<kBf>(o[r][b][i], f[2 * i][0], f[2 * i + 1][0], f[2 * i][1], f[2 * i + 1][1], w[u][0], w[u][1]);
             }
         }
     }
@@ -408,7 +406,7 @@ struct KvWarp {
             if constexpr (kMx) value_scales<EDGE>(rec[n], lo - n * kKvRecord, hi - n * kKvRecord, rel[n], lane);
         }
         // softmax
-        uint32_t whi[N][RT][2], wlo[N][RT][2];
+        Weights weights[N];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             // tokens g (0) and g + 8 (1): scores, and exponents of the weights.  A score is rounded before m is taken from it
@@ -475,14 +473,14 @@ struct KvWarp {
             for (int n = 0; n < N; ++n)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    uint32_t hi16, lo16;
-                    split_pair<kBf>(w[n][2 * i], w[n][2 * i + 1], hi16, lo16);
-                    whi[n][r][i] = transpose8x8(hi16);
-                    wlo[n][r][i] = transpose8x8(lo16);
+                    uint32_t part[kParts];
+                    split_pair<kBf>(w[n][2 * i], w[n][2 * i + 1], part);
+#pragma unroll
+                    for (int u = 0; u < kParts; ++u) weights[n][r][u][i] = transpose8x8(part[u]);
                 }
         }
 #pragma unroll
-        for (int n = 0; n < N; ++n) values<EDGE>(rec[n], lo - n * kKvRecord, hi - n * kKvRecord, whi[n], wlo[n], rel[n], lane);
+        for (int n = 0; n < N; ++n) values<EDGE>(rec[n], lo - n * kKvRecord, hi - n * kKvRecord, weights[n], rel[n], lane);
     }
 
     // the sum of weights of head 2t + c of tile r
@@ -1168,9 +1166,11 @@ int kv_attend_tiles(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, c
 // The query is one operand where its type fits it exactly.
 template <int FMT, int NB>
 int kv_attend_rows(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status, cudaStream_t stream) {
-    return a.type == kTypeBf16 || (a.type == kTypeF16 && FMT != kKvBf16)
-               ? kv_attend_tiles<FMT, NB, 1>(pool, seqs, a, work, status, stream)
-               : kv_attend_tiles<FMT, NB, 2>(pool, seqs, a, work, status, stream);
+    if (a.type == kTypeBf16 || (a.type == kTypeF16 && FMT != kKvBf16))
+        return kv_attend_tiles<FMT, NB, 1>(pool, seqs, a, work, status, stream);
+    if constexpr (FMT == kKvBf16)
+        if (a.type == kTypeF32) return kv_attend_tiles<FMT, NB, 3>(pool, seqs, a, work, status, stream);
+    return kv_attend_tiles<FMT, NB, 2>(pool, seqs, a, work, status, stream);
 }
 template <int FMT, int NB, int HALVES>
 cudaError_t kv_attend_tiles_init() {
@@ -1182,8 +1182,11 @@ cudaError_t kv_attend_tiles_init() {
 }
 template <int FMT, int NB>
 cudaError_t kv_attend_rows_init() {
-    const cudaError_t e = kv_attend_tiles_init<FMT, NB, 1>();
-    return e == cudaSuccess ? kv_attend_tiles_init<FMT, NB, 2>() : e;
+    cudaError_t e = kv_attend_tiles_init<FMT, NB, 1>();
+    if (e == cudaSuccess) e = kv_attend_tiles_init<FMT, NB, 2>();
+    if constexpr (FMT == kKvBf16)
+        if (e == cudaSuccess) e = kv_attend_tiles_init<FMT, NB, 3>();
+    return e;
 }
 
 template <int FMT>

@@ -49,3 +49,43 @@ def test_bf16_results_are_the_rounding_of_a_result_in_32_bits(fmt, dim, group, n
     got = out[0].double().cpu()
     low, high = ((want - tol).float().bfloat16().double(), (want + tol).float().bfloat16().double())
     assert ((got >= low) & (got <= high)).all(), float(((got < low) | (got > high)).double().mean())
+
+
+@pytest.mark.parametrize("fmt", ["f16", "bf16", "mx8", "mx4"])
+@pytest.mark.parametrize("dim,group", [(64, 5), (128, 16), (256, 3)])
+def test_queries_in_32_bits_keep_them(fmt, dim, group):
+    """Keys with one element that is not zero: a score is one product, of a number of 24 bits and 1.  It is off by the
+    query's split (f16: 11 + 11 bits, 2^-22 with room; bf16: three times 8, less), the sum of the parts (2 u, u = 2^-23) and the roundings of the scale,
+    its product and the distance to the maximum: 2^-22 + 4 u = 2^-20.7 of |x|, here below 2^-20.  lse carries it once and
+    exp2's 2^-22, out twice (weight and sum), with 2^-22 from the weights' split, the sums' 32 u and the split's floor, n 2^-29 max|v|."""
+    heads, n, scale, u = 1, 16, 8.0, 2.0 ** -23
+    s = Sequences(fmt, dim, heads, 16, [n])
+    k = torch.zeros((n, heads, dim), device="cuda")
+    k[torch.arange(n), 0, torch.arange(n) * (dim // n) + 1] = 1.0
+    v = tensors(n, heads, dim, "f32", 71)[1]
+    s.append(k, v, [0], [n])
+    q = torch.randn((1, heads * group, dim), generator=torch.Generator().manual_seed(72)).cuda()
+    out, lse = s.attend(q, [n], scale)
+    s.sync()
+    sv = stored(v, fmt)
+    want, wanted, size, top = formula(q[0], k, sv, scale, group)
+    d = 2.0 ** -20 * top
+    assert ((lse[0].double().cpu() - wanted).abs() <= d + 2.0 ** -21 + 2.0 ** -22 * wanted.abs()).all()
+    tol = (4 * d + 4 * 2.0 ** -22 + 32 * u)[:, None] * size + n * 2.0 ** -29 * sv.abs().max().item()
+    assert ((out[0].double().cpu() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", ["f16", "bf16", "mx8", "mx4"])
+def test_a_single_token_gives_its_value(fmt):
+    """Whatever its score, the weight is divided by itself: what is left is its split (f16 2^-24, bf16 in three parts less),
+    the sum of the parts (3 u, u = 2^-23), the approximate quotient (2 u), two products (u), and for block scales one more
+    rounding of exp2's argument (ln 2 2^-21, 3 u)."""
+    dim, rows = 64, 64
+    s = Sequences(fmt, dim, 1, 16, [1])
+    k, v = tensors(1, 1, dim, "f32", 73)
+    s.append(k, v, [0], [1])
+    q = torch.randn((1, rows, dim), generator=torch.Generator().manual_seed(74)).cuda()
+    out, _ = s.attend(q, [1], 0.3)
+    s.sync()
+    sv = stored(v, fmt)[0, 0]
+    assert ((out[0].double() - sv).abs() <= 12 * 2.0 ** -23 * sv.abs()).all()
