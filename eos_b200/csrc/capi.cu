@@ -104,12 +104,7 @@ __global__ void bounded_wait_probe_kernel(long long limit_cycles, int* status) {
     if (threadIdx.x == 0 && (!ok || abort_flag != 0)) atomicExch(status, kStatusPipelineTimeout);
 }
 
-int read_status(EosB200Runtime* rt, cudaStream_t s, char** err) {
-    int st = 0;
-    CUDA_TRY(cudaMemcpyAsync(&st, rt->d_status, sizeof(int), cudaMemcpyDeviceToHost, s));
-    CUDA_TRY(cudaStreamSynchronize(s));
-    if (st == kStatusOk) return EOS_B200_OK;
-    cudaMemsetAsync(rt->d_status, 0, sizeof(int), s);  // reported once
+std::string status_text(int st) {
     const char* what = "unknown device status";
     if (st == kStatusBadTokenId) what = "input_ids value out of range [0, vocab)";
     else if (st == kStatusBadTypeId) what = "token_type_ids value out of range";
@@ -117,7 +112,16 @@ int read_status(EosB200Runtime* rt, cudaStream_t s, char** err) {
     else if (st == kStatusBadPage) what = "page id outside the cache, or a position behind the sequence's page table";
     else if (st == kStatusBadSequence) what = "length, start or row offset of a sequence out of range";
     else if (st == kStatusPipelineTimeout) what = "a bounded wait inside a kernel ran out (pipeline timeout)";
-    return fail(err, std::string("device status ") + std::to_string(st) + ": " + what, EOS_B200_DEVICE_STATUS);
+    return std::string("device status ") + std::to_string(st) + ": " + what;
+}
+
+int read_status(EosB200Runtime* rt, cudaStream_t s, char** err) {
+    int st = 0;
+    CUDA_TRY(cudaMemcpyAsync(&st, rt->d_status, sizeof(int), cudaMemcpyDeviceToHost, s));
+    CUDA_TRY(cudaStreamSynchronize(s));
+    if (st == kStatusOk) return EOS_B200_OK;
+    cudaMemsetAsync(rt->d_status, 0, sizeof(int), s);  // reported once
+    return fail(err, status_text(st), EOS_B200_DEVICE_STATUS);
 }
 }  // namespace
 
@@ -3708,7 +3712,10 @@ struct EosB200KvCache {
     EosB200Runtime* rt = nullptr;
     KvPool pool{};
     KvWork work{};
+    std::mutex lock;            // of `reported`
+    int reported[kKvErrors] = {};
 };
+static_assert(kStatusBadPage == kStatusPipelineTimeout + 1 && kStatusBadSequence == kStatusPipelineTimeout + 2, "KvWork::errors");
 
 namespace {
 
@@ -3779,13 +3786,14 @@ int eos_b200_kv_cache_create(EosB200Runtime* rt, int64_t pages, int page_size, i
     c->rt = rt;
     // one allocation: the pages, then the workspace (its counts first), each part 256-byte aligned
     const auto part = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
-    const size_t ctas = (size_t)rt->sm_count, pool_bytes = part((size_t)(pages * page_bytes)), count_bytes = part(3 * ctas * sizeof(int)),
+    const size_t ctas = (size_t)rt->sm_count, pool_bytes = part((size_t)(pages * page_bytes)), count_bytes = part((3 * ctas + kKvErrors) * sizeof(int)),
                  slot_bytes = part(ctas * kv_slot_floats(head_dim) * sizeof(float));
     cudaError_t e = dev_alloc(&p.base, pool_bytes + count_bytes + slot_bytes + ctas * 2 * kKvMaxRows * (head_dim + 3) * sizeof(float));
     c->pool = p;
     c->work.ctas = rt->sm_count;
     if (e == cudaSuccess) {
         c->work.count = reinterpret_cast<int*>(p.base + pool_bytes);
+        c->work.errors = c->work.count + 3 * ctas;
         c->work.slots = reinterpret_cast<float*>(p.base + pool_bytes + count_bytes);
         c->work.partial = reinterpret_cast<float*>(p.base + pool_bytes + count_bytes + slot_bytes);
         e = cudaMemsetAsync(p.base, 0, pool_bytes + count_bytes, rt->stream);
@@ -3824,7 +3832,7 @@ int eos_b200_kv_cache_append_device(EosB200KvCache* c, const void* d_key, const 
     if (stats != nullptr) std::memset(stats, 0, sizeof(*stats));
     if (tokens == 0 || batch == 0) return EOS_B200_OK;
     CUDA_TRY(cudaSetDevice(c->rt->device));
-    launch_kv_append(c->pool, seqs, k, v, type, tokens, c->rt->d_status, pick_stream(c->rt, stream));
+    launch_kv_append(c->pool, seqs, k, v, type, tokens, c->work.errors, pick_stream(c->rt, stream));
     CUDA_TRY(cudaGetLastError());
     if (stats != nullptr) stats->kernel_launches = 1;
     return EOS_B200_OK;
@@ -3843,7 +3851,7 @@ int eos_b200_kv_cache_read_device(EosB200KvCache* c, void* d_key, void* d_value,
     if (stats != nullptr) std::memset(stats, 0, sizeof(*stats));
     if (tokens == 0 || batch == 0) return EOS_B200_OK;
     CUDA_TRY(cudaSetDevice(c->rt->device));
-    launch_kv_read(c->pool, seqs, k, v, type, tokens, c->rt->d_status, pick_stream(c->rt, stream));
+    launch_kv_read(c->pool, seqs, k, v, type, tokens, c->work.errors, pick_stream(c->rt, stream));
     CUDA_TRY(cudaGetLastError());
     if (stats != nullptr) stats->kernel_launches = 1;
     return EOS_B200_OK;
@@ -3884,7 +3892,7 @@ int eos_b200_kv_cache_attend_device(EosB200KvCache* c, const void* d_query, int 
     a.scale_log2 = (float)((double)scale * 1.4426950408889634);
     a.window = window;
     CUDA_TRY(cudaSetDevice(c->rt->device));
-    const int launches = launch_kv_attend(c->pool, seqs, a, c->work, c->rt->d_status, pick_stream(c->rt, stream));
+    const int launches = launch_kv_attend(c->pool, seqs, a, c->work, c->work.errors, pick_stream(c->rt, stream));
     CUDA_TRY(cudaGetLastError());
     if (stats != nullptr) stats->kernel_launches = launches;
     return EOS_B200_OK;
@@ -3893,7 +3901,21 @@ int eos_b200_kv_cache_attend_device(EosB200KvCache* c, const void* d_query, int 
 int eos_b200_kv_cache_sync(EosB200KvCache* c, void* stream, char** err) {
     if (c == nullptr) return fail(err, "kv_cache_sync: null cache");
     CUDA_TRY(cudaSetDevice(c->rt->device));
-    return read_status(c->rt, pick_stream(c->rt, stream), err);
+    const cudaStream_t s = pick_stream(c->rt, stream);
+    int met[kKvErrors];
+    CUDA_TRY(cudaMemcpyAsync(met, c->work.errors, sizeof(met), cudaMemcpyDeviceToHost, s));
+    CUDA_TRY(cudaStreamSynchronize(s));
+    std::string what;
+    {
+        std::lock_guard<std::mutex> guard(c->lock);
+        for (int i = 0; i < kKvErrors; ++i) {
+            // (another thread's sync may have seen later counts: the difference is then not above 0)
+            if ((int)((unsigned)met[i] - (unsigned)c->reported[i]) <= 0) continue;
+            c->reported[i] = met[i];
+            what += (what.empty() ? "" : "; ") + status_text(kStatusPipelineTimeout + i);
+        }
+    }
+    return what.empty() ? EOS_B200_OK : fail(err, what, EOS_B200_DEVICE_STATUS);
 }
 
 }  // extern "C"

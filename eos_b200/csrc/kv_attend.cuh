@@ -670,7 +670,7 @@ __device__ __forceinline__ float load_part(const float* p) {
 
 template <int FMT, int NB, int RT, int HALVES>
 __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
-    kv_attend_kernel(KvPool pool, KvSeqs seqs, KvAttend a, KvSplit split, int* status) {
+    kv_attend_kernel(KvPool pool, KvSeqs seqs, KvAttend a, KvSplit split, int* errors) {
     using Shape = KvShape<FMT, NB, RT, HALVES>;
     constexpr int D = 32 * NB, kRows = Shape::kRows, kMaxWarps = Shape::kMaxWarps, kMaxStages = Shape::kMaxStages;
     extern __shared__ __align__(128) uint8_t smem[];          // rings
@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
 #pragma unroll 1
     for (int b = tid * per; b < min((tid + 1) * per, seqs.batch); ++b) {
         int lo, hi;
-        if (!kv_span(pool, seqs, a.window, b, lo, hi) && blockIdx.x == 0) atomicExch(status, kStatusBadSequence);
+        if (!kv_span(pool, seqs, a.window, b, lo, hi) && blockIdx.x == 0) kv_report(errors, kStatusBadSequence);
         mine += kv_records(lo, hi);
     }
     int64_t upto = mine;
@@ -748,7 +748,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
     const int64_t tpart = split.by_teams(c1 - c0 + teams - 1);
     const int64_t t0 = min(c0 + team * tpart, c1);
     int left = (int)min(min(t0 + tpart, c1) - t0, (int64_t)0x7fffffff);   // records of the team that are not yet done with
-    if (tpart > 0x7fffffff && tid == 0) atomicExch(status, kStatusBadSequence);   // (2^31 records a warp: lengths gone wrong)
+    if (tpart > 0x7fffffff && tid == 0) kv_report(errors, kStatusBadSequence);   // (2^31 records a warp: lengths gone wrong)
 
     if (left > 0) {
         KvWalk at;
@@ -830,7 +830,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
                             if (src != nullptr) {
                                 kv_copy_record(ring_at + st * Shape::kRecord, src + lane * Shape::kRecord, Shape::kRecord, full_at + 8 * st, policy);
                             } else {
-                                atomicExch(status, kStatusBadPage);
+                                kv_report(errors, kStatusBadPage);
                                 mbar_arrive(full_at + 8 * st);
                             }
                         }
@@ -923,7 +923,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
             at.next_unit(pool, seqs, a.window, per_seq);
         }
         if (!alive && lane == 0) {
-            atomicExch(status, kStatusPipelineTimeout);
+            kv_report(errors, kStatusPipelineTimeout);
             // the copies still under way must land before the CTA leaves: the last fill of every stage
             for (int i = 0; rw == 0 && i < stages; ++i) {
                 s_drain[warp] = 0;
@@ -1118,7 +1118,7 @@ struct KvAttendInstance {
     static cudaError_t init() {
         return cudaFuncSetAttribute(kv_attend_kernel<FMT, NB, RT, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmemMax);
     }
-    static int launch(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
+    static int launch(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors,
                       cudaStream_t stream) {
         KvSplit split{};
         // warps for the rows of a key head: as many as it takes to cover them, a power of two, at most 8 (64 or 128 rows)
@@ -1147,7 +1147,7 @@ struct KvAttendInstance {
         split.count = work.count;
         split.slots = work.slots;
         split.partial = work.partial;
-        kv_attend_kernel<FMT, NB, RT, HALVES><<<work.ctas, 32 * warps, split.teams * split.ring_bytes, stream>>>(pool, seqs, a, split, status);
+        kv_attend_kernel<FMT, NB, RT, HALVES><<<work.ctas, 32 * warps, split.teams * split.ring_bytes, stream>>>(pool, seqs, a, split, errors);
         return 1;
     }
 };
@@ -1158,19 +1158,19 @@ struct KvAttendInstance {
 // to convert, 113 against 108 (of 128: 82 against 80).
 constexpr bool kv_two_tiles(int fmt, int nb, int halves) { return fmt >= kKvMx8 && nb * (16 + 8 * halves) <= 144; }
 template <int FMT, int NB, int HALVES>
-int kv_attend_tiles(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status, cudaStream_t stream) {
+int kv_attend_tiles(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors, cudaStream_t stream) {
     if constexpr (kv_two_tiles(FMT, NB, HALVES))
-        if (a.group > 8) return KvAttendInstance<FMT, NB, 2, HALVES>::launch(pool, seqs, a, work, status, stream);
-    return KvAttendInstance<FMT, NB, 1, HALVES>::launch(pool, seqs, a, work, status, stream);
+        if (a.group > 8) return KvAttendInstance<FMT, NB, 2, HALVES>::launch(pool, seqs, a, work, errors, stream);
+    return KvAttendInstance<FMT, NB, 1, HALVES>::launch(pool, seqs, a, work, errors, stream);
 }
 // The query is one operand where its type fits it exactly.
 template <int FMT, int NB>
-int kv_attend_rows(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status, cudaStream_t stream) {
+int kv_attend_rows(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors, cudaStream_t stream) {
     if (a.type == kTypeBf16 || (a.type == kTypeF16 && FMT != kKvBf16))
-        return kv_attend_tiles<FMT, NB, 1>(pool, seqs, a, work, status, stream);
+        return kv_attend_tiles<FMT, NB, 1>(pool, seqs, a, work, errors, stream);
     if constexpr (FMT == kKvBf16)
-        if (a.type == kTypeF32) return kv_attend_tiles<FMT, NB, 3>(pool, seqs, a, work, status, stream);
-    return kv_attend_tiles<FMT, NB, 2>(pool, seqs, a, work, status, stream);
+        if (a.type == kTypeF32) return kv_attend_tiles<FMT, NB, 3>(pool, seqs, a, work, errors, stream);
+    return kv_attend_tiles<FMT, NB, 2>(pool, seqs, a, work, errors, stream);
 }
 template <int FMT, int NB, int HALVES>
 cudaError_t kv_attend_tiles_init() {
@@ -1190,14 +1190,14 @@ cudaError_t kv_attend_rows_init() {
 }
 
 template <int FMT>
-int kv_attend_format(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status, cudaStream_t stream) {
+int kv_attend_format(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors, cudaStream_t stream) {
     switch (pool.blocks) {
-        case 1: return kv_attend_rows<FMT, 1>(pool, seqs, a, work, status, stream);
-        case 2: return kv_attend_rows<FMT, 2>(pool, seqs, a, work, status, stream);
-        case 3: return kv_attend_rows<FMT, 3>(pool, seqs, a, work, status, stream);
-        case 4: return kv_attend_rows<FMT, 4>(pool, seqs, a, work, status, stream);
-        case 6: return kv_attend_rows<FMT, 6>(pool, seqs, a, work, status, stream);
-        default: return kv_attend_rows<FMT, 8>(pool, seqs, a, work, status, stream);
+        case 1: return kv_attend_rows<FMT, 1>(pool, seqs, a, work, errors, stream);
+        case 2: return kv_attend_rows<FMT, 2>(pool, seqs, a, work, errors, stream);
+        case 3: return kv_attend_rows<FMT, 3>(pool, seqs, a, work, errors, stream);
+        case 4: return kv_attend_rows<FMT, 4>(pool, seqs, a, work, errors, stream);
+        case 6: return kv_attend_rows<FMT, 6>(pool, seqs, a, work, errors, stream);
+        default: return kv_attend_rows<FMT, 8>(pool, seqs, a, work, errors, stream);
     }
 }
 template <int FMT>

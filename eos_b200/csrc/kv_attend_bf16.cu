@@ -3,9 +3,9 @@
 
 namespace eosb {
 
-int kv_attend_bf16(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
+int kv_attend_bf16(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors,
                  cudaStream_t stream) {
-    return kv_attend_format<kKvBf16>(pool, seqs, a, work, status, stream);
+    return kv_attend_format<kKvBf16>(pool, seqs, a, work, errors, stream);
 }
 cudaError_t kv_attend_bf16_init(int blocks) { return kv_attend_format_init<kKvBf16>(blocks); }
 

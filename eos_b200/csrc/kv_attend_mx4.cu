@@ -3,9 +3,9 @@
 
 namespace eosb {
 
-int kv_attend_mx4(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
+int kv_attend_mx4(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors,
                  cudaStream_t stream) {
-    return kv_attend_format<kKvMx4>(pool, seqs, a, work, status, stream);
+    return kv_attend_format<kKvMx4>(pool, seqs, a, work, errors, stream);
 }
 cudaError_t kv_attend_mx4_init(int blocks) { return kv_attend_format_init<kKvMx4>(blocks); }
 

@@ -7,32 +7,32 @@
 namespace eosb {
 
 void launch_kv_append(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type,
-                      int64_t tokens, int* status, cudaStream_t stream) {
+                      int64_t tokens, int* errors, cudaStream_t stream) {
     switch (pool.format) {
-        case kKvF16: return kv_append_f16(pool, seqs, key, value, type, tokens, status, stream);
-        case kKvBf16: return kv_append_bf16(pool, seqs, key, value, type, tokens, status, stream);
-        case kKvMx8: return kv_append_mx8(pool, seqs, key, value, type, tokens, status, stream);
-        default: return kv_append_mx4(pool, seqs, key, value, type, tokens, status, stream);
+        case kKvF16: return kv_append_f16(pool, seqs, key, value, type, tokens, errors, stream);
+        case kKvBf16: return kv_append_bf16(pool, seqs, key, value, type, tokens, errors, stream);
+        case kKvMx8: return kv_append_mx8(pool, seqs, key, value, type, tokens, errors, stream);
+        default: return kv_append_mx4(pool, seqs, key, value, type, tokens, errors, stream);
     }
 }
 
 void launch_kv_read(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
-                    int* status, cudaStream_t stream) {
+                    int* errors, cudaStream_t stream) {
     switch (pool.format) {
-        case kKvF16: return kv_read_f16(pool, seqs, key, value, type, tokens, status, stream);
-        case kKvBf16: return kv_read_bf16(pool, seqs, key, value, type, tokens, status, stream);
-        case kKvMx8: return kv_read_mx8(pool, seqs, key, value, type, tokens, status, stream);
-        default: return kv_read_mx4(pool, seqs, key, value, type, tokens, status, stream);
+        case kKvF16: return kv_read_f16(pool, seqs, key, value, type, tokens, errors, stream);
+        case kKvBf16: return kv_read_bf16(pool, seqs, key, value, type, tokens, errors, stream);
+        case kKvMx8: return kv_read_mx8(pool, seqs, key, value, type, tokens, errors, stream);
+        default: return kv_read_mx4(pool, seqs, key, value, type, tokens, errors, stream);
     }
 }
 
-int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
+int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors,
                      cudaStream_t stream) {
     switch (pool.format) {
-        case kKvF16: return kv_attend_f16(pool, seqs, a, work, status, stream);
-        case kKvBf16: return kv_attend_bf16(pool, seqs, a, work, status, stream);
-        case kKvMx8: return kv_attend_mx8(pool, seqs, a, work, status, stream);
-        default: return kv_attend_mx4(pool, seqs, a, work, status, stream);
+        case kKvF16: return kv_attend_f16(pool, seqs, a, work, errors, stream);
+        case kKvBf16: return kv_attend_bf16(pool, seqs, a, work, errors, stream);
+        case kKvMx8: return kv_attend_mx8(pool, seqs, a, work, errors, stream);
+        default: return kv_attend_mx4(pool, seqs, a, work, errors, stream);
     }
 }
 

@@ -83,9 +83,9 @@ struct KvRows {             // keys or values of a call, [tokens, heads, dim] wi
 };
 
 void launch_kv_append(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type,
-                      int64_t tokens, int* status, cudaStream_t stream);
+                      int64_t tokens, int* errors, cudaStream_t stream);
 void launch_kv_read(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
-                    int* status, cudaStream_t stream);
+                    int* errors, cudaStream_t stream);
 
 struct KvAttend {
     const void* query;      // [batch, q_heads, dim], strides in elements
@@ -105,14 +105,16 @@ struct KvWork {
     float* slots;           // [ctas][kv_slot_floats(dim)]: partial results of the CTAs' warps
     float* partial;         // [ctas][2][kKvMaxRows][dim + 3]: of the CTAs
     int* count;             // [3 ctas], zero between calls
+    int* errors;            // [kKvErrors] what append, read and attend met; the counts only grow, the host remembers what it has reported
 };
+constexpr int kKvErrors = 3;           // pipeline timeout, bad page, bad sequence: kStatusPipelineTimeout and the two codes behind it
 constexpr int kKvMaxRows = 128;        // query heads of one unit, at most
 // 128 rows, or (small heads, 16 warps) 256
 __host__ __device__ constexpr int kv_slot_floats(int dim) { return kKvMaxRows * (dim + 3) + (dim <= 96 ? 128 * (dim + 3) : 0); }
 
 // cudaSuccess once the kernels of this format and dim are ready on the current device
 cudaError_t kv_init(int format, int blocks);
-int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* status,
+int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors,
                      cudaStream_t stream);
 
 }  // namespace eosb

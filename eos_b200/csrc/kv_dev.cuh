@@ -103,6 +103,10 @@ __device__ __forceinline__ void load_pair_scales(const uint8_t* p, uint32_t (&w)
         if constexpr (NB > 6) w[3] = v.w;
     }
 }
+// ---------------------------------------------------------------- errors
+// Counts an error that a call met (see KvWork).
+__device__ __forceinline__ void kv_report(int* errors, int code) { atomicAdd(errors + (code - kStatusPipelineTimeout), 1); }
+
 // ---------------------------------------------------------------- pages
 // The record of `rec` (record index in sequence b) and head h; null when the table or the page id is out of range.
 __device__ __forceinline__ uint8_t* kv_record(const KvPool& pool, const KvSeqs& s, int b, int rec, int h) {

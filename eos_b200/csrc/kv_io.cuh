@@ -33,7 +33,7 @@ struct KvUnit {
     int64_t row0;     // row of position 0 of the sequence (may be negative: rows are row0 + position)
     bool ok;
 };
-__device__ __forceinline__ KvUnit kv_unit(const KvSeqs& s, int64_t tokens, int64_t u, int lane, int* status) {
+__device__ __forceinline__ KvUnit kv_unit(const KvSeqs& s, int64_t tokens, int64_t u, int lane, int* errors) {
     KvUnit r;
     r.ok = false;
     int64_t row, n, first = 0;
@@ -59,7 +59,7 @@ __device__ __forceinline__ KvUnit kv_unit(const KvSeqs& s, int64_t tokens, int64
     }
     if (n == 0) return r;
     if (n < 0 || row < 0 || row + n > tokens || start < 0 || start + n > 0x7fffffffLL) {
-        if (lane == 0) atomicExch(status, kStatusBadSequence);
+        if (lane == 0) kv_report(errors, kStatusBadSequence);
         return r;
     }
     const int64_t rec = (start >> 4) + first;
@@ -178,7 +178,7 @@ __host__ __device__ constexpr int kv_append_blocks(int fmt, int nb, int type) {
 }
 template <int FMT, int NB, int TYPE>
 __global__ void __launch_bounds__(kKvIoWarps * 32, kv_append_blocks(FMT, NB, TYPE))
-    kv_append_kernel(KvPool pool, KvSeqs seqs, KvRows key, KvRows value, int64_t tokens, int64_t units, int* status) {
+    kv_append_kernel(KvPool pool, KvSeqs seqs, KvRows key, KvRows value, int64_t tokens, int64_t units, int* errors) {
     constexpr bool kMx = FMT >= kKvMx8;
     constexpr int KP = kv_key_piece(FMT), VP = kv_value_piece(FMT), NS = kv_scale_stride(NB), ES = TYPE == kTypeF32 ? 4 : 2;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kKvIoWarps * 32, kv_append_blocks(FMT, NB, TYP
     const int64_t u = w / pool.heads;
     if (u >= units) return;
     const int h = (int)(w - u * pool.heads);
-    const KvUnit un = kv_unit(seqs, tokens, u, lane, status);
+    const KvUnit un = kv_unit(seqs, tokens, u, lane, errors);
     if (!un.ok) return;
     const int base = un.rec * kKvRecord;
     const bool full = un.hi - un.lo == kKvRecord && key.vec && value.vec;   // the usual record of a prompt: no conditions on the loads
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kKvIoWarps * 32, kv_append_blocks(FMT, NB, TYP
     // the rows are on their way while the page is looked up
     uint8_t* rec = kv_record(pool, seqs, un.b, un.rec, h);
     if (rec == nullptr) {
-        if (lane == 0) atomicExch(status, kStatusBadPage);
+        if (lane == 0) kv_report(errors, kStatusBadPage);
         return;
     }
     // ---- values: lane (g, t) owns elements 4 g .. + 3 of every block for the tokens 2t, 2t+1, 2t+8, 2t+9
@@ -482,7 +482,7 @@ __device__ __forceinline__ void store_out(uint8_t* p, int vec, const float (&x)[
 
 template <int FMT, int NB, int TYPE>
 __global__ void __launch_bounds__(kKvIoWarps * 32)
-    kv_read_kernel(KvPool pool, KvSeqs seqs, KvRows key, KvRows value, int64_t tokens, int64_t units, int* status) {
+    kv_read_kernel(KvPool pool, KvSeqs seqs, KvRows key, KvRows value, int64_t tokens, int64_t units, int* errors) {
     constexpr bool kMx = FMT >= kKvMx8;
     constexpr int KP = kv_key_piece(FMT), VP = kv_value_piece(FMT), NS = kv_scale_stride(NB), ES = TYPE == kTypeF32 ? 4 : 2;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -490,11 +490,11 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
     const int64_t u = w / pool.heads;
     if (u >= units) return;
     const int h = (int)(w - u * pool.heads);
-    const KvUnit un = kv_unit(seqs, tokens, u, lane, status);
+    const KvUnit un = kv_unit(seqs, tokens, u, lane, errors);
     if (!un.ok) return;
     const uint8_t* rec = kv_record(pool, seqs, un.b, un.rec, h);
     if (rec == nullptr) {
-        if (lane == 0) atomicExch(status, kStatusBadPage);
+        if (lane == 0) kv_report(errors, kStatusBadPage);
         return;
     }
     const int base = un.rec * kKvRecord;
@@ -581,32 +581,32 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
 inline int64_t kv_units(const KvSeqs& s, int64_t tokens) { return s.cu == nullptr ? tokens : (tokens >> 4) + 2 * (int64_t)s.batch; }
 
 template <bool READ, int FMT, int NB, int TYPE>
-void kv_io_launch(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int64_t tokens, int* status,
+void kv_io_launch(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int64_t tokens, int* errors,
                   cudaStream_t stream) {
     const int64_t units = kv_units(seqs, tokens);
     const unsigned blocks = (unsigned)((units * pool.heads + kKvIoWarps - 1) / kKvIoWarps);
-    if constexpr (READ) kv_read_kernel<FMT, NB, TYPE><<<blocks, kKvIoWarps * 32, 0, stream>>>(pool, seqs, key, value, tokens, units, status);
-    else kv_append_kernel<FMT, NB, TYPE><<<blocks, kKvIoWarps * 32, 0, stream>>>(pool, seqs, key, value, tokens, units, status);
+    if constexpr (READ) kv_read_kernel<FMT, NB, TYPE><<<blocks, kKvIoWarps * 32, 0, stream>>>(pool, seqs, key, value, tokens, units, errors);
+    else kv_append_kernel<FMT, NB, TYPE><<<blocks, kKvIoWarps * 32, 0, stream>>>(pool, seqs, key, value, tokens, units, errors);
 }
 template <bool READ, int FMT, int NB>
 void kv_io_type(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
-                int* status, cudaStream_t stream) {
+                int* errors, cudaStream_t stream) {
     switch (type) {
-        case kTypeF32: return kv_io_launch<READ, FMT, NB, kTypeF32>(pool, seqs, key, value, tokens, status, stream);
-        case kTypeF16: return kv_io_launch<READ, FMT, NB, kTypeF16>(pool, seqs, key, value, tokens, status, stream);
-        default: return kv_io_launch<READ, FMT, NB, kTypeBf16>(pool, seqs, key, value, tokens, status, stream);
+        case kTypeF32: return kv_io_launch<READ, FMT, NB, kTypeF32>(pool, seqs, key, value, tokens, errors, stream);
+        case kTypeF16: return kv_io_launch<READ, FMT, NB, kTypeF16>(pool, seqs, key, value, tokens, errors, stream);
+        default: return kv_io_launch<READ, FMT, NB, kTypeBf16>(pool, seqs, key, value, tokens, errors, stream);
     }
 }
 template <bool READ, int FMT>
 void kv_io_format(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
-                  int* status, cudaStream_t stream) {
+                  int* errors, cudaStream_t stream) {
     switch (pool.blocks) {
-        case 1: return kv_io_type<READ, FMT, 1>(pool, seqs, key, value, type, tokens, status, stream);
-        case 2: return kv_io_type<READ, FMT, 2>(pool, seqs, key, value, type, tokens, status, stream);
-        case 3: return kv_io_type<READ, FMT, 3>(pool, seqs, key, value, type, tokens, status, stream);
-        case 4: return kv_io_type<READ, FMT, 4>(pool, seqs, key, value, type, tokens, status, stream);
-        case 6: return kv_io_type<READ, FMT, 6>(pool, seqs, key, value, type, tokens, status, stream);
-        default: return kv_io_type<READ, FMT, 8>(pool, seqs, key, value, type, tokens, status, stream);
+        case 1: return kv_io_type<READ, FMT, 1>(pool, seqs, key, value, type, tokens, errors, stream);
+        case 2: return kv_io_type<READ, FMT, 2>(pool, seqs, key, value, type, tokens, errors, stream);
+        case 3: return kv_io_type<READ, FMT, 3>(pool, seqs, key, value, type, tokens, errors, stream);
+        case 4: return kv_io_type<READ, FMT, 4>(pool, seqs, key, value, type, tokens, errors, stream);
+        case 6: return kv_io_type<READ, FMT, 6>(pool, seqs, key, value, type, tokens, errors, stream);
+        default: return kv_io_type<READ, FMT, 8>(pool, seqs, key, value, type, tokens, errors, stream);
     }
 }
 

@@ -4,12 +4,12 @@
 namespace eosb {
 
 void kv_append_mx4(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
-                  int* status, cudaStream_t stream) {
-    kv_io_format<false, kKvMx4>(pool, seqs, key, value, type, tokens, status, stream);
+                  int* errors, cudaStream_t stream) {
+    kv_io_format<false, kKvMx4>(pool, seqs, key, value, type, tokens, errors, stream);
 }
 void kv_read_mx4(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
-                int* status, cudaStream_t stream) {
-    kv_io_format<true, kKvMx4>(pool, seqs, key, value, type, tokens, status, stream);
+                int* errors, cudaStream_t stream) {
+    kv_io_format<true, kKvMx4>(pool, seqs, key, value, type, tokens, errors, stream);
 }
 
 cudaError_t kv_io_mx4_init(int blocks) { return kv_io_format_init<kKvMx4>(blocks); }

@@ -616,7 +616,8 @@ EOS_B200_API int eos_b200_kv_cache_attend_device(EosB200KvCache* cache, const vo
                                                  int window, void* d_out, float* d_lse, void* stream, EosB200Stats* stats,
                                                  char** err);
 /* Waits for `stream` (NULL: the runtime's stream) and returns EOS_B200_DEVICE_STATUS if a kernel of the calls above met
- * a page, position or length out of range, or gave up on a bounded wait. */
+ * a page, position or length out of range, or gave up on a bounded wait.  What one cache's calls met is reported once, by that
+ * cache's sync alone. */
 EOS_B200_API int eos_b200_kv_cache_sync(EosB200KvCache* cache, void* stream, char** err);
 
 /* Seeded synthetic data on the device (bench / tests): n rows of dim N(0,1) values, optionally

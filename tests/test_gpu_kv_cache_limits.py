@@ -89,3 +89,55 @@ def test_a_single_token_gives_its_value(fmt):
     s.sync()
     sv = stored(v, fmt)[0, 0]
     assert ((out[0].double() - sv).abs() <= 12 * 2.0 ** -23 * sv.abs()).all()
+
+
+def test_errors_stay_with_their_cache():
+    """What a call on one cache met is reported by that cache's sync, once, whatever else its runtime runs meanwhile, and by no other's."""
+    import eos_b200
+    from eos_b200 import synth
+    dim, heads, n = 64, 2, 40
+    rt = eos_b200.Runtime(0)
+    a, b = (Sequences(fmt, dim, heads, 16, [n], seed=i, runtime=rt) for i, fmt in enumerate(("f16", "mx8")))
+    k, v = tensors(n, heads, dim, "f16", 81)
+    q = tensors(1, heads, dim, "f16", 82)[0]
+    encoder = eos_b200.BertEmbedder(rt, **synth.make_q8_encoder(1, 128, 2, 256, vocab=200, max_pos=64, seed=1, head_out=64))
+    ids, mask, _ = synth.make_batch(2, 16, 200, 5, 16, seed=2)
+    error = eos_b200.EosB200DeviceStatusError
+
+    def others():
+        b.append(k, v, [0], [n])
+        b.attend(q, [n], 0.1)
+        b.read([0], [n], "f16")
+        b.sync()
+        encoder.run(ids, mask)
+
+    good = a.table.clone()
+    a.append(k, v, [0], [n])
+    a.sync()
+    for call, what in ((lambda: a.append(k, v, [0], [n]), "page"), (lambda: a.read([0], [n], "f16"), "page"),
+                       (lambda: a.attend(q, [n], 0.1), "page"), (lambda: a.append(k, v, [-1], [n]), "start")):
+        a.table.copy_(good)
+        if what == "page":
+            a.table[0, 1] = a.pages
+        call()
+        others()
+        with pytest.raises(error, match=what):
+            a.sync()
+        a.sync()
+        others()
+    # both at once
+    a.table[0, 0] = -1
+    a.attend(q, [n], 0.1)
+    b.attend(q, [-1], 0.1)
+    with pytest.raises(error, match="length"):
+        b.sync()
+    with pytest.raises(error, match="page"):
+        a.sync()
+    # two kinds in one cache are both named
+    a.attend(q, [n], 0.1)
+    a.attend(q, [-7], 0.1)
+    with pytest.raises(error, match="page.*length"):
+        a.sync()
+    a.sync()
+    b.sync()
+    encoder.close()
