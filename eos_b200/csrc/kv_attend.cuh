@@ -609,8 +609,6 @@ __device__ __forceinline__ bool kv_span(const KvPool& pool, const KvSeqs& s, int
     lo = window > 0 ? max(hi - window, 0) : 0;
     return n >= 0 && n <= room;
 }
-__device__ __forceinline__ int kv_records(int lo, int hi) { return hi > lo ? (hi + kKvRecord - 1) / kKvRecord - lo / kKvRecord : 0; }
-
 
 // A walk over the records of a range, in order: the unit (b, hu) and the record r of its n.
 struct KvWalk {
@@ -806,7 +804,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
             const int h = (int)split.by_chunks(at.hu), row0 = (at.hu - h * split.chunks) * chunk_rows + rw * kRows;
             w.load_query(a, (int64_t)at.b * a.seq_stride + (int64_t)h * a.group * a.head_stride, row0, a.group, lane);
             // the unit's span relative to the next record's first token
-            int lo = at.lo - (at.lo / kKvRecord + at.r) * kKvRecord, hi = lo + at.hi - at.lo;
+            int lo = at.lo - (at.lo / kKvRecord + at.r) * kKvRecord, hi = lo + (at.hi - at.lo);
             const int row_warps = opaque(split.row_warps);
             const int batch = stages >> 1;
             int fresh = opaque(1);                       // the query is on its way

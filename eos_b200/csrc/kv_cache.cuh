@@ -60,6 +60,9 @@ __host__ __device__ constexpr int kv_lane_offset(int bytes, int lane, int p) {
     return plane * 512 + (rest >= 8 ? 256 + lane * 4 + in - 8 : lane * 4 + in);
 }
 
+// Records that the positions [lo, hi) of a sequence lie in, for any positions that an int holds.
+__host__ __device__ inline int kv_records(int lo, int hi) { return hi > lo ? (hi - 1) / kKvRecord + 1 - lo / kKvRecord : 0; }
+
 struct KvPool {
     uint8_t* base;
     int64_t pages;

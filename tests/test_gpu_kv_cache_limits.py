@@ -6,7 +6,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from tests.test_gpu_kv_cache import DTYPES, Sequences, stored, tensors  # noqa: E402
+from tests.test_gpu_kv_cache import DTYPES, Sequences, check_attend, same, stored, tensors  # noqa: E402
 
 
 def formula(q, k, v, scale, group):
@@ -141,3 +141,48 @@ def test_errors_stay_with_their_cache():
     a.sync()
     b.sync()
     encoder.close()
+
+
+def test_the_longest_sequences():
+    """Positions up to 2^31 - 2 and a length of 2^31 - 1, the largest there are, on pages that a table names again and again;
+    another sequence of the call is not touched by it."""
+    import eos_b200
+    rt = eos_b200.Runtime(0)
+    dim, heads, group, page, wide, last, n = 32, 1, 3, 65536, 32768, 2 ** 31 - 1, 1000
+    cache = eos_b200.KvCache(rt, 3, page, heads, dim, "mx8")
+    table = torch.zeros((2, wide), dtype=torch.int32, device="cuda")
+    table[0, -1], table[1] = 1, 2
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    k, v = tensors(n + 40, heads, dim, "f32", 91)
+    q = tensors(2, group, dim, "f32", 92)[0]
+    st = torch.cuda.current_stream().cuda_stream
+    starts, cu, lengths = ints(last - n, 0), ints(0, n, n + 40), ints(last, 40)
+    cache.append_device(k.data_ptr(), v.data_ptr(), "f32", n + 40, 2, table.data_ptr(), wide, starts.data_ptr(), cu.data_ptr(), stream=st)
+    rk, rv = torch.zeros_like(k), torch.zeros_like(v)
+    cache.read_device(rk.data_ptr(), rv.data_ptr(), "f32", n + 40, 2, table.data_ptr(), wide, starts.data_ptr(), cu.data_ptr(), stream=st)
+    cache.sync(st)
+    sk, sv = stored(k, "mx8"), stored(v, "mx8")
+    assert same(rk, sk) and same(rv, sv)
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+    for window in (1, 333, n):
+        cache.attend_device(q.data_ptr(), "f32", group, 2, table.data_ptr(), wide, lengths.data_ptr(), out.data_ptr(), 0.2, window,
+                            lse.data_ptr(), stream=st)
+        cache.sync(st)
+        spans = [(sk[n - window:n], sk[n:][-min(window, 40):]), (sv[n - window:n], sv[n:][-min(window, 40):])]
+        check_attend(q, spans, [min(window, n), min(window, 40)], 0.2, 0, "mx8", out, lse, group)
+    # all of it: 2^31 - 1 - n tokens of zeros, whose weights are 1, and the last n
+    cache.attend_device(q.data_ptr(), "f32", group, 2, table.data_ptr(), wide, lengths.data_ptr(), out.data_ptr(), 0.2, 0, lse.data_ptr(),
+                        stream=st)
+    cache.sync(st)
+    check_attend(q[1:], [sk[n:][None], sv[n:][None]], [40], 0.2, 0, "mx8", out[1:], lse[1:], group)
+    p = torch.exp(0.2 * (sk[:n, 0] @ q[0].double().T))           # [n, group]
+    total = last - n + p.sum(0)
+    # weights and sums as in check_attend; of the ones, 2^7 each, a lane's sums are exact below 2^31 and a few are rounded, 2^-20
+    assert ((lse[0].double() - torch.log(total)).abs() <= 2.0 ** -19).all()
+    want = (p.T @ sv[:n, 0]) / total[:, None]
+    size = (p.T @ sv[:n, 0].abs()) / total[:, None]
+    # (the floor of a weight's split: 2^-31 of the largest weight, and sums over n weighted values)
+    big = (0.2 * (sk[:n, 0].abs() @ q[0].double().abs().T)).max()
+    tol = (4 * float(big) * (dim + 8) * 2.0 ** -23 + n * 2.0 ** -23 + 2.0 ** -18) * size + n * 2.0 ** -29 * (p / total * sv[:n, 0].abs().amax(-1)[:, None]).amax(0)[:, None]
+    assert ((out[0].double() - want).abs() <= tol).all()
+    cache.close()

@@ -68,6 +68,31 @@ def test_record_layout_is_a_bijection(tmp_path):
     assert subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout == "ok\n"
 
 
+def run_cpp(tmp_path, body):
+    """Compiles a main() with the cache's host-side header and runs it; it prints ok."""
+    src, exe = tmp_path / "check.cpp", tmp_path / "check"
+    src.write_text("#include <climits>\n#include <cstdio>\n#include <cstdlib>\n#include <set>\n#include <utility>\n#include <vector>\n"
+                   '#include "kv_cache.cuh"\nusing namespace eosb;\n' + body)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    subprocess.check_call(["g++", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover", "-I",
+                           os.path.join(ROOT, "eos_b200", "csrc"), "-I", os.path.join(cuda, "include"), str(src), "-o", str(exe)])
+    assert subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout == "ok\n"
+
+
+def test_records_of_a_span_up_to_the_largest_position(tmp_path):
+    run_cpp(tmp_path, r"""
+int main() {
+    const int ends[] = {0, 1, 15, 16, 17, 31, 32, 1000, 65536, INT_MAX - 33, INT_MAX - 17, INT_MAX - 16, INT_MAX - 15, INT_MAX - 14, INT_MAX - 1, INT_MAX};
+    for (int lo : ends)
+        for (int hi : ends) {
+            const long long want = hi > lo ? ((long long)hi + 15) / 16 - lo / 16 : 0;
+            if (kv_records(lo, hi) != want) return 1;
+        }
+    std::puts("ok");
+}
+""")
+
+
 def test_work_units_cover_every_record_once():
     """The unit arithmetic of an append / read: sequence b starts at unit cu[b] // 16 + 2 b, unit i of a sequence is its
     i-th touched record, and tokens // 16 + 2 batch units are enough."""
