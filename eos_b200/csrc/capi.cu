@@ -89,18 +89,22 @@ cudaStream_t pick_stream(EosB200Runtime* rt, void* stream) {
 }
 
 // One warp waits on an mbarrier nobody ever arrives on, with the given limit; the wait gives up, and the kernel
-// reports it through the status word exactly as the pipelines do.
+// reports it through the status word exactly as the pipelines do -- if it also gives up as one where the odd lanes alone do,
+// whose barrier nobody arrives on, while that of the others has completed.
 __global__ void bounded_wait_probe_kernel(long long limit_cycles, int* status) {
-    __shared__ __align__(8) unsigned long long bar;
-    __shared__ int abort_flag;
+    __shared__ __align__(8) unsigned long long bar[2];
+    __shared__ int abort_flag, parted;
     if (threadIdx.x == 0) {
-        abort_flag = 0;
-        mbar_init(smem_u32(&bar), 1);
+        abort_flag = parted = 0;
+        mbar_init(smem_u32(&bar[0]), 1);
+        mbar_init(smem_u32(&bar[1]), 1);
         mbar_fence_init();
+        mbar_arrive(smem_u32(&bar[0]));
     }
     __syncwarp();
-    const bool ok = mbar_wait_limit(smem_u32(&bar), 0, &abort_flag, limit_cycles);
+    const bool ok = mbar_wait_limit(smem_u32(&bar[1]), 0, &abort_flag, limit_cycles);
     __syncwarp();
+    if (mbar_wait_warp(smem_u32(&bar[threadIdx.x & 1]), 0, false, 0, 0, &parted, limit_cycles)) return;
     if (threadIdx.x == 0 && (!ok || abort_flag != 0)) atomicExch(status, kStatusPipelineTimeout);
 }
 

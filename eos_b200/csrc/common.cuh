@@ -73,6 +73,18 @@ __device__ __forceinline__ bool mbar_wait_limit(uint32_t bar, uint32_t parity, v
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
     return mbar_wait_limit(bar, parity, abort_flag, kWaitLimitCycles);
 }
+// The same by all 32 lanes of a warp, for one barrier or (`two`, the same in all lanes) a second one as well: if one lane has given
+// up, the answer is false in all of them.  (Lanes that poll for themselves may part there, one giving up just before the phase
+// completes for the others.)
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, bool two, uint32_t bar2, uint32_t parity2,
+                                               volatile int* abort_flag, long long limit_cycles = kWaitLimitCycles) {
+    bool done = mbar_try_wait(bar, parity);
+    if (two) done = mbar_try_wait(bar2, parity2) && done;
+    if (__all_sync(0xffffffffu, done)) return true;
+    done = mbar_wait_limit(bar, parity, abort_flag, limit_cycles);
+    if (two) done = done && mbar_wait_limit(bar2, parity2, abort_flag, limit_cycles);
+    return __all_sync(0xffffffffu, done);
+}
 
 // ---------------------------------------------------------------- fences
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }

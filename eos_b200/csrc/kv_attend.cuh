@@ -797,7 +797,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
         KvWarp<FMT, NB, RT, HALVES> w;
         int stage = 0, fill = 0, empty = rw == 0 ? stages : 0;   // stage to read next; stage to fill next, stages to fill
         uint32_t phase = 0, fill_phase = 1;
-        bool alive = true;   // no wait has run out
+        bool alive = true;   // no wait has run out (the same in all lanes)
 #pragma unroll 1
         while (true) {
             int seg = min(at.n - at.r, left);   // records of the unit here
@@ -847,13 +847,13 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
                 }
                 const int take = Shape::kPair && j > 1 && lo <= 0 && hi >= 2 * kKvRecord && pair ? 2 : 1;
                 const int next = stage + 1 == stages ? 0 : stage + 1;
-                alive = alive && mbar_wait(full_at + 8 * stage, phase, &s_abort);
+                alive = alive && mbar_wait_warp(full_at + 8 * stage, phase, Shape::kPair && take == 2, full_at + 8 * next,
+                                                next == 0 ? phase ^ 1u : phase, &s_abort);
                 const uint8_t* here = ring + stage * Shape::kRecord;
                 const bool ok = alive && s_ok[team][stage];
                 bool one = ok;
                 if constexpr (Shape::kPair) {
                     if (take == 2) {   // (all tokens of both count)
-                        alive = alive && mbar_wait(full_at + 8 * next, next == 0 ? phase ^ 1u : phase, &s_abort);
                         const uint8_t* there = ring + next * Shape::kRecord;
                         const bool ok2 = alive && s_ok[team][next];
                         one = ok != ok2;   // a record that is missing is left out

@@ -186,3 +186,17 @@ def test_the_longest_sequences():
     tol = (4 * float(big) * (dim + 8) * 2.0 ** -23 + n * 2.0 ** -23 + 2.0 ** -18) * size + n * 2.0 ** -29 * (p / total * sv[:n, 0].abs().amax(-1)[:, None]).amax(0)[:, None]
     assert ((out[0].double() - want).abs() <= tol).all()
     cache.close()
+
+
+def test_a_warp_gives_up_as_one():
+    """The wait of the attention's warps: where half of the lanes give up and the others do not, all have given up.  The
+    self-test reports its time-out only then."""
+    import eos_b200
+    rt = eos_b200.Runtime(0)
+    for _ in range(3):
+        with pytest.raises(eos_b200.EosB200DeviceStatusError, match="timeout"):
+            rt.selftest_bounded_wait(200_000)
+    s = Sequences("mx8", 64, 1, 16, [40], runtime=rt)
+    s.append(*tensors(40, 1, 64, "f16", 95), [0], [40])
+    s.sync()
+    rt.close()
