@@ -44,7 +44,9 @@ __device__ __forceinline__ int opaque(int x) {
     return x;
 }
 
-constexpr float kKvMaxInit = -1.5e38f;   // below every score; finite, so that 2^(x - m) of a masked score is 0 and not NaN
+// The least fp32 number: no score is below it.  Finite, so that 2^(x - m) of a masked score is 0 and not NaN.  (A distance from it
+// may be infinite: a first score above 0 less it, and the second maximum by which it moves.  Both are then taken anew.)
+constexpr float kKvMaxInit = -3.402823466e38f;
 constexpr float kKvHead = 7.f, kKvLag = 15.f;   // m = ceil(largest score) - 7; weights up to 2^15
 constexpr int kKvQueryExp = 13;                  // query rows are scaled to a largest magnitude in [2^13, 2^14)
 

@@ -200,3 +200,50 @@ def test_a_warp_gives_up_as_one():
     s.append(*tensors(40, 1, 64, "f16", 95), [0], [40])
     s.sync()
     rt.close()
+
+
+@pytest.mark.parametrize("fmt", ["f16", "bf16", "mx8", "mx4"])
+@pytest.mark.parametrize("top", [1e38, 1.6e38, 2.2e38])
+def test_scores_as_low_as_fp32_goes(fmt, top):
+    """All scores of a row close to -top, times log2(e) down to -3.2e38: the softmax is that of their differences, here none or
+    more than any weight.  And both ends in one row."""
+    dim, n = 32, 40
+    _, v = tensors(n, 1, dim, "f16", 5)
+    v = stored(v, fmt).half()
+    k = torch.zeros((n, 1, dim), device="cuda", dtype=torch.float16)
+    k[:, 0, 0] = -2.0
+    k[[3, 37], 0, 0] = -1.0
+    k[20, 0, 1] = 2.0                                      # (the second query's one large score)
+    s = Sequences(fmt, dim, 1, 16, [n])
+    s.append(k, v, [0], [n])
+    q = torch.zeros((1, 2, dim), device="cuda")
+    q[0, :, 0] = top / 2 * 2.0 ** -100                     # scores -top, and -top / 2 of tokens 3 and 37
+    q[0, 1, 1] = top / 2 * 2.0 ** -100                     # token 20: 0 = -top + top
+    out, lse = s.attend(q, [n], 2.0 ** 100)
+    s.sync()
+    two = v[[3, 37], 0].double()
+    tol = (2.0 ** -14 if fmt == "bf16" else 2.0 ** -20) * two.abs().mean(0) + 2.0 ** -24 * two.abs().amax()
+    assert ((out[0, 0].double() - two.mean(0)).abs() <= tol).all()
+    assert abs(float(lse[0, 0]) + top / 2) <= 2.0 ** -20 * top
+    assert ((out[0, 1].double() - v[20, 0].double()).abs() <= 2.0 ** -20 * v[20, 0].abs() + 2.0 ** -24).all()
+    assert abs(float(lse[0, 1])) <= 2.0 ** -20 * top
+    # every score the same, at the lowest
+    k[:, 0, :2] = torch.tensor([-2.0, 0.0], device="cuda")
+    s.append(k, v, [0], [n])
+    out, lse = s.attend(q, [n], 2.0 ** 100)
+    s.sync()
+    mean, size = v[:, 0].double().mean(0), v[:, 0].double().abs().mean(0)
+    assert ((out[0] - mean).abs() <= (n + 16) * 2.0 ** -23 * size + 2.0 ** -24).all()
+    assert ((lse[0].double() + top).abs() <= 2.0 ** -20 * top).all()
+    # and at the highest
+    out, lse = s.attend(-q, [n], 2.0 ** 100)
+    s.sync()
+    assert ((out[0] - mean).abs() <= (n + 16) * 2.0 ** -23 * size + 2.0 ** -24).all()
+    assert ((lse[0].double() - top).abs() <= 2.0 ** -20 * top).all()
+    # a row that rises from the lowest to the highest, record by record
+    k[:, 0, 0] = torch.linspace(-2, 2, 5, device="cuda").half().repeat_interleave(8)
+    s.append(k, v, [0], [n])
+    out, lse = s.attend(q, [n], 2.0 ** 100)
+    s.sync()
+    assert ((out[0] - v[32:, 0].double().mean(0)).abs() <= 24 * 2.0 ** -23 * v[32:, 0].double().abs().mean(0) + 2.0 ** -24).all()
+    assert ((lse[0].double() - top).abs() <= 2.0 ** -20 * top).all()
