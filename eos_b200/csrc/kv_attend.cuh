@@ -103,7 +103,8 @@ struct KvWarp {
     using Weights = uint32_t[RT][kParts][2];
 
     uint32_t q[RT][NB][4 * HALVES];   // head g of each tile, elements 32 b + 8 t .. + 7: the largest parts, then the next
-    float2 qs[RT];                    // heads 2t and 2t + 1: factor of the raw sums, scale log2(e) 2^(query exponent)
+    float2 qs[RT];                    // heads 2t and 2t + 1: factor of the raw sums, scale log2(e) 2^(query exponent), less ks
+    float ks;                         // (mx formats) factor of the key scales, a power of two
     float2 nm[RT], nd[RT];            // heads 2t, 2t + 1: minus the lagging maxima of x; of x + e relative to those (mx formats)
     float l[RT][2];                   // this lane's part of the sum of weights
     float o[RT][NB][2][4];            // [block][i]: elements 32 b + 4 g + 2 i (0, 1) and + 2 i + 1 (2, 3) of heads 2t, 2t + 1
@@ -145,40 +146,54 @@ struct KvWarp {
                 }
         }
     }
-    // ... then the operands.  f16: each row is divided by a power of two first, so that no magnitude leaves f16's range.
+    // ... then the operands.  f16: each row is divided by a power of two first, so that no magnitude leaves f16's range.  It is
+    // multiplied back behind the sum -- over block-scaled keys, whose sum with it might leave fp32's range where the score does
+    // not, as far as it is common to the rows and below 1, into the key scales (one packed product a block, 1 % over mx4).
     // One operand: the type is f16 or bf16 (over a bf16 cache bf16); more: f32 (over a bf16 cache two: f16).
     __device__ __forceinline__ void convert_query(const KvAttend& a, int lane) {
         const bool f16 = opaque(a.type) == kTypeF16;
+        auto pair = [&](int r, int b, int i) {
+            if constexpr (!kWide) {
+                const uint32_t w = q[r][b][i];
+                if constexpr (kBf) return HALVES == 1 ? bf16x2_floats(w) : f16x2_floats(w);
+                const float2 x = f16x2_floats(w), y = bf16x2_floats(w);
+                return make_float2(f16 ? x.x : y.x, f16 ? x.y : y.y);
+            } else {
+                return make_float2(__uint_as_float(q[r][b][2 * i]), __uint_as_float(q[r][b][2 * i + 1]));
+            }
+        };
+        uint32_t e[RT], back = 127u + kKvQueryExp;   // exponents of the rows; what they are taken back relative to behind the sum
+        if constexpr (!kBf) {
+            uint32_t most = 0;
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-            split_row(a, r, lane, [&](int b, int i) {
-                if constexpr (!kWide) {
-                    const uint32_t w = q[r][b][i];
-                    if constexpr (kBf) return HALVES == 1 ? bf16x2_floats(w) : f16x2_floats(w);
-                    const float2 x = f16x2_floats(w), y = bf16x2_floats(w);
-                    return make_float2(f16 ? x.x : y.x, f16 ? x.y : y.y);
-                } else {
-                    return make_float2(__uint_as_float(q[r][b][2 * i]), __uint_as_float(q[r][b][2 * i + 1]));
-                }
-            });
+            for (int r = 0; r < RT; ++r) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 x = pair(r, b, i);
+                        top = max(top, max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu));
+                    }
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                e[r] = min(max(top >> 23, kKvQueryExp + 1u), 254u);
+                most = max(most, e[r]);
+            }
+            if constexpr (kMx) {
+                back = min(back, __reduce_max_sync(0xffffffffu, most));
+                ks = __uint_as_float((back - kKvQueryExp) << 23);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) split_row(r, lane, e[r], back, a.scale_log2, [&](int b, int i) { return pair(r, b, i); });
     }
     template <typename F>
-    __device__ __forceinline__ void split_row(const KvAttend& a, int r, int lane, F&& pair) {
-        float inv = 1.f, factor = a.scale_log2;
+    __device__ __forceinline__ void split_row(int r, int lane, uint32_t e, uint32_t back, float factor, F&& pair) {
+        float inv = 1.f;
         if constexpr (!kBf) {
-            uint32_t top = 0;
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 x = pair(b, i);
-                    top = max(top, max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu));
-                }
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const uint32_t e = min(max(top >> 23, kKvQueryExp + 1u), 254u);
             inv = __uint_as_float((254u + kKvQueryExp - e) << 23);
-            factor *= __uint_as_float((e - kKvQueryExp) << 23);
+            factor *= __uint_as_float((127u + e - back) << 23);   // (e and back are at least 14: an exponent of -126 or more)
         }
         // the factors of heads 2t and 2t + 1 are those of the lanes with g = 2t and 2t + 1
         qs[r].x = __shfl_sync(0xffffffffu, factor, 8 * (lane & 3));
@@ -254,7 +269,7 @@ struct KvWarp {
                     f16_of_e2m1x8(k0[b], f[0], f[1], f[2], f[3]);
                     f16_of_e2m1x8(k1[b], h[0], h[1], h[2], h[3]);
                 }
-                const float s0 = scale_at(e0[b / 4], b & 3), s1 = scale_at(e1[b / 4], b & 3);
+                const float2 sk = mul2(make_float2(scale_at(e0[b / 4], b & 3), scale_at(e1[b / 4], b & 3)), make_float2(ks, ks));
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
                     float c[4] = {0.f, 0.f, 0.f, 0.f};
@@ -263,8 +278,8 @@ struct KvWarp {
                         mma_16x8x16<false>(c, f[0], h[0], f[1], h[1], q[r][b][4 * u], q[r][b][4 * u + 1]);
                         mma_16x8x16<false>(c, f[2], h[2], f[3], h[3], q[r][b][4 * u + 2], q[r][b][4 * u + 3]);
                     }
-                    s[r][0] = fmaf(c[0], s0, s[r][0]), s[r][1] = fmaf(c[1], s0, s[r][1]);
-                    s[r][2] = fmaf(c[2], s1, s[r][2]), s[r][3] = fmaf(c[3], s1, s[r][3]);
+                    s[r][0] = fmaf(c[0], sk.x, s[r][0]), s[r][1] = fmaf(c[1], sk.x, s[r][1]);
+                    s[r][2] = fmaf(c[2], sk.y, s[r][2]), s[r][3] = fmaf(c[3], sk.y, s[r][3]);
                 }
             }
         }

@@ -247,3 +247,21 @@ def test_scores_as_low_as_fp32_goes(fmt, top):
     s.sync()
     assert ((out[0] - v[32:, 0].double().mean(0)).abs() <= 24 * 2.0 ** -23 * v[32:, 0].double().abs().mean(0) + 2.0 ** -24).all()
     assert ((lse[0].double() - top).abs() <= 2.0 ** -20 * top).all()
+
+
+@pytest.mark.parametrize("fmt", ["mx8", "mx4"])
+@pytest.mark.parametrize("power", [-118, -100, 60, 100, 112, 118])
+def test_keys_of_any_size_under_queries_of_the_opposite(fmt, power):
+    """Block-scaled keys of 2^power under queries of 2^-power, all of one sign: the scores are of ordinary size, and so must all be
+    that leads to them.  One query of the group is far smaller than the others: its scores are zeros nearly."""
+    dim, n, group = 128, 70, 3
+    s = Sequences(fmt, dim, 1, 16, [n])
+    g = torch.Generator().manual_seed(97)
+    k = (torch.rand((n, 1, dim), generator=g) * 2.0 ** power).cuda()
+    v = torch.randn((n, 1, dim), generator=g).cuda()
+    q = (torch.rand((1, group, dim), generator=g) * 2.0 ** -power).cuda()
+    q[0, 1] *= 2.0 ** -6
+    s.append(k, v, [0], [n])
+    out, lse = s.attend(q, [n], 0.125)
+    s.sync()
+    check_attend(q, ([stored(k, fmt)], [stored(v, fmt)]), [n], 0.125, 0, fmt, out, lse, group)
