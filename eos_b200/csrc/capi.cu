@@ -3872,7 +3872,8 @@ int eos_b200_kv_cache_attend_device(EosB200KvCache* c, const void* d_query, int 
         return fail(err, "kv_cache_attend: q_heads " + std::to_string(q_heads) + " is not a multiple of the cache's " +
                              std::to_string(c->pool.heads) + " key heads");
     if (q_heads > 65536) return fail(err, "kv_cache_attend: more than 65536 query heads");
-    if (!std::isfinite(scale)) return fail(err, "kv_cache_attend: scale must be finite");
+    const float scale_log2 = (float)((double)scale * 1.4426950408889634);
+    if (!std::isfinite(scale_log2)) return fail(err, "kv_cache_attend: scale must be finite, its magnitude at most 2.3e38");
     if (window < 0) return fail(err, "kv_cache_attend: negative window");
     if (query_seq_stride < 0 || query_head_stride < 0) return fail(err, "kv_cache_attend: negative stride");
     if (stats != nullptr) std::memset(stats, 0, sizeof(*stats));
@@ -3893,7 +3894,7 @@ int eos_b200_kv_cache_attend_device(EosB200KvCache* c, const void* d_query, int 
     a.group = q_heads / c->pool.heads;
     a.out = d_out;
     a.lse = d_lse;
-    a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+    a.scale_log2 = scale_log2;
     a.window = window;
     CUDA_TRY(cudaSetDevice(c->rt->device));
     const int launches = launch_kv_attend(c->pool, seqs, a, c->work, c->work.errors, pick_stream(c->rt, stream));

@@ -606,7 +606,8 @@ EOS_B200_API int eos_b200_kv_cache_read_device(EosB200KvCache* cache, void* d_ke
  * are appended before the call when it attends to itself.
  * batch is at most 65535.  Positions on a page that is out of range are left out and eos_b200_kv_cache_sync reports it; a
  * length that is negative or longer than the page table is cut, and reported too.  Rows that meet an infinity or a NaN are
- * not finite; other rows are not touched by it.
+ * not finite; other rows are not touched by it.  scale q, the sums q . k and the scores scale q . k have to stay within fp32's range
+ * (|scale| itself: at most 2.3e38).
  * Enqueued, allocation-free and capturable as above; calls of one cache share its workspace and must be ordered (one
  * stream, or events between streams; replays of graphs that hold them likewise): overlapping ones give wrong results, and may
  * go on giving them.  Two caches are independent. */

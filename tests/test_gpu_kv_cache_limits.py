@@ -265,3 +265,18 @@ def test_keys_of_any_size_under_queries_of_the_opposite(fmt, power):
     out, lse = s.attend(q, [n], 0.125)
     s.sync()
     check_attend(q, ([stored(k, fmt)], [stored(v, fmt)]), [n], 0.125, 0, fmt, out, lse, group)
+
+
+def test_refusals_at_the_limits():
+    """Arguments that no kernel could use: a scale that leaves fp32's range in base 2."""
+    import eos_b200
+    rt = eos_b200.Runtime(0)
+    c = eos_b200.KvCache(rt, 4, 16, 2, 64, "mx8")
+    x, i = torch.zeros((4, 2, 64), device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda")
+    p, t = x.data_ptr(), i.data_ptr()
+    ok = dict(d_query=p, type="f32", q_heads=2, batch=1, d_page_table=t, max_pages=1, d_lengths=t, d_out=p + 1024, scale=1.0)
+    for scale in (2.4e38, -3.4e38):
+        with pytest.raises(eos_b200.EosB200Error, match="scale"):
+            c.attend_device(**{**ok, "scale": scale})
+    c.attend_device(**{**ok, "scale": 2.3e38, "stream": torch.cuda.current_stream().cuda_stream})
+    c.sync(torch.cuda.current_stream().cuda_stream)
