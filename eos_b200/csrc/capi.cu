@@ -3731,15 +3731,18 @@ int row_alignment(const void* p, int64_t stride_a, int64_t stride_b, int type) {
     return all % 32 == 0 ? 2 : all % 16 == 0 ? 1 : 0;
 }
 
-// What append and read check alike; fills the kernels' views.
-std::string kv_rows_check(const EosB200KvCache* c, const void* key, const void* value, int type, int64_t tokens,
+// whether 4-byte accesses at p are aligned (null: yes)
+bool word_aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
+
+// What append and read check alike; fills the kernels' views.  The reason of a refusal, or null.
+const char* kv_rows_check(const EosB200KvCache* c, const void* key, const void* value, int type, int64_t tokens,
                           const EosB200KvStrides* st, int batch, const int32_t* table, int max_pages, const int32_t* starts,
                           const int32_t* cu, KvSeqs* seqs, KvRows* k, KvRows* v) {
     if (type < EOS_B200_TYPE_F32 || type > EOS_B200_TYPE_BF16) return "unknown element type";
     if (tokens < 0 || batch < 0) return "negative token or sequence count";
     if (tokens > 0x7fffffffLL) return "more than 2^31 - 1 tokens in one call";
     if (cu == nullptr && tokens != batch) return "without row offsets there is one token per sequence (tokens == batch)";
-    if (tokens == 0 || batch == 0) return "";
+    if (tokens == 0 || batch == 0) return nullptr;
     if (key == nullptr || value == nullptr || table == nullptr || starts == nullptr) return "null argument";
     if (max_pages <= 0) return "max_pages must be positive";
     const int64_t dim = c->pool.dim, row = dim * c->pool.heads;
@@ -3748,12 +3751,13 @@ std::string kv_rows_check(const EosB200KvCache* c, const void* key, const void* 
     if (s.key_token < 0 || s.key_head < 0 || s.value_token < 0 || s.value_head < 0) return "negative stride";
     if (reinterpret_cast<uintptr_t>(key) % type_bytes(type) != 0 || reinterpret_cast<uintptr_t>(value) % type_bytes(type) != 0)
         return "key or value is not aligned to its element type";
+    if (!word_aligned(table) || !word_aligned(starts) || !word_aligned(cu)) return "page table, starts or row offsets are not 4-byte aligned";
     // blocks of eight warps, one (record, head) each
     if ((tokens / kKvRecord + 2 * (int64_t)batch + 1) * c->pool.heads / 8 >= 0x7fffffffLL) return "too many tokens x heads in one call";
     *seqs = {table, max_pages, batch, starts, cu, nullptr};
     *k = {const_cast<void*>(key), s.key_token, s.key_head, row_alignment(key, s.key_token, s.key_head, type)};
     *v = {const_cast<void*>(value), s.value_token, s.value_head, row_alignment(value, s.value_token, s.value_head, type)};
-    return "";
+    return nullptr;
 }
 
 }  // namespace
@@ -3830,9 +3834,9 @@ int eos_b200_kv_cache_append_device(EosB200KvCache* c, const void* d_key, const 
     if (c == nullptr) return fail(err, "kv_cache_append: null cache");
     KvSeqs seqs{};
     KvRows k{}, v{};
-    const std::string why = kv_rows_check(c, d_key, d_value, type, tokens, strides, batch, d_page_table, max_pages, d_starts,
-                                          d_cu_tokens, &seqs, &k, &v);
-    if (!why.empty()) return fail(err, "kv_cache_append: " + why);
+    const char* why = kv_rows_check(c, d_key, d_value, type, tokens, strides, batch, d_page_table, max_pages, d_starts,
+                                    d_cu_tokens, &seqs, &k, &v);
+    if (why != nullptr) return fail(err, std::string("kv_cache_append: ") + why);
     if (stats != nullptr) std::memset(stats, 0, sizeof(*stats));
     if (tokens == 0 || batch == 0) return EOS_B200_OK;
     CUDA_TRY(cudaSetDevice(c->rt->device));
@@ -3849,9 +3853,9 @@ int eos_b200_kv_cache_read_device(EosB200KvCache* c, void* d_key, void* d_value,
     if (c == nullptr) return fail(err, "kv_cache_read: null cache");
     KvSeqs seqs{};
     KvRows k{}, v{};
-    const std::string why = kv_rows_check(c, d_key, d_value, type, tokens, strides, batch, d_page_table, max_pages, d_starts,
-                                          d_cu_tokens, &seqs, &k, &v);
-    if (!why.empty()) return fail(err, "kv_cache_read: " + why);
+    const char* why = kv_rows_check(c, d_key, d_value, type, tokens, strides, batch, d_page_table, max_pages, d_starts,
+                                    d_cu_tokens, &seqs, &k, &v);
+    if (why != nullptr) return fail(err, std::string("kv_cache_read: ") + why);
     if (stats != nullptr) std::memset(stats, 0, sizeof(*stats));
     if (tokens == 0 || batch == 0) return EOS_B200_OK;
     CUDA_TRY(cudaSetDevice(c->rt->device));
@@ -3883,6 +3887,8 @@ int eos_b200_kv_cache_attend_device(EosB200KvCache* c, const void* d_query, int 
     if (max_pages <= 0) return fail(err, "kv_cache_attend: max_pages must be positive");
     if (reinterpret_cast<uintptr_t>(d_query) % type_bytes(type) != 0) return fail(err, "kv_cache_attend: query is not aligned to its element type");
     if (reinterpret_cast<uintptr_t>(d_out) % 16 != 0) return fail(err, "kv_cache_attend: out must be 16-byte aligned");
+    if (!word_aligned(d_lse) || !word_aligned(d_page_table) || !word_aligned(d_lengths))
+        return fail(err, "kv_cache_attend: lse, page table or lengths are not 4-byte aligned");
     KvSeqs seqs = {d_page_table, max_pages, batch, nullptr, nullptr, d_lengths};
     KvAttend a{};
     a.query = d_query;

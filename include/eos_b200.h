@@ -584,7 +584,7 @@ typedef struct {
  * twice among the pages written), and calls that run at the same time must write different pages (16 tokens share words);
  * other positions may be read by other calls meanwhile.
  * Enqueued on `stream` (NULL: the runtime's stream) without synchronising, allocation-free, and may be captured into a
- * graph; all arrays are device memory and are read when the kernel runs.  Sequences whose entries are out of range
+ * graph; all arrays are device memory, aligned to their elements, and are read when the kernel runs.  Sequences whose entries are out of range
  * (negative, behind the page table, a page id outside the cache) are skipped as far as they are, and
  * eos_b200_kv_cache_sync reports it. */
 EOS_B200_API int eos_b200_kv_cache_append_device(EosB200KvCache* cache, const void* d_key, const void* d_value, int type,

@@ -268,7 +268,7 @@ def test_keys_of_any_size_under_queries_of_the_opposite(fmt, power):
 
 
 def test_refusals_at_the_limits():
-    """Arguments that no kernel could use: a scale that leaves fp32's range in base 2."""
+    """Arguments that no kernel could use: a scale that leaves fp32's range in base 2, arrays of words that are not aligned."""
     import eos_b200
     rt = eos_b200.Runtime(0)
     c = eos_b200.KvCache(rt, 4, 16, 2, 64, "mx8")
@@ -278,5 +278,13 @@ def test_refusals_at_the_limits():
     for scale in (2.4e38, -3.4e38):
         with pytest.raises(eos_b200.EosB200Error, match="scale"):
             c.attend_device(**{**ok, "scale": scale})
+    for bad in (dict(d_lse=p + 2046), dict(d_page_table=t + 1), dict(d_lengths=t + 2)):
+        with pytest.raises(eos_b200.EosB200Error, match="aligned"):
+            c.attend_device(**{**ok, **bad})
+    rows = dict(d_key=p, d_value=p + 1024, type="f32", tokens=1, batch=1, d_page_table=t, max_pages=1, d_starts=t)
+    for call in (c.append_device, c.read_device):
+        for bad in (dict(d_page_table=t + 2), dict(d_starts=t + 1), dict(d_cu_tokens=t + 3)):
+            with pytest.raises(eos_b200.EosB200Error, match="aligned"):
+                call(**{**rows, **bad})
     c.attend_device(**{**ok, "scale": 2.3e38, "stream": torch.cuda.current_stream().cuda_stream})
     c.sync(torch.cuda.current_stream().cuda_stream)
