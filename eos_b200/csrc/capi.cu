@@ -3714,6 +3714,7 @@ int eos_b200_token_pool_encode(EosB200TokenPool* tp, const int32_t* h_tokens, co
 // ------------------------------------------------------------------------------------------------
 struct EosB200KvCache {
     EosB200Runtime* rt = nullptr;
+    int device = 0;             // (destroying the cache does not look at the runtime)
     KvPool pool{};
     KvWork work{};
     std::mutex lock;            // of `reported`
@@ -3792,6 +3793,7 @@ int eos_b200_kv_cache_create(EosB200Runtime* rt, int64_t pages, int page_size, i
     EosB200KvCache* c = new (std::nothrow) EosB200KvCache();
     if (c == nullptr) return fail(err, "kv_cache_create: out of host memory");
     c->rt = rt;
+    c->device = rt->device;
     // one allocation: the pages, then the workspace (its counts first), each part 256-byte aligned
     const auto part = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
     const size_t ctas = (size_t)rt->sm_count, pool_bytes = part((size_t)(pages * page_bytes)), count_bytes = part((3 * ctas + kKvErrors) * sizeof(int)),
@@ -3818,7 +3820,7 @@ int eos_b200_kv_cache_create(EosB200Runtime* rt, int64_t pages, int page_size, i
 
 void eos_b200_kv_cache_destroy(EosB200KvCache* c) {
     if (c == nullptr) return;
-    cudaSetDevice(c->rt->device);
+    cudaSetDevice(c->device);
     dev_free(c->pool.base);
     delete c;
 }

@@ -288,3 +288,28 @@ def test_refusals_at_the_limits():
                 call(**{**rows, **bad})
     c.attend_device(**{**ok, "scale": 2.3e38, "stream": torch.cuda.current_stream().cuda_stream})
     c.sync(torch.cuda.current_stream().cuda_stream)
+
+
+def test_a_cache_may_outlive_its_runtime():
+    """Where both are garbage of one cycle the runtime may go first; the cache then frees what it holds without looking at it,
+    and leaves no error behind for the next call."""
+    import ctypes
+
+    import eos_b200
+    from eos_b200 import _lib
+    dim, n = 64, 40
+    k, v = tensors(n, 1, dim, "f16", 101)
+    for _ in range(4):
+        s = Sequences("mx8", dim, 1, 16, [n])
+        s.append(k, v, [0], [n])
+        s.sync()
+        _lib.lib().eos_b200_runtime_destroy(s.rt.handle)
+        s.rt.handle = ctypes.c_void_p()
+        other = Sequences("mx4", dim, 1, 16, [n])            # (takes the freed memory)
+        junk = [eos_b200.Runtime(0) for _ in range(3)]
+        for rt in junk:
+            rt.close()
+        s.cache.close()
+        other.append(k, v, [0], [n])
+        other.sync()
+        assert same(other.read([0], [n])[0], stored(k, "mx4"))
