@@ -3754,7 +3754,7 @@ const char* kv_rows_check(const EosB200KvCache* c, const void* key, const void* 
         return "key or value is not aligned to its element type";
     if (!word_aligned(table) || !word_aligned(starts) || !word_aligned(cu)) return "page table, starts or row offsets are not 4-byte aligned";
     // blocks of eight warps, one (record, head) each
-    if ((tokens / kKvRecord + 2 * (int64_t)batch + 1) * c->pool.heads / 8 >= 0x7fffffffLL) return "too many tokens x heads in one call";
+    if ((tokens / kKvRecord + 2 * (int64_t)batch + 1) * c->pool.heads / 8 >= 0x7ffffffeLL) return "too many tokens x heads in one call";
     *seqs = {table, max_pages, batch, starts, cu, nullptr};
     *k = {const_cast<void*>(key), s.key_token, s.key_head, row_alignment(key, s.key_token, s.key_head, type)};
     *v = {const_cast<void*>(value), s.value_token, s.value_head, row_alignment(value, s.value_token, s.value_head, type)};

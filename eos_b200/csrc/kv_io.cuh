@@ -72,6 +72,17 @@ __device__ __forceinline__ KvUnit kv_unit(const KvSeqs& s, int64_t tokens, int64
     return r;
 }
 
+// The row offsets of a call, looked over by one block (the last; the work's own would not meet all that is wrong, for where offsets
+// descend the search above passes sequences by): ascending from 0 or more to `tokens` or less.
+__device__ __forceinline__ void kv_check_offsets(const KvSeqs& s, int64_t tokens, int* errors) {
+    bool bad = false;
+    for (int b = threadIdx.x; b < s.batch; b += blockDim.x) {
+        const int from = __ldg(s.cu + b), to = __ldg(s.cu + b + 1);
+        bad |= from < 0 || to < from || to > tokens;
+    }
+    if (__syncthreads_or(bad) && threadIdx.x == 0) kv_report(errors, kStatusBadSequence);
+}
+
 // ---------------------------------------------------------------- elements
 // N (4 or 8) consecutive elements of a call's tensor, as they lie in memory
 template <int TYPE, int N>
@@ -184,7 +195,10 @@ __global__ void __launch_bounds__(kKvIoWarps * 32, kv_append_blocks(FMT, NB, TYP
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t w = (int64_t)blockIdx.x * kKvIoWarps + (threadIdx.x >> 5);
     const int64_t u = w / pool.heads;
-    if (u >= units) return;
+    if (u >= units) {   // (all warps of the last block)
+        if (seqs.cu != nullptr && blockIdx.x == gridDim.x - 1) kv_check_offsets(seqs, tokens, errors);
+        return;
+    }
     const int h = (int)(w - u * pool.heads);
     const KvUnit un = kv_unit(seqs, tokens, u, lane, errors);
     if (!un.ok) return;
@@ -488,7 +502,10 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t w = (int64_t)blockIdx.x * kKvIoWarps + (threadIdx.x >> 5);
     const int64_t u = w / pool.heads;
-    if (u >= units) return;
+    if (u >= units) {   // (all warps of the last block)
+        if (seqs.cu != nullptr && blockIdx.x == gridDim.x - 1) kv_check_offsets(seqs, tokens, errors);
+        return;
+    }
     const int h = (int)(w - u * pool.heads);
     const KvUnit un = kv_unit(seqs, tokens, u, lane, errors);
     if (!un.ok) return;
@@ -584,7 +601,7 @@ template <bool READ, int FMT, int NB, int TYPE>
 void kv_io_launch(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int64_t tokens, int* errors,
                   cudaStream_t stream) {
     const int64_t units = kv_units(seqs, tokens);
-    const unsigned blocks = (unsigned)((units * pool.heads + kKvIoWarps - 1) / kKvIoWarps);
+    const unsigned blocks = (unsigned)((units * pool.heads + kKvIoWarps - 1) / kKvIoWarps) + (seqs.cu != nullptr ? 1u : 0u);   // (kv_check_offsets)
     if constexpr (READ) kv_read_kernel<FMT, NB, TYPE><<<blocks, kKvIoWarps * 32, 0, stream>>>(pool, seqs, key, value, tokens, units, errors);
     else kv_append_kernel<FMT, NB, TYPE><<<blocks, kKvIoWarps * 32, 0, stream>>>(pool, seqs, key, value, tokens, units, errors);
 }

@@ -585,8 +585,8 @@ typedef struct {
  * other positions may be read by other calls meanwhile.
  * Enqueued on `stream` (NULL: the runtime's stream) without synchronising, allocation-free, and may be captured into a
  * graph; all arrays are device memory, aligned to their elements, and are read when the kernel runs.  Sequences whose entries are out of range
- * (negative, behind the page table, a page id outside the cache) are skipped as far as they are, and
- * eos_b200_kv_cache_sync reports it. */
+ * (negative, behind the page table, a page id outside the cache, row offsets that descend or pass `tokens`) are skipped as far
+ * as they are -- beside descending offsets other sequences' rows may be, too -- and eos_b200_kv_cache_sync reports it. */
 EOS_B200_API int eos_b200_kv_cache_append_device(EosB200KvCache* cache, const void* d_key, const void* d_value, int type,
                                                  int64_t tokens, const EosB200KvStrides* strides, int batch,
                                                  const int32_t* d_page_table, int max_pages, const int32_t* d_starts,

@@ -313,3 +313,45 @@ def test_a_cache_may_outlive_its_runtime():
         other.append(k, v, [0], [n])
         other.sync()
         assert same(other.read([0], [n])[0], stored(k, "mx4"))
+
+
+@pytest.mark.parametrize("counts", [[100, -80, 40], [64, -64, 64], [200, -300, 150, -50], [10, -1, 0], [0, 0, 120, -120, 0, 0]])
+def test_row_offsets_that_run_backwards_are_reported(counts):
+    """Rows between offsets that descend belong to no one sequence; whichever of them are written or read, the call is reported,
+    and what other sequences hold stays."""
+    import eos_b200
+    dim, heads, n = 32, 2, 208
+    batch = len(counts)
+    s = Sequences("mx8", dim, heads, 16, [n] * batch)
+    k, v = tensors(n, heads, dim, "f16", 98)
+    s.append(k, v, [0] * batch, counts)
+    with pytest.raises(eos_b200.EosB200DeviceStatusError, match="row offset"):
+        s.sync()
+    cu = [sum(counts[:i]) for i in range(batch + 1)]
+    rows = s._ints(cu), s._ints([0] * batch)
+    rk, rv = torch.full_like(k, 9.0), torch.full_like(v, 9.0)
+    s.cache.read_device(rk.data_ptr(), rv.data_ptr(), "f16", n, batch, s.table.data_ptr(), s.max_pages, rows[1].data_ptr(),
+                        rows[0].data_ptr(), stream=torch.cuda.current_stream().cuda_stream)
+    with pytest.raises(eos_b200.EosB200DeviceStatusError, match="row offset"):
+        s.sync()
+    s.sync()
+    s.append(k[:batch].contiguous(), v[:batch].contiguous(), [n - 1] * batch)     # (and the cache works on)
+    s.sync()
+
+
+def test_many_row_offsets():
+    """More sequences than a block has threads, one of them at the end."""
+    import eos_b200
+    batch, n = 2000, 3
+    s = Sequences("f16", 32, 1, 16, [n] * batch)
+    k, v = tensors(n * batch, 1, 32, "f16", 99)
+    s.append(k, v, [0] * batch, [n] * batch)
+    s.sync()
+    rk, rv = s.read([0] * batch, [n] * batch, "f16")
+    assert same(rk, k) and same(rv, v)
+    s.append(k, v, [0] * batch, [n] * (batch - 1) + [-1])
+    with pytest.raises(eos_b200.EosB200DeviceStatusError, match="row offset"):
+        s.sync()
+    s.append(k, v, [0] * batch, [n] * (batch - 1) + [n + 1])
+    with pytest.raises(eos_b200.EosB200DeviceStatusError, match="row offset"):
+        s.sync()
