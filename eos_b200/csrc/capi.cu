@@ -3796,14 +3796,14 @@ int eos_b200_kv_cache_create(EosB200Runtime* rt, int64_t pages, int page_size, i
     c->device = rt->device;
     // one allocation: the pages, then the workspace (its counts first), each part 256-byte aligned
     const auto part = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
-    const size_t ctas = (size_t)rt->sm_count, pool_bytes = part((size_t)(pages * page_bytes)), count_bytes = part((3 * ctas + kKvErrors) * sizeof(int)),
+    const size_t ctas = (size_t)rt->sm_count, pool_bytes = part((size_t)(pages * page_bytes)), count_bytes = part((3 * ctas + 1) * sizeof(uint64_t) + kKvErrors * sizeof(int)),
                  slot_bytes = part(ctas * kv_slot_floats(head_dim) * sizeof(float));
     cudaError_t e = dev_alloc(&p.base, pool_bytes + count_bytes + slot_bytes + ctas * 2 * kKvMaxRows * (head_dim + 3) * sizeof(float));
     c->pool = p;
     c->work.ctas = rt->sm_count;
     if (e == cudaSuccess) {
-        c->work.count = reinterpret_cast<int*>(p.base + pool_bytes);
-        c->work.errors = c->work.count + 3 * ctas;
+        c->work.count = reinterpret_cast<uint64_t*>(p.base + pool_bytes);
+        c->work.errors = reinterpret_cast<int*>(c->work.count + 3 * ctas + 1);
         c->work.slots = reinterpret_cast<float*>(p.base + pool_bytes + count_bytes);
         c->work.partial = reinterpret_cast<float*>(p.base + pool_bytes + count_bytes + slot_bytes);
         e = cudaMemsetAsync(p.base, 0, pool_bytes + count_bytes, rt->stream);

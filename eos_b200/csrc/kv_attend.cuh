@@ -556,6 +556,11 @@ struct KvQuotient {
 // its range altogether; at most its first and its last unit are partial.  Partial results are joined in shared memory by the
 // CTA, and what is still partial then (at most two units a CTA) through the workspace by whichever of the unit's CTAs is done
 // last.  All joins run in a fixed order: same bits every time.  (A second kernel for that join cost 4 to 7 us a call.)
+// The counts behind "last" are never set back: they carry the number of the call, and a count that holds a smaller one is raised
+// to it first.  So whatever calls that overlapped against the rules have left there, the next one finds its counts at zero.  The
+// number: every CTA of a call reads how many CTAs have run before its own, over all calls, and then adds itself; divided by the CTAs
+// of a call that is the same for all of them.  (0 to 0.3 us a call; counts zeroed by
+// the CTA that is done with them last 0.6 to 1.2, calls numbered by what the additions return 0.3 to 1.3.)
 // ------------------------------------------------------------------------------------------------
 // (Groups of 12: one sequence of 2000 tokens and 8 heads, 16 CTAs a unit, 14.4 us instead of 12.9, of 131071 56.5 instead of
 // 55.3.  Ranges of at least 16 records: 1000 tokens 14.6 us instead of 12.2.)
@@ -607,6 +612,8 @@ __device__ __forceinline__ int64_t kv_div(int64_t a, int64_t b) {   // not negat
     return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : kv_div64(a, b);
 }
 
+constexpr unsigned long long kKvCall = 1024;   // more than a call ever counts to
+
 struct KvSplit {
     int chunks;                     // chunks of query heads per key head
     int row_warps;                  // warps that share a record, each with its own rows
@@ -615,7 +622,8 @@ struct KvSplit {
     KvDiv by_ctas, by_per_seq, by_teams, by_page, by_chunks;   // (by_page: records of a page)
     float* slots;                   // [ctas][kv_slot_floats]: partial results of the warps' first units
     float* partial;                 // [ctas][2][rows][dim + 3]: of the CTAs, numerators of all rows, then (m, d, l) of each
-    int* count;                     // [ctas][2], [ctas]: parts of a group, groups of a unit that are done; zero between calls
+    unsigned long long* count;      // [ctas][2], [ctas]: parts of a group, groups of a unit that are done, under the call's number
+                                    // times kKvCall; [1]: CTAs that have run
 };
 
 // positions of sequence b that are attended to: [lo, hi)
@@ -696,6 +704,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
     __shared__ int64_t s_from[2 * kMaxWarps];                    // first record, among all, of the slot's unit, and
     __shared__ int s_long[2 * kMaxWarps];                        // its records
     __shared__ int s_turn[2];                                 // whether this CTA joins its first / last unit's parts
+    __shared__ __align__(8) unsigned long long s_call;        // CTAs that have run before this one; the call's number times kKvCall
     __shared__ __align__(8) uint64_t s_full[kMaxWarps][kMaxStages], s_empty[kMaxWarps][kMaxStages];
     __shared__ uint8_t s_ok[kMaxWarps][kMaxStages];              // whether the record could be fetched
     __shared__ int s_abort, s_drain[kMaxWarps];
@@ -714,6 +723,10 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
         return last ? reinterpret_cast<float*>(smem + of * split.ring_bytes) + (w - of * split.row_warps) * Shape::kPartial
                     : split.slots + (int64_t)blockIdx.x * kv_slot_floats(D) + w * Shape::kPartial;
     };
+
+    const bool numbers = tid == threads - 1;   // the thread that sees to the call's number, waited for behind the records
+    if (numbers)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(&s_call)), "l"(split.count + 3 * gridDim.x) : "memory");
 
     // ---- records of all sequences, scanned by the CTA
     const int per = (seqs.batch + threads - 1) / threads;
@@ -972,33 +985,54 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
         const int e_first = starts ? __ffs(starts) - 1 : 0, e_last = starts ? 31 - __clz(starts) : 0;
         const uint32_t m_first = starts ? run_from(e_first) : 0u, m_last = starts ? run_from(e_last) : 0u;
         const bool open_first = m_first && !(begun & m_first), open_last = m_last && (begun & m_last) && !(ended & m_last);
-        int owner[2], parts[2];         // the CTA that such a unit begins in, and how many hold parts of it
+        const bool open = open_first || open_last;
+        int owner[2] = {0, 0}, parts[2] = {1, 1};   // the CTA that such a unit begins in, and how many hold parts of it
+        if (open) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int at_slot = slot_of(i ? e_last : e_first, 0);
+                owner[i] = (int)kv_div(s_from[at_slot], part);
+                parts[i] = (int)kv_div(s_from[at_slot] + s_long[at_slot] - 1, part) - owner[i] + 1;
+            }
+        }
         bool turn[2];                   // whether this CTA joins them
-#pragma unroll 1
-        for (int phase_no = 0; phase_no < 3; ++phase_no) {
-            if (phase_no == 1) {
-                if (!open_first && !open_last) break;
+        // the count of a unit's group of CTAs (phase 1) or of its groups (2), and how far it goes
+        auto count_of = [&](int i, int phase_no, int& of) {
+            const int group = ((int)blockIdx.x - owner[i]) / kKvGroup, lead = owner[i] + group * kKvGroup;
+            of = phase_no == 1 ? min(kKvGroup, parts[i] - group * kKvGroup) : (parts[i] + kKvGroup - 1) / kKvGroup;
+            return phase_no == 1 ? split.count + 2 * lead + (lead == owner[i] ? 1 : 0) : split.count + 2 * gridDim.x + owner[i];
+        };
+        if (numbers) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            asm volatile("red.relaxed.gpu.global.add.u64 [%0], 1;" ::"l"(split.count + 3 * gridDim.x) : "memory");
+            if (open) {   // (the counts that this CTA may add to, raised while the warps' results are joined)
+                s_call = (unsigned long long)split.by_ctas((int64_t)s_call) * kKvCall;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int at_slot = slot_of(i ? e_last : e_first, 0);
-                    owner[i] = (int)kv_div(s_from[at_slot], part);
-                    parts[i] = (int)kv_div(s_from[at_slot] + s_long[at_slot] - 1, part) - owner[i] + 1;
+                    if (!(i ? open_last : open_first)) continue;
+                    for (int n = 1; n <= (parts[i] > kKvGroup ? 2 : 1); ++n) {
+                        int of;
+                        asm volatile("red.relaxed.gpu.global.max.u64 [%0], %1;" ::"l"(count_of(i, n, of)), "l"(s_call) : "memory");
+                    }
                 }
             }
+        }
+#pragma unroll 1
+        for (int phase_no = 0; phase_no < 3; ++phase_no) {
+            if (phase_no == 1 && !open) break;
             if (phase_no > 0) {
+                const bool first = phase_no == 1 ? open_first : turn[0] && parts[0] > kKvGroup,
+                           second = phase_no == 1 ? open_last : turn[1] && parts[1] > kKvGroup;   // what there is to count
                 __syncthreads();   // the CTA's parts are written
                 if (tid < 64 && lane == 0) {   // warp 0 for the first unit, warp 1 for the last
                     const int i = tid >> 5;
-                    const int group = ((int)blockIdx.x - owner[i]) / kKvGroup, groups = (parts[i] + kKvGroup - 1) / kKvGroup;
-                    const int lead = owner[i] + group * kKvGroup;
-                    int* count = phase_no == 1 ? split.count + 2 * lead + (lead == owner[i] ? 1 : 0) : split.count + 2 * gridDim.x + owner[i];
-                    const int of = phase_no == 1 ? min(kKvGroup, parts[i] - group * kKvGroup) : groups;
-                    bool mine_now = false;
-                    if (phase_no == 1 ? (i ? open_last : open_first) : (s_turn[i] && groups > 1)) {
-                        int done;
-                        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(done) : "l"(count) : "memory");
-                        mine_now = done == of - 1;
-                        if (mine_now) *count = 0;   // for the next call
+                    int of;
+                    const unsigned long long* count = count_of(i, phase_no, of);
+                    bool mine_now = i ? second : first;
+                    if (mine_now) {
+                        unsigned long long done;
+                        asm volatile("atom.acq_rel.gpu.global.add.u64 %0, [%1], 1;" : "=l"(done) : "l"(count) : "memory");
+                        mine_now = done == s_call + of - 1;
                     }
                     s_turn[i] = mine_now;
                 }
@@ -1159,7 +1193,7 @@ struct KvAttendInstance {
         split.by_teams = KvDiv(split.teams);
         split.by_page = KvDiv(pool.records_per_page);
         split.by_chunks = KvDiv(split.chunks);
-        split.count = work.count;
+        split.count = reinterpret_cast<unsigned long long*>(work.count);
         split.slots = work.slots;
         split.partial = work.partial;
         kv_attend_kernel<FMT, NB, RT, HALVES><<<work.ctas, 32 * warps, split.teams * split.ring_bytes, stream>>>(pool, seqs, a, split, errors);

@@ -107,7 +107,7 @@ struct KvWork {
     int ctas;               // one per SM
     float* slots;           // [ctas][kv_slot_floats(dim)]: partial results of the CTAs' warps
     float* partial;         // [ctas][2][kKvMaxRows][dim + 3]: of the CTAs
-    int* count;             // [3 ctas], zero between calls
+    uint64_t* count;        // [3 ctas], and how many CTAs have run (see kv_attend.cuh); zero at first, never set back
     int* errors;            // [kKvErrors] what append, read and attend met; the counts only grow, the host remembers what it has reported
 };
 constexpr int kKvErrors = 3;           // pipeline timeout, bad page, bad sequence: kStatusPipelineTimeout and the two codes behind it

@@ -609,8 +609,8 @@ EOS_B200_API int eos_b200_kv_cache_read_device(EosB200KvCache* cache, void* d_ke
  * not finite; other rows are not touched by it.  scale q, the sums q . k and the scores scale q . k have to stay within fp32's range
  * (|scale| itself: at most 2.3e38).
  * Enqueued, allocation-free and capturable as above; calls of one cache share its workspace and must be ordered (one
- * stream, or events between streams; replays of graphs that hold them likewise): overlapping ones give wrong results, and may
- * go on giving them.  Two caches are independent. */
+ * stream, or events between streams; replays of graphs that hold them likewise): overlapping ones give wrong results (and calls
+ * behind them right ones).  Two caches are independent. */
 EOS_B200_API int eos_b200_kv_cache_attend_device(EosB200KvCache* cache, const void* d_query, int type, int q_heads,
                                                  int64_t query_seq_stride, int64_t query_head_stride, int batch,
                                                  const int32_t* d_page_table, int max_pages, const int32_t* d_lengths, float scale,

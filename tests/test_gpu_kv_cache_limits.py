@@ -355,3 +355,29 @@ def test_many_row_offsets():
     s.append(k, v, [0] * batch, [n] * (batch - 1) + [n + 1])
     with pytest.raises(eos_b200.EosB200DeviceStatusError, match="row offset"):
         s.sync()
+
+
+def test_attends_that_overlapped_leave_nothing_behind():
+    """Attends of one cache that no order keeps apart share its workspace, and their results are not to be used.  Those of
+    calls behind them, in order again, are right: every call leaves the workspace's counts as it wants to find them."""
+    dim, heads, group = 64, 2, 4
+    shapes = [([20000, 3000], 0), ([20000, 3000], 700), ([1, 3000], 0), ([12000, 0], 0)]
+    s = Sequences("mx8", dim, heads, 64, [20000, 3000])
+    k, v = tensors(23000, heads, dim, "f16", 105)
+    s.append(k, v, [0, 0], [20000, 3000])
+    q = tensors(2, heads * group, dim, "f16", 106)[0]
+    want = [s.attend(q, n, 0.125, window) for n, window in shapes]
+    lengths = [s._ints(n) for n, _ in shapes]
+    streams = [torch.cuda.Stream() for _ in shapes]
+    outs = [torch.empty_like(q) for _ in shapes]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for _ in range(20):
+            for (_, window), n, out, stream in zip(shapes, lengths, outs, streams):
+                s.cache.attend_device(q.data_ptr(), "f16", heads * group, 2, s.table.data_ptr(), s.max_pages, n.data_ptr(),
+                                      out.data_ptr(), 0.125, window, stream=stream.cuda_stream)
+        torch.cuda.synchronize()
+        for (n, window), (out, lse) in zip(shapes, want):
+            again, lse2 = s.attend(q, n, 0.125, window)
+            assert same(again, out) and same(lse2, lse)
+    s.sync()
