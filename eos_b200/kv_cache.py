@@ -6,6 +6,7 @@ All tensors are device memory, given by address; calls enqueue on a stream and r
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from typing import Optional, Tuple, Union
 
 from . import _lib
@@ -30,13 +31,31 @@ def _stream(stream: Optional[int]) -> Optional[int]:
     return 1 if stream == 0 else stream
 
 
+class _Results(threading.local):
+    """Where a thread's calls leave launches and error: made once, which a call of a few microseconds notices."""
+
+    def __init__(self):
+        self.stats, self.err = Stats(), C.c_char_p()
+        self.refs = C.byref(self.stats), C.byref(self.err)
+
+    def done(self, rc: int) -> int:
+        if rc:
+            err, self.err = self.err, C.c_char_p()
+            self.refs = C.byref(self.stats), C.byref(self.err)
+            _lib.check(rc, err)
+        return self.stats.kernel_launches
+
+
 class KvCache:
     """`pages` pages of `page_size` tokens (a multiple of 16) x `kv_heads` heads of `head_dim` elements (32, 64, 96, 128,
     192 or 256), keys and values, on the runtime's device.  The caller hands pages out: row b of a page table
     [batch, max_pages] int32 lists the pages of sequence b in order.
 
     format: "f16" / "bf16" hold the rounded values, "mx8" e4m3 and "mx4" e2m1 codes with one power-of-two scale for every 32
-    elements of a head's vector (the smallest that saturates nothing)."""
+    elements of a head's vector (the smallest that saturates nothing).
+
+    Several threads may call one cache; what their calls enqueue is ordered by streams: attends of one cache one after the other,
+    appends that overlap on different pages."""
 
     def __init__(self, rt: Runtime, pages: int, page_size: int, kv_heads: int, head_dim: int, format: str = "mx8"):
         if format not in FORMATS:
@@ -47,19 +66,10 @@ class KvCache:
         _lib.call("eos_b200_kv_cache_create", rt.handle, int(pages), int(page_size), int(kv_heads), int(head_dim),
                   FORMATS[format], C.byref(self.handle))
         rt._adopt(self)
-        # one call in flight per handle: the result structures are made once, which a call of a few microseconds notices
         lib = _lib.lib()
         self._append, self._read = lib.eos_b200_kv_cache_append_device, lib.eos_b200_kv_cache_read_device
         self._attend = lib.eos_b200_kv_cache_attend_device
-        self._stats, self._err = Stats(), C.c_char_p()
-        self._stats_ref, self._err_ref = C.byref(self._stats), C.byref(self._err)
-
-    def _done(self, rc: int) -> int:
-        if rc:
-            err, self._err = self._err, C.c_char_p()
-            self._err_ref = C.byref(self._err)
-            _lib.check(rc, err)
-        return self._stats.kernel_launches
+        self._results = _Results()
 
     @property
     def page_bytes(self) -> int:
@@ -72,18 +82,20 @@ class KvCache:
         """Writes new tokens: d_key, d_value [tokens, kv_heads, head_dim]; sequence b owns the rows d_cu_tokens[b] up to
         d_cu_tokens[b + 1] and writes them from position d_starts[b] on (None: one token per sequence).  strides: elements
         between (key tokens, key heads, value tokens, value heads).  Returns kernels launched."""
-        return self._done(self._append(self.handle, d_key, d_value, _type(type), tokens,
-                                       None if strides is None else C.byref(KvStrides(*strides)), batch, d_page_table,
-                                       max_pages, d_starts, d_cu_tokens, _stream(stream), self._stats_ref, self._err_ref))
+        r = self._results
+        return r.done(self._append(self.handle, d_key, d_value, _type(type), tokens,
+                                   None if strides is None else C.byref(KvStrides(*strides)), batch, d_page_table, max_pages,
+                                   d_starts, d_cu_tokens, _stream(stream), *r.refs))
 
     def read_device(self, d_key: int, d_value: int, type: Union[str, int], tokens: int, batch: int, d_page_table: int,
                     max_pages: int, d_starts: int, d_cu_tokens: Optional[int] = None,
                     strides: Optional[Tuple[int, int, int, int]] = None, stream: Optional[int] = None) -> int:
         """The inverse of append_device with the same arguments: d_key, d_value receive the cached values.  Rows behind
         the last sequence are left as they were."""
-        return self._done(self._read(self.handle, d_key, d_value, _type(type), tokens,
-                                     None if strides is None else C.byref(KvStrides(*strides)), batch, d_page_table, max_pages,
-                                     d_starts, d_cu_tokens, _stream(stream), self._stats_ref, self._err_ref))
+        r = self._results
+        return r.done(self._read(self.handle, d_key, d_value, _type(type), tokens,
+                                 None if strides is None else C.byref(KvStrides(*strides)), batch, d_page_table, max_pages,
+                                 d_starts, d_cu_tokens, _stream(stream), *r.refs))
 
     def attend_device(self, d_query: int, type: Union[str, int], q_heads: int, batch: int, d_page_table: int, max_pages: int,
                       d_lengths: int, d_out: int, scale: float, window: int = 0, d_lse: Optional[int] = None,
@@ -92,9 +104,9 @@ class KvCache:
         d_lengths[b] cached positions; out [batch, q_heads, head_dim] of the query's type, d_lse [batch, q_heads] fp32 the
         logarithm of the softmax denominators.  Query head i reads key head i // (q_heads // kv_heads).  query_strides:
         elements between sequences and between heads, 0: contiguous.  Returns kernels launched."""
-        return self._done(self._attend(self.handle, d_query, _type(type), q_heads, query_strides[0], query_strides[1], batch,
-                                       d_page_table, max_pages, d_lengths, scale, window, d_out, d_lse, _stream(stream),
-                                       self._stats_ref, self._err_ref))
+        r = self._results
+        return r.done(self._attend(self.handle, d_query, _type(type), q_heads, query_strides[0], query_strides[1], batch,
+                                   d_page_table, max_pages, d_lengths, scale, window, d_out, d_lse, _stream(stream), *r.refs))
 
     def sync(self, stream: Optional[int] = None) -> None:
         """Waits for the stream; raises EosB200DeviceStatusError if a kernel met a page, position or length out of range."""

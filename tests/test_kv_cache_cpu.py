@@ -215,3 +215,64 @@ def test_refusals_without_a_device():
             _lib.call(name, *args)
     assert _lib.lib().eos_b200_kv_cache_page_bytes(None) == 0
     _lib.lib().eos_b200_kv_cache_destroy(None)
+
+
+class FakeLibrary:
+    """Entry points that wait for another call in flight before they answer: with the token count as launches, or an error."""
+
+    def __init__(self):
+        import threading
+        self.both = threading.Barrier(2, timeout=20)
+        self.freed = []
+
+    def eos_b200_kv_cache_create(self, *args):
+        return 0
+
+    def eos_b200_kv_cache_destroy(self, handle):
+        pass
+
+    def eos_b200_free_cstring(self, p):
+        self.freed.append(p)
+
+    def _rows(self, handle, key, value, type_, tokens, strides, batch, *rest):
+        stats, err = (r._obj for r in rest[-2:])
+        stats.kernel_launches = tokens
+        if batch < 0:
+            err.value = b"refused %d" % tokens
+        self.both.wait()       # both have written
+        self.both.wait()
+        return 1 if batch < 0 else 0
+
+    eos_b200_kv_cache_append_device = eos_b200_kv_cache_read_device = _rows
+
+    def eos_b200_kv_cache_attend_device(self, handle, query, type_, q_heads, *rest):
+        return self._rows(handle, None, None, type_, q_heads, None, rest[2], *rest)
+
+
+def fake_cache(monkeypatch):
+    from types import SimpleNamespace
+
+    import eos_b200
+    from eos_b200 import _lib
+    fake = FakeLibrary()
+    monkeypatch.setattr(_lib, "lib", lambda: fake)
+    return eos_b200.KvCache(SimpleNamespace(handle=None, _adopt=lambda child: None), 1, 16, 1, 64), fake
+
+
+def test_calls_of_two_threads_keep_their_results_apart(monkeypatch):
+    """ctypes lets other threads run during a call: launches and errors are those of the thread's own call."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    import eos_b200
+    cache, fake = fake_cache(monkeypatch)
+    calls = [lambda n, b: cache.append_device(1, 1, "f16", n, b, 1, 1, 1), lambda n, b: cache.read_device(1, 1, "f16", n, b, 1, 1, 1),
+             lambda n, b: cache.attend_device(1, "f16", n, b, 1, 1, 1, 1, 1.0)]
+    with ThreadPoolExecutor(2) as pool:
+        for one in calls:
+            for two in calls:
+                got = [pool.submit(one, 3, 1), pool.submit(two, 5, 1)]
+                assert [g.result(30) for g in got] == [3, 5]
+                got = [pool.submit(one, 7, -1), pool.submit(two, 9, -1)]
+                errors = [g.exception(30) for g in got]
+                assert all(isinstance(e, eos_b200.EosB200Error) for e in errors) and [str(e) for e in errors] == ["refused 7", "refused 9"]
+    assert len(fake.freed) == 2 * len(calls) ** 2
