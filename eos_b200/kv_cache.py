@@ -31,6 +31,14 @@ def _stream(stream: Optional[int]) -> Optional[int]:
     return 1 if stream == 0 else stream
 
 
+def _strides(strides: Optional[Tuple[int, int, int, int]]):
+    if strides is None:
+        return None
+    if len(strides) != 4:
+        raise ValueError(f"strides are (key token, key head, value token, value head), got {strides!r}")
+    return C.byref(KvStrides(*strides))
+
+
 class _Results(threading.local):
     """Where a thread's calls leave launches and error: made once, which a call of a few microseconds notices."""
 
@@ -84,8 +92,8 @@ class KvCache:
         between (key tokens, key heads, value tokens, value heads).  Returns kernels launched."""
         r = self._results
         return r.done(self._append(self.handle, d_key, d_value, _type(type), tokens,
-                                   None if strides is None else C.byref(KvStrides(*strides)), batch, d_page_table, max_pages,
-                                   d_starts, d_cu_tokens, _stream(stream), *r.refs))
+                                   _strides(strides), batch, d_page_table, max_pages, d_starts, d_cu_tokens, _stream(stream),
+                                   *r.refs))
 
     def read_device(self, d_key: int, d_value: int, type: Union[str, int], tokens: int, batch: int, d_page_table: int,
                     max_pages: int, d_starts: int, d_cu_tokens: Optional[int] = None,
@@ -94,8 +102,8 @@ class KvCache:
         the last sequence are left as they were."""
         r = self._results
         return r.done(self._read(self.handle, d_key, d_value, _type(type), tokens,
-                                 None if strides is None else C.byref(KvStrides(*strides)), batch, d_page_table, max_pages,
-                                 d_starts, d_cu_tokens, _stream(stream), *r.refs))
+                                 _strides(strides), batch, d_page_table, max_pages, d_starts, d_cu_tokens, _stream(stream),
+                                 *r.refs))
 
     def attend_device(self, d_query: int, type: Union[str, int], q_heads: int, batch: int, d_page_table: int, max_pages: int,
                       d_lengths: int, d_out: int, scale: float, window: int = 0, d_lse: Optional[int] = None,
@@ -104,6 +112,8 @@ class KvCache:
         d_lengths[b] cached positions; out [batch, q_heads, head_dim] of the query's type, d_lse [batch, q_heads] fp32 the
         logarithm of the softmax denominators.  Query head i reads key head i // (q_heads // kv_heads).  query_strides:
         elements between sequences and between heads, 0: contiguous.  Returns kernels launched."""
+        if len(query_strides) != 2:
+            raise ValueError(f"query_strides are (sequence, head), got {query_strides!r}")
         r = self._results
         return r.done(self._attend(self.handle, d_query, _type(type), q_heads, query_strides[0], query_strides[1], batch,
                                    d_page_table, max_pages, d_lengths, scale, window, d_out, d_lse, _stream(stream), *r.refs))

@@ -276,3 +276,14 @@ def test_calls_of_two_threads_keep_their_results_apart(monkeypatch):
                 errors = [g.exception(30) for g in got]
                 assert all(isinstance(e, eos_b200.EosB200Error) for e in errors) and [str(e) for e in errors] == ["refused 7", "refused 9"]
     assert len(fake.freed) == 2 * len(calls) ** 2
+
+
+def test_strides_of_the_wrong_count_are_refused(monkeypatch):
+    cache, _ = fake_cache(monkeypatch)
+    for call in (cache.append_device, cache.read_device):
+        for strides in ((64, 64), (64, 64, 64), (64,) * 5, ()):
+            with pytest.raises(ValueError, match="strides"):
+                call(1, 1, "f16", 1, 1, 1, 1, 1, strides=strides)
+    for strides in ((64,), (64, 64, 64), ()):
+        with pytest.raises(ValueError, match="strides"):
+            cache.attend_device(1, "f16", 1, 1, 1, 1, 1, 1, 1.0, query_strides=strides)
