@@ -34,6 +34,7 @@
 #include <algorithm>
 
 #include "kv_dev.cuh"
+#include "kv_split.cuh"
 
 namespace eosb {
 
@@ -548,9 +549,9 @@ struct KvQuotient {
 };
 
 // ------------------------------------------------------------------------------------------------
-// Split of the work.  Units are (sequence, key head, chunk of query heads); the records of all units, one unit after
-// the other, are cut into equal ranges, one for each CTA and within it for each warp, wherever the cuts fall: lengths may
-// differ as they like.  (Where whole units make ranges that are hardly longer, the CTAs' cuts are between units: nothing is
+// Split of the work (its arithmetic: kv_split.cuh).  Units are (sequence, key head, chunk of query heads); the records of all
+// units, one unit after the other, are cut into equal ranges, one for each CTA and within it for each warp, wherever the cuts
+// fall: lengths may differ as they like.  (Where whole units make ranges that are hardly longer, the CTAs' cuts are between units: nothing is
 // left to join across CTAs, which takes 3 to 4 us.  96 sequences of 32 to 64 records, one unit each: 35 -> 30 us; 128 units of 7
 // to 44: 14.8 -> 11.9; 8 of 32, on 8 CTAs instead of 32: 11.2, the same.)  A warp writes what it holds of units that lie in
 // its range altogether; at most its first and its last unit are partial.  Partial results are joined in shared memory by the
@@ -559,14 +560,9 @@ struct KvQuotient {
 // The counts behind "last" are never set back: they carry the number of the call, and a count that holds a smaller one is raised
 // to it first.  So whatever calls that overlapped against the rules have left there, the next one finds its counts at zero.  The
 // number: every CTA of a call reads how many CTAs have run before its own, over all calls, and then adds itself; divided by the CTAs
-// of a call that is the same for all of them.  (0 to 0.3 us a call; counts zeroed by
-// the CTA that is done with them last 0.6 to 1.2, calls numbered by what the additions return 0.3 to 1.3.)
+// of a call that is the same for all of them.  (0 to 0.3 us a call; counts zeroed by the CTA that is done with them last 0.6 to
+// 1.2, calls numbered by what the additions return 0.3 to 1.3.)
 // ------------------------------------------------------------------------------------------------
-// (Groups of 12: one sequence of 2000 tokens and 8 heads, 16 CTAs a unit, 14.4 us instead of 12.9, of 131071 56.5 instead of
-// 55.3.  Ranges of at least 16 records: 1000 tokens 14.6 us instead of 12.2.)
-constexpr int kKvGroup = 24;        // neighbouring CTAs whose parts are joined first (at most 31 groups of it, for 744 SMs)
-constexpr int kKvMinRecords = 8;    // records of a CTA, at least
-constexpr int kKvWhole = 24;        // records more than an equal range that a CTA may take to keep its units whole
 
 // Shape of a CTA.  Each warp (or team of warps that share records) has a ring of records in shared memory, filled by
 // bulk copies: one copy a record, since a record is contiguous.  The partial result of a warp's last unit goes into its
@@ -591,26 +587,6 @@ struct KvShape {
     static_assert(kMaxWarps * kPartial <= kv_slot_floats(32 * NB) && kMaxWarps * kPartial * 4 <= kSmemMax && kSmemMax / 4 / kRecord >= 3 &&
                       kPartial * 4 % 32 == 0 && kRecord % 16 == 0, "rings, slots");
 };
-
-__device__ __noinline__ inline int64_t kv_div64(int64_t a, int64_t b) { return a / b; }
-
-// Division of a number that is not negative by a constant of the launch: below 2^31 floor(a / d) = a m >> s with
-// s = 31 + ceil(log2 d), m = ceil(2^s / d) -- the excess a (m d - 2^s) / (d 2^s) is below 2^31 / 2^s <= 1 / d.
-struct KvDiv {
-    uint32_t d, m;
-    int s;
-    KvDiv() = default;
-    explicit KvDiv(uint32_t by) : d(by), s(31) {
-        while ((1ull << (s - 31)) < by) ++s;
-        m = (uint32_t)(((s < 63 ? 1ull << s : 0) + by - 1) / by);
-    }
-    __device__ __forceinline__ int64_t operator()(int64_t a) const {
-        return a >> 31 ? kv_div64(a, d) : (int64_t)((uint64_t)(uint32_t)a * m >> s);
-    }
-};
-__device__ __forceinline__ int64_t kv_div(int64_t a, int64_t b) {   // not negative; the 32-bit division is far shorter
-    return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : kv_div64(a, b);
-}
 
 constexpr unsigned long long kKvCall = 1024;   // more than a call ever counts to
 
@@ -759,10 +735,10 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
     }
     s_before[tid] = base + upto - mine;
     total *= per_seq;
-    const int64_t part = max(split.by_ctas(total + gridDim.x - 1), (int64_t)kKvMinRecords);
+    const int64_t part = kv_part(split.by_ctas, total);
     // Whole units, as many for each CTA, where no range gets much longer by it
     const int64_t units = (int64_t)seqs.batch * per_seq, whole = split.by_ctas(units + gridDim.x - 1);
-    const bool cut = __syncthreads_or(per > 1 || whole * mine > part + kKvWhole);
+    const bool cut = __syncthreads_or(per > 1 || !kv_keep_whole(whole, mine, part));
     auto range_begin = [&](int64_t cta) -> int64_t {
         if (cut) return min(cta * part, total);
         const int64_t u = cta * whole;
@@ -773,10 +749,10 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
         return s_before[b] * per_seq + (u - (int64_t)b * per_seq) * kv_records(lo, hi);
     };
     const int64_t c0 = range_begin(blockIdx.x), c1 = range_begin((int64_t)blockIdx.x + 1);
-    const int64_t tpart = split.by_teams(c1 - c0 + teams - 1);
-    const int64_t t0 = min(c0 + team * tpart, c1);
-    int left = (int)min(min(t0 + tpart, c1) - t0, (int64_t)0x7fffffff);   // records of the team that are not yet done with
-    if (tpart > 0x7fffffff && tid == 0) kv_report(errors, kStatusBadSequence);   // (2^31 records a warp: lengths gone wrong)
+    const KvRange range = kv_team_range(split.by_teams, c0, c1, team);
+    const int64_t t0 = range.begin;
+    int left = (int)min(range.end - t0, (int64_t)0x7fffffff);   // records of the team that are not yet done with
+    if (range.part > 0x7fffffff && tid == 0) kv_report(errors, kStatusBadSequence);   // (2^31 records a warp: lengths gone wrong)
 
     if (left > 0) {
         KvWalk at;
@@ -942,7 +918,7 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
                 if (lane == 0) {
                     s_unit[2 * warp + which] = (int64_t)at.b << 32 | at.hu;
                     s_ends[2 * warp + which] = (begins ? 1 : 0) | (ends ? 2 : 0) | (last ? 4 : 0);
-                    s_from[2 * warp + which] = min(t0 + tpart, c1) - left - at.r;
+                    s_from[2 * warp + which] = range.end - left - at.r;
                     s_long[2 * warp + which] = at.n;
                 }
             }
@@ -986,22 +962,16 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
         const uint32_t m_first = starts ? run_from(e_first) : 0u, m_last = starts ? run_from(e_last) : 0u;
         const bool open_first = m_first && !(begun & m_first), open_last = m_last && (begun & m_last) && !(ended & m_last);
         const bool open = open_first || open_last;
-        int owner[2] = {0, 0}, parts[2] = {1, 1};   // the CTA that such a unit begins in, and how many hold parts of it
+        KvHolders holders[2] = {};      // the CTAs that hold parts of such a unit
         if (open) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int at_slot = slot_of(i ? e_last : e_first, 0);
-                owner[i] = (int)kv_div(s_from[at_slot], part);
-                parts[i] = (int)kv_div(s_from[at_slot] + s_long[at_slot] - 1, part) - owner[i] + 1;
+                holders[i] = kv_holders(s_from[at_slot], s_long[at_slot], part);
             }
         }
         bool turn[2];                   // whether this CTA joins them
-        // the count of a unit's group of CTAs (phase 1) or of its groups (2), and how far it goes
-        auto count_of = [&](int i, int phase_no, int& of) {
-            const int group = ((int)blockIdx.x - owner[i]) / kKvGroup, lead = owner[i] + group * kKvGroup;
-            of = phase_no == 1 ? min(kKvGroup, parts[i] - group * kKvGroup) : (parts[i] + kKvGroup - 1) / kKvGroup;
-            return phase_no == 1 ? split.count + 2 * lead + (lead == owner[i] ? 1 : 0) : split.count + 2 * gridDim.x + owner[i];
-        };
+        auto join_of = [&](int i, int phase_no) { return kv_join(holders[i], blockIdx.x, phase_no, gridDim.x); };
         if (numbers) {
             asm volatile("cp.async.wait_all;" ::: "memory");
             asm volatile("red.relaxed.gpu.global.add.u64 [%0], 1;" ::"l"(split.count + 3 * gridDim.x) : "memory");
@@ -1010,10 +980,8 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     if (!(i ? open_last : open_first)) continue;
-                    for (int n = 1; n <= (parts[i] > kKvGroup ? 2 : 1); ++n) {
-                        int of;
-                        asm volatile("red.relaxed.gpu.global.max.u64 [%0], %1;" ::"l"(count_of(i, n, of)), "l"(s_call) : "memory");
-                    }
+                    for (int n = 1; n <= (holders[i].parts > kKvGroup ? 2 : 1); ++n)
+                        asm volatile("red.relaxed.gpu.global.max.u64 [%0], %1;" ::"l"(split.count + join_of(i, n).count), "l"(s_call) : "memory");
                 }
             }
         }
@@ -1021,18 +989,17 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
         for (int phase_no = 0; phase_no < 3; ++phase_no) {
             if (phase_no == 1 && !open) break;
             if (phase_no > 0) {
-                const bool first = phase_no == 1 ? open_first : turn[0] && parts[0] > kKvGroup,
-                           second = phase_no == 1 ? open_last : turn[1] && parts[1] > kKvGroup;   // what there is to count
+                const bool first = phase_no == 1 ? open_first : turn[0] && holders[0].parts > kKvGroup,
+                           second = phase_no == 1 ? open_last : turn[1] && holders[1].parts > kKvGroup;   // what there is to count
                 __syncthreads();   // the CTA's parts are written
                 if (tid < 64 && lane == 0) {   // warp 0 for the first unit, warp 1 for the last
                     const int i = tid >> 5;
-                    int of;
-                    const unsigned long long* count = count_of(i, phase_no, of);
+                    const KvJoin join = join_of(i, phase_no);
                     bool mine_now = i ? second : first;
                     if (mine_now) {
                         unsigned long long done;
-                        asm volatile("atom.acq_rel.gpu.global.add.u64 %0, [%1], 1;" : "=l"(done) : "l"(count) : "memory");
-                        mine_now = done == s_call + of - 1;
+                        asm volatile("atom.acq_rel.gpu.global.add.u64 %0, [%1], 1;" : "=l"(done) : "l"(split.count + join.count) : "memory");
+                        mine_now = done == s_call + join.n - 1;
                     }
                     s_turn[i] = mine_now;
                 }
@@ -1065,18 +1032,16 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
                     to = partial_of(blockIdx.x, begun & members ? 1 : 0);
                 } else {
                     if (!(task ? turn[1] : turn[0])) continue;
-                    const int own = task ? owner[1] : owner[0], all = task ? parts[1] : parts[0];
-                    const int group = ((int)blockIdx.x - own) / kKvGroup, groups = (all + kKvGroup - 1) / kKvGroup;
-                    const int lead = phase_no == 1 ? own + group * kKvGroup : own;
-                    const int n = phase_no == 1 ? min(kKvGroup, all - group * kKvGroup) : groups;
-                    const int cta = lead + (phase_no == 1 ? 1 : kKvGroup) * min(lane, n - 1);
-                    const float* rows = partial_of(cta, cta == own ? 1 : 0);
+                    const KvHolders held = task ? holders[1] : holders[0];
+                    const KvJoin join = kv_join(held, blockIdx.x, phase_no, gridDim.x);
+                    const int cta = join.lead + join.step * min(lane, join.n - 1);
+                    const float* rows = partial_of(cta, cta == held.owner ? 1 : 0);
                     from = rows + row * D;
                     from_stats = rows + chunk_rows * D + 3 * row;
-                    members = (1u << n) - 1u;
+                    members = (1u << join.n) - 1u;
                     u = __shfl_sync(0xffffffffu, unit, task ? e_last : e_first);
-                    final_row = phase_no == 2 || groups == 1;
-                    to = partial_of(lead, lead == own ? 1 : 0);
+                    final_row = phase_no == 2 || held.parts <= kKvGroup;
+                    to = partial_of(join.lead, join.lead == held.owner ? 1 : 0);
                 }
                 constexpr int kQuads = (D + 127) / 128;   // lane: elements 4 lane + 128 i .. + 3
                 const bool member = members >> lane & 1u;

@@ -1,4 +1,4 @@
-// Paged key-value cache: host-side interface of its kernels (kv_cache.cu, kv_attend_*.cu) and the page layout.
+// Paged key-value cache: host-side interface of its kernels (kv_cache.cu, kv_attend_*.cu) and the page layout (how work is cut: kv_split.cuh).
 //
 // A page holds page_size tokens of every head; the unit of the layout is the RECORD: the keys and values of 16
 // consecutive tokens of one head, contiguous, 16-byte aligned,

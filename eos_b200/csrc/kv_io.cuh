@@ -19,20 +19,13 @@
 // starts, rows and page table, and the record's old bytes one after the other.
 #pragma once
 #include "kv_dev.cuh"
+#include "kv_split.cuh"
 
 namespace eosb {
 
 constexpr int kKvIoWarps = 8;
 
-// The sequence and record that work unit u of a call stands for.  Sequence b starts at unit cu[b] / 16 + 2 b: n tokens
-// that start anywhere in a record touch at most floor((n + 30) / 16) records, and the gap to sequence b + 1 is at least
-// that.  Warp-wide search, 32 probes a step; lanes agree on the result.
-struct KvUnit {
-    int b, rec;       // sequence, record index within the sequence
-    int lo, hi;       // positions [lo, hi) of the record that the call covers
-    int64_t row0;     // row of position 0 of the sequence (may be negative: rows are row0 + position)
-    bool ok;
-};
+// The sequence and record that work unit u of a call stands for.  Warp-wide search, 32 probes a step; lanes agree on the result.
 __device__ __forceinline__ KvUnit kv_unit(const KvSeqs& s, int64_t tokens, int64_t u, int lane, int* errors) {
     KvUnit r;
     r.ok = false;
@@ -46,7 +39,7 @@ __device__ __forceinline__ KvUnit kv_unit(const KvSeqs& s, int64_t tokens, int64
         while (hi - lo > 1) {
             const int step = (hi - lo + 31) >> 5;
             const int probe = lo + lane * step;
-            const bool below = lane == 0 || (probe < hi && (int64_t)(__ldg(s.cu + probe) >> 4) + 2 * (int64_t)probe <= u);
+            const bool below = lane == 0 || (probe < hi && kv_unit_start(__ldg(s.cu + probe), probe) <= u);
             const int top = 31 - __clz(__ballot_sync(0xffffffffu, below));
             lo += top * step;
             hi = min(hi, lo + step);
@@ -55,20 +48,14 @@ __device__ __forceinline__ KvUnit kv_unit(const KvSeqs& s, int64_t tokens, int64
         row = __ldg(s.cu + lo);
         start = __ldg(s.starts + lo);
         n = (int64_t)__ldg(s.cu + lo + 1) - row;
-        first = u - ((int64_t)(row >> 4) + 2 * (int64_t)lo);
+        first = u - kv_unit_start((int)row, lo);
     }
     if (n == 0) return r;
     if (n < 0 || row < 0 || row + n > tokens || start < 0 || start + n > 0x7fffffffLL) {
         if (lane == 0) kv_report(errors, kStatusBadSequence);
         return r;
     }
-    const int64_t rec = (start >> 4) + first;
-    if (first < 0 || rec * kKvRecord >= start + n) return r;
-    r.rec = (int)rec;
-    r.lo = (int)max(start, rec * kKvRecord);
-    r.hi = (int)min(start + n, (rec + 1) * kKvRecord);
-    r.row0 = row - start;
-    r.ok = true;
+    r.ok = kv_place(r, row, n, start, first);
     return r;
 }
 
@@ -594,13 +581,10 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
 }
 
 // ---------------------------------------------------------------- launches
-// Work units of a call: see kv_unit.  The rows behind the last sequence belong to no unit.
-inline int64_t kv_units(const KvSeqs& s, int64_t tokens) { return s.cu == nullptr ? tokens : (tokens >> 4) + 2 * (int64_t)s.batch; }
-
 template <bool READ, int FMT, int NB, int TYPE>
 void kv_io_launch(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int64_t tokens, int* errors,
                   cudaStream_t stream) {
-    const int64_t units = kv_units(seqs, tokens);
+    const int64_t units = kv_units(seqs.cu != nullptr, tokens, seqs.batch);
     const unsigned blocks = (unsigned)((units * pool.heads + kKvIoWarps - 1) / kKvIoWarps) + (seqs.cu != nullptr ? 1u : 0u);   // (kv_check_offsets)
     if constexpr (READ) kv_read_kernel<FMT, NB, TYPE><<<blocks, kKvIoWarps * 32, 0, stream>>>(pool, seqs, key, value, tokens, units, errors);
     else kv_append_kernel<FMT, NB, TYPE><<<blocks, kKvIoWarps * 32, 0, stream>>>(pool, seqs, key, value, tokens, units, errors);

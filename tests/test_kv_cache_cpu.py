@@ -287,3 +287,168 @@ def test_strides_of_the_wrong_count_are_refused(monkeypatch):
     for strides in ((64,), (64, 64, 64), ()):
         with pytest.raises(ValueError, match="strides"):
             cache.attend_device(1, "f16", 1, 1, 1, 1, 1, 1, 1.0, query_strides=strides)
+
+
+def test_divisions_by_constants_of_a_launch(tmp_path):
+    run_cpp(tmp_path, r"""
+#include "kv_split.cuh"
+int main() {
+    std::srand(1);
+    const long long fixed[] = {0, 1, 2, 15, 16, 147, 148, 149, (1ll << 31) - 2, (1ll << 31) - 1, 1ll << 31, (1ll << 31) + 1, 1ll << 40};
+    for (int i = 0; i < 3000; ++i) {
+        const uint32_t d = i < 2000 ? i + 1 : i < 2030 ? 1u << (i - 2000) : 1u + (uint32_t)std::rand();
+        const KvDiv by(d);
+        for (long long a : fixed)
+            if (by(a) != a / d || kv_div(a, d) != a / d) return 1;
+        for (int j = 0; j < 200; ++j) {
+            const long long r = std::rand(), k = r / d * d;   // and next to multiples
+            for (long long a : {r, k, k + d - 1, k ? k - 1 : 0})
+                if (by(a) != a / d || kv_div(a, d) != a / d) return 2;
+        }
+    }
+    std::puts("ok");
+}
+""")
+
+
+def test_work_units_place_every_row_once(tmp_path):
+    """The kernels' own arithmetic: every position of every sequence is in one unit, with the row that belongs to it."""
+    run_cpp(tmp_path, r"""
+#include "kv_split.cuh"
+int main() {
+    std::srand(2);
+    const int some[] = {0, 1, 2, 15, 16, 17, 31};
+    for (int round = 0; round < 400; ++round) {
+        const int batch = 1 + std::rand() % 40;
+        std::vector<int> n(batch), start(batch), cu(1, 0);
+        for (int b = 0; b < batch; ++b) {
+            n[b] = std::rand() % 3 ? some[std::rand() % 7] : std::rand() % 200;
+            start[b] = std::rand() % 4 ? std::rand() % 100 : INT_MAX - n[b] - std::rand() % 20;
+            cu.push_back(cu.back() + n[b]);
+        }
+        const int tokens = cu.back() + std::rand() % 20;   // rows behind the last sequence
+        std::set<std::pair<int, int>> seen;
+        for (int64_t u = 0; u < kv_units(true, tokens, batch); ++u) {
+            int b = 0;
+            for (int i = 1; i < batch; ++i)
+                if (kv_unit_start(cu[i], i) <= u) b = i;
+            KvUnit w{};
+            if (n[b] == 0 || !kv_place(w, cu[b], n[b], start[b], u - kv_unit_start(cu[b], b))) continue;
+            if (w.lo >= w.hi || w.lo / 16 != w.rec || (w.hi - 1) / 16 != w.rec) return 1;
+            for (int64_t p = w.lo; p < w.hi; ++p) {
+                const int64_t row = w.row0 + p;
+                if (row < cu[b] || row >= cu[b + 1] || p != start[b] + (row - cu[b])) return 2;
+                if (!seen.insert({b, (int)row}).second) return 3;
+            }
+        }
+        if ((int)seen.size() != cu.back()) return 4;
+        for (int b = 0; b < batch; ++b) {   // without row offsets: a unit a sequence
+            KvUnit w{};
+            if (start[b] == INT_MAX) continue;
+            if (!kv_place(w, b, 1, start[b], 0) || w.lo != start[b] || w.hi != start[b] + 1 || w.row0 + w.lo != b) return 5;
+        }
+        if (kv_units(false, batch, batch) != batch) return 6;
+    }
+    std::puts("ok");
+}
+""")
+
+
+def test_parts_of_a_unit_are_joined_once(tmp_path):
+    """The kernel's own ranges and joins: what teams and CTAs hold of every unit, who joins it and which count says so."""
+    run_cpp(tmp_path, r"""
+#include <map>
+#include "kv_split.cuh"
+struct Part { int unit, records, which; KvHolders held; };
+int main() {
+    std::srand(3);
+    for (int round = 0; round < 1500; ++round) {
+        const int all_ctas[] = {1, 3, 24, 25, 49, 148, 744}, all_teams[] = {1, 2, 3, 4, 8, 12, 16};
+        const int ctas = all_ctas[std::rand() % 7], teams = all_teams[std::rand() % 7], units = 1 + std::rand() % 60;
+        std::vector<int64_t> n(units), from(units + 1, 0);
+        const int kind = std::rand() % 3;
+        for (int u = 0; u < units; ++u) {
+            n[u] = kind == 0 ? 1 + std::rand() % 9 : kind == 1 ? 1 + std::rand() % 400 : u == units / 2 ? 1 + std::rand() % 20000 : 1 + std::rand() % 50;
+            from[u + 1] = from[u] + n[u];
+        }
+        const int64_t total = from[units];
+        const KvDiv by_ctas(ctas), by_teams(teams);
+        const int64_t part = kv_part(by_ctas, total);
+        if (part * ctas < total || part < kKvMinRecords) return 1;
+        std::vector<int64_t> whole(units, 0);
+        std::map<std::pair<int, int>, Part> parts;   // (cta, which)
+        for (int c = 0; c < ctas; ++c) {
+            const int64_t c0 = kv_least(c * part, total), c1 = kv_least((c + 1) * part, total);
+            struct Entry { int unit; bool begins, ends; int records; int64_t from; };
+            std::vector<Entry> entries;
+            int64_t reached = c0;
+            for (int t = 0; t < teams; ++t) {
+                const KvRange r = kv_team_range(by_teams, c0, c1, t);
+                if (r.begin != reached || r.end < r.begin) return 2;
+                reached = r.end;
+                for (int64_t at = r.begin; at < r.end;) {
+                    int u = 0;
+                    while (from[u + 1] <= at) ++u;
+                    const int64_t end = kv_least(from[u + 1], r.end);
+                    const bool begins = at == from[u], ends = end == from[u + 1];
+                    if (begins && ends) whole[u] += n[u];
+                    else entries.push_back({u, begins, ends, (int)(end - at), from[u]});
+                    at = end;
+                }
+            }
+            if (reached != c1) return 3;
+            for (size_t i = 0; i < entries.size();) {   // runs of equal units
+                size_t j = i;
+                bool begun = false, ended = false;
+                int records = 0;
+                for (; j < entries.size() && entries[j].unit == entries[i].unit; ++j) {
+                    begun |= entries[j].begins, ended |= entries[j].ends;
+                    records += entries[j].records;
+                }
+                const int u = entries[i].unit;
+                if (begun && ended) whole[u] += records;
+                else {
+                    if (begun ? j != entries.size() : i != 0) return 4;   // only the first and the last run are open
+                    if (parts.count({c, begun ? 1 : 0})) return 5;
+                    parts[{c, begun ? 1 : 0}] = {u, records, begun ? 1 : 0, kv_holders(from[u], n[u], part)};
+                }
+                i = j;
+            }
+        }
+        std::map<int, std::pair<int, int>> counts;   // count -> (unit, lead)
+        std::map<int, int> arrivals;
+        for (auto& [key, p] : parts) {
+            const int c = key.first, u = p.unit;
+            if (c < p.held.owner || c >= p.held.owner + p.held.parts || p.which != (c == p.held.owner ? 1 : 0)) return 6;
+            whole[u] += p.records;
+            const KvJoin a = kv_join(p.held, c, 1, ctas);
+            if (c < a.lead || c >= a.lead + a.n * a.step || a.n > kKvGroup || a.n > 31) return 7;
+            for (int i = 0; i < a.n; ++i) {
+                auto q = parts.find({a.lead + i * a.step, a.lead + i * a.step == p.held.owner ? 1 : 0});
+                if (q == parts.end() || q->second.unit != u) return 8;
+            }
+            if (a.count < 0 || a.count >= 2 * ctas || !counts.emplace(a.count, std::make_pair(u, a.lead)).second && counts[a.count] != std::make_pair(u, a.lead)) return 9;
+            if (++arrivals[a.count] > a.n) return 10;
+            if (arrivals[a.count] == a.n && p.held.parts > kKvGroup) {   // this group is joined: phase 2
+                const KvJoin g = kv_join(p.held, c, 2, ctas);
+                if (g.lead != p.held.owner || g.n > 31 || g.count < 2 * ctas || g.count >= 3 * ctas) return 11;
+                if (!counts.emplace(g.count, std::make_pair(u, -1)).second && counts[g.count] != std::make_pair(u, -1)) return 12;
+                bool leads = false;
+                for (int i = 0; i < g.n; ++i) leads |= g.lead + i * g.step == a.lead;
+                if (!leads || ++arrivals[g.count] > g.n) return 13;
+            }
+        }
+        for (auto& [key, p] : parts) {   // every count is reached
+            const KvJoin a = kv_join(p.held, key.first, 1, ctas);
+            if (arrivals[a.count] != a.n) return 14;
+            const KvJoin g = kv_join(p.held, key.first, 2, ctas);
+            if (p.held.parts > kKvGroup && arrivals[g.count] != g.n) return 15;
+        }
+        for (int u = 0; u < units; ++u)
+            if (whole[u] != n[u]) return 16;
+        // whole units: those that fit a little more than an equal range
+        if (!kv_keep_whole(1, part + kKvWhole, part) || kv_keep_whole(1, part + kKvWhole + 1, part)) return 17;
+    }
+    std::puts("ok");
+}
+""")
