@@ -1,5 +1,8 @@
 """Paged key-value cache on the device, at the limits of what its calls allow: the bits that results carry, the range of
 scores and lengths, errors and workspaces of caches that live side by side."""
+import random
+
+import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -381,3 +384,65 @@ def test_attends_that_overlapped_leave_nothing_behind():
             again, lse2 = s.attend(q, n, 0.125, window)
             assert same(again, out) and same(lse2, lse)
     s.sync()
+
+
+@pytest.mark.parametrize("fmt,type_,dim,group", [("bf16", "bf16", 128, 130), ("mx4", "f32", 64, 200), ("f16", "f16", 96, 70), ("mx8", "bf16", 32, 300),
+                                                 ("bf16", "f32", 256, 65)])
+def test_many_query_heads_over_a_sequence_that_is_cut(fmt, type_, dim, group):
+    """Several chunks of query heads for a key head, the last one short, in units that tens of CTAs hold parts of: joined by
+    neighbours, over the groups, and beside a short sequence."""
+    lengths = [9, 13001]
+    s = Sequences(fmt, dim, 1, 64, lengths, seed=4)
+    k, v = tensors(sum(lengths), 1, dim, type_, 111)
+    s.append(k, v, [0, 0], lengths)
+    q = tensors(2, group, dim, type_, 112)[0]
+    scale = 2 * dim ** -0.5
+    out, lse = s.attend(q, lengths, scale)
+    s.sync()
+    cut = lambda x: torch.split(stored(x, fmt), lengths)  # noqa: E731
+    check_attend(q, (cut(k), cut(v)), lengths, scale, 0, fmt, out, lse, group)
+    again, lse2 = s.attend(q, lengths, scale)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("seed", range(48))
+def test_shapes_at_random(seed):
+    """Any format, type, head size, sharing, page and lengths: written in two calls, read back from anywhere, attended to through
+    any strides and windows."""
+    r = random.Random(1000 + seed)
+    fmt, type_, dim = r.choice(["f16", "bf16", "mx8", "mx4"]), r.choice(["f32", "f16", "bf16"]), r.choice([32, 64, 96, 128, 192, 256])
+    heads, group = r.choice([1, 2, 3, 5, 8]), r.choice([1, 2, 3, 4, 7, 8, 9, 12, 16, 17, 31, 40, 65])
+    page, batch, window = r.choice([16, 32, 48, 80, 256]), r.choice([1, 2, 3, 7, 20, 60, 150]), r.choice([0, 0, 0, 1, 15, 16, 17, 100, 1000])
+    most = max(1, min(4000, 200000 // (batch * heads * max(1, group // 4) * dim // 64 + 1)))
+    n = [r.choice([0, 1, r.randint(0, most), int(most ** r.random()), most]) for _ in range(batch)]
+    n[0] = max(n[0], 1)
+    s = Sequences(fmt, dim, heads, page, n, seed=seed)
+    k, v = tensors(sum(n), heads, dim, type_, seed)
+    first = [r.randint(0, x) for x in n]
+    at = np.cumsum([0] + n)
+    rows = lambda lo, hi: np.concatenate([np.arange(at[b] + lo[b], at[b] + hi[b]) for b in range(batch)])  # noqa: E731
+    for lo, hi in (([0] * batch, first), (first, n)):
+        some = rows(lo, hi)
+        if len(some):
+            s.append(k[some].contiguous(), v[some].contiguous(), lo, [b - a for a, b in zip(lo, hi)])
+    sk, sv = stored(k, fmt), stored(v, fmt)
+    lo = [r.randint(0, x) for x in n]
+    hi = [r.randint(a, x) for a, x in zip(lo, n)]
+    rk, rv = s.read(lo, [b - a for a, b in zip(lo, hi)], fill=-3.0)
+    some = rows(lo, hi)
+    assert same(rk[:len(some)], sk[some]) and same(rv[:len(some)], sv[some]) and (rk[len(some):] == -3).all()
+    q = tensors(batch, heads * group, dim, type_, seed + 1)[0]
+    strides, view = (0, 0), q
+    if r.random() < 0.5:
+        head, more, off = dim + r.choice([0, 1, 8, 4]), r.choice([0, 3, 8]), r.choice([0, 1, 8])
+        strides = heads * group * head + more, head
+        view = torch.as_strided(torch.zeros(batch * strides[0] + 8, dtype=q.dtype, device="cuda"), q.shape, strides + (1,), off)
+        view.copy_(q)
+    scale = dim ** -0.5 * r.choice([1, 1, 0.1, 3, -1])
+    out, lse = s.attend(view, n, scale, window, strides, shape=q.shape)
+    s.sync()
+    few = sorted({0, batch - 1} | {r.randrange(batch) for _ in range(3)})
+    check_attend(q[few], [[x[at[b]:at[b + 1]] for b in few] for x in (sk, sv)], [n[b] for b in few], scale, window, fmt, out[few], lse[few], group)
+    assert torch.isfinite(out.float()).all()
+    again, lse2 = s.attend(view, n, scale, window, strides, shape=q.shape)
+    assert same(out, again) and same(lse, lse2)
