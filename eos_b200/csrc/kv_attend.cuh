@@ -7,29 +7,34 @@
 // formed transposed: S^T = K q^T with the tokens as the 16 rows and 8 query heads of the key head as the columns, then
 // O^T += V^T P^T with 16 elements of the values as the rows.  The few query heads that share a key head fill the narrow
 // side of the instruction, keys and values its wide one, and the accumulators take half of what heads as rows would.
-// (tcgen05 wants 128 rows of keys in shared memory, in an operand type: the conversion of the codes would have to be
-// written back there first, and the weights once more through it; the kernel is bound by HBM and by the conversions.)
+// (tcgen05 wants 128 rows and its operands in shared memory or TMEM.  Its 16-bit kinds would have the codes converted and written
+// back there first, and the weights once more; its block-scaled kinds take the codes as they are, but then query and weights have
+// to be sums of several e4m3 numbers, and the value scales, one for 32 elements of a token, run along the wrong axis.  The 16-bit
+// formats are at HBM's rate without it.)
 //
 // Every fp32 factor -- the weights, and a query that does not fit the operand type (fp32, or f16 over a bf16 cache) -- is
 // the sum of two 16-bit operands, so the products carry 22 bits.  Over a bf16 cache, whose operands hold 8, it is the sum of
 // three for fp32 queries and results, 24 bits, and of two, 16, for 16-bit ones, which keep 11 at most (an f16 query is exact in
-// two; its lse stays that of 32 bits, for it is taken before the split).  The cached value is never split: it is exact in its operand type.  (Weights in one f16 operand where the result is bf16 saved 7 us of 90 over mx4 and 1 of 64 over mx8, and
-// moved one result in twenty to a neighbouring bf16 number: results are the rounding of one in 32 bits, whatever their type.)
+// two; its lse stays that of 32 bits, for it is taken before the split).  The cached value is never split: it is exact in its
+// operand type.  (Weights in one f16 operand where the result is bf16 saved 7 us of 90 over mx4 and 1 of 64 over mx8, and moved
+// one result in twenty to a neighbouring bf16 number.)
 //
 // The maxima are integers, and lag: m is set 7 below the largest score and moves only when a score passes m + 15, so most
 // records do no rescaling and no shuffles, and weights use f16's range from both ends: they stay below 2^15, and what
 // f16 cannot hold (2^-25) is 2^-31 of the row's largest weight.  A weight and its value's scale are multiplied before the
 // split: w = 2^(x - m + e - d) with e the largest scale exponent of the token's blocks and d a second lagging maximum,
-// relative to the first, so that the bound holds whatever the scales; the blocks' own exponents, relative to e, are f16 factors of the split weights
-// (four multiplications a block where scaling the codes takes eight), so the codes enter the mma as they are.
+// relative to the first, so that the bound holds whatever the scales; the blocks' own exponents, relative to e, are f16 factors of
+// the split weights (four multiplications a block where scaling the codes takes eight), so the codes enter the mma as they are.
 //
 // What bounds it (GPU time of a call, heads of 128 unless said; floor: the records' bytes at 6540 GB/s).  f16, 32 sequences of
 // 8192 tokens, 8 key heads with 8 query heads each: 174 to 179 us, 6.0 to 6.2 TB/s, floor 164: HBM.  mx8, one sequence of
 // 131071 tokens, 8 key heads with 4 query heads each: 55 us, 5.0 TB/s, floor 42: the loop runs at HBM's rate, and the rest is
 // a call's constant part -- launch and exit 2.5 us, lengths, page ids and the first records one after the other 4 us, joins
 // 4 to 5 us, of which 3 to 4 are those across CTAs.  mx4, 16 sequences of 4000 to 32768 tokens, 8 key heads with 8 query
-// heads each: 90 us, 3.4 TB/s, floor 47: the conversion of the codes and the split of the weights, some 400 instructions
-// a warp and record, of which 170 run at half rate.  One short sequence: 7 us, launch and latencies.
+// heads each: 90 us, 3.4 TB/s, floor 47: no one unit -- 425 instructions a warp and record, of which 173 run at half rate, fill 55 %
+// of the issue slots and 38 % of that pipe; the rest is the latency of dependent instructions that four warps a scheduler do not
+// hide (wait 1.8, math pipe 0.8, barriers 0.7, shared memory 0.6 stalls an instruction), and 10 to 12 us of prologue and joins.  Spills are
+// two loads in 425 instructions.  One short sequence: 8 us, launch and latencies.
 #pragma once
 #include <algorithm>
 
@@ -573,7 +578,7 @@ struct KvShape {
     // 65536 / (32 warps)
     static constexpr int kRegisters = 8 * NB * RT + 4 * NB * RT * HALVES;
     // (16 instead of 12 for mx8 and heads of 128: a batch of up to 4097 tokens 68 us instead of 63; 12 instead of 16 for mx4:
-    // 96 instead of 90, whose spills of some 80 bytes cost less than the warps bring.)
+    // 96 instead of 90, whose spills cost less than the warps bring.)
     // Two records at a time where a record is much arithmetic for few bytes: mx8, 131071 tokens, 56.5 us instead of 61.3 one
     // at a time, mx4 89.6 instead of 96.8; 16-bit formats lose by it, heads of 64 under fp32 queries 38.4 instead of 32.8.
     static constexpr bool kPair = FMT >= kKvMx8 && NB * RT <= 4;

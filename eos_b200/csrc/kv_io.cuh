@@ -168,8 +168,9 @@ __device__ __forceinline__ void store_lane(uint8_t* plane0, int lane, const uint
 // Raw words that a lane holds of the keys, or of the values.  The block-scaled formats are bound by latency, so the values
 // are loaded when the keys are done with, and the registers that saves go to more warps (16-bit rows of 128 to mx8: 32
 // warps an SM 159 us with the read back (155 now), 24 warps 168, 16 warps with all loads first 176; fetching the values' rows into
-// the L2 meanwhile brings nothing); the plain formats run at HBM's
-// rate with all loads first.
+// the L2 meanwhile brings nothing); the plain formats run at HBM's rate with all loads first.  The warps are bought with spills
+// (-Xptxas -v, bytes stored and loaded a thread): 16-bit rows of 128 to mx8 64 registers, 124 and 140, to mx4 48 and 80; of 192
+// 80 registers, 168 to 176 and 196 to 204, to mx4 80 to 88 and 128 to 140; of 256 to mx8 32 and 32; of 96 64 and 96; fp32 rows 4 to 48.
 __host__ __device__ constexpr int kv_raw_words(int nb, int type) { return type == kTypeF32 ? 16 * nb : 8 * nb; }
 __host__ __device__ constexpr int kv_append_blocks(int fmt, int nb, int type) {
     return fmt < kKvMx8 ? 1 : kv_raw_words(nb, type) <= 32 ? 4 : kv_raw_words(nb, type) <= 48 ? 3 : kv_raw_words(nb, type) <= 64 ? 2 : 1;

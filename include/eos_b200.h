@@ -566,7 +566,8 @@ EOS_B200_API int eos_b200_token_pool_encode(EosB200TokenPool* tp, const int32_t*
 #define EOS_B200_KV_MX8 2
 #define EOS_B200_KV_MX4 3
 typedef struct EosB200KvCache EosB200KvCache;
-/* Allocates `pages` pages (zeroed) of page_size tokens x kv_heads heads, keys and values. */
+/* Allocates `pages` pages (zeroed) of page_size tokens x kv_heads heads, keys and values, and a workspace for the cache's attention
+ * calls: 11 MB at head_dim 32, 30 MB at 128, 59 MB at 256. */
 EOS_B200_API int eos_b200_kv_cache_create(EosB200Runtime* rt, int64_t pages, int page_size, int kv_heads, int head_dim, int format,
                                           EosB200KvCache** out, char** err);
 EOS_B200_API void eos_b200_kv_cache_destroy(EosB200KvCache* cache);
@@ -600,10 +601,11 @@ EOS_B200_API int eos_b200_kv_cache_read_device(EosB200KvCache* cache, void* d_ke
                                                EosB200Stats* stats, char** err);
 /* Attention of one new token per sequence: query [batch, q_heads, head_dim] of `type`, query head i reads key head
  * i / (q_heads / kv_heads).  Sequence b attends to positions [max(0, n - window), n), n = d_lengths[b] (window 0: all
- * of them):  out = sum_j softmax_j(scale q . k_j) v_j, sums in fp32, rounded to `type` into d_out [batch, q_heads, head_dim]
+ * of them):  out = sum_j softmax_j(scale q . k_j) v_j, sums in fp32 of weights (and fp32 queries) of 22 bits or more (over BF16 pages
+ * 24 under fp32 queries, 16 under 16-bit ones), rounded to `type` into d_out [batch, q_heads, head_dim]
  * (contiguous, 16-byte aligned, apart from the query); d_lse (nullable) [batch, q_heads] fp32 receives
- * ln sum_j exp(scale q . k_j).  A sequence with n = 0 gives zeros and -infinity.  query_seq_stride / query_head_stride in elements, 0: contiguous.  The new token's own key and value
- * are appended before the call when it attends to itself.
+ * ln sum_j exp(scale q . k_j).  A sequence with n = 0 gives zeros and -infinity.  query_seq_stride / query_head_stride in elements,
+ * 0: contiguous.  The new token's own key and value are appended before the call when it attends to itself.
  * batch is at most 65535.  Positions on a page that is out of range are left out and eos_b200_kv_cache_sync reports it; a
  * length that is negative or longer than the page table is cut, and reported too.  Rows that meet an infinity or a NaN are
  * not finite; other rows are not touched by it.  scale q, the sums q . k and the scores scale q . k have to stay within fp32's range
