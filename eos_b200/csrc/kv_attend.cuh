@@ -296,17 +296,23 @@ struct KvWarp {
     template <bool EDGE>
     __device__ __forceinline__ void value_scales(const uint8_t* rec, int lo, int hi, uint32_t (&rel)[2][NB], int lane) const {
         const int t = lane & 3;
-        uint32_t tops[2], odd = 0;
+        uint32_t tops[2], live[2] = {0xffffffffu, 0xffffffffu}, odd = 0;
+        if constexpr (EDGE) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int tok = 2 * t + 8 * p;
+                live[p] = kv_live_bytes(tok >= lo && tok < hi, tok + 1 >= lo && tok + 1 < hi);
+            }
+        }
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
             uint32_t w[(NB + 1) / 2];
             load_pair_scales<NB>(rec + kv_value_scale_offset(FMT, NB) + (t + 4 * p) * 2 * kv_scale_stride(NB), w);
-            tops[p] = *reinterpret_cast<const uint32_t*>(rec + kv_value_top_offset(FMT, NB) + 4 * (t + 4 * p));
+            tops[p] = *reinterpret_cast<const uint32_t*>(rec + kv_value_top_offset(FMT, NB) + 4 * (t + 4 * p)) & live[p];
             odd |= tops[p];
-            // bytes 60 - 4 (top - e): with zeros below them, the f16 numbers 2^(e - top), top - e <= 14
-            const uint32_t c = 0x3c3c3c3cu - __byte_perm(tops[p], 0, 0x1010) * 4u;
+            const uint32_t both = __byte_perm(tops[p], 0, 0x1010);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) rel[p][b] = __byte_perm(w[b / 2] * 4u + c, 0, b & 1 ? 0x3424 : 0x1404);
+            for (int b = 0; b < NB; ++b) rel[p][b] = __byte_perm(kv_relative_scales(w[b / 2] & live[p], both), 0, b & 1 ? 0x3424 : 0x1404);
         }
         if (__any_sync(0xffffffffu, (odd & 0xffff0000u) != 0u)) {
 #pragma unroll

@@ -52,6 +52,12 @@ __host__ __device__ constexpr int kv_record_bytes(int format, int blocks) {
     return kv_value_top_offset(format, blocks) + (format <= kKvBf16 ? 0 : 32);
 }
 constexpr int kKvNear = 14;   // exponents below a token's largest that the attention kernel's ordinary path covers
+// Scale bytes of a token pair's values, two blocks of (first token, second token), relative to the tokens' largest (tops: twice
+// the pair's): bytes 60 - 4 (top - e), with zeros below them the f16 numbers 2^(e - top) for top - e <= kKvNear.  Four
+// subtractions in one, right as long as no byte leaves its place; a token that does not count may hold anything -- it may be
+// written meanwhile, its top already and its scales not yet -- so its bytes are masked first.
+__host__ __device__ inline uint32_t kv_relative_scales(uint32_t scales, uint32_t tops) { return scales * 4u + (0x3c3c3c3cu - tops * 4u); }
+__host__ __device__ inline uint32_t kv_live_bytes(bool first, bool second) { return (first ? 0x00ff00ffu : 0u) | (second ? 0xff00ff00u : 0u); }
 // offset of byte p of a lane's `bytes` bytes (planes of 16, then 8, then 4 bytes per lane)
 __host__ __device__ constexpr int kv_lane_offset(int bytes, int lane, int p) {
     const int plane = p >> 4, in = p & 15, rest = bytes - (plane << 4);

@@ -446,3 +446,40 @@ def test_shapes_at_random(seed):
     assert torch.isfinite(out.float()).all()
     again, lse2 = s.attend(view, n, scale, window, strides, shape=q.shape)
     assert same(out, again) and same(lse, lse2)
+
+
+@pytest.mark.parametrize("fmt", ["f16", "mx8", "mx4"])
+def test_attends_and_reads_while_the_next_tokens_are_appended(fmt):
+    """What lies behind the length may be written while the positions before it are read: tokens of very unlike size, zeros and
+    values that are not finite, at the places beside the last one and in the same words."""
+    dim, heads, group, n, more = 128, 2, 4, [1001, 40], 9
+    s = Sequences(fmt, dim, heads, 32, [x + more for x in n])
+    k, v = tensors(sum(n), heads, dim, "f16", 121)
+    s.append(k, v, [0, 0], n)
+    q = tensors(2, heads * group, dim, "f16", 122)[0]
+    want, lse = s.attend(q, n, 0.125)
+    rk, rv = s.read([0, 0], n, "f16")
+    table = []                                       # rows of `more` tokens for each sequence
+    for size in (2.0 ** -14, 1.0, 2.0 ** 12, float("nan"), 0.0):
+        x = tensors(2 * more, heads, dim, "f32", 123)[1] * size
+        x[:, :, 32:64] *= 2.0 ** -18
+        table.append(x)
+    reader, writer = torch.cuda.Stream(), torch.cuda.Stream()
+    cu, at, lengths, zero = s._ints([0, more, 2 * more]), s._ints(n), s._ints(n), s._ints([0, 0])
+    all_cu = s._ints([0, n[0], n[0] + n[1]])
+    outs = [torch.empty_like(q) for _ in range(60)]
+    reads = [(torch.empty_like(rk), torch.empty_like(rv)) for _ in outs]
+    torch.cuda.synchronize()
+    for i, (out, (k2, v2)) in enumerate(zip(outs, reads)):
+        for j in range(3):
+            x = table[(3 * i + j) % len(table)]
+            s.cache.append_device(x.data_ptr(), x.data_ptr(), "f32", 2 * more, 2, s.table.data_ptr(), s.max_pages, at.data_ptr(),
+                                  cu.data_ptr(), stream=writer.cuda_stream)
+        s.cache.attend_device(q.data_ptr(), "f16", heads * group, 2, s.table.data_ptr(), s.max_pages, lengths.data_ptr(),
+                              out.data_ptr(), 0.125, stream=reader.cuda_stream)
+        s.cache.read_device(k2.data_ptr(), v2.data_ptr(), "f16", sum(n), 2, s.table.data_ptr(), s.max_pages, zero.data_ptr(),
+                            all_cu.data_ptr(), stream=reader.cuda_stream)
+    torch.cuda.synchronize()
+    for out, (k2, v2) in zip(outs, reads):
+        assert same(out, want) and same(k2, rk) and same(v2, rv)
+    s.sync()

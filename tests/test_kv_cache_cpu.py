@@ -452,3 +452,31 @@ int main() {
     std::puts("ok");
 }
 """)
+
+
+def test_scales_of_a_live_token_beside_one_that_is_being_written(tmp_path):
+    """An attention may read a record while the token behind the last is appended: whatever bytes that one has at the moment, the live
+    token's come out as they are."""
+    run_cpp(tmp_path, r"""
+int main() {
+    std::srand(4);
+    for (int round = 0; round < 2000000; ++round) {
+        const int live = std::rand() % 3;   // the first, the second, both
+        uint32_t top[2], e[2][2];
+        for (int i = 0; i < 2; ++i) {
+            top[i] = std::rand() % 255;
+            for (int b = 0; b < 2; ++b) {
+                const int down = std::rand() % (kKvNear + 1);
+                e[b][i] = live == i || live == 2 ? (top[i] > (uint32_t)down ? top[i] - down : 0) : std::rand() % 256;
+            }
+        }
+        const uint32_t mask = kv_live_bytes(live != 1, live != 0);
+        const uint32_t scales = e[0][0] | e[0][1] << 8 | e[1][0] << 16 | e[1][1] << 24, pair = top[0] | top[1] << 8;
+        const uint32_t got = kv_relative_scales(scales & mask, (pair | pair << 16) & mask);
+        for (int i = 0; i < 2; ++i)
+            for (int b = 0; b < 2; ++b)
+                if ((live == i || live == 2) && (got >> (16 * b + 8 * i) & 255) != 60 - 4 * (top[i] - e[b][i])) return 1;
+    }
+    std::puts("ok");
+}
+""")
