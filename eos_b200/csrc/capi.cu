@@ -3718,7 +3718,7 @@ struct EosB200KvCache {
     KvPool pool{};
     KvWork work{};
     std::mutex lock;            // of `reported`
-    int reported[kKvErrors] = {};
+    uint64_t reported[kKvErrors] = {};
 };
 static_assert(kStatusBadPage == kStatusPipelineTimeout + 1 && kStatusBadSequence == kStatusPipelineTimeout + 2, "KvWork::errors");
 
@@ -3796,14 +3796,14 @@ int eos_b200_kv_cache_create(EosB200Runtime* rt, int64_t pages, int page_size, i
     c->device = rt->device;
     // one allocation: the pages, then the workspace (its counts first), each part 256-byte aligned
     const auto part = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
-    const size_t ctas = (size_t)rt->sm_count, pool_bytes = part((size_t)(pages * page_bytes)), count_bytes = part((3 * ctas + 1) * sizeof(uint64_t) + kKvErrors * sizeof(int)),
+    const size_t ctas = (size_t)rt->sm_count, pool_bytes = part((size_t)(pages * page_bytes)), count_bytes = part((3 * ctas + 1 + kKvErrors) * sizeof(uint64_t)),
                  slot_bytes = part(ctas * kv_slot_floats(head_dim) * sizeof(float));
     cudaError_t e = dev_alloc(&p.base, pool_bytes + count_bytes + slot_bytes + ctas * 2 * kKvMaxRows * (head_dim + 3) * sizeof(float));
     c->pool = p;
     c->work.ctas = rt->sm_count;
     if (e == cudaSuccess) {
         c->work.count = reinterpret_cast<uint64_t*>(p.base + pool_bytes);
-        c->work.errors = reinterpret_cast<int*>(c->work.count + 3 * ctas + 1);
+        c->work.errors = c->work.count + 3 * ctas + 1;
         c->work.slots = reinterpret_cast<float*>(p.base + pool_bytes + count_bytes);
         c->work.partial = reinterpret_cast<float*>(p.base + pool_bytes + count_bytes + slot_bytes);
         e = cudaMemsetAsync(p.base, 0, pool_bytes + count_bytes, rt->stream);
@@ -3915,15 +3915,14 @@ int eos_b200_kv_cache_sync(EosB200KvCache* c, void* stream, char** err) {
     if (c == nullptr) return fail(err, "kv_cache_sync: null cache");
     CUDA_TRY(cudaSetDevice(c->rt->device));
     const cudaStream_t s = pick_stream(c->rt, stream);
-    int met[kKvErrors];
+    uint64_t met[kKvErrors];
     CUDA_TRY(cudaMemcpyAsync(met, c->work.errors, sizeof(met), cudaMemcpyDeviceToHost, s));
     CUDA_TRY(cudaStreamSynchronize(s));
     std::string what;
     {
         std::lock_guard<std::mutex> guard(c->lock);
         for (int i = 0; i < kKvErrors; ++i) {
-            // (another thread's sync may have seen later counts: the difference is then not above 0)
-            if ((int)((unsigned)met[i] - (unsigned)c->reported[i]) <= 0) continue;
+            if (met[i] <= c->reported[i]) continue;   // (less: another thread's sync has seen later counts)
             c->reported[i] = met[i];
             what += (what.empty() ? "" : "; ") + status_text(kStatusPipelineTimeout + i);
         }

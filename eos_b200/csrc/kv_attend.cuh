@@ -680,7 +680,7 @@ __device__ __forceinline__ float load_part(const float* p) {
 
 template <int FMT, int NB, int RT, int HALVES>
 __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
-    kv_attend_kernel(KvPool pool, KvSeqs seqs, KvAttend a, KvSplit split, int* errors) {
+    kv_attend_kernel(KvPool pool, KvSeqs seqs, KvAttend a, KvSplit split, uint64_t* errors) {
     using Shape = KvShape<FMT, NB, RT, HALVES>;
     constexpr int D = 32 * NB, kRows = Shape::kRows, kMaxWarps = Shape::kMaxWarps, kMaxStages = Shape::kMaxStages;
     extern __shared__ __align__(128) uint8_t smem[];          // rings
@@ -845,11 +845,11 @@ __global__ void __launch_bounds__(KvShape<FMT, NB, RT, HALVES>::kMaxThreads, 1)
                             if (src != nullptr) {
                                 kv_copy_record(ring_at + st * Shape::kRecord, src + lane * Shape::kRecord, Shape::kRecord, full_at + 8 * st, policy);
                             } else {
-                                kv_report(errors, kStatusBadPage);
                                 mbar_arrive(full_at + 8 * st);
                             }
                         }
                     }
+                    if (src == nullptr && lane == 0) kv_report(errors, kStatusBadPage);
                     if (row_warps > 1) alive = __all_sync(0xffffffffu, alive);
                     if (src != nullptr) src += k * Shape::kRecord;
                     run -= k;
@@ -1143,7 +1143,7 @@ struct KvAttendInstance {
     static cudaError_t init() {
         return cudaFuncSetAttribute(kv_attend_kernel<FMT, NB, RT, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmemMax);
     }
-    static int launch(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors,
+    static int launch(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, uint64_t* errors,
                       cudaStream_t stream) {
         KvSplit split{};
         // warps for the rows of a key head: as many as it takes to cover them, a power of two, at most 8 (64 or 128 rows)
@@ -1183,14 +1183,14 @@ struct KvAttendInstance {
 // to convert, 113 against 108 (of 128: 82 against 80).
 constexpr bool kv_two_tiles(int fmt, int nb, int halves) { return fmt >= kKvMx8 && nb * (16 + 8 * halves) <= 144; }
 template <int FMT, int NB, int HALVES>
-int kv_attend_tiles(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors, cudaStream_t stream) {
+int kv_attend_tiles(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, uint64_t* errors, cudaStream_t stream) {
     if constexpr (kv_two_tiles(FMT, NB, HALVES))
         if (a.group > 8) return KvAttendInstance<FMT, NB, 2, HALVES>::launch(pool, seqs, a, work, errors, stream);
     return KvAttendInstance<FMT, NB, 1, HALVES>::launch(pool, seqs, a, work, errors, stream);
 }
 // The query is one operand where its type fits it exactly.
 template <int FMT, int NB>
-int kv_attend_rows(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors, cudaStream_t stream) {
+int kv_attend_rows(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, uint64_t* errors, cudaStream_t stream) {
     if (a.type == kTypeBf16 || (a.type == kTypeF16 && FMT != kKvBf16))
         return kv_attend_tiles<FMT, NB, 1>(pool, seqs, a, work, errors, stream);
     if constexpr (FMT == kKvBf16)
@@ -1215,7 +1215,7 @@ cudaError_t kv_attend_rows_init() {
 }
 
 template <int FMT>
-int kv_attend_format(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors, cudaStream_t stream) {
+int kv_attend_format(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, uint64_t* errors, cudaStream_t stream) {
     switch (pool.blocks) {
         case 1: return kv_attend_rows<FMT, 1>(pool, seqs, a, work, errors, stream);
         case 2: return kv_attend_rows<FMT, 2>(pool, seqs, a, work, errors, stream);
@@ -1237,10 +1237,10 @@ cudaError_t kv_attend_format_init(int blocks) {
     }
 }
 
-int kv_attend_f16(const KvPool&, const KvSeqs&, const KvAttend&, const KvWork&, int*, cudaStream_t);
-int kv_attend_bf16(const KvPool&, const KvSeqs&, const KvAttend&, const KvWork&, int*, cudaStream_t);
-int kv_attend_mx8(const KvPool&, const KvSeqs&, const KvAttend&, const KvWork&, int*, cudaStream_t);
-int kv_attend_mx4(const KvPool&, const KvSeqs&, const KvAttend&, const KvWork&, int*, cudaStream_t);
+int kv_attend_f16(const KvPool&, const KvSeqs&, const KvAttend&, const KvWork&, uint64_t*, cudaStream_t);
+int kv_attend_bf16(const KvPool&, const KvSeqs&, const KvAttend&, const KvWork&, uint64_t*, cudaStream_t);
+int kv_attend_mx8(const KvPool&, const KvSeqs&, const KvAttend&, const KvWork&, uint64_t*, cudaStream_t);
+int kv_attend_mx4(const KvPool&, const KvSeqs&, const KvAttend&, const KvWork&, uint64_t*, cudaStream_t);
 cudaError_t kv_attend_f16_init(int blocks);
 cudaError_t kv_attend_bf16_init(int blocks);
 cudaError_t kv_attend_mx8_init(int blocks);

@@ -3,7 +3,7 @@
 
 namespace eosb {
 
-int kv_attend_mx4(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors,
+int kv_attend_mx4(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, uint64_t* errors,
                  cudaStream_t stream) {
     return kv_attend_format<kKvMx4>(pool, seqs, a, work, errors, stream);
 }

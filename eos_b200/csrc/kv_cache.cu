@@ -7,7 +7,7 @@
 namespace eosb {
 
 void launch_kv_append(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type,
-                      int64_t tokens, int* errors, cudaStream_t stream) {
+                      int64_t tokens, uint64_t* errors, cudaStream_t stream) {
     switch (pool.format) {
         case kKvF16: return kv_append_f16(pool, seqs, key, value, type, tokens, errors, stream);
         case kKvBf16: return kv_append_bf16(pool, seqs, key, value, type, tokens, errors, stream);
@@ -17,7 +17,7 @@ void launch_kv_append(const KvPool& pool, const KvSeqs& seqs, const KvRows& key,
 }
 
 void launch_kv_read(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
-                    int* errors, cudaStream_t stream) {
+                    uint64_t* errors, cudaStream_t stream) {
     switch (pool.format) {
         case kKvF16: return kv_read_f16(pool, seqs, key, value, type, tokens, errors, stream);
         case kKvBf16: return kv_read_bf16(pool, seqs, key, value, type, tokens, errors, stream);
@@ -26,7 +26,7 @@ void launch_kv_read(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, c
     }
 }
 
-int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors,
+int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, uint64_t* errors,
                      cudaStream_t stream) {
     switch (pool.format) {
         case kKvF16: return kv_attend_f16(pool, seqs, a, work, errors, stream);

@@ -92,9 +92,9 @@ struct KvRows {             // keys or values of a call, [tokens, heads, dim] wi
 };
 
 void launch_kv_append(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type,
-                      int64_t tokens, int* errors, cudaStream_t stream);
+                      int64_t tokens, uint64_t* errors, cudaStream_t stream);
 void launch_kv_read(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
-                    int* errors, cudaStream_t stream);
+                    uint64_t* errors, cudaStream_t stream);
 
 struct KvAttend {
     const void* query;      // [batch, q_heads, dim], strides in elements
@@ -114,7 +114,7 @@ struct KvWork {
     float* slots;           // [ctas][kv_slot_floats(dim)]: partial results of the CTAs' warps
     float* partial;         // [ctas][2][kKvMaxRows][dim + 3]: of the CTAs
     uint64_t* count;        // [3 ctas], and how many CTAs have run (see kv_attend.cuh); zero at first, never set back
-    int* errors;            // [kKvErrors] what append, read and attend met; the counts only grow, the host remembers what it has reported
+    uint64_t* errors;       // [kKvErrors] what append, read and attend met; the counts only grow, the host remembers what it has reported
 };
 constexpr int kKvErrors = 3;           // pipeline timeout, bad page, bad sequence: kStatusPipelineTimeout and the two codes behind it
 constexpr int kKvMaxRows = 128;        // query heads of one unit, at most
@@ -123,7 +123,7 @@ __host__ __device__ constexpr int kv_slot_floats(int dim) { return kKvMaxRows * 
 
 // cudaSuccess once the kernels of this format and dim are ready on the current device
 cudaError_t kv_init(int format, int blocks);
-int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, int* errors,
+int launch_kv_attend(const KvPool& pool, const KvSeqs& seqs, const KvAttend& a, const KvWork& work, uint64_t* errors,
                      cudaStream_t stream);
 
 }  // namespace eosb

@@ -98,7 +98,9 @@ __device__ __forceinline__ void load_pair_scales(const uint8_t* p, uint32_t (&w)
 }
 // ---------------------------------------------------------------- errors
 // Counts an error that a call met (see KvWork).
-__device__ __forceinline__ void kv_report(int* errors, int code) { atomicAdd(errors + (code - kStatusPipelineTimeout), 1); }
+__device__ __forceinline__ void kv_report(uint64_t* errors, int code) {
+    atomicAdd(reinterpret_cast<unsigned long long*>(errors) + (code - kStatusPipelineTimeout), 1ull);
+}
 
 // ---------------------------------------------------------------- pages
 // The record of `rec` (record index in sequence b) and head h; null when the table or the page id is out of range.

@@ -26,7 +26,7 @@ namespace eosb {
 constexpr int kKvIoWarps = 8;
 
 // The sequence and record that work unit u of a call stands for.  Warp-wide search, 32 probes a step; lanes agree on the result.
-__device__ __forceinline__ KvUnit kv_unit(const KvSeqs& s, int64_t tokens, int64_t u, int lane, int* errors) {
+__device__ __forceinline__ KvUnit kv_unit(const KvSeqs& s, int64_t tokens, int64_t u, int lane, uint64_t* errors) {
     KvUnit r;
     r.ok = false;
     int64_t row, n, first = 0;
@@ -61,7 +61,7 @@ __device__ __forceinline__ KvUnit kv_unit(const KvSeqs& s, int64_t tokens, int64
 
 // The row offsets of a call, looked over by one block (the last; the work's own would not meet all that is wrong, for where offsets
 // descend the search above passes sequences by): ascending from 0 or more to `tokens` or less.
-__device__ __forceinline__ void kv_check_offsets(const KvSeqs& s, int64_t tokens, int* errors) {
+__device__ __forceinline__ void kv_check_offsets(const KvSeqs& s, int64_t tokens, uint64_t* errors) {
     bool bad = false;
     for (int b = threadIdx.x; b < s.batch; b += blockDim.x) {
         const int from = __ldg(s.cu + b), to = __ldg(s.cu + b + 1);
@@ -177,7 +177,7 @@ __host__ __device__ constexpr int kv_append_blocks(int fmt, int nb, int type) {
 }
 template <int FMT, int NB, int TYPE>
 __global__ void __launch_bounds__(kKvIoWarps * 32, kv_append_blocks(FMT, NB, TYPE))
-    kv_append_kernel(KvPool pool, KvSeqs seqs, KvRows key, KvRows value, int64_t tokens, int64_t units, int* errors) {
+    kv_append_kernel(KvPool pool, KvSeqs seqs, KvRows key, KvRows value, int64_t tokens, int64_t units, uint64_t* errors) {
     constexpr bool kMx = FMT >= kKvMx8;
     constexpr int KP = kv_key_piece(FMT), VP = kv_value_piece(FMT), NS = kv_scale_stride(NB), ES = TYPE == kTypeF32 ? 4 : 2;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -484,7 +484,7 @@ __device__ __forceinline__ void store_out(uint8_t* p, int vec, const float (&x)[
 
 template <int FMT, int NB, int TYPE>
 __global__ void __launch_bounds__(kKvIoWarps * 32)
-    kv_read_kernel(KvPool pool, KvSeqs seqs, KvRows key, KvRows value, int64_t tokens, int64_t units, int* errors) {
+    kv_read_kernel(KvPool pool, KvSeqs seqs, KvRows key, KvRows value, int64_t tokens, int64_t units, uint64_t* errors) {
     constexpr bool kMx = FMT >= kKvMx8;
     constexpr int KP = kv_key_piece(FMT), VP = kv_value_piece(FMT), NS = kv_scale_stride(NB), ES = TYPE == kTypeF32 ? 4 : 2;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kKvIoWarps * 32)
 
 // ---------------------------------------------------------------- launches
 template <bool READ, int FMT, int NB, int TYPE>
-void kv_io_launch(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int64_t tokens, int* errors,
+void kv_io_launch(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int64_t tokens, uint64_t* errors,
                   cudaStream_t stream) {
     const int64_t units = kv_units(seqs.cu != nullptr, tokens, seqs.batch);
     const unsigned blocks = (unsigned)((units * pool.heads + kKvIoWarps - 1) / kKvIoWarps) + (seqs.cu != nullptr ? 1u : 0u);   // (kv_check_offsets)
@@ -592,7 +592,7 @@ void kv_io_launch(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, con
 }
 template <bool READ, int FMT, int NB>
 void kv_io_type(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
-                int* errors, cudaStream_t stream) {
+                uint64_t* errors, cudaStream_t stream) {
     switch (type) {
         case kTypeF32: return kv_io_launch<READ, FMT, NB, kTypeF32>(pool, seqs, key, value, tokens, errors, stream);
         case kTypeF16: return kv_io_launch<READ, FMT, NB, kTypeF16>(pool, seqs, key, value, tokens, errors, stream);
@@ -601,7 +601,7 @@ void kv_io_type(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const
 }
 template <bool READ, int FMT>
 void kv_io_format(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
-                  int* errors, cudaStream_t stream) {
+                  uint64_t* errors, cudaStream_t stream) {
     switch (pool.blocks) {
         case 1: return kv_io_type<READ, FMT, 1>(pool, seqs, key, value, type, tokens, errors, stream);
         case 2: return kv_io_type<READ, FMT, 2>(pool, seqs, key, value, type, tokens, errors, stream);
@@ -637,8 +637,8 @@ cudaError_t kv_io_format_init(int blocks) {
 }
 
 #define EOSB_KV_IO(name)                                                                                                   \
-    void kv_append_##name(const KvPool&, const KvSeqs&, const KvRows&, const KvRows&, int, int64_t, int*, cudaStream_t);   \
-    void kv_read_##name(const KvPool&, const KvSeqs&, const KvRows&, const KvRows&, int, int64_t, int*, cudaStream_t);     \
+    void kv_append_##name(const KvPool&, const KvSeqs&, const KvRows&, const KvRows&, int, int64_t, uint64_t*, cudaStream_t);   \
+    void kv_read_##name(const KvPool&, const KvSeqs&, const KvRows&, const KvRows&, int, int64_t, uint64_t*, cudaStream_t);     \
     cudaError_t kv_io_##name##_init(int blocks);
 EOSB_KV_IO(f16)
 EOSB_KV_IO(bf16)

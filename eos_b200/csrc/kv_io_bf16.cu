@@ -4,11 +4,11 @@
 namespace eosb {
 
 void kv_append_bf16(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
-                  int* errors, cudaStream_t stream) {
+                  uint64_t* errors, cudaStream_t stream) {
     kv_io_format<false, kKvBf16>(pool, seqs, key, value, type, tokens, errors, stream);
 }
 void kv_read_bf16(const KvPool& pool, const KvSeqs& seqs, const KvRows& key, const KvRows& value, int type, int64_t tokens,
-                int* errors, cudaStream_t stream) {
+                uint64_t* errors, cudaStream_t stream) {
     kv_io_format<true, kKvBf16>(pool, seqs, key, value, type, tokens, errors, stream);
 }
 

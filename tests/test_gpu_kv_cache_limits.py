@@ -483,3 +483,25 @@ def test_attends_and_reads_while_the_next_tokens_are_appended(fmt):
     for out, (k2, v2) in zip(outs, reads):
         assert same(out, want) and same(k2, rk) and same(v2, rv)
     s.sync()
+
+
+def test_a_table_that_names_no_page():
+    """2^27 records of two sequences, none of them on a page: nothing is attended to, and it is reported, once."""
+    import eos_b200
+    rt = eos_b200.Runtime(0)
+    dim, page, wide = 32, 65536, 32768
+    cache = eos_b200.KvCache(rt, 1, page, 1, dim, "mx4")
+    table = torch.full((2, wide), -1, dtype=torch.int32, device="cuda")
+    table[1, 1:] = 1
+    q = tensors(2, 2, dim, "f16", 131)[0]
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    lengths = torch.tensor([2 ** 30, 2 ** 30], dtype=torch.int32, device="cuda")
+    for _ in range(2):
+        cache.attend_device(q.data_ptr(), "f16", 2, 2, table.data_ptr(), wide, lengths.data_ptr(), out.data_ptr(), 0.2, 0, lse.data_ptr(),
+                            stream=st)
+        with pytest.raises(eos_b200.EosB200DeviceStatusError, match="page"):
+            cache.sync(st)
+        assert (out == 0).all() and (lse == float("-inf")).all()
+    cache.sync(st)
+    cache.close()
