@@ -242,7 +242,7 @@ struct KvWarp {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) c[r][i >> 2][i & 3] = 0.f;
 #pragma unroll
-            for (int h = 0; h < HALVES; ++h)
+            for (int h = HALVES - 1; h >= 0; --h)   // the smallest parts first: a sum is cut at its size in every step
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -280,7 +280,7 @@ struct KvWarp {
                 for (int r = 0; r < RT; ++r) {
                     float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int u = 0; u < HALVES; ++u) {
+                    for (int u = HALVES - 1; u >= 0; --u) {
                         mma_16x8x16<false>(c, f[0], h[0], f[1], h[1], q[r][b][4 * u], q[r][b][4 * u + 1]);
                         mma_16x8x16<false>(c, f[2], h[2], f[3], h[3], q[r][b][4 * u + 2], q[r][b][4 * u + 3]);
                     }
